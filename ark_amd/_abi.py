@@ -134,5 +134,25 @@ class GradSpan(C.Structure):
     _fields_ = [("dst", C.c_void_p), ("src", C.c_void_p), ("n", C.c_uint64)]
 
 
+# include/ark_act.h
+ACT_F16 = 0
+ACT_BF16 = 1
+ACT_F32 = 2
+ACT_GROUP = 32
+ACT_ACCUMULATE = 1
+ACT_TRANSPOSED = 2
+
+
+# include/ark_rope.h
+ROPE_HALF = 0
+ROPE_INTERLEAVED = 1
+ROPE_MAX_HEAD = 512
+ROPE_SCALE_NONE = 0
+ROPE_SCALE_LINEAR = 1
+ROPE_SCALE_NTK = 2
+ROPE_SCALE_YARN = 3
+ROPE_SCALE_BANDS = 4
+
+
 # every struct whose size ark_opt_struct_sizes reports, in its order
 ALL_STRUCTS = STRUCTS + (CodecSpan, CkptRecord, CkptInfo, GradSpan)

@@ -27,7 +27,7 @@ class ArkOptError(RuntimeError):
 
 def _declare(L):
     P = C.c_void_p
-    u64, u32, i32, f32 = C.c_uint64, C.c_uint32, C.c_int32, C.c_float
+    u64, u32, i32, f32, f64 = C.c_uint64, C.c_uint32, C.c_int32, C.c_float, C.c_double
     H = C.c_void_p  # opaque handle
     sig = {
         "ark_opt_abi_version": ([], C.c_int),
@@ -82,6 +82,20 @@ def _declare(L):
         "ark_grad_embed_scatter_noalloc": ([P, u32, u32, P, P, u32, P], C.c_int),
         "ark_grad_plan_run_final": ([H, H], C.c_int),
         "ark_grad_embed_scatter_final": ([P, u32, u32, P, P, u32, H], C.c_int),
+        "ark_act_bytes": ([u64, u64, C.POINTER(u64)], C.c_int),
+        "ark_act_pack": ([P, u64, u32, u64, u64, P, P], C.c_int),
+        "ark_act_unpack": ([P, u64, u64, u32, P, u64, P], C.c_int),
+        "ark_act_weight_grad": ([P, u32, u64, u64, P, u64, u32, u64, P, u64, u32, P], C.c_int),
+        "ark_rope_frequencies": ([u32, f64, u32, C.POINTER(f64), C.POINTER(f64),
+                                  C.POINTER(f64)], C.c_int),
+        "ark_rope_create": ([u32, u32, u32, C.POINTER(f64), f64, C.POINTER(H)], C.c_int),
+        "ark_rope_destroy": ([H], C.c_int),
+        # layouts are host arrays of four uint64, passed by address
+        "ark_rope_apply": ([H, u32, u64, u64, P, u32, u64] + [P] * 8 + [u32, P], C.c_int),
+        "ark_rope_norm": ([H, u32, u64, u64, P, u32, u64, f32, P, P, u32] + [P] * 10 + [P],
+                          C.c_int),
+        "ark_rope_norm_backward": ([H, u32, u64, u64, P, u32, u64, f32, P, P, u32] + [P] * 16
+                                   + [u32, P], C.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)

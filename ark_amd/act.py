@@ -1,0 +1,123 @@
+"""Activations kept in 8 bits for the backward pass (include/ark_act.h) for
+torch tensors, and the weight gradient that reads them.
+
+``pack(x)`` keeps a layer's input as an ``Act8`` of half the bytes (a quarter
+of fp32's); ``weight_grad(kept, dy)`` is the weight gradient x^T dy from it, in
+fp32, written to or added into the gradients an optimizer steps on;
+``unpack(kept)`` gives the values back.
+"""
+import ctypes as C
+
+from . import _abi
+from ._lib import check, lib, current_stream as _stream
+
+_TYPES = None
+
+
+def _types():
+    global _TYPES
+    if _TYPES is None:
+        import torch
+        _TYPES = {torch.float16: _abi.ACT_F16, torch.bfloat16: _abi.ACT_BF16,
+                  torch.float32: _abi.ACT_F32}
+    return _TYPES
+
+
+def _code(t, what):
+    code = _types().get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what} holds {t.dtype}: float16, bfloat16 and float32 are taken")
+    return code
+
+
+def _rows(t, what):
+    """(address, row stride) of a 2-D device tensor whose rows are contiguous."""
+    if t.dim() != 2:
+        raise ValueError(f"{what} has {t.dim()} dimensions, not 2")
+    if not t.is_cuda:
+        raise ValueError(f"{what} is not a device tensor")
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        raise ValueError(f"{what}: the values of a row do not follow one another")
+    return t.data_ptr(), t.stride(0)
+
+
+class Act8:
+    """The 8-bit form of a (tokens, columns) array of ``dtype``: ``data`` holds
+    33 bytes for every 32 tokens of a column."""
+
+    __slots__ = ("tokens", "columns", "dtype", "data")
+
+    def __init__(self, tokens, columns, dtype, device=None, data=None):
+        import torch
+        if dtype not in _types():
+            raise ValueError(f"dtype {dtype}: float16, bfloat16 and float32 are taken")
+        if tokens < 0 or columns < 0:
+            raise ValueError(f"sizes {tokens} x {columns}")
+        n = -(-tokens // _abi.ACT_GROUP) * columns * (_abi.ACT_GROUP + 1)
+        if data is None:
+            data = torch.empty(n, dtype=torch.uint8, device=device or "cuda")
+        elif data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() != n:
+            raise ValueError(f"data must be {n} contiguous uint8")
+        self.tokens, self.columns, self.dtype, self.data = tokens, columns, dtype, data
+
+    @property
+    def nbytes(self):
+        return self.data.numel()
+
+
+def pack(x, out=None):
+    """The 8-bit form of x (tokens x columns, rows of any stride), in ``out``
+    (an Act8 of the same sizes and type) or a new one."""
+    code = _code(x, "x")
+    p, stride = _rows(x, "x")
+    t, c = x.shape
+    if out is None:
+        out = Act8(t, c, x.dtype, x.device)
+    elif (out.tokens, out.columns, out.dtype) != (t, c, x.dtype) or out.data.device != x.device:
+        raise ValueError(f"out is {out.tokens} x {out.columns} {out.dtype}, x {t} x {c} {x.dtype}")
+    check(lib().ark_act_pack(p, stride, code, t, c, out.data.data_ptr(), _stream(x)))
+    return out
+
+
+def unpack(kept, out=None):
+    """The values of an Act8, in ``out`` (tokens x columns, rows of any stride)
+    or a new tensor of the type they were packed from."""
+    import torch
+    if out is None:
+        out = torch.empty((kept.tokens, kept.columns), dtype=kept.dtype, device=kept.data.device)
+    elif tuple(out.shape) != (kept.tokens, kept.columns) or out.device != kept.data.device:
+        raise ValueError(f"out is {tuple(out.shape)}, the activation {kept.tokens} x "
+                         f"{kept.columns}")
+    p, stride = _rows(out, "out")
+    check(lib().ark_act_unpack(kept.data.data_ptr(), kept.tokens, kept.columns,
+                               _code(out, "out"), p, stride, _stream(out)))
+    return out
+
+
+def weight_grad(kept, dy, dw=None, accumulate=False, layout="in_out"):
+    """dw (+)= x^T dy from the Act8 ``kept`` of x (tokens x columns) and dy
+    (tokens x outputs; float16 for an activation packed from float16, bfloat16
+    for any).  dw is float32, columns x outputs ("in_out") or outputs x columns
+    ("out_in"), rows of any stride; a new tensor when None.  accumulate adds to
+    it."""
+    import torch
+    if layout not in ("in_out", "out_in"):
+        raise ValueError(f"layout {layout!r}: 'in_out' or 'out_in'")
+    dp, dstride = _rows(dy, "dy")
+    if dy.shape[0] != kept.tokens or dy.device != kept.data.device:
+        raise ValueError(f"dy has {dy.shape[0]} rows, the activation {kept.tokens}")
+    n = dy.shape[1]
+    shape = (kept.columns, n) if layout == "in_out" else (n, kept.columns)
+    if dw is None:
+        if accumulate:
+            raise ValueError("accumulate needs a dw")
+        dw = torch.empty(shape, dtype=torch.float32, device=dy.device)
+    elif tuple(dw.shape) != shape or dw.dtype != torch.float32 or dw.device != dy.device:
+        raise ValueError(f"dw is {tuple(dw.shape)} {dw.dtype}, not {shape} float32")
+    wp, wstride = _rows(dw, "dw")
+    flags = (_abi.ACT_ACCUMULATE if accumulate else 0) | (
+        _abi.ACT_TRANSPOSED if layout == "out_in" else 0)
+    check(lib().ark_act_weight_grad(kept.data.data_ptr(), _types()[kept.dtype], kept.tokens,
+                                    kept.columns, dp, dstride, _code(dy, "dy"), n, wp, wstride,
+                                    flags, _stream(dy)))
+    return dw

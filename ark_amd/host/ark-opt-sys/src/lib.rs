@@ -288,6 +288,80 @@ extern "C" {
                                           stream: *mut c_void) -> c_int;
 }
 
+// ---- include/ark_act.h (no reference counterpart) ----------------------------
+
+pub const ARK_ACT_F16: u32 = 0;
+pub const ARK_ACT_BF16: u32 = 1;
+pub const ARK_ACT_F32: u32 = 2;
+pub const ARK_ACT_GROUP: u64 = 32;
+pub const ARK_ACT_ACCUMULATE: u32 = 1;
+pub const ARK_ACT_TRANSPOSED: u32 = 2;
+
+extern "C" {
+    /// Activations kept in 8 bits for the backward pass.
+    pub fn ark_act_bytes(tokens: u64, columns: u64, bytes: *mut u64) -> c_int;
+    pub fn ark_act_pack(x: *const c_void, x_stride: u64, dtype: u32, tokens: u64, columns: u64,
+                        act: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn ark_act_unpack(act: *const c_void, tokens: u64, columns: u64, dtype: u32,
+                          x: *mut c_void, x_stride: u64, stream: *mut c_void) -> c_int;
+    /// The weight gradient from an 8-bit input, into fp32 gradients.
+    pub fn ark_act_weight_grad(act: *const c_void, act_dtype: u32, tokens: u64, columns: u64,
+                               dy: *const c_void, dy_stride: u64, dy_dtype: u32, outputs: u64,
+                               dw: *mut f32, dw_stride: u64, flags: u32,
+                               stream: *mut c_void) -> c_int;
+}
+
+// ---- include/ark_rope.h (the rotation of `objc/bridge.m:229-411`; the norm of
+// heads has no reference counterpart) -------------------------------------------
+
+pub const ARK_ROPE_HALF: u32 = 0;
+pub const ARK_ROPE_INTERLEAVED: u32 = 1;
+pub const ARK_ROPE_MAX_HEAD: u32 = 512;
+pub const ARK_ROPE_SCALE_NONE: u32 = 0;
+pub const ARK_ROPE_SCALE_LINEAR: u32 = 1;
+pub const ARK_ROPE_SCALE_NTK: u32 = 2;
+pub const ARK_ROPE_SCALE_YARN: u32 = 3;
+pub const ARK_ROPE_SCALE_BANDS: u32 = 4;
+
+/// Opaque rotation of a model.
+#[repr(C)]
+pub struct ark_rope {
+    _private: [u8; 0],
+}
+
+extern "C" {
+    pub fn ark_rope_frequencies(rotary_dim: u32, base: f64, scaling: u32, params: *const f64,
+                                inv_freq: *mut f64, magnitude: *mut f64) -> c_int;
+    pub fn ark_rope_create(head_dim: u32, rotary_dim: u32, layout: u32, inv_freq: *const f64,
+                           magnitude: f64, out: *mut *mut ark_rope) -> c_int;
+    pub fn ark_rope_destroy(rope: *mut ark_rope) -> c_int;
+    pub fn ark_rope_apply(rope: *const ark_rope, dtype: u32, batch: u64, tokens: u64,
+                          positions: *const c_void, position_bytes: u32, start: u64,
+                          q: *const c_void, q_layout: *const u64, q_out: *mut c_void,
+                          q_out_layout: *const u64, k: *const c_void, k_layout: *const u64,
+                          k_out: *mut c_void, k_out_layout: *const u64, inverse: u32,
+                          stream: *mut c_void) -> c_int;
+    /// The norm of every head of q and k with the rotation, forward and backward.
+    pub fn ark_rope_norm(rope: *const ark_rope, dtype: u32, batch: u64, tokens: u64,
+                         positions: *const c_void, position_bytes: u32, start: u64, eps: f32,
+                         gain_q: *const c_void, gain_k: *const c_void, gain_dtype: u32,
+                         q: *const c_void, q_layout: *const u64, q_out: *mut c_void,
+                         q_out_layout: *const u64, q_act: *mut c_void, k: *const c_void,
+                         k_layout: *const u64, k_out: *mut c_void, k_out_layout: *const u64,
+                         k_act: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn ark_rope_norm_backward(rope: *const ark_rope, dtype: u32, batch: u64, tokens: u64,
+                                  positions: *const c_void, position_bytes: u32, start: u64,
+                                  eps: f32, gain_q: *const c_void, gain_k: *const c_void,
+                                  gain_dtype: u32, dq: *const c_void, dq_layout: *const u64,
+                                  q: *const c_void, q_layout: *const u64, q_act: *const c_void,
+                                  q_grad: *mut c_void, q_grad_layout: *const u64,
+                                  dgain_q: *mut f32, dk: *const c_void, dk_layout: *const u64,
+                                  k: *const c_void, k_layout: *const u64, k_act: *const c_void,
+                                  k_grad: *mut c_void, k_grad_layout: *const u64,
+                                  dgain_k: *mut f32, accumulate: u32,
+                                  stream: *mut c_void) -> c_int;
+}
+
 // ---- include/ark_synth.h (no reference counterpart: test and bench inputs) ---
 
 extern "C" {
