@@ -86,6 +86,9 @@ def _declare(L):
         "ark_act_pack": ([P, u64, u32, u64, u64, P, P], C.c_int),
         "ark_act_unpack": ([P, u64, u64, u32, P, u64, P], C.c_int),
         "ark_act_weight_grad": ([P, u32, u64, u64, P, u64, u32, u64, P, u64, u32, P], C.c_int),
+        "ark_act_weight_grad_workspace": ([u64, u64, u64, u64, C.POINTER(u64)], C.c_int),
+        "ark_act_weight_grad_noalloc": ([P, u32, u64, u64, P, u64, u32, u64, P, u64, u32, P, u64,
+                                         P], C.c_int),
         "ark_rope_frequencies": ([u32, f64, u32, C.POINTER(f64), C.POINTER(f64),
                                   C.POINTER(f64)], C.c_int),
         "ark_rope_create": ([u32, u32, u32, C.POINTER(f64), f64, C.POINTER(H)], C.c_int),

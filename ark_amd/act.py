@@ -117,7 +117,13 @@ def weight_grad(kept, dy, dw=None, accumulate=False, layout="in_out"):
     wp, wstride = _rows(dw, "dw")
     flags = (_abi.ACT_ACCUMULATE if accumulate else 0) | (
         _abi.ACT_TRANSPOSED if layout == "out_in" else 0)
-    check(lib().ark_act_weight_grad(kept.data.data_ptr(), _types()[kept.dtype], kept.tokens,
-                                    kept.columns, dp, dstride, _code(dy, "dy"), n, wp, wstride,
-                                    flags, _stream(dy)))
+    need = C.c_uint64()
+    check(lib().ark_act_weight_grad_workspace(kept.tokens, kept.columns, dstride, n,
+                                              C.byref(need)))
+    # torch's allocator hands a stream's memory back to it without waiting
+    ws = torch.empty(need.value, dtype=torch.uint8, device=dy.device) if need.value else None
+    check(lib().ark_act_weight_grad_noalloc(
+        kept.data.data_ptr(), _types()[kept.dtype], kept.tokens, kept.columns, dp, dstride,
+        _code(dy, "dy"), n, wp, wstride, flags, ws.data_ptr() if need.value else None, need.value,
+        _stream(dy)))
     return dw

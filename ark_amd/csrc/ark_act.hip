@@ -1,5 +1,9 @@
 // ark_act.hip -- activations kept in 8 bits and the weight gradient that reads
 // them (include/ark_act.h).
+#include <atomic>
+#include <type_traits>
+#include <utility>
+
 #include "ark_act.hpp"
 #include "ark_common.hpp"
 
@@ -63,38 +67,509 @@ __global__ __launch_bounds__(kLanes) void unpack_kernel(const uint8_t* __restric
   }
 }
 
-// 16 x 16 outputs a block, one a lane; both operands' tiles staged in LDS one
-// group of rows at a time.
+// ---- the weight gradient -----------------------------------------------------
+//
+// dw = act^T dy: rows m are act's columns, columns n are dy's, and the sum runs
+// over tokens.  A block of eight waves, four along m and two along n, forms a
+// tile of 64 MF x 32 NF outputs, a wave MF x NF matrix instructions of 16 x 16
+// over 32 tokens, a group of the 8-bit form.  act's layout is the instruction's
+// operand already: 32 tokens of a column follow one another, so a lane's eight
+// are 8 bytes, widened in registers under the column's exponent (exactly).  dy
+// lies the other way (tokens are its rows) and turns on its way out of LDS,
+// by the transposing read.  A step is 64 tokens: the next step's tile travels
+// from memory in registers while this one's is multiplied out of LDS, two LDS
+// buffers by turns, one barrier a step.
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+// words at any even address (gfx950 takes unaligned global accesses)
+typedef uint32_t u32_a2 __attribute__((aligned(2)));
+typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32x4_a1 __attribute__((ext_vector_type(4), aligned(1)));
+
+#define ARK_LDS __attribute__((address_space(3)))
+
+template <typename V>
+__device__ __forceinline__ ARK_LDS V* lds_at(uint32_t byte) {
+  return (ARK_LDS V*)(uintptr_t)byte;
+}
+
+constexpr uint32_t kStep = 64;                      // tokens a step
+constexpr uint32_t kStepGroups = kStep / ARK_ACT_GROUP;
+
+struct GradArgs {
+  const uint8_t* q;        // act's values
+  const uint8_t* e;        // and exponents
+  const uint16_t* dy;
+  float* dw;
+  float* partial;          // [splits][tiles][tile's values in lane order], or NULL
+  uint64_t tokens, dy_stride, dw_stride, groups;
+  uint32_t columns, outputs;
+  uint32_t m_tiles, n_tiles, splits, steps;  // steps of all splits together
+  uint32_t accumulate, vec;                  // vec: dw takes 16-byte stores
+};
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
+                                                                __builtin_bit_cast(u16x2, b)));
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void grad_kernel(const uint8_t* __restrict__ q,
-                                                   const uint8_t* __restrict__ e, uint64_t tokens,
-                                                   uint32_t columns, const T* __restrict__ dy,
-                                                   uint64_t dy_stride, uint32_t outputs,
-                                                   float* __restrict__ dw, uint64_t dw_stride,
-                                                   uint32_t flags) {
-  __shared__ float xs[16][ARK_ACT_GROUP + 1], ys[ARK_ACT_GROUP][17];
-  const uint32_t lc = threadIdx.x / 16, lo = threadIdx.x % 16;
-  const uint32_t c = blockIdx.x * 16 + lc, o = blockIdx.y * 16 + lo;
-  float sum = 0.0f;
-  for (uint64_t t0 = 0, g = 0; t0 < tokens; t0 += ARK_ACT_GROUP, ++g) {
-    for (uint32_t i = threadIdx.x; i < 16 * ARK_ACT_GROUP; i += 256) {
-      const uint32_t cc = i / ARK_ACT_GROUP, t = i % ARK_ACT_GROUP;
-      const uint32_t col = blockIdx.x * 16 + cc;
-      xs[cc][t] = col < columns ? act_value(q[(g * columns + col) * ARK_ACT_GROUP + t],
-                                            act_up(e[g * columns + col]))
-                                : 0.0f;
-      const uint32_t tt = i / 16, oo = blockIdx.y * 16 + i % 16;
-      ys[tt][i % 16] = t0 + tt < tokens && oo < outputs ? (float)dy[(t0 + tt) * dy_stride + oo]
-                                                        : 0.0f;
+struct Mat;
+template <>
+struct Mat<_Float16> {
+  typedef f16x8 Frag;
+  static __device__ __forceinline__ f32x4 mul(Frag a, Frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  // The instructions keep fewer bits of a product whose fp16 factor is
+  // subnormal, so a column is multiplied by the power of two that takes its
+  // largest exponent to 9 (65024 at most; 10, where |q| <= 63, stays): all its
+  // values are then normal but those 2^22 times smaller than its largest.  The
+  // sums are scaled back at the end, exactly.
+  static constexpr bool kShift = true;
+  static __device__ __forceinline__ uint32_t shift(uint32_t top) {
+    return top >= 143u ? 0u : 142u - top;
+  }
+  // what LDS holds of an exponent byte: 2^(e + shift) twice (at least 2^-24)
+  static __device__ __forceinline__ uint32_t scale(uint32_t s, uint32_t shift) {
+    const uint32_t h = __builtin_bit_cast(
+        uint16_t, (_Float16)(s == 255u ? act_up(s) : __uint_as_float((s - 6u + shift) << 23)));
+    return h | h << 16;
+  }
+  // eight bytes q + 128 -> q 2^e: the byte becomes the low mantissa of
+  // 1024 + q + 128, which fp16 holds, and both steps after it are exact
+  static __device__ __forceinline__ Frag widen(u32x2 w, uint32_t scale) {
+    const f16x2 s = __builtin_bit_cast(f16x2, scale);
+    const f16x2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t b = i < 2 ? w.x : w.y;
+      const uint32_t u = __builtin_amdgcn_perm(0x64646464u, b, i % 2 ? 0x04030402u : 0x04010400u);
+      r[i] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2, u) + off) * s);
+    }
+    return __builtin_bit_cast(Frag, r);
+  }
+};
+template <>
+struct Mat<__bf16> {
+  typedef bf16x8 Frag;
+  static __device__ __forceinline__ f32x4 mul(Frag a, Frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static constexpr bool kShift = false;  // bf16 has fp32's range
+  static __device__ __forceinline__ uint32_t shift(uint32_t) { return 0; }
+  static __device__ __forceinline__ uint32_t scale(uint32_t s, uint32_t) {
+    return __float_as_uint(act_up(s));
+  }
+  // q 2^e has at most 7 significant bits, so fp32's upper half is all of it
+  static __device__ __forceinline__ Frag widen(u32x2 w, uint32_t scale) {
+    const float s = __uint_as_float(scale);
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t b = (i < 2 ? w.x : w.y) ^ 0x80808080u;
+      const float lo = (float)(int8_t)(b >> (i % 2 * 16)) * s;
+      const float hi = (float)(int8_t)(b >> (i % 2 * 16 + 8)) * s;
+      r[i] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+    }
+    return __builtin_bit_cast(Frag, r);
+  }
+};
+
+// N neighbouring outputs of a token of dy.
+template <uint32_t N>
+struct Row {
+  uint32_t v[(N + 1) / 2] = {};
+  __device__ __forceinline__ void load(const char* p) {
+    if constexpr (N == 4) {
+      const u32x2_a2 t = *(const ARK_GLOBAL u32x2_a2*)p;
+      v[0] = t.x, v[1] = t.y;
+    } else if constexpr (N == 2) {
+      v[0] = *(const ARK_GLOBAL u32_a2*)p;
+    } else {
+      v[0] = ld_g<uint16_t>(p);
+    }
+  }
+  // drops the first n
+  __device__ __forceinline__ void shift(uint32_t n) {
+    if constexpr (N == 4) {
+      const uint64_t t = ((uint64_t)v[1] << 32 | v[0]) >> (n % 4 * 16);
+      v[0] = (uint32_t)t, v[1] = (uint32_t)(t >> 32);
+    } else if constexpr (N == 2) {
+      v[0] >>= n % 2 * 16;
+    }
+  }
+  // output c of this token and of the next
+  __device__ __forceinline__ uint32_t pair(const Row& next, uint32_t c) const {
+    return __builtin_amdgcn_perm(next.v[c / 2], v[c / 2], c % 2 ? 0x07060302u : 0x05040100u);
+  }
+};
+
+// f(0), f(1), ... f(N - 1), each index a constant.
+template <typename F, uint32_t... I>
+__device__ __forceinline__ void each(F f, std::integer_sequence<uint32_t, I...>) {
+  (f(std::integral_constant<uint32_t, I>()), ...);
+}
+template <uint32_t N, typename F>
+__device__ __forceinline__ void each(F f) {
+  each(f, std::make_integer_sequence<uint32_t, N>());
+}
+
+// A tile's shape, its LDS buffer and what a lane stages of it.
+template <uint32_t MF, uint32_t NF, uint32_t WN>
+struct Tile {
+  static constexpr uint32_t kLanes = 256 * WN;
+  static constexpr uint32_t kM = 64 * MF, kN = 16 * NF * WN;
+  static constexpr uint32_t kRow = kStep * 2;                    // bytes of an output of dy
+  static constexpr uint32_t kB = 0;                              // dy, then act, then scales
+  static constexpr uint32_t kA = kN * kRow;
+  static constexpr uint32_t kS = kA + kStepGroups * kM * ARK_ACT_GROUP;
+  static constexpr uint32_t kBytes = kS + kStepGroups * kM * 4;
+  static_assert(kBytes % kRow == 0, "a buffer starts at a multiple of a row");
+  static constexpr uint32_t kWide = NF / 2;                      // outputs a lane stages of 8 tokens
+  static constexpr uint32_t kAAll = kStepGroups * kM * 2;        // 16-byte chunks of act
+  static constexpr uint32_t kAChunks = (kAAll + kLanes - 1) / kLanes;
+  static constexpr uint32_t kScales = kStepGroups * kM;
+  static constexpr uint32_t kSChunks = (kScales + kLanes - 1) / kLanes;
+  static constexpr uint32_t kTop = 2 * kBytes;                   // a column's largest exponent
+  static constexpr uint32_t kLds = kTop + kM * 4;
+  static constexpr uint32_t kPhases = 2 * NF;                    // of MF products a step
+  static constexpr uint32_t kAhead = NF >= 4 ? 3 : 1;            // dy's reads ahead of them
+  // dy lies in LDS as [output][token], 128 bytes an output, its 16-byte chunks (8
+  // tokens) permuted so that neither the eight lanes that write one chunk of
+  // outputs kWide apart nor the eight that read one chunk of neighbouring
+  // outputs meet in a bank: bits 2-4 of the output, bit 1 on top of bit 4.
+  static __device__ __forceinline__ uint32_t swizzle(uint32_t n) {
+    return (n >> 2 & 7u) ^ (n >> 1 & 1u) << 2;
+  }
+};
+
+// One lane's four values of a 16 x 16 tile at (m, n): four neighbours of dw's
+// rows, which SWAP makes n ([columns][outputs]) and otherwise m (transposed).
+template <bool SWAP>
+__device__ __forceinline__ void grad_out(const GradArgs& a, uint32_t m, uint32_t n, uint32_t lane,
+                                         f32x4 v) {
+  const uint32_t row = (SWAP ? m : n) + lane % 16, col = (SWAP ? n : m) + lane / 16 * 4;
+  const uint32_t rows = SWAP ? a.columns : a.outputs, cols = SWAP ? a.outputs : a.columns;
+  if (row >= rows || col >= cols) return;
+  float* p = a.dw + row * a.dw_stride + col;
+  if (a.vec && col + 4 <= cols) {
+    if (a.accumulate) v += *(const f32x4*)p;
+    *(f32x4*)p = v;
+    return;
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < 4; ++k)
+    if (col + k < cols) p[k] = a.accumulate ? p[k] + v[k] : v[k];
+}
+
+// ANY: any stride and number of outputs; otherwise offsets inside a step fit 32
+// bits and there are eight outputs at least.
+template <typename T, uint32_t MF, uint32_t NF, uint32_t WN, bool SWAP, bool ANY>
+__global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
+  typedef typename std::conditional<ANY, uint64_t, uint32_t>::type Off;
+  typedef Tile<MF, NF, WN> L;
+  typedef Mat<T> M;
+  extern __shared__ __align__(16) uint8_t lds[];
+  const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  const uint32_t wm = wave % 4, wn = wave / 4, li = lane % 16, lg = lane / 16;
+  // blocks of one XCD (every eighth) take neighbouring tiles of one split, which
+  // share their operands in its L2
+  const uint32_t tiles = a.m_tiles * a.n_tiles, all = gridDim.x;
+  const uint32_t per = all / 8, rest = all % 8, xcd = blockIdx.x % 8;
+  const uint32_t id = xcd * per + (xcd < rest ? xcd : rest) + blockIdx.x / 8;
+  const uint32_t split = id / tiles, tile = id % tiles;
+  const uint32_t m0 = tile % a.m_tiles * L::kM, n0 = tile / a.m_tiles * L::kN;
+  const uint32_t s0 = (uint32_t)((uint64_t)a.steps * split / a.splits);
+  const uint32_t s1 = (uint32_t)((uint64_t)a.steps * (split + 1) / a.splits);
+
+  // What this lane stages of a step: 16 bytes of dy (8 outputs of a token) or of
+  // act at a time, and one exponent, at these offsets from the step's start.  No
+  // load needs a bound: outputs past the last are loaded from the last eight and
+  // shifted into place, columns, tokens and groups past the last repeat it, whose
+  // products are never stored or meet dy's zeros.
+  typedef Row<L::kWide> R;
+  R rb[8];
+  u32x4 ra[L::kAChunks];
+  uint32_t rs[L::kSChunks], shift[L::kSChunks] = {};
+  uint32_t* top = (uint32_t*)(lds + L::kTop);
+  constexpr uint32_t kAcross = L::kN / L::kWide;  // lanes of a token
+  const uint32_t b_row = tid / kAcross * 8, b_n = tid % kAcross * L::kWide;
+  const bool edge = n0 + L::kN > a.outputs && a.outputs % L::kWide;
+  const uint32_t b_col = n0 + b_n + L::kWide <= a.outputs ? n0 + b_n : a.outputs - L::kWide;
+  Off oa[L::kAChunks], os[L::kSChunks], ob = ((Off)b_row * (Off)a.dy_stride + b_col) * 2;  // bytes
+  // lanes past the last chunk stage it once more
+  const auto a_chunk = [&](uint32_t i) {
+    return min(tid + i * L::kLanes, L::kAAll - 1);
+  };
+  const auto s_chunk = [&](uint32_t i) { return min(tid + i * L::kLanes, L::kScales - 1); };
+  const auto place = [&](uint32_t groups) {  // of the step
+    const auto at = [&](uint32_t g, uint32_t m) {
+      return (Off)(g < groups ? g : groups - 1) * a.columns + (m < a.columns ? m : a.columns - 1);
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < L::kAChunks; ++i) {
+      const uint32_t c = a_chunk(i), r = c % (L::kM * 2);
+      oa[i] = at(c / (L::kM * 2), m0 + r / 2) * ARK_ACT_GROUP + r % 2 * 16;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < L::kSChunks; ++i)
+      os[i] = at(s_chunk(i) / L::kM, m0 + s_chunk(i) % L::kM);
+  };
+  const auto load = [&](uint32_t step) {
+    const char* dy = (const char*)(a.dy + (uint64_t)step * kStep * a.dy_stride);
+    if (step + 1 < a.steps) {
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) rb[i].load(dy + (uint64_t)i * a.dy_stride * 2 + ob);
+    } else {
+      const uint32_t n = (uint32_t)(a.tokens - (uint64_t)step * kStep);
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+        const uint32_t t = b_row + i < n ? b_row + i : n - 1;
+        rb[i].load(dy + ((Off)t * (Off)a.dy_stride + b_col) * 2);
+      }
+      place((uint32_t)(a.groups - (uint64_t)step * kStepGroups));
+    }
+    const uint64_t g0 = (uint64_t)step * kStepGroups * a.columns;
+    const char *q = (const char*)a.q + g0 * ARK_ACT_GROUP, *e = (const char*)a.e + g0;
+#pragma unroll
+    for (uint32_t i = 0; i < L::kAChunks; ++i) ra[i] = ld_g<u32x4>(q + oa[i]);
+#pragma unroll
+    for (uint32_t i = 0; i < L::kSChunks; ++i) rs[i] = ld_g<uint8_t>(e + os[i]);
+  };
+  // LDS is addressed in bytes.
+  const uint32_t base = (uint32_t)(uintptr_t)(ARK_LDS uint8_t*)lds;
+  const auto put_b = [&](uint32_t buf, uint32_t c) {  // output b_n + c
+    const uint32_t n = b_n + c;
+    u32x4 v;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) v[k] = rb[2 * k].pair(rb[2 * k + 1], c);
+    *lds_at<u32x4>(buf + n * L::kRow + (b_row / 8 ^ L::swizzle(n)) * 16) = v;
+  };
+  const auto put_a = [&](uint32_t buf, uint32_t i) {
+    *lds_at<u32x4>(buf + L::kA + a_chunk(i) * 16) = ra[i];
+  };
+  const auto put_s = [&](uint32_t buf, uint32_t i) {
+    *lds_at<uint32_t>(buf + L::kS + s_chunk(i) * 4) = M::scale(rs[i], shift[i]);
+  };
+  const auto store = [&](uint32_t buf, uint32_t step) {
+    if (edge) {
+      const uint32_t drop = n0 + b_n + L::kWide > a.outputs ? n0 + b_n + L::kWide - a.outputs : 0;
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) rb[i].shift(drop);
+    }
+    if (step + 1 == a.steps) {
+      const uint32_t n = (uint32_t)(a.tokens - (uint64_t)step * kStep);
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i)
+        if (b_row + i >= n) rb[i] = R();
+    }
+#pragma unroll
+    for (uint32_t c = 0; c < L::kWide; ++c) put_b(buf, c);
+#pragma unroll
+    for (uint32_t i = 0; i < L::kAChunks; ++i) put_a(buf, i);
+#pragma unroll
+    for (uint32_t i = 0; i < L::kSChunks; ++i) put_s(buf, i);
+  };
+
+  if (s0 < s1) {
+    place(kStepGroups);
+    load(s0);
+  }
+  if constexpr (M::kShift) {
+    for (uint32_t i = tid; i < L::kM; i += L::kLanes) top[i] = 109;
+    __syncthreads();
+    // the columns' exponents over the split, 16 columns of a group at a time
+    const uint32_t groups = (uint32_t)((uint64_t)s1 * kStepGroups < a.groups
+                                           ? (uint64_t)s1 * kStepGroups : a.groups);
+    const uint32_t m = tid % (L::kM / 16) * 16;
+    if (a.columns >= 16 && m0 + m < a.columns) {
+      const uint32_t c = m0 + m + 16 <= a.columns ? m0 + m : a.columns - 16;
+      u32x4 even = {0, 0, 0, 0}, odd = even;  // bytes 0 and 2, 1 and 3 of each word
+#pragma unroll 4
+      for (uint32_t g = s0 * kStepGroups + tid / (L::kM / 16); g < groups;
+           g += L::kLanes / (L::kM / 16)) {
+        const u32x4 v = *(const ARK_GLOBAL u32x4_a1*)(a.e + (uint64_t)g * a.columns + c);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+          even[k] = max_u16x2(even[k], v[k] & 0x00FF00FFu);
+          odd[k] = max_u16x2(odd[k], v[k] >> 8 & 0x00FF00FFu);
+        }
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < 16; ++k) {
+        const uint32_t v = (k % 2 ? odd : even)[k / 4] >> (k % 4 / 2 * 16) & 0xFFFFu;
+        if (c + k >= m0) atomicMax(&top[c + k - m0], v);
+      }
+    } else if (a.columns < 16 && tid < a.columns) {  // one tile, m0 = 0
+      for (uint32_t g = s0 * kStepGroups; g < groups; ++g)
+        atomicMax(&top[tid], (uint32_t)a.e[(uint64_t)g * a.columns + tid]);
     }
     __syncthreads();
-    for (uint32_t t = 0; t < ARK_ACT_GROUP; ++t) sum = __builtin_fmaf(xs[lc][t], ys[t][lo], sum);
+#pragma unroll
+    for (uint32_t i = 0; i < L::kSChunks; ++i) shift[i] = M::shift(top[s_chunk(i) % L::kM]);
+  }
+
+  f32x4 acc[MF][NF];
+#pragma unroll
+  for (uint32_t i = 0; i < MF; ++i)
+#pragma unroll
+    for (uint32_t j = 0; j < NF; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  // A step's products go in phases: the four (MF) that share dy's fragment j.
+  // dy's fragments are read kAhead phases before their products, act's of the
+  // next group while this one's are used.  The barrier comes when the last of
+  // the step's reads is done, before its last kAhead phases, which then read
+  // the next step's first fragments.
+  typename M::Frag b[L::kAhead + 1], x[2][MF];
+  u32x4 w[MF];
+  uint32_t sc[MF];
+  const uint32_t b_first = wn * NF * 16 + li;
+  const uint32_t b_get = b_first * L::kRow + (lg * 2 ^ L::swizzle(b_first)) * 16;
+  const uint32_t a_m = wm * MF * 16 + li;
+  const uint32_t a_get = L::kA + (lg / 2 * L::kM + a_m) * ARK_ACT_GROUP + lg % 2 * 16;
+  const uint32_t s_get = L::kS + (lg / 2 * L::kM + a_m) * 4;
+  const auto read_b = [&](uint32_t buf, uint32_t phase) {
+    const uint32_t h = phase / NF, j = phase % NF;
+    // 16 outputs on, bit 4 turns over, and with it the swizzle's bit 2
+    b[phase % (L::kAhead + 1)] = *lds_at<typename M::Frag>(
+        ((buf + b_get) ^ (h * 16 + j % 2 * 64)) + j * 16 * L::kRow);
+  };
+  const auto read_a = [&](uint32_t buf) {
+#pragma unroll
+    for (uint32_t i = 0; i < MF; ++i) {
+      w[i] = *lds_at<u32x4>(buf + a_get + i * 16 * ARK_ACT_GROUP);
+      sc[i] = *lds_at<uint32_t>(buf + s_get + i * 64);
+    }
+  };
+  const auto widen = [&](uint32_t h, uint32_t i) {
+    x[h][i] = M::widen(h ? u32x2{w[i].z, w[i].w} : u32x2{w[i].x, w[i].y}, sc[i]);
+  };
+  static_assert(L::kPhases % (L::kAhead + 1) == 0, "a step starts at b[0]");
+  if (s0 < s1) {
+    store(base, s0);
+    if (s0 + 1 < s1) load(s0 + 1);
     __syncthreads();
+#pragma unroll
+    for (uint32_t p = 0; p < L::kAhead; ++p) read_b(base, p);
+    read_a(base);
+#pragma unroll
+    for (uint32_t i = 0; i < MF; ++i) widen(0, i);
   }
-  if (c < columns && o < outputs) {
-    float* p = dw + (flags & ARK_ACT_TRANSPOSED ? o * dw_stride + c : c * dw_stride + o);
-    *p = flags & ARK_ACT_ACCUMULATE ? *p + sum : sum;
+  // A plain step's stores and loads one at a time: what the chunk's registers
+  // hold goes to the next step's buffer, and the chunk after it is asked for.
+  constexpr uint32_t kItemsB = L::kWide + 8, kItems = kItemsB + L::kAChunks + L::kSChunks;
+  const auto pass_on = [&](auto item, uint32_t buf, uint32_t step) {
+    constexpr uint32_t k = decltype(item)::value;
+    const uint64_t t0 = (uint64_t)step * kStep, g0 = (uint64_t)step * kStepGroups * a.columns;
+    if constexpr (k < L::kWide) {
+      put_b(buf, k);
+    } else if constexpr (k < kItemsB) {
+      constexpr uint32_t i = k - L::kWide;
+      Off o = ob;
+      asm("" : "+v"(o));  // kept apart from the base, which then stays scalar
+      rb[i].load((const char*)(a.dy + (t0 + i) * a.dy_stride) + o);
+    } else if constexpr (k < kItemsB + L::kAChunks) {
+      constexpr uint32_t i = k - kItemsB;
+      Off o = oa[i];
+      asm("" : "+v"(o));
+      put_a(buf, i);
+      ra[i] = ld_g<u32x4>((const char*)a.q + g0 * ARK_ACT_GROUP + o);
+    } else {
+      constexpr uint32_t i = k - kItemsB - L::kAChunks;
+      Off o = os[i];
+      asm("" : "+v"(o));
+      put_s(buf, i);
+      rs[i] = ld_g<uint8_t>((const char*)a.e + g0 + o);
+    }
+  };
+  const auto multiply = [&](uint32_t s, auto whole) {
+    constexpr bool kPlain = decltype(whole)::value;
+    constexpr uint32_t kLast = L::kPhases - L::kAhead;  // first phase past the barrier
+    const uint32_t odd = (s - s0) % 2;
+    const uint32_t cur = base + odd * L::kBytes, nxt = base + (odd ^ 1u) * L::kBytes;
+    each<L::kPhases>([&](auto phase) __attribute__((always_inline)) {
+      constexpr uint32_t p = decltype(phase)::value, h = p / NF, j = p % NF;
+      if constexpr (p + L::kAhead < L::kPhases)
+        read_b(cur, p + L::kAhead);
+      else
+        read_b(nxt, p + L::kAhead - L::kPhases);
+      if constexpr (p == kLast) read_a(nxt);
+      if constexpr (kPlain) {
+        each<kItems>([&](auto k) __attribute__((always_inline)) {
+          if constexpr (p == k * kLast / kItems) pass_on(k, nxt, s + 2);
+        });
+      } else {
+        if (p == 0 && s + 1 < s1) store(nxt, s + 1);
+        if (p == 1 && s + 2 < s1) load(s + 2);
+      }
+      // the other half's fragments, over the last phases of this one's
+      constexpr uint32_t kOver = NF < MF ? NF : h == 1 && L::kAhead < MF ? L::kAhead : MF;
+#pragma unroll
+      for (uint32_t i = 0; i < MF; ++i)
+        if (j == NF - kOver + i * kOver / MF) widen(h ^ 1u, i);
+#pragma unroll
+      for (uint32_t i = 0; i < MF; ++i)
+        acc[i][j] = SWAP ? M::mul(b[p % (L::kAhead + 1)], x[h][i], acc[i][j])
+                         : M::mul(x[h][i], b[p % (L::kAhead + 1)], acc[i][j]);
+      if constexpr (p + 1 == kLast) __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  // steps whose loads and stores are plain, then the others
+  uint32_t s = s0;
+  if (!edge)
+    for (; s + 2 < s1 && s + 3 < a.steps; ++s) multiply(s, std::true_type());
+  for (; s < s1; ++s) multiply(s, std::false_type());
+  if constexpr (M::kShift) {
+#pragma unroll
+    for (uint32_t i = 0; i < MF; ++i) {
+      f32x4 f;
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) {
+        const uint32_t m = (wm * MF + i) * 16 + (SWAP ? li : lg * 4 + k);
+        f[k] = __uint_as_float((127u - M::shift(top[m])) << 23);
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < NF; ++j) acc[i][j] *= f;
+    }
   }
+
+  if (a.partial) {
+    f32x4* out = (f32x4*)a.partial + (uint64_t)id * MF * NF * L::kLanes + tid;
+#pragma unroll
+    for (uint32_t i = 0; i < MF; ++i)
+#pragma unroll
+      for (uint32_t j = 0; j < NF; ++j) out[(i * NF + j) * L::kLanes] = acc[i][j];
+    return;
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < MF; ++i)
+#pragma unroll
+    for (uint32_t j = 0; j < NF; ++j)
+      grad_out<SWAP>(a, m0 + (wm * MF + i) * 16, n0 + (wn * NF + j) * 16, lane, acc[i][j]);
+}
+
+// The splits' partial tiles added in order.
+template <uint32_t MF, uint32_t NF, uint32_t WN, bool SWAP>
+__global__ __launch_bounds__(256 * WN) void grad_sum_kernel(GradArgs a) {
+  typedef Tile<MF, NF, WN> L;
+  const uint32_t tiles = a.m_tiles * a.n_tiles;
+  const uint32_t tile = blockIdx.x / (MF * NF), f = blockIdx.x % (MF * NF);
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const f32x4* p = (const f32x4*)a.partial +
+                   ((uint64_t)tile * MF * NF + f) * L::kLanes + threadIdx.x;
+  const uint64_t step = (uint64_t)tiles * MF * NF * L::kLanes;
+  f32x4 s = p[0];
+  for (uint32_t k = 1; k < a.splits; ++k) s += p[k * step];
+  grad_out<SWAP>(a, tile % a.m_tiles * L::kM + (wave % 4 * MF + f / NF) * 16,
+                 tile / a.m_tiles * L::kN + (wave / 4 * NF + f % NF) * 16, lane, s);
 }
 
 int check_dtype(uint32_t dtype, const char* what) {
@@ -175,6 +650,179 @@ void launch_unpack(const uint8_t* act, uint64_t tokens, uint64_t columns, void* 
                      (uint32_t)columns, (elem_t<DT>*)x, stride);
 }
 
+// How a call is cut: the tile (64 mf x 16 nf wn outputs) and the splits of the
+// tokens, each summed by blocks of its own.
+struct Cut {
+  uint32_t mf, nf, wn, splits;
+  uint64_t tiles;
+  // the splits' partial tiles
+  uint64_t bytes() const {
+    return splits > 1 ? tiles * splits * (64 * mf) * (16 * nf * wn) * 4 : 0;
+  }
+};
+
+// Microseconds a step of 64 tokens takes a tile's block: alone on its compute
+// unit, and its share of a unit full of blocks (MI355X, fp16, 16384 tokens).
+struct Pace {
+  uint32_t mf, nf, wn;
+  float alone, full;
+};
+constexpr Pace kPaces[] = {{3, 8, 2, 1.24f, 1.40f}, {3, 8, 1, 0.90f, 0.76f},
+                           {2, 4, 1, 0.60f, 0.39f}, {1, 4, 1, 0.47f, 0.25f}};
+
+// The cut expected to end first: the tile's pace times the blocks the fullest
+// of 256 compute units gets, and for splits a launch and the partial tiles'
+// way to memory and back at 4 TB/s.
+Cut cut_of(uint64_t tokens, uint64_t columns, uint64_t outputs, bool any) {
+  const uint64_t steps = (tokens + kStep - 1) / kStep;
+  const auto tiles = [&](uint32_t mf, uint32_t n) {
+    return ((columns + 64 * mf - 1) / (64 * mf)) * ((outputs + n - 1) / n);
+  };
+  if (any || steps == 0) return {1, 2, 2, 1, tiles(1, 64)};
+  Cut best = {};
+  float best_us = 0.0f;
+  for (const Pace& p : kPaces) {
+    const uint64_t t = tiles(p.mf, 16 * p.nf * p.wn);
+    for (uint32_t k = 1; k <= 32 && k <= steps; ++k) {
+      const uint64_t per_unit = (t * k + 255) / 256;
+      const float pace = per_unit * p.full > p.alone ? per_unit * p.full : p.alone;
+      const Cut c = {p.mf, p.nf, p.wn, k, t};
+      const float us = (float)((steps + k - 1) / k) * pace +
+                       (k > 1 ? 4.0f + (float)c.bytes() * 2.0f / 4e6f : 0.0f);
+      if (best.mf == 0 || us < best_us) best = c, best_us = us;
+    }
+  }
+  return best;
+}
+
+// Offsets inside a step's rows of dy and act fit 32 bits, and a lane's four
+// outputs are there; other calls take the kernel that asks for neither.
+bool needs_any(uint64_t columns, uint64_t dy_stride, uint64_t outputs) {
+  return outputs < 4 || dy_stride >= (1u << 25) || columns >= (1u << 25);
+}
+
+template <typename T, uint32_t MF, uint32_t NF, uint32_t WN, bool SWAP, bool ANY>
+int launch_grad(const GradArgs& a, hipStream_t s) {
+  typedef Tile<MF, NF, WN> L;
+  const void* kernel = (const void*)grad_kernel<T, MF, NF, WN, SWAP, ANY>;
+  static std::atomic<uint64_t> ready{0};  // devices that know the kernel's LDS
+  int dev = 0;
+  ARK_HIP(hipGetDevice(&dev));
+  if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1u)) {
+    ARK_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds));
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  const uint64_t tiles = (uint64_t)a.m_tiles * a.n_tiles;
+  hipLaunchKernelGGL((grad_kernel<T, MF, NF, WN, SWAP, ANY>), dim3((uint32_t)(tiles * a.splits)),
+                     dim3(L::kLanes), L::kLds, s, a);
+  ARK_HIP(hipGetLastError());
+  if (a.splits > 1) {
+    hipLaunchKernelGGL((grad_sum_kernel<MF, NF, WN, SWAP>), dim3((uint32_t)(tiles * MF * NF)),
+                       dim3(L::kLanes), 0, s, a);
+    ARK_HIP(hipGetLastError());
+  }
+  return ARK_OPT_OK;
+}
+
+template <typename T, uint32_t MF, uint32_t NF, uint32_t WN, bool ANY = false>
+int launch_tile(const GradArgs& a, bool transposed, hipStream_t s) {
+  return transposed ? launch_grad<T, MF, NF, WN, false, ANY>(a, s)
+                    : launch_grad<T, MF, NF, WN, true, ANY>(a, s);
+}
+
+template <typename T>
+int run_grad(const GradArgs& a, const Cut& c, bool any, bool transposed, hipStream_t s) {
+  if (any) return launch_tile<T, 1, 2, 2, true>(a, transposed, s);
+  if (c.mf == 3 && c.wn == 2) return launch_tile<T, 3, 8, 2>(a, transposed, s);
+  if (c.mf == 3) return launch_tile<T, 3, 8, 1>(a, transposed, s);
+  if (c.mf == 2) return launch_tile<T, 2, 4, 1>(a, transposed, s);
+  return launch_tile<T, 1, 4, 1>(a, transposed, s);
+}
+
+// The call's checks and launches; workspace NULL: one of the library's own.
+int weight_grad(const void* act, uint32_t act_dtype, uint64_t tokens, uint64_t columns,
+                const void* dy, uint64_t dy_stride, uint32_t dy_dtype, uint64_t outputs,
+                float* dw, uint64_t dw_stride, uint32_t flags, bool given, void* workspace,
+                uint64_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = check_dtype(act_dtype, "act_dtype"))) return rc;
+  if (dy_dtype != ARK_ACT_F16 && dy_dtype != ARK_ACT_BF16)
+    return ark::fail(ARK_OPT_EINVAL, "dy_dtype %u: dy is fp16 or bf16", dy_dtype);
+  if (dy_dtype == ARK_ACT_F16 && act_dtype != ARK_ACT_F16)
+    return ark::fail(ARK_OPT_EINVAL,
+                     "fp16 dy needs an act packed from fp16 (others' values may not fit fp16)");
+  if (flags & ~(ARK_ACT_ACCUMULATE | ARK_ACT_TRANSPOSED))
+    return ark::fail(ARK_OPT_EINVAL, "flags %#x unknown", flags);
+  if ((rc = check_sizes(tokens, columns)) || (rc = check_sizes(tokens, outputs))) return rc;
+  if (columns == 0 || outputs == 0) return ARK_OPT_OK;
+  if (((uintptr_t)dy % 2) || ((uintptr_t)dw % 4))
+    return ark::fail(ARK_OPT_EINVAL, "dy or dw not aligned to its element");
+  uint64_t dyb, dwb;
+  const bool tr = flags & ARK_ACT_TRANSPOSED;
+  if ((rc = rows_bytes(tokens, outputs, dy_stride, 2, false, "dy", &dyb))) return rc;
+  if ((rc = rows_bytes(tr ? outputs : columns, tr ? columns : outputs, dw_stride, 4, true, "dw",
+                       &dwb)))
+    return rc;
+  const uint64_t ab = 33 * ark::act_groups(tokens) * columns;
+  if (ark::overlaps(dw, dwb, act, ab) || ark::overlaps(dw, dwb, dy, dyb))
+    return ark::fail(ARK_OPT_EINVAL, "dw overlaps act or dy");
+  if (tokens == 0 && (flags & ARK_ACT_ACCUMULATE)) return ARK_OPT_OK;
+  const bool any = needs_any(columns, dy_stride, outputs);
+  const Cut c = cut_of(tokens, columns, outputs, any);
+  const uint64_t steps = (tokens + kStep - 1) / kStep;
+  if (steps >= (1ull << 31) || c.tiles >= (1ull << 31) / 32 || c.tiles * c.mf * c.nf >= (1ull << 31))
+    return ark::fail(ARK_OPT_EINVAL, "tokens, columns or outputs too large");
+  ark::BufferChecker checker;
+  if (given && c.bytes()) {
+    if (workspace_bytes < c.bytes())
+      return ark::fail(ARK_OPT_EINVAL, "workspace of %llu B, %llu B needed",
+                       (unsigned long long)workspace_bytes, (unsigned long long)c.bytes());
+    if ((uintptr_t)workspace % 16)
+      return ark::fail(ARK_OPT_EINVAL, "workspace %p is not 16-byte aligned", workspace);
+    if (ark::overlaps(workspace, c.bytes(), act, ab) || ark::overlaps(workspace, c.bytes(), dy, dyb) ||
+        ark::overlaps(workspace, c.bytes(), dw, dwb))
+      return ark::fail(ARK_OPT_EINVAL, "workspace overlaps act, dy or dw");
+    if ((rc = checker.check(workspace, c.bytes(), "workspace", 0))) return rc;
+  }
+  if (tokens && (rc = check_act(act, tokens, columns, &checker))) return rc;
+  if ((rc = checker.check(dy, dyb, "dy", 0))) return rc;
+  if ((rc = checker.check(dw, dwb, "dw", 0))) return rc;
+  {
+    const void* d[2] = {dw, workspace};  // dw may be an optimizer's gradient
+    const uint64_t b[2] = {dwb, given ? c.bytes() : 0};
+    ark::opt_units_invalidate(d, b, given ? 2 : 1);
+  }
+  const hipStream_t s = (hipStream_t)stream;
+  GradArgs a = {};
+  a.groups = ark::act_groups(tokens);
+  a.q = (const uint8_t*)act;
+  a.e = a.q + a.groups * columns * ARK_ACT_GROUP;
+  a.dy = (const uint16_t*)dy;
+  a.dw = dw;
+  a.tokens = tokens;
+  a.dy_stride = dy_stride;
+  a.dw_stride = dw_stride;
+  a.columns = (uint32_t)columns;
+  a.outputs = (uint32_t)outputs;
+  a.accumulate = flags & ARK_ACT_ACCUMULATE ? 1u : 0u;
+  a.vec = ((uintptr_t)dw % 16 == 0 && dw_stride % 4 == 0) ? 1u : 0u;
+  a.steps = (uint32_t)steps;
+  a.m_tiles = (uint32_t)((columns + 64 * c.mf - 1) / (64 * c.mf));
+  a.n_tiles = (uint32_t)((outputs + 16 * c.nf * c.wn - 1) / (16 * c.nf * c.wn));
+  a.splits = c.splits;
+  ark::StreamBuf buf;
+  if (c.splits > 1) {
+    a.partial = (float*)workspace;
+    if (!given) {
+      const hipError_t e = buf.alloc(c.bytes(), s);
+      if (e != hipSuccess) return ark::hip_fail(e, "workspace of ark_act_weight_grad");
+      a.partial = (float*)buf.p;
+    }
+  }
+  return dy_dtype == ARK_ACT_F16 ? run_grad<_Float16>(a, c, any, tr, s)
+                                 : run_grad<__bf16>(a, c, any, tr, s);
+}
+
 }  // namespace
 
 extern "C" {
@@ -234,51 +882,28 @@ int ark_act_unpack(const void* act, uint64_t tokens, uint64_t columns, uint32_t 
 int ark_act_weight_grad(const void* act, uint32_t act_dtype, uint64_t tokens, uint64_t columns,
                         const void* dy, uint64_t dy_stride, uint32_t dy_dtype, uint64_t outputs,
                         float* dw, uint64_t dw_stride, uint32_t flags, void* stream) {
+  return weight_grad(act, act_dtype, tokens, columns, dy, dy_stride, dy_dtype, outputs, dw,
+                     dw_stride, flags, false, nullptr, 0, stream);
+}
+
+int ark_act_weight_grad_workspace(uint64_t tokens, uint64_t columns, uint64_t dy_stride,
+                                  uint64_t outputs, uint64_t* bytes) {
+  if (!bytes) return ark::fail(ARK_OPT_EINVAL, "bytes is NULL");
+  *bytes = 0;
   int rc;
-  if ((rc = check_dtype(act_dtype, "act_dtype"))) return rc;
-  if (dy_dtype != ARK_ACT_F16 && dy_dtype != ARK_ACT_BF16)
-    return ark::fail(ARK_OPT_EINVAL, "dy_dtype %u: dy is fp16 or bf16", dy_dtype);
-  if (dy_dtype == ARK_ACT_F16 && act_dtype != ARK_ACT_F16)
-    return ark::fail(ARK_OPT_EINVAL,
-                     "fp16 dy needs an act packed from fp16 (others' values may not fit fp16)");
-  if (flags & ~(ARK_ACT_ACCUMULATE | ARK_ACT_TRANSPOSED))
-    return ark::fail(ARK_OPT_EINVAL, "flags %#x unknown", flags);
   if ((rc = check_sizes(tokens, columns)) || (rc = check_sizes(tokens, outputs))) return rc;
-  if (columns == 0 || outputs == 0) return ARK_OPT_OK;
-  if (((uintptr_t)dy % 2) || ((uintptr_t)dw % 4))
-    return ark::fail(ARK_OPT_EINVAL, "dy or dw not aligned to its element");
-  uint64_t dyb, dwb;
-  const bool tr = flags & ARK_ACT_TRANSPOSED;
-  if ((rc = rows_bytes(tokens, outputs, dy_stride, 2, false, "dy", &dyb))) return rc;
-  if ((rc = rows_bytes(tr ? outputs : columns, tr ? columns : outputs, dw_stride, 4, true, "dw",
-                       &dwb)))
-    return rc;
-  const uint64_t ab = 33 * ark::act_groups(tokens) * columns;
-  if (ark::overlaps(dw, dwb, act, ab) || ark::overlaps(dw, dwb, dy, dyb))
-    return ark::fail(ARK_OPT_EINVAL, "dw overlaps act or dy");
-  if (tokens == 0 && (flags & ARK_ACT_ACCUMULATE)) return ARK_OPT_OK;
-  ark::BufferChecker checker;
-  if (tokens && (rc = check_act(act, tokens, columns, &checker))) return rc;
-  if ((rc = checker.check(dy, dyb, "dy", 0))) return rc;
-  if ((rc = checker.check(dw, dwb, "dw", 0))) return rc;
-  {
-    const void* d = dw;  // dw may be an optimizer's gradient
-    ark::opt_units_invalidate(&d, &dwb, 1);
-  }
-  const hipStream_t s = (hipStream_t)stream;
-  const uint8_t* q = (const uint8_t*)act;
-  const uint8_t* e = q + ark::act_groups(tokens) * columns * ARK_ACT_GROUP;
-  const dim3 grid((uint32_t)((columns + 15) / 16), (uint32_t)((outputs + 15) / 16));
-  if (dy_dtype == ARK_ACT_F16)
-    hipLaunchKernelGGL(grad_kernel<_Float16>, grid, dim3(256), 0, s, q, e, tokens,
-                       (uint32_t)columns, (const _Float16*)dy, dy_stride, (uint32_t)outputs, dw,
-                       dw_stride, flags);
-  else
-    hipLaunchKernelGGL(grad_kernel<__bf16>, grid, dim3(256), 0, s, q, e, tokens,
-                       (uint32_t)columns, (const __bf16*)dy, dy_stride, (uint32_t)outputs, dw,
-                       dw_stride, flags);
-  ARK_HIP(hipGetLastError());
+  if (columns && outputs)
+    *bytes = cut_of(tokens, columns, outputs, needs_any(columns, dy_stride, outputs)).bytes();
   return ARK_OPT_OK;
+}
+
+int ark_act_weight_grad_noalloc(const void* act, uint32_t act_dtype, uint64_t tokens,
+                                uint64_t columns, const void* dy, uint64_t dy_stride,
+                                uint32_t dy_dtype, uint64_t outputs, float* dw,
+                                uint64_t dw_stride, uint32_t flags, void* workspace,
+                                uint64_t workspace_bytes, void* stream) {
+  return weight_grad(act, act_dtype, tokens, columns, dy, dy_stride, dy_dtype, outputs, dw,
+                     dw_stride, flags, true, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -309,6 +309,14 @@ extern "C" {
                                dy: *const c_void, dy_stride: u64, dy_dtype: u32, outputs: u64,
                                dw: *mut f32, dw_stride: u64, flags: u32,
                                stream: *mut c_void) -> c_int;
+    /// The same with a workspace of the caller's.
+    pub fn ark_act_weight_grad_workspace(tokens: u64, columns: u64, dy_stride: u64, outputs: u64,
+                                         bytes: *mut u64) -> c_int;
+    pub fn ark_act_weight_grad_noalloc(act: *const c_void, act_dtype: u32, tokens: u64,
+                                       columns: u64, dy: *const c_void, dy_stride: u64,
+                                       dy_dtype: u32, outputs: u64, dw: *mut f32, dw_stride: u64,
+                                       flags: u32, workspace: *mut c_void, workspace_bytes: u64,
+                                       stream: *mut c_void) -> c_int;
 }
 
 // ---- include/ark_rope.h (the rotation of `objc/bridge.m:229-411`; the norm of

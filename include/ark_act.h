@@ -77,6 +77,20 @@ int ark_act_weight_grad(const void *act, uint32_t act_dtype, uint64_t tokens, ui
                         const void *dy, uint64_t dy_stride, uint32_t dy_dtype, uint64_t outputs,
                         float *dw, uint64_t dw_stride, uint32_t flags, void *stream);
 
+/* ark_act_weight_grad with the same arguments and bits, for callers that keep
+ * their own workspace (loops whose host time counts, code that cannot
+ * allocate): ark_act_weight_grad_workspace bytes of device memory, aligned to
+ * 16, that the call's work uses until it ends.  Few or one large sum need
+ * none (0 bytes; workspace may then be NULL).  The other call takes such memory
+ * from the library's kept slots or the stream-ordered pool. */
+int ark_act_weight_grad_workspace(uint64_t tokens, uint64_t columns, uint64_t dy_stride,
+                                  uint64_t outputs, uint64_t *bytes);
+int ark_act_weight_grad_noalloc(const void *act, uint32_t act_dtype, uint64_t tokens,
+                                uint64_t columns, const void *dy, uint64_t dy_stride,
+                                uint32_t dy_dtype, uint64_t outputs, float *dw,
+                                uint64_t dw_stride, uint32_t flags, void *workspace,
+                                uint64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
