@@ -7,7 +7,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 
 def build(force=True, arch="gfx950"):
     """Compile ark_amd/lib/libark_opt.so; force=True rebuilds every time."""
-    cmd = ["make", "-C", os.path.join(_HERE, "csrc"), f"ARCH={arch}"]
+    cmd = ["make", "-j8", "-C", os.path.join(_HERE, "csrc"), f"ARCH={arch}"]
     if force:
         cmd.insert(1, "-B")
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)

@@ -26,7 +26,6 @@ struct Part {
   Array y;           // the output
   const void* gain;  // head_dim values
   uint8_t* act;      // 8-bit form written or read, or NULL
-  float* partial;    // backward: the gain's gradient, one row of head_dim a block
   uint32_t heads;
 };
 
@@ -34,10 +33,13 @@ struct Args {
   Part part[2];
   const uint64_t* turns;  // 2^64 inv_freq / (2 pi) of every pair
   const void* positions;
-  uint64_t start, batch, tokens;
+  float* partial;         // backward: [part][block][head_dim] of the gains' gradients
+  uint64_t start, tokens, all;  // all: batch * tokens
   float magnitude, eps;
-  uint32_t position_bytes, head, rotary, inverse, gain_dtype;
-  uint64_t rows[2];       // batch * tokens * heads
+  uint32_t position_bytes, head, rotary, layout, inverse, gain_dtype;
+  uint32_t lanes;         // of a row: a power of two
+  uint32_t tile;          // tokens a block takes at once
+  uint32_t slices;        // tiles_kernel: blocks that share a group's heads
 };
 
 // sin and cos of an angle given in turns / 2^32, by eighths: |r| <= pi / 4
@@ -63,10 +65,10 @@ __device__ __forceinline__ void sincos_turns(uint32_t phase, float* s, float* c)
   *c = __uint_as_float(__float_as_uint(v) ^ (((k + 1u) & 2u) << 30));
 }
 
-__device__ __forceinline__ int64_t position_at(const Args& a, uint64_t b, uint64_t t) {
-  if (!a.positions) return (int64_t)(a.start + t);
-  const uint64_t i = b * a.tokens + t;
-  return a.position_bytes == 8 ? ((const int64_t*)a.positions)[i] : ((const int32_t*)a.positions)[i];
+__device__ __forceinline__ int64_t position_at(const Args& a, uint64_t bt) {
+  if (!a.positions) return (int64_t)(a.start + (bt < a.tokens ? bt : bt % a.tokens));
+  return a.position_bytes == 8 ? ((const int64_t*)a.positions)[bt]
+                               : ((const int32_t*)a.positions)[bt];
 }
 
 // Top 32 bits of position * turns, modulo a whole turn.
@@ -80,111 +82,512 @@ __device__ __forceinline__ float gain_at(const Args& a, const void* gain, uint32
   return ((const float*)gain)[j];
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
+// The value of the lane that differs in one bit, 1 to 32.
+template <uint32_t BIT>
+__device__ __forceinline__ uint32_t across(uint32_t v) {
+  if constexpr (BIT == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, false);   // quad 1032
+  if constexpr (BIT == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, false);   // quad 2301
+  if constexpr (BIT == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, false);  // row_ror 8
+  if constexpr (BIT == 4 || BIT == 16) return __builtin_amdgcn_ds_swizzle(v, BIT << 10 | 0x1F);
+  return __shfl_xor(v, BIT);
+}
+template <uint32_t BIT>
+__device__ __forceinline__ float across(float v) {
+  return __uint_as_float(across<BIT>(__float_as_uint(v)));
+}
+
+// The sum over the lanes of a row, 8 to 64 of them, in every lane.
+__device__ __forceinline__ float row_sum(float v, uint32_t lanes) {
+  v += across<1>(v);
+  v += across<2>(v);
+  v += across<4>(v);
+  if (lanes >= 16) v += across<8>(v);
+  if (lanes >= 32) v += across<16>(v);
+  if (lanes == 64) v += across<32>(v);
   return v;
 }
 
 enum Op { kRope, kNorm, kBack };
 
 constexpr uint32_t kBlock = 256, kWaves = 4;
-constexpr uint32_t kPairs = ARK_ROPE_MAX_HEAD / 2 / 64;  // pairs of a row a lane takes
 
-// A wave takes rows (a head of a token) one after another; its lanes take the
-// row's pairs 64 apart, the pairs past the rotary ones being neighbours.
-template <uint32_t DT, uint32_t LAYOUT, Op OP>
-__global__ __launch_bounds__(kBlock) void rows_kernel(Args a) {
-  const Part& P = a.part[blockIdx.y];
+// N neighbouring elements as they lie in memory, at any element's alignment
+// (gfx950 takes unaligned global accesses).
+template <uint32_t DT, uint32_t N>
+struct Raw {
+  static constexpr uint32_t kWords = DT == ARK_ACT_F32 ? N : (N + 1) / 2;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (uint32_t i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ void load(const elem_t<DT>* p) {
+    if constexpr (DT != ARK_ACT_F32 && N == 1) {
+      w[0] = ld_g<uint16_t>(p);
+    } else {
+      typedef uint32_t T __attribute__((ext_vector_type(kWords), aligned(DT == ARK_ACT_F32 ? 4 : 2)));
+      const T v = *(const ARK_GLOBAL T*)p;
+#pragma unroll
+      for (uint32_t i = 0; i < kWords; ++i) w[i] = v[i];
+    }
+  }
+  __device__ __forceinline__ void store(elem_t<DT>* p) const {
+    if constexpr (DT != ARK_ACT_F32 && N == 1) {
+      st_g<uint16_t>(p, (uint16_t)w[0]);
+    } else {
+      typedef uint32_t T __attribute__((ext_vector_type(kWords), aligned(DT == ARK_ACT_F32 ? 4 : 2)));
+      T v;
+#pragma unroll
+      for (uint32_t i = 0; i < kWords; ++i) v[i] = w[i];
+      *(ARK_GLOBAL T*)p = v;
+    }
+  }
+  __device__ __forceinline__ float get(uint32_t i) const {
+    if constexpr (DT == ARK_ACT_F32)
+      return __uint_as_float(w[i]);
+    else if constexpr (DT == ARK_ACT_F16)
+      return h2f(w[i / 2] >> (i % 2 * 16) & 0xFFFFu);
+    else
+      return __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+  }
+  __device__ __forceinline__ void set(uint32_t i, float f) {
+    if constexpr (DT == ARK_ACT_F32) {
+      w[i] = __float_as_uint(f);
+    } else {
+      const uint32_t b = __builtin_bit_cast(uint16_t, narrow<elem_t<DT>>(f));
+      w[i / 2] = i % 2 ? w[i / 2] | b << 16 : b;
+    }
+  }
+};
+
+// N elements of a and N after them, in order, to every other one and those
+// between; and back.
+template <uint32_t DT, uint32_t N>
+__device__ __forceinline__ void unmix(Raw<DT, N>& a, Raw<DT, N>& b) {
+  uint32_t t[2 * N], *const aw = a.w, *const bw = b.w;
+  if constexpr (DT == ARK_ACT_F32) {
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) t[i] = aw[i], t[N + i] = bw[i];
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) aw[i] = t[2 * i], bw[i] = t[2 * i + 1];
+  } else if constexpr (N > 1) {
+#pragma unroll
+    for (uint32_t i = 0; i < N / 2; ++i) t[i] = aw[i], t[N / 2 + i] = bw[i];
+#pragma unroll
+    for (uint32_t i = 0; i < N / 2; ++i) {
+      aw[i] = __builtin_amdgcn_perm(t[2 * i + 1], t[2 * i], 0x05040100u);
+      bw[i] = __builtin_amdgcn_perm(t[2 * i + 1], t[2 * i], 0x07060302u);
+    }
+  }
+}
+template <uint32_t DT, uint32_t N>
+__device__ __forceinline__ void mix(Raw<DT, N>& a, Raw<DT, N>& b) {
+  uint32_t t[2 * N], *const aw = a.w, *const bw = b.w;
+  if constexpr (DT == ARK_ACT_F32) {
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) t[2 * i] = aw[i], t[2 * i + 1] = bw[i];
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) aw[i] = t[i], bw[i] = t[N + i];
+  } else if constexpr (N > 1) {
+#pragma unroll
+    for (uint32_t i = 0; i < N / 2; ++i) {
+      t[2 * i] = __builtin_amdgcn_perm(bw[i], aw[i], 0x05040100u);
+      t[2 * i + 1] = __builtin_amdgcn_perm(bw[i], aw[i], 0x07060302u);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < N / 2; ++i) aw[i] = t[i], bw[i] = t[N / 2 + i];
+  }
+}
+
+// A row (a head of a token) over its lanes: a lane takes V neighbouring pairs,
+// and of long rows with V = 1 the pairs 64 on too, K in all.  Pairs past the
+// rotary ones are made of what is left of the head the same way, and turn by
+// nothing.  A lane's pairs are two stretches of V elements, u and v, in the half
+// layout; in the interleaved one they are one of 2V, sorted once loaded.
+template <uint32_t DT, uint32_t V, uint32_t K>
+struct Row {
+  static constexpr uint32_t kE = V * K;
   typedef elem_t<DT> T;
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const uint32_t half = a.rotary / 2, pairs = half + (a.head - a.rotary + 1) / 2;
-  uint32_t ju[kPairs], jv[kPairs];
-  bool hu[kPairs], hv[kPairs];
-  float gu[kPairs], gv[kPairs], su[kPairs] = {}, sv[kPairs] = {};
+  uint32_t pair[K], eu[K], ev[K];
+  bool on[K], pairs_v[K];
+  uint32_t half;
+  bool mixed;  // interleaved
+  __device__ __forceinline__ Row(const Args& a, uint32_t lane) {
+    half = a.rotary / 2;
+    mixed = a.layout == ARK_ROPE_INTERLEAVED;
+    const uint32_t rest = (a.head - a.rotary + 1) / 2;
 #pragma unroll
-  for (uint32_t i = 0; i < kPairs; ++i) {
-    const uint32_t p = lane + 64 * i;
-    const bool rot = p < half;
-    ju[i] = rot ? (LAYOUT == ARK_ROPE_HALF ? p : 2 * p) : a.rotary + 2 * (p - half);
-    jv[i] = rot && LAYOUT == ARK_ROPE_HALF ? p + half : ju[i] + 1;
-    hu[i] = p < pairs;
-    hv[i] = p < pairs && jv[i] < a.head;
-    gu[i] = OP != kRope && hu[i] ? gain_at(a, P.gain, ju[i]) : 0.0f;
-    gv[i] = OP != kRope && hv[i] ? gain_at(a, P.gain, jv[i]) : 0.0f;
-  }
-  const uint64_t columns = (uint64_t)P.heads * a.head;
-  const uint64_t groups = (a.batch * a.tokens + ARK_ACT_GROUP - 1) / ARK_ACT_GROUP;
-  const uint8_t* exps = P.act ? P.act + groups * columns * ARK_ACT_GROUP : nullptr;
-  const uint64_t rows = a.rows[blockIdx.y];
-  for (uint64_t row = (uint64_t)blockIdx.x * kWaves + wave; row < rows;
-       row += (uint64_t)gridDim.x * kWaves) {
-    const uint64_t bt = row / P.heads, h = row % P.heads;
-    const uint64_t b = bt / a.tokens, t = bt % a.tokens;
-    const int64_t pos = position_at(a, b, t);
-    const T* x = (const T*)P.x.p + b * P.x.sb + t * P.x.st + h * P.x.sh;
-    const T* dy = OP == kBack ? (const T*)P.dy.p + b * P.dy.sb + t * P.dy.st + h * P.dy.sh : x;
-    float xu[kPairs], xv[kPairs], du[kPairs], dv[kPairs], sn[kPairs], cs[kPairs];
-    float sq = 0.0f, along = 0.0f;
-    const auto load = [&](uint32_t j) -> float {
-      if (OP != kBack || !P.act) return (float)x[j];
-      const uint64_t col = h * a.head + j, g = bt / ARK_ACT_GROUP;
-      return act_value(P.act[(g * columns + col) * ARK_ACT_GROUP + bt % ARK_ACT_GROUP],
-                       act_up(exps[g * columns + col]));
-    };
-#pragma unroll
-    for (uint32_t i = 0; i < kPairs; ++i) {
-      xu[i] = hu[i] ? load(ju[i]) : 0.0f;
-      xv[i] = hv[i] ? load(jv[i]) : 0.0f;
-      const uint32_t p = lane + 64 * i;
-      sn[i] = 0.0f;
-      cs[i] = 1.0f;
-      if (p < half) {
-        sincos_turns(phase_of(pos, a.turns[p]), &sn[i], &cs[i]);
-        sn[i] *= a.inverse || OP == kBack ? -a.magnitude : a.magnitude;
-        cs[i] *= a.magnitude;
-      }
-      if (OP == kBack) {
-        const float u = hu[i] ? (float)dy[ju[i]] : 0.0f, v = hv[i] ? (float)dy[jv[i]] : 0.0f;
-        du[i] = u * cs[i] - v * sn[i];
-        dv[i] = u * sn[i] + v * cs[i];
-        along += du[i] * gu[i] * xu[i] + dv[i] * gv[i] * xv[i];
-      }
-      sq += xu[i] * xu[i] + xv[i] * xv[i];
-    }
-    float r = 1.0f;
-    if (OP != kRope) r = 1.0f / __builtin_sqrtf(wave_sum(sq) / (float)a.head + a.eps);
-    if (OP == kBack) along = wave_sum(along) / (float)a.head * r * r;
-    T* y = (T*)P.y.p + b * P.y.sb + t * P.y.st + h * P.y.sh;
-#pragma unroll
-    for (uint32_t i = 0; i < kPairs; ++i) {
-      float u, v;
-      if (OP == kBack) {
-        su[i] += du[i] * xu[i] * r;
-        sv[i] += dv[i] * xv[i] * r;
-        u = r * (du[i] * gu[i] - xu[i] * along);
-        v = r * (dv[i] * gv[i] - xv[i] * along);
+    for (uint32_t k = 0; k < K; ++k) {
+      pair[k] = (lane + 64 * k) * V;
+      const uint32_t p = pair[k];
+      on[k] = p < half + rest;
+      if (mixed) {
+        eu[k] = 2 * p;
+        ev[k] = 2 * p + (V == 1 ? 1 : V);  // as loaded
       } else {
-        const float nu = OP == kNorm ? xu[i] * r * gu[i] : xu[i];
-        const float nv = OP == kNorm ? xv[i] * r * gv[i] : xv[i];
-        u = nu * cs[i] - nv * sn[i];
-        v = nu * sn[i] + nv * cs[i];
+        eu[k] = p < half ? p : a.rotary + p - half;
+        ev[k] = p < half ? half + p : a.rotary + rest + p - half;
       }
-      if (hu[i]) y[ju[i]] = narrow<T>(u);
-      if (hv[i]) y[jv[i]] = narrow<T>(v);
+      pairs_v[k] = on[k] && ev[k] < a.head;
     }
   }
-  if (OP == kBack) {
-    __shared__ float sum[kWaves][ARK_ROPE_MAX_HEAD];
+  struct Data {
+    Raw<DT, V> u[K], v[K];
+    __device__ __forceinline__ void load(const Row& r, const T* p) {
 #pragma unroll
-    for (uint32_t i = 0; i < kPairs; ++i) {
-      if (hu[i]) sum[wave][ju[i]] = su[i];
-      if (hv[i]) sum[wave][jv[i]] = sv[i];
+      for (uint32_t k = 0; k < K; ++k) {
+        u[k].clear();
+        v[k].clear();
+        if (r.on[k]) u[k].load(p + r.eu[k]);
+        if (r.pairs_v[k]) v[k].load(p + r.ev[k]);
+      }
     }
+    // what the interleaved layout loaded, e0 e1 ..., to e0 e2 ... and e1 e3 ...
+    __device__ __forceinline__ void sort(const Row& r) {
+      if (V > 1 && r.mixed)
+#pragma unroll
+        for (uint32_t k = 0; k < K; ++k) unmix(u[k], v[k]);
+    }
+    __device__ __forceinline__ void store(const Row& r, T* p) {
+      if (V > 1 && r.mixed)
+#pragma unroll
+        for (uint32_t k = 0; k < K; ++k) mix(u[k], v[k]);
+#pragma unroll
+      for (uint32_t k = 0; k < K; ++k) {
+        if (r.on[k]) u[k].store(p + r.eu[k]);
+        if (r.pairs_v[k]) v[k].store(p + r.ev[k]);
+      }
+    }
+    // element `second` of the lane's pair e
+    __device__ __forceinline__ float get(uint32_t e, bool second) const {
+      return second ? v[e / V].get(e % V) : u[e / V].get(e % V);
+    }
+    __device__ __forceinline__ void set(uint32_t e, bool second, float f) {
+      second ? v[e / V].set(e % V, f) : u[e / V].set(e % V, f);
+    }
+  };
+  // where element `second` of pair e lies in the row
+  __device__ __forceinline__ uint32_t at(uint32_t e, bool second) const {
+    const uint32_t k = e / V, i = e % V;
+    return mixed ? eu[k] + 2 * i + second : (second ? ev[k] : eu[k]) + i;
+  }
+  __device__ __forceinline__ bool has(uint32_t e, bool second) const {
+    return second ? pairs_v[e / V] : on[e / V];
+  }
+  __device__ __forceinline__ void gains(const Args& a, const void* g, float* gu, float* gv) const {
+#pragma unroll
+    for (uint32_t e = 0; e < kE; ++e) {
+      gu[e] = has(e, false) ? gain_at(a, g, at(e, false)) : 0.0f;
+      gv[e] = has(e, true) ? gain_at(a, g, at(e, true)) : 0.0f;
+    }
+  }
+  // the pairs' cosines and sines from a token's line of the block's table
+  __device__ __forceinline__ void turn(const float2* line, float* c, float* s) const {
+#pragma unroll
+    for (uint32_t e = 0; e < kE; ++e) c[e] = 1.0f, s[e] = 0.0f;
+#pragma unroll
+    for (uint32_t k = 0; k < K; ++k)
+      if (pair[k] < half)
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) {
+          const float2 t = line[pair[k] + i];
+          c[k * V + i] = t.x, s[k * V + i] = t.y;
+        }
+  }
+  // y = the rotation of x, or of x r gain
+  template <Op OP>
+  __device__ __forceinline__ void forward(const Args& a, const Data& x, const float* gu,
+                                          const float* gv, const float* c, const float* s,
+                                          Data* y) const {
+    float u[kE], v[kE], r = 1.0f, q = 0.0f;
+#pragma unroll
+    for (uint32_t e = 0; e < kE; ++e) {
+      u[e] = x.get(e, false), v[e] = x.get(e, true);
+      q = __builtin_fmaf(u[e], u[e], q);
+      q = __builtin_fmaf(v[e], v[e], q);
+    }
+    if constexpr (OP == kNorm)
+      r = 1.0f / __builtin_sqrtf(row_sum(q, a.lanes) / (float)a.head + a.eps);
+#pragma unroll
+    for (uint32_t e = 0; e < kE; ++e) {
+      const float nu = OP == kNorm ? u[e] * (r * gu[e]) : u[e];
+      const float nv = OP == kNorm ? v[e] * (r * gv[e]) : v[e];
+      y->set(e, false, __builtin_fmaf(nu, c[e], -(nv * s[e])));
+      y->set(e, true, __builtin_fmaf(nu, s[e], nv * c[e]));
+    }
+  }
+  // dx from dy and x, and dy rotated back times x r into the gain's sums
+  __device__ __forceinline__ void backward(const Args& a, const Data& dy, const float* xu,
+                                           const float* xv, const float* gu, const float* gv,
+                                           const float* c, const float* s, float* su, float* sv,
+                                           Data* dx) const {
+    float du[kE], dv[kE], q = 0.0f, along = 0.0f;
+#pragma unroll
+    for (uint32_t e = 0; e < kE; ++e) {
+      const float u = dy.get(e, false), v = dy.get(e, true);
+      du[e] = __builtin_fmaf(u, c[e], v * s[e]);
+      dv[e] = __builtin_fmaf(v, c[e], -(u * s[e]));
+      q = __builtin_fmaf(xu[e], xu[e], q);
+      q = __builtin_fmaf(xv[e], xv[e], q);
+      along = __builtin_fmaf(du[e] * gu[e], xu[e], along);
+      along = __builtin_fmaf(dv[e] * gv[e], xv[e], along);
+    }
+    const float n = 1.0f / (float)a.head;
+    const float r = 1.0f / __builtin_sqrtf(row_sum(q, a.lanes) * n + a.eps);
+    along = row_sum(along, a.lanes) * n * r * r;
+#pragma unroll
+    for (uint32_t e = 0; e < kE; ++e) {
+      su[e] = __builtin_fmaf(du[e], xu[e] * r, su[e]);
+      sv[e] = __builtin_fmaf(dv[e], xv[e] * r, sv[e]);
+      dx->set(e, false, r * __builtin_fmaf(-xu[e], along, du[e] * gu[e]));
+      dx->set(e, true, r * __builtin_fmaf(-xv[e], along, dv[e] * gv[e]));
+    }
+  }
+  // a wave's sums of the gain's gradient, its rows' lanes together, into LDS
+  __device__ __forceinline__ void gather(const Args& a, float* su, float* sv, float* out) const {
+#pragma unroll
+    for (uint32_t e = 0; e < kE; ++e) {
+      if (a.lanes <= 8) su[e] += across<8>(su[e]), sv[e] += across<8>(sv[e]);
+      if (a.lanes <= 16) su[e] += across<16>(su[e]), sv[e] += across<16>(sv[e]);
+      if (a.lanes <= 32) su[e] += across<32>(su[e]), sv[e] += across<32>(sv[e]);
+      if (threadIdx.x % 64 < a.lanes) {
+        if (has(e, false)) out[at(e, false)] = su[e];
+        if (has(e, true)) out[at(e, true)] = sv[e];
+      }
+    }
+  }
+};
+
+// What a block keeps of its tokens in LDS: their cosines and sines, one line of
+// rotary / 2 a token, and where each token starts in the part's x, dy and y.
+struct Tokens {
+  float2* turns;
+  uint64_t* at;  // [token][x, dy, y]
+  __device__ __forceinline__ Tokens(const Args& a, uint8_t* lds) {
+    at = (uint64_t*)lds;
+    turns = (float2*)(lds + a.tile * 24);
+  }
+  __device__ __forceinline__ void fill(const Args& a, const Part& p, uint64_t first, uint32_t n,
+                                       bool back) const {
+    const uint32_t half = a.rotary / 2;
+    for (uint32_t i = threadIdx.x; i < n * 3; i += kBlock) {
+      const uint64_t bt = first + i / 3;
+      const Array& r = i % 3 == 0 ? p.x : i % 3 == 1 ? p.dy : p.y;
+      uint64_t b = 0, t = bt;
+      if (a.all != a.tokens) b = bt / a.tokens, t = bt % a.tokens;
+      at[i] = b * r.sb + t * r.st;
+    }
+    for (uint32_t i = threadIdx.x; i < n * half; i += kBlock) {
+      float s, c;
+      sincos_turns(phase_of(position_at(a, first + i / half), a.turns[i % half]), &s, &c);
+      turns[i] = make_float2(c * a.magnitude, s * (back ? -a.magnitude : a.magnitude));
+    }
+  }
+};
+
+// Rows of tokens taken `tile` at a time by every block in turn: a wave takes 64
+// / lanes rows at once, neighbouring heads of a token, kUnroll times over before
+// it works on the first.
+template <uint32_t DT, Op OP, uint32_t V, uint32_t K>
+__global__ __launch_bounds__(kBlock) void rows_kernel(Args a) {
+  typedef Row<DT, V, K> R;
+  typedef elem_t<DT> T;
+  constexpr uint32_t kUnroll = V == 4 ? 2 : 1;
+  extern __shared__ __align__(16) uint8_t lds[];
+  const Tokens tok(a, lds);
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const R row(a, lane % a.lanes);
+  const uint32_t at_once = 64 / a.lanes;
+  const Part& P = a.part[blockIdx.y];
+  const uint64_t columns = (uint64_t)P.heads * a.head;
+  float su[R::kE] = {}, sv[R::kE] = {}, gu[R::kE], gv[R::kE];
+  if (OP != kRope && P.heads) row.gains(a, P.gain, gu, gv);  // no heads: no gain
+  for (uint64_t first = (uint64_t)blockIdx.x * a.tile; first < a.all;
+       first += (uint64_t)gridDim.x * a.tile) {
+    const uint32_t n = (uint32_t)(a.all - first < a.tile ? a.all - first : a.tile);
+    __syncthreads();
+    tok.fill(a, P, first, n, OP != kBack && a.inverse);
+    __syncthreads();
+    {
+      const uint8_t* exps = P.act + (a.all + ARK_ACT_GROUP - 1) / ARK_ACT_GROUP * columns * ARK_ACT_GROUP;
+      for (uint32_t r0 = wave * at_once; r0 < n * P.heads; r0 += kWaves * at_once * kUnroll) {
+        typename R::Data x[kUnroll], dy[kUnroll];
+        uint32_t t[kUnroll], h[kUnroll];
+        bool in[kUnroll];
+#pragma unroll
+        for (uint32_t i = 0; i < kUnroll; ++i) {
+          const uint32_t r = r0 + i * kWaves * at_once + lane / a.lanes;
+          in[i] = r < n * P.heads;
+          t[i] = in[i] ? r / P.heads : 0;
+          h[i] = in[i] ? r - t[i] * P.heads : 0;
+          if (OP != kBack || !P.act)
+            x[i].load(row, (const T*)P.x.p + tok.at[t[i] * 3] + h[i] * P.x.sh);
+          if (OP == kBack)
+            dy[i].load(row, (const T*)P.dy.p + tok.at[t[i] * 3 + 1] + h[i] * P.dy.sh);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kUnroll; ++i) {
+          float c[R::kE], s[R::kE];
+          row.turn(tok.turns + t[i] * (a.rotary / 2), c, s);
+          if (OP != kBack || !P.act) x[i].sort(row);
+          if (OP == kBack) dy[i].sort(row);
+          typename R::Data y;
+          if constexpr (OP == kBack) {
+            float xu[R::kE], xv[R::kE];
+            const uint64_t bt = first + t[i], g = bt / ARK_ACT_GROUP;
+            const auto kept = [&](uint32_t e, bool second) {
+              if (!row.has(e, second)) return 0.0f;
+              const uint64_t col = g * columns + h[i] * a.head + row.at(e, second);
+              return act_value(P.act[col * ARK_ACT_GROUP + bt % ARK_ACT_GROUP], act_up(exps[col]));
+            };
+#pragma unroll
+            for (uint32_t e = 0; e < R::kE; ++e) {
+              xu[e] = P.act ? kept(e, false) : x[i].get(e, false);
+              xv[e] = P.act ? kept(e, true) : x[i].get(e, true);
+            }
+            if (!in[i])  // a row that is not there adds nothing to the gain
+#pragma unroll
+              for (uint32_t e = 0; e < R::kE; ++e) xu[e] = xv[e] = 0.0f;
+            if (!in[i]) dy[i] = typename R::Data();
+            row.backward(a, dy[i], xu, xv, gu, gv, c, s, su, sv, &y);
+          } else {
+            row.template forward<OP>(a, x[i], gu, gv, c, s, &y);
+          }
+          if (in[i]) y.store(row, (T*)P.y.p + tok.at[t[i] * 3 + 2] + h[i] * P.y.sh);
+        }
+      }
+    }
+  }
+  if constexpr (OP == kBack) {
+    float* sum = (float*)lds;
+    __syncthreads();
+    row.gather(a, su, sv, sum + wave * a.head);
     __syncthreads();
     for (uint32_t j = threadIdx.x; j < a.head; j += kBlock)
-      P.partial[(uint64_t)blockIdx.x * a.head + j] =
-          (sum[0][j] + sum[1][j]) + (sum[2][j] + sum[3][j]);
+      a.partial[((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.head + j] =
+          (sum[j] + sum[a.head + j]) + (sum[2 * a.head + j] + sum[3 * a.head + j]);
+  }
+}
+
+// The norm of 32 tokens of a head at a time, with the 8-bit form of its input:
+// written by the forward pass, read by the backward pass.  A wave holds the
+// tile, kIt rows a lane, neighbouring tokens, so that a column's largest
+// magnitude is its lanes' and its bytes a lane's are neighbours.
+template <uint32_t DT, bool BACK, uint32_t V, uint32_t kIt>
+__global__ __launch_bounds__(kBlock) void tiles_kernel(Args a) {
+  typedef Row<DT, V, 1> R;
+  typedef elem_t<DT> T;
+  constexpr uint32_t kLanes = 2 * kIt;  // of a row: 64 / (32 / kIt)
+  typedef uint32_t Bytes __attribute__((ext_vector_type(kIt / 4), aligned(4)));
+  extern __shared__ __align__(16) uint8_t lds[];
+  const Tokens tok(a, lds);
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, mine = lane / kLanes * kIt;
+  const R row(a, lane % kLanes);
+  const uint64_t groups = (a.all + ARK_ACT_GROUP - 1) / ARK_ACT_GROUP;
+  const Part& P = a.part[blockIdx.y];
+  const uint64_t columns = (uint64_t)P.heads * a.head;
+  float su[R::kE] = {}, sv[R::kE] = {}, gu[R::kE], gv[R::kE];
+  if (P.heads) row.gains(a, P.gain, gu, gv);  // no heads: no gain
+  const uint32_t slice = blockIdx.x % a.slices;
+  for (uint64_t g = blockIdx.x / a.slices; g < groups; g += gridDim.x / a.slices) {
+    const uint64_t first = g * ARK_ACT_GROUP;
+    const uint32_t n = (uint32_t)(a.all - first < ARK_ACT_GROUP ? a.all - first : ARK_ACT_GROUP);
+    __syncthreads();
+    tok.fill(a, P, first, n, false);
+    __syncthreads();
+    {
+      for (uint32_t h = slice * kWaves + wave; h < P.heads; h += a.slices * kWaves) {
+        uint8_t* const q = P.act + (g * columns + h * a.head) * ARK_ACT_GROUP;
+        uint8_t* const exps = P.act + groups * columns * ARK_ACT_GROUP + g * columns + h * a.head;
+        typename R::Data in[kIt];
+#pragma unroll
+        for (uint32_t i = 0; i < kIt; ++i) {
+          const uint32_t t = mine + i;
+          const Array& from = BACK ? P.dy : P.x;
+          if (t < n)
+            in[i].load(row, (const T*)from.p + tok.at[t * 3 + BACK] + h * from.sh);
+          else
+            in[i] = typename R::Data();
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kIt; ++i) in[i].sort(row);
+        Bytes b[R::kE][2];
+        float up[R::kE][2];
+#pragma unroll
+        for (uint32_t e = 0; e < R::kE; ++e)
+#pragma unroll
+          for (uint32_t k = 0; k < 2; ++k) {
+            if (!row.has(e, k)) {
+              b[e][k] = Bytes(), up[e][k] = 0.0f;
+              continue;
+            }
+            uint8_t* const at = q + row.at(e, k) * ARK_ACT_GROUP + mine;
+            if constexpr (BACK) {
+              b[e][k] = *(const ARK_GLOBAL Bytes*)at;
+              up[e][k] = act_up(ld_g<uint8_t>(exps + row.at(e, k)));
+            }
+          }
+        if constexpr (!BACK) {
+          uint32_t most[R::kE][2];
+#pragma unroll
+          for (uint32_t e = 0; e < R::kE; ++e)
+#pragma unroll
+            for (uint32_t k = 0; k < 2; ++k) {
+              uint32_t m = 0;
+#pragma unroll
+              for (uint32_t i = 0; i < kIt; ++i)
+                m = max(m, __float_as_uint(in[i].get(e, k)) & 0x7FFFFFFFu);
+              if (kLanes <= 8) m = max(m, across<8>(m));
+              if (kLanes <= 16) m = max(m, across<16>(m));
+              if (kLanes <= 32) m = max(m, across<32>(m));
+              most[e][k] = m;
+            }
+#pragma unroll
+          for (uint32_t e = 0; e < R::kE; ++e)
+#pragma unroll
+            for (uint32_t k = 0; k < 2; ++k) {
+              const uint32_t s = act_exponent<DT>(most[e][k]);
+              const float down = act_down(s);
+              Bytes w = Bytes();
+#pragma unroll
+              for (uint32_t i = 0; i < kIt; ++i)
+                w[i / 4] |= act_byte<DT>(in[i].get(e, k), s, down) << (i % 4 * 8);
+              if (row.has(e, k)) {
+                *(ARK_GLOBAL Bytes*)(q + row.at(e, k) * ARK_ACT_GROUP + mine) = w;
+                if (mine == 0) st_g<uint8_t>(exps + row.at(e, k), (uint8_t)s);
+              }
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kIt; ++i) {
+          const uint32_t t = mine + i;
+          float c[R::kE], s[R::kE];
+          row.turn(tok.turns + (t < n ? t : 0) * (a.rotary / 2), c, s);
+          typename R::Data y;
+          if constexpr (BACK) {
+            float xu[R::kE], xv[R::kE];
+#pragma unroll
+            for (uint32_t e = 0; e < R::kE; ++e) {
+              xu[e] = act_value(b[e][0][i / 4] >> (i % 4 * 8) & 255u, up[e][0]);
+              xv[e] = act_value(b[e][1][i / 4] >> (i % 4 * 8) & 255u, up[e][1]);
+            }
+            row.backward(a, in[i], xu, xv, gu, gv, c, s, su, sv, &y);
+          } else {
+            row.template forward<kNorm>(a, in[i], gu, gv, c, s, &y);
+          }
+          if (t < n) y.store(row, (T*)P.y.p + tok.at[t * 3 + 2] + h * P.y.sh);
+        }
+      }
+    }
+  }
+  if constexpr (BACK) {
+    float* sum = (float*)lds;
+    __syncthreads();
+    row.gather(a, su, sv, sum + wave * a.head);
+    __syncthreads();
+    for (uint32_t j = threadIdx.x; j < a.head; j += kBlock)
+      a.partial[((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.head + j] =
+          (sum[j] + sum[a.head + j]) + (sum[2 * a.head + j] + sum[3 * a.head + j]);
   }
 }
 
@@ -194,7 +597,7 @@ template <uint32_t DT>
 __global__ __launch_bounds__(kBlock) void keep_kernel(Args a) {
   const Part& P = a.part[blockIdx.z];
   if (!P.act) return;
-  const uint64_t columns = (uint64_t)P.heads * a.head, n = a.batch * a.tokens;
+  const uint64_t columns = (uint64_t)P.heads * a.head, n = a.all;
   const uint64_t groups = (n + ARK_ACT_GROUP - 1) / ARK_ACT_GROUP;
   const uint64_t i = (uint64_t)blockIdx.x * kBlock + threadIdx.x;
   if (i >= groups * columns) return;
@@ -217,33 +620,132 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(Args a) {
   P.act[groups * columns * ARK_ACT_GROUP + i] = (uint8_t)s;
 }
 
-// The gain's gradient from the blocks' rows, added in order.
-__global__ __launch_bounds__(64) void gain_kernel(const float* __restrict__ partial, uint32_t rows,
-                                                  uint32_t head, float* __restrict__ dq,
-                                                  float* __restrict__ dk, uint32_t accumulate) {
-  const uint32_t j = blockIdx.x * 64 + threadIdx.x;
-  float* out = blockIdx.y ? dk : dq;
-  if (j >= head || !out) return;
+// The gains' gradients from the blocks' rows, added in order: 64 rows' runs by
+// the lanes of a column, then those.
+constexpr uint32_t kGainColumns = 16, kGainRuns = 64;
+__global__ __launch_bounds__(kGainColumns * kGainRuns) void gain_kernel(
+    const float* __restrict__ partial, uint32_t rows, uint32_t head, float* __restrict__ dq,
+    float* __restrict__ dk, uint32_t accumulate) {
+  __shared__ float sum[kGainRuns][kGainColumns];
+  const uint32_t c = threadIdx.x % kGainColumns, run = threadIdx.x / kGainColumns;
+  const uint32_t j = blockIdx.x * kGainColumns + c;
   const float* p = partial + (uint64_t)blockIdx.y * rows * head + j;
   float s = 0.0f;
-  for (uint32_t i = 0; i < rows; ++i) s += p[(uint64_t)i * head];
-  out[j] = accumulate ? out[j] + s : s;
+  if (j < head)
+#pragma unroll 8
+    for (uint32_t i = run; i < rows; i += kGainRuns) s += p[(uint64_t)i * head];
+  sum[run][c] = s;
+  __syncthreads();
+  for (uint32_t half = kGainRuns / 2; half; half /= 2) {
+    if (run < half) sum[run][c] += sum[run + half][c];
+    __syncthreads();
+  }
+  float* out = blockIdx.y ? dk : dq;
+  if (run == 0 && j < head && out) out[j] = accumulate ? out[j] + sum[0][c] : sum[0][c];
 }
 
-constexpr uint32_t kMaxBlocks = 1024;
+// How a row goes over lanes: V pairs a lane where the head and its rotary part
+// are whole chunks of 2V, and the wave's lanes for a row, at least eight.
+struct Shape2 {
+  uint32_t v, k, lanes;
+};
+Shape2 row_shape(uint32_t head, uint32_t rotary) {
+  const uint32_t both = head | rotary;
+  const uint32_t v = both % 8 == 0 ? 4 : both % 4 == 0 && head <= 256 ? 2 : 1;
+  const uint32_t need = ((head + 1) / 2 + v - 1) / v;
+  uint32_t lanes = v == 4 ? 8 : v == 2 ? 32 : 64;
+  while (lanes < need && lanes < 64) lanes *= 2;
+  return {v, need > 64 ? 4u : 1u, lanes};
+}
+
+template <uint32_t DT, Op OP>
+void rows_of(const Shape2& w, dim3 grid, uint32_t lds, hipStream_t s, const Args& a) {
+  if (w.v == 4)
+    hipLaunchKernelGGL((rows_kernel<DT, OP, 4, 1>), grid, dim3(kBlock), lds, s, a);
+  else if (w.v == 2)
+    hipLaunchKernelGGL((rows_kernel<DT, OP, 2, 1>), grid, dim3(kBlock), lds, s, a);
+  else if (w.k == 1)
+    hipLaunchKernelGGL((rows_kernel<DT, OP, 1, 1>), grid, dim3(kBlock), lds, s, a);
+  else
+    hipLaunchKernelGGL((rows_kernel<DT, OP, 1, 4>), grid, dim3(kBlock), lds, s, a);
+}
+template <uint32_t DT, bool BACK>
+void tiles_of(const Shape2& w, dim3 grid, uint32_t lds, hipStream_t s, const Args& a) {
+#define ARK_TILES(V, L)                                                                  \
+  if (w.v == V && w.lanes == L)                                                          \
+    hipLaunchKernelGGL((tiles_kernel<DT, BACK, V, L / 2>), grid, dim3(kBlock), lds, s, a);
+  ARK_TILES(4, 8)
+  ARK_TILES(4, 16)
+  ARK_TILES(4, 32)
+  ARK_TILES(2, 32)
+  ARK_TILES(2, 64)
+  ARK_TILES(1, 64)
+#undef ARK_TILES
+}
+
+// Rows of one line of the table kept small enough for eight blocks a unit.
+uint32_t rows_tile(const Args& a) {
+  const uint32_t line = 24 + a.rotary / 2 * 8;
+  uint32_t most = 16384 / line;
+  if (most > 32) most = 32;
+  // a thousand blocks before tokens share one
+  const uint64_t want = (a.all + 1023) / 1024;
+  return want < 1 ? 1 : want < most ? (uint32_t)want : most;
+}
+uint32_t block_lds(const Args& a) {
+  const uint32_t t = a.tile * (24 + a.rotary / 2 * 8), sum = kWaves * a.head * 4;
+  return t > sum ? t : sum;
+}
 
 template <Op OP>
-void launch_rows(uint32_t dtype, uint32_t layout, dim3 grid, hipStream_t s, const Args& a) {
-#define ARK_ROWS(DT, LY)                                                                       \
-  if (dtype == DT && layout == LY)                                                             \
-    hipLaunchKernelGGL((rows_kernel<DT, LY, OP>), grid, dim3(kBlock), 0, s, a);
-  ARK_ROWS(ARK_ACT_F16, ARK_ROPE_HALF)
-  ARK_ROWS(ARK_ACT_BF16, ARK_ROPE_HALF)
-  ARK_ROWS(ARK_ACT_F32, ARK_ROPE_HALF)
-  ARK_ROWS(ARK_ACT_F16, ARK_ROPE_INTERLEAVED)
-  ARK_ROWS(ARK_ACT_BF16, ARK_ROPE_INTERLEAVED)
-  ARK_ROWS(ARK_ACT_F32, ARK_ROPE_INTERLEAVED)
-#undef ARK_ROWS
+uint32_t launch_rows(uint32_t dtype, Args* a, hipStream_t s, bool launch = true) {
+  const Shape2 w = row_shape(a->head, a->rotary);
+  a->lanes = w.lanes;
+  a->tile = rows_tile(*a);
+  const uint64_t tiles = (a->all + a->tile - 1) / a->tile;
+  const uint32_t most = OP == kBack ? 1024 : 1u << 20;
+  const uint32_t blocks = (uint32_t)(tiles < most ? tiles : most);
+  if (!launch || !blocks) return blocks;
+  const dim3 grid(blocks, a->part[1].heads ? 2 : 1);
+  if (dtype == ARK_ACT_F16)
+    rows_of<ARK_ACT_F16, OP>(w, grid, block_lds(*a), s, *a);
+  else if (dtype == ARK_ACT_BF16)
+    rows_of<ARK_ACT_BF16, OP>(w, grid, block_lds(*a), s, *a);
+  else
+    rows_of<ARK_ACT_F32, OP>(w, grid, block_lds(*a), s, *a);
+  return blocks;
+}
+
+// Whether a wave can hold 32 tokens of a head: at most 128 values a lane.
+bool tiles_fit(const Args& a) {
+  const Shape2 w = row_shape(a.head, a.rotary);
+  return w.k == 1 && w.v * w.lanes <= 128;
+}
+
+template <bool BACK>
+uint32_t launch_tiles(uint32_t dtype, Args* a, hipStream_t s, bool launch = true) {
+  const Shape2 w = row_shape(a->head, a->rotary);
+  a->lanes = w.lanes;
+  a->tile = ARK_ACT_GROUP;
+  const uint64_t groups = ark::act_groups(a->all);
+  const uint32_t heads = a->part[0].heads > a->part[1].heads ? a->part[0].heads : a->part[1].heads;
+  // blocks share a group's heads until there are about 1500
+  uint32_t slices = (heads + kWaves - 1) / kWaves;
+  while (slices > 1 && groups * (slices - 1) >= 1536) --slices;
+  a->slices = slices;
+  uint64_t by = groups;
+  const uint32_t most = (BACK ? 2048u : 1u << 20) / slices;
+  if (by > most) by = most;
+  const uint32_t blocks = (uint32_t)by * slices;
+  if (!launch || !blocks) return blocks;
+  const dim3 grid(blocks, a->part[1].heads ? 2 : 1);
+  if (dtype == ARK_ACT_F16)
+    tiles_of<ARK_ACT_F16, BACK>(w, grid, block_lds(*a), s, *a);
+  else if (dtype == ARK_ACT_BF16)
+    tiles_of<ARK_ACT_BF16, BACK>(w, grid, block_lds(*a), s, *a);
+  else
+    tiles_of<ARK_ACT_F32, BACK>(w, grid, block_lds(*a), s, *a);
+  return blocks;
 }
 
 }  // namespace
@@ -430,14 +932,6 @@ int check_memory(const Given* g, int n, const Flat* f, int nf) {
   return ARK_OPT_OK;
 }
 
-// Blocks for the larger of the two parts; a third dimension is not needed, the
-// kernel's loop takes what is left.
-uint32_t row_blocks(const Args& a, uint32_t most) {
-  const uint64_t rows = a.rows[0] > a.rows[1] ? a.rows[0] : a.rows[1];
-  const uint64_t blocks = (rows + kWaves - 1) / kWaves;
-  return (uint32_t)(blocks < most ? blocks : most);
-}
-
 Args base_args(const ark_rope* r, uint64_t batch, uint64_t tokens, const void* positions,
                uint32_t position_bytes, uint64_t start) {
   Args a = {};
@@ -445,11 +939,12 @@ Args base_args(const ark_rope* r, uint64_t batch, uint64_t tokens, const void* p
   a.positions = positions;
   a.position_bytes = position_bytes;
   a.start = start;
-  a.batch = batch;
   a.tokens = tokens;
+  a.all = batch * tokens;
   a.magnitude = r->magnitude;
   a.head = r->head;
   a.rotary = r->rotary;
+  a.layout = r->layout;
   return a;
 }
 
@@ -600,12 +1095,10 @@ int ark_rope_apply(const ark_rope* r, uint32_t dtype, uint64_t batch, uint64_t t
     a.part[i].x = array_of(g[2 * i + 1]);
     a.part[i].y = array_of(g[2 * i]);
     a.part[i].heads = heads[i];
-    a.rows[i] = batch * tokens * heads[i];
   }
   ark::DeviceGuard guard(r->device);
   if (!guard.ok) return ark::fail(ARK_OPT_EHIP, "cannot select device %d", r->device);
-  launch_rows<kRope>(dtype, r->layout, dim3(row_blocks(a, 1u << 20), heads[1] ? 2 : 1),
-                     (hipStream_t)stream, a);
+  launch_rows<kRope>(dtype, &a, (hipStream_t)stream);
   ARK_HIP(hipGetLastError());
   return ARK_OPT_OK;
 }
@@ -658,10 +1151,15 @@ int ark_rope_norm(const ark_rope* r, uint32_t dtype, uint64_t batch, uint64_t to
     a.part[i].y = array_of(g[2 * i]);
     a.part[i].heads = heads[i];
     a.part[i].gain = gains[i];
-    a.rows[i] = n * heads[i];
     a.part[i].act = (uint8_t*)acts[i];
     const uint64_t values = ark::act_groups(n) * heads[i] * r->head;
     most = acts[i] && values > most ? values : most;
+  }
+  // both parts' tiles and 8-bit forms in one pass, or each in its own
+  if (q_act && (k_act || !heads[1]) && tiles_fit(a)) {
+    launch_tiles<false>(dtype, &a, (hipStream_t)stream);
+    ARK_HIP(hipGetLastError());
+    return ARK_OPT_OK;
   }
   if (most) {
     const dim3 grid((uint32_t)((most + kBlock - 1) / kBlock), 1, heads[1] ? 2 : 1);
@@ -673,8 +1171,7 @@ int ark_rope_norm(const ark_rope* r, uint32_t dtype, uint64_t batch, uint64_t to
       hipLaunchKernelGGL(keep_kernel<ARK_ACT_F32>, grid, dim3(kBlock), 0, (hipStream_t)stream, a);
     ARK_HIP(hipGetLastError());
   }
-  launch_rows<kNorm>(dtype, r->layout, dim3(row_blocks(a, 1u << 20), heads[1] ? 2 : 1),
-                     (hipStream_t)stream, a);
+  launch_rows<kNorm>(dtype, &a, (hipStream_t)stream);
   ARK_HIP(hipGetLastError());
   return ARK_OPT_OK;
 }
@@ -742,22 +1239,26 @@ int ark_rope_norm_backward(const ark_rope* r, uint32_t dtype, uint64_t batch, ui
     a.part[i].heads = heads[i];
     a.part[i].gain = gains[i];
     a.part[i].act = (uint8_t*)acts[i];
-    a.rows[i] = n * heads[i];
   }
   ark::DeviceGuard guard(r->device);
   if (!guard.ok) return ark::fail(ARK_OPT_EHIP, "cannot select device %d", r->device);
   const hipStream_t st = (hipStream_t)stream;
-  const uint32_t blocks = row_blocks(a, kMaxBlocks);
+  const bool tiled = has[0] && q_act && (k_act || !has[1]) && tiles_fit(a);
+  const uint32_t blocks = empty ? 0
+                          : tiled ? launch_tiles<true>(dtype, &a, st, false)
+                                  : launch_rows<kBack>(dtype, &a, st, false);
   ark::StreamBuf buf;
   if (blocks) {
     const hipError_t e = buf.alloc((uint64_t)2 * blocks * r->head * 4, st);
     if (e != hipSuccess) return ark::hip_fail(e, "workspace of ark_rope_norm_backward");
-    for (int i = 0; i < 2; ++i) a.part[i].partial = (float*)buf.p + (uint64_t)i * blocks * r->head;
-    launch_rows<kBack>(dtype, r->layout, dim3(blocks, 2), st, a);
+    a.partial = (float*)buf.p;
+    tiled ? launch_tiles<true>(dtype, &a, st)
+          : launch_rows<kBack>(dtype, &a, st);
     ARK_HIP(hipGetLastError());
   }
-  hipLaunchKernelGGL(gain_kernel, dim3((r->head + 63) / 64, dk_layout ? 2 : 1), dim3(64), 0, st,
-                     (const float*)buf.p, blocks, r->head, dgain_q, dgain_k, accumulate);
+  hipLaunchKernelGGL(gain_kernel, dim3((r->head + kGainColumns - 1) / kGainColumns, dk_layout ? 2 : 1),
+                     dim3(kGainColumns * kGainRuns), 0, st, (const float*)buf.p, blocks, r->head,
+                     dgain_q, dgain_k, accumulate);
   ARK_HIP(hipGetLastError());
   return ARK_OPT_OK;
 }
