@@ -8,23 +8,17 @@ fp32, written to or added into the gradients an optimizer steps on;
 """
 import ctypes as C
 
+import torch
+
 from . import _abi
 from ._lib import check, lib, current_stream as _stream
 
-_TYPES = None
-
-
-def _types():
-    global _TYPES
-    if _TYPES is None:
-        import torch
-        _TYPES = {torch.float16: _abi.ACT_F16, torch.bfloat16: _abi.ACT_BF16,
-                  torch.float32: _abi.ACT_F32}
-    return _TYPES
+_TYPES = {torch.float16: _abi.ACT_F16, torch.bfloat16: _abi.ACT_BF16,
+          torch.float32: _abi.ACT_F32}
 
 
 def _code(t, what):
-    code = _types().get(t.dtype)
+    code = _TYPES.get(t.dtype)
     if code is None:
         raise ValueError(f"{what} holds {t.dtype}: float16, bfloat16 and float32 are taken")
     return code
@@ -48,8 +42,7 @@ class Act8:
     __slots__ = ("tokens", "columns", "dtype", "data")
 
     def __init__(self, tokens, columns, dtype, device=None, data=None):
-        import torch
-        if dtype not in _types():
+        if dtype not in _TYPES:
             raise ValueError(f"dtype {dtype}: float16, bfloat16 and float32 are taken")
         if tokens < 0 or columns < 0:
             raise ValueError(f"sizes {tokens} x {columns}")
@@ -82,7 +75,6 @@ def pack(x, out=None):
 def unpack(kept, out=None):
     """The values of an Act8, in ``out`` (tokens x columns, rows of any stride)
     or a new tensor of the type they were packed from."""
-    import torch
     if out is None:
         out = torch.empty((kept.tokens, kept.columns), dtype=kept.dtype, device=kept.data.device)
     elif tuple(out.shape) != (kept.tokens, kept.columns) or out.device != kept.data.device:
@@ -100,7 +92,6 @@ def weight_grad(kept, dy, dw=None, accumulate=False, layout="in_out"):
     for any).  dw is float32, columns x outputs ("in_out") or outputs x columns
     ("out_in"), rows of any stride; a new tensor when None.  accumulate adds to
     it."""
-    import torch
     if layout not in ("in_out", "out_in"):
         raise ValueError(f"layout {layout!r}: 'in_out' or 'out_in'")
     dp, dstride = _rows(dy, "dy")
@@ -123,7 +114,7 @@ def weight_grad(kept, dy, dw=None, accumulate=False, layout="in_out"):
     # torch's allocator hands a stream's memory back to it without waiting
     ws = torch.empty(need.value, dtype=torch.uint8, device=dy.device) if need.value else None
     check(lib().ark_act_weight_grad_noalloc(
-        kept.data.data_ptr(), _types()[kept.dtype], kept.tokens, kept.columns, dp, dstride,
+        kept.data.data_ptr(), _TYPES[kept.dtype], kept.tokens, kept.columns, dp, dstride,
         _code(dy, "dy"), n, wp, wstride, flags, ws.data_ptr() if need.value else None, need.value,
         _stream(dy)))
     return dw

@@ -13,58 +13,138 @@ using namespace ark::dev;
 
 constexpr uint32_t kLanes = 256;
 
-// One lane per column of a group: 32 loads, the largest magnitude, 32 bytes.
-template <uint32_t DT>
+// N columns of a row as they lie in memory, at any element's alignment.
+template <uint32_t DT, uint32_t N>
+struct Columns {
+  static constexpr uint32_t kWords = DT == ARK_ACT_F32 ? N : N / 2;
+  typedef uint32_t V __attribute__((ext_vector_type(kWords), aligned(DT == ARK_ACT_F32 ? 4 : 2)));
+  V v;
+  __device__ __forceinline__ float get(uint32_t c) const {
+    if constexpr (DT == ARK_ACT_F32) return __uint_as_float(v[c]);
+    const uint32_t h = v[c / 2];
+    if constexpr (DT == ARK_ACT_BF16) return __uint_as_float(c % 2 ? h & 0xFFFF0000u : h << 16);
+    return h2f(h >> (c % 2 * 16) & 0xFFFFu);
+  }
+};
+
+// A lane takes N columns of a group: 32 loads, no lane needs another's to find
+// its columns' largest magnitudes, and 32 N bytes that follow one another.  The
+// columns past the last whole N are the last N again, written twice alike.
+template <uint32_t DT, uint32_t N>
 __global__ __launch_bounds__(kLanes) void pack_kernel(const elem_t<DT>* __restrict__ x,
                                                       uint64_t stride, uint64_t tokens,
                                                       uint32_t columns, uint8_t* __restrict__ q,
                                                       uint8_t* __restrict__ e) {
-  const uint32_t c = blockIdx.x * kLanes + threadIdx.x;
+  typedef Columns<DT, N> C;
+  const uint32_t c0 = (blockIdx.x * kLanes + threadIdx.x) * N;
   const uint64_t g = blockIdx.y + (uint64_t)gridDim.y * blockIdx.z;
   const uint64_t t0 = g * ARK_ACT_GROUP;
-  if (c >= columns || t0 >= tokens) return;
+  if (c0 >= columns || t0 >= tokens) return;
+  const uint32_t c = c0 + N <= columns ? c0 : columns - N;
   const uint32_t n = (uint32_t)(tokens - t0 < ARK_ACT_GROUP ? tokens - t0 : ARK_ACT_GROUP);
   const elem_t<DT>* row = x + t0 * stride + c;
-  float v[ARK_ACT_GROUP];
-  uint32_t most = 0;
+  C v[ARK_ACT_GROUP];
+  if (n == ARK_ACT_GROUP) {
 #pragma unroll
-  for (uint32_t i = 0; i < ARK_ACT_GROUP; ++i) {
-    v[i] = i < n ? (float)row[i * stride] : 0.0f;
-    const uint32_t a = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-    most = a > most ? a : most;
+    for (uint32_t i = 0; i < ARK_ACT_GROUP; ++i)
+      v[i].v = *(const ARK_GLOBAL typename C::V*)(row + i * stride);
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < ARK_ACT_GROUP; ++i) {
+      v[i].v = typename C::V();
+      if (i < n) v[i].v = *(const ARK_GLOBAL typename C::V*)(row + i * stride);
+    }
   }
-  const uint32_t s = act_exponent<DT>(most);
-  const float down = act_down(s);
-  uint32_t w[ARK_ACT_GROUP / 4] = {};
+  typename C::V most = typename C::V();
 #pragma unroll
   for (uint32_t i = 0; i < ARK_ACT_GROUP; ++i)
-    w[i / 4] |= act_byte<DT>(v[i], s, down) << (i % 4 * 8);
-  u32x4* out = (u32x4*)(q + (g * columns + c) * ARK_ACT_GROUP);
-  out[0] = u32x4{w[0], w[1], w[2], w[3]};
-  out[1] = u32x4{w[4], w[5], w[6], w[7]};
-  e[g * columns + c] = (uint8_t)s;
+#pragma unroll
+    for (uint32_t k = 0; k < C::kWords; ++k)
+      most[k] = DT == ARK_ACT_F32 ? max(most[k], v[i].v[k] & 0x7FFFFFFFu)
+                                  : max_u16x2(most[k], v[i].v[k] & 0x7FFF7FFFu);
+  C top;
+  top.v = most;
+  uint8_t* out = q + (g * columns + c) * ARK_ACT_GROUP;
+#pragma unroll
+  for (uint32_t k = 0; k < N; ++k) {
+    const ActScale s = act_scale<DT>(__float_as_uint(top.get(k)));
+    u32x4 w[2];
+#pragma unroll
+    for (uint32_t i = 0; i < ARK_ACT_GROUP / 4; ++i)
+      w[i / 4][i % 4] = act_bytes4(s, v[4 * i].get(k), v[4 * i + 1].get(k), v[4 * i + 2].get(k),
+                                   v[4 * i + 3].get(k));
+    st_g<u32x4>(out + k * ARK_ACT_GROUP, w[0]);
+    st_g<u32x4>(out + k * ARK_ACT_GROUP + 16, w[1]);
+    st_g<uint8_t>(e + g * columns + c + k, (uint8_t)s.s);
+  }
 }
 
-template <uint32_t DT>
+template <uint32_t DT, uint32_t N>
 __global__ __launch_bounds__(kLanes) void unpack_kernel(const uint8_t* __restrict__ q,
                                                         const uint8_t* __restrict__ e,
                                                         uint64_t tokens, uint32_t columns,
                                                         elem_t<DT>* __restrict__ x,
                                                         uint64_t stride) {
-  const uint32_t c = blockIdx.x * kLanes + threadIdx.x;
+  typedef Columns<DT, N> C;
+  const uint32_t c0 = (blockIdx.x * kLanes + threadIdx.x) * N;
   const uint64_t g = blockIdx.y + (uint64_t)gridDim.y * blockIdx.z;
   const uint64_t t0 = g * ARK_ACT_GROUP;
-  if (c >= columns || t0 >= tokens) return;
+  if (c0 >= columns || t0 >= tokens) return;
+  const uint32_t c = c0 + N <= columns ? c0 : columns - N;
   const uint32_t n = (uint32_t)(tokens - t0 < ARK_ACT_GROUP ? tokens - t0 : ARK_ACT_GROUP);
-  const u32x4* in = (const u32x4*)(q + (g * columns + c) * ARK_ACT_GROUP);
-  const u32x4 a = in[0], b = in[1];
-  const float up = act_up(e[g * columns + c]);
+  u32x4 w[N][2];
+  float up[N];
+#pragma unroll
+  for (uint32_t k = 0; k < N; ++k) {
+    const uint8_t* in = q + (g * columns + c + k) * ARK_ACT_GROUP;
+    w[k][0] = ld_g<u32x4>(in);
+    w[k][1] = ld_g<u32x4>(in + 16);
+    up[k] = act_up(ld_g<uint8_t>(e + g * columns + c + k));
+  }
   elem_t<DT>* row = x + t0 * stride + c;
 #pragma unroll
   for (uint32_t i = 0; i < ARK_ACT_GROUP; ++i) {
-    const uint32_t w = i < 16 ? a[i / 4] : b[i / 4 - 4];
-    if (i < n) row[i * stride] = narrow<elem_t<DT>>(act_value(w >> (i % 4 * 8) & 255u, up));
+    float f[N];
+#pragma unroll
+    for (uint32_t k = 0; k < N; ++k)
+      f[k] = act_value(w[k][i / 16][i / 4 % 4] >> (i % 4 * 8) & 255u, up[k]);
+    typename C::V v;
+#pragma unroll
+    for (uint32_t k = 0; k < C::kWords; ++k) {
+      if constexpr (DT == ARK_ACT_F32)
+        v[k] = __float_as_uint(f[k]);
+      else
+        v[k] = narrow2<DT>(f[2 * k], f[2 * k + 1]);
+    }
+    if (i < n) *(ARK_GLOBAL typename C::V*)(row + i * stride) = v;
   }
+}
+
+// The same for a single column.
+template <uint32_t DT>
+__global__ __launch_bounds__(kLanes) void pack1_kernel(const elem_t<DT>* __restrict__ x,
+                                                       uint64_t stride, uint64_t tokens,
+                                                       uint8_t* __restrict__ q,
+                                                       uint8_t* __restrict__ e) {
+  const uint64_t g = (uint64_t)blockIdx.x * kLanes + threadIdx.x, t0 = g * ARK_ACT_GROUP;
+  if (t0 >= tokens) return;
+  uint32_t most = 0;
+  const auto at = [&](uint32_t i) { return t0 + i < tokens ? (float)x[(t0 + i) * stride] : 0.0f; };
+  for (uint32_t i = 0; i < ARK_ACT_GROUP; ++i)
+    most = max(most, __float_as_uint(at(i)) & 0x7FFFFFFFu);
+  const ActScale s = act_scale<DT>(most);
+  for (uint32_t i = 0; i < ARK_ACT_GROUP; i += 4)
+    st_g<uint32_t>(q + t0 + i, act_bytes4(s, at(i), at(i + 1), at(i + 2), at(i + 3)));
+  e[g] = (uint8_t)s.s;
+}
+template <uint32_t DT>
+__global__ __launch_bounds__(kLanes) void unpack1_kernel(const uint8_t* __restrict__ q,
+                                                         const uint8_t* __restrict__ e,
+                                                         uint64_t tokens,
+                                                         elem_t<DT>* __restrict__ x,
+                                                         uint64_t stride) {
+  const uint64_t t = (uint64_t)blockIdx.x * kLanes + threadIdx.x;
+  if (t < tokens) x[t * stride] = (elem_t<DT>)act_value(q[t], act_up(e[t / ARK_ACT_GROUP]));
 }
 
 // ---- the weight gradient -----------------------------------------------------
@@ -110,13 +190,6 @@ struct GradArgs {
   uint32_t m_tiles, n_tiles, splits, steps;  // steps of all splits together
   uint32_t accumulate, vec;                  // vec: dw takes 16-byte stores
 };
-
-typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
-                                                                __builtin_bit_cast(u16x2, b)));
-}
 
 template <typename T>
 struct Mat;
@@ -632,22 +705,38 @@ int check_copy(const void* x, uint64_t x_stride, uint32_t dtype, uint64_t tokens
   return checker.check(x, *x_bytes, "x", 0);
 }
 
+// Columns a lane takes: two (4 bytes of 16-bit rows), which fills the wave slots
+// best; fp32's two are 8 bytes.
+constexpr uint32_t kWide = 2;
+
 template <uint32_t DT>
 void launch_pack(const void* x, uint64_t stride, uint64_t tokens, uint64_t columns, uint8_t* act,
                  hipStream_t s) {
   const uint64_t groups = ark::act_groups(tokens);
-  hipLaunchKernelGGL(pack_kernel<DT>, group_grid((columns + kLanes - 1) / kLanes, groups),
-                     dim3(kLanes), 0, s, (const elem_t<DT>*)x, stride, tokens, (uint32_t)columns,
-                     act, act + groups * columns * ARK_ACT_GROUP);
+  uint8_t* e = act + groups * columns * ARK_ACT_GROUP;
+  const elem_t<DT>* p = (const elem_t<DT>*)x;
+  if (columns < kWide)
+    hipLaunchKernelGGL(pack1_kernel<DT>, dim3((uint32_t)((groups + kLanes - 1) / kLanes)),
+                       dim3(kLanes), 0, s, p, stride, tokens, act, e);
+  else
+    hipLaunchKernelGGL((pack_kernel<DT, kWide>),
+                       group_grid((columns + kLanes * kWide - 1) / (kLanes * kWide), groups),
+                       dim3(kLanes), 0, s, p, stride, tokens, (uint32_t)columns, act, e);
 }
 
 template <uint32_t DT>
 void launch_unpack(const uint8_t* act, uint64_t tokens, uint64_t columns, void* x, uint64_t stride,
                    hipStream_t s) {
   const uint64_t groups = ark::act_groups(tokens);
-  hipLaunchKernelGGL(unpack_kernel<DT>, group_grid((columns + kLanes - 1) / kLanes, groups),
-                     dim3(kLanes), 0, s, act, act + groups * columns * ARK_ACT_GROUP, tokens,
-                     (uint32_t)columns, (elem_t<DT>*)x, stride);
+  const uint8_t* e = act + groups * columns * ARK_ACT_GROUP;
+  elem_t<DT>* p = (elem_t<DT>*)x;
+  if (columns < kWide)
+    hipLaunchKernelGGL(unpack1_kernel<DT>, dim3((uint32_t)((tokens + kLanes - 1) / kLanes)),
+                       dim3(kLanes), 0, s, act, e, tokens, p, stride);
+  else
+    hipLaunchKernelGGL((unpack_kernel<DT, kWide>),
+                       group_grid((columns + kLanes * kWide - 1) / (kLanes * kWide), groups),
+                       dim3(kLanes), 0, s, act, e, tokens, (uint32_t)columns, p, stride);
 }
 
 // How a call is cut: the tile (64 mf x 16 nf wn outputs) and the splits of the

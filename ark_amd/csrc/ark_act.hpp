@@ -37,12 +37,20 @@ struct Elem<ARK_ACT_F32> {
 template <uint32_t DT>
 using elem_t = typename Elem<DT>::T;
 
-// fp32 -> T with the fp32 value formed first: fp16's conversion must not merge
-// with the multiply before it (see f2h).
-template <typename T>
-__device__ __forceinline__ T narrow(float f) {
-  asm("" : "+v"(f));
-  return (T)f;
+// Two fp32 values to 16 bits each, to nearest even, the first in the low half.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+template <uint32_t DT>
+__device__ __forceinline__ uint32_t narrow2(float a, float b) {
+  typedef elem_t<DT> T2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), T2));
+}
+
+// The magnitudes of two 16-bit values, the larger of each pair of halves: ordered
+// as whole numbers, inf and NaN above all others.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
+                                                                __builtin_bit_cast(u16x2, b)));
 }
 
 // The exponent byte of a group whose largest magnitude has the fp32 bits
@@ -66,14 +74,29 @@ __device__ __forceinline__ float act_up(uint32_t s) {
   return __uint_as_float(s == 255u ? 0x7FC00000u : (s - 6u) << 23);
 }
 
-// The byte of x in a group of exponent byte s: q + 128, with |q| held to 127,
-// or to 63 at fp16's top exponent.  A group that is NaN stores q = 0.
+// What quantises a group: x 2^-e rounds to a whole number in the last place of
+// 1.5 * 2^23 + 128, whose low byte then is q + 128.  |x| is held to 127 * 2^e
+// first (63 * 2^10 at fp16's top exponent), which binds only where e is the
+// largest there is.  A group that is NaN gets bytes that mean nothing.
+struct ActScale {
+  uint32_t s;
+  float down, most;
+};
 template <uint32_t DT>
-__device__ __forceinline__ uint32_t act_byte(float x, uint32_t s, float down) {
-  float q = __builtin_rintf(x * down);
-  const float most = DT == ARK_ACT_F16 && s >= 143u ? 63.0f : 127.0f;
-  q = __builtin_fminf(__builtin_fmaxf(q, -most), most);
-  return s == 255u ? 128u : (uint32_t)((int)q + 128);
+__device__ __forceinline__ ActScale act_scale(uint32_t most) {
+  const uint32_t s = act_exponent<DT>(most);
+  return {s, act_down(s), act_up(s) * (DT == ARK_ACT_F16 && s >= 143u ? 63.0f : 127.0f)};
+}
+// Four values' bytes, the first lowest.
+__device__ __forceinline__ uint32_t act_bytes4(const ActScale& a, float x0, float x1, float x2,
+                                               float x3) {
+  const auto one = [&](float x) {
+    return __float_as_uint(__builtin_fmaf(__builtin_amdgcn_fmed3f(x, -a.most, a.most), a.down,
+                                          12583040.0f));
+  };
+  const uint32_t lo = __builtin_amdgcn_perm(one(x1), one(x0), 0x0C0C0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(one(x3), one(x2), 0x04000C0Cu);
+  return lo | hi;
 }
 __device__ __forceinline__ float act_value(uint32_t byte, float up) {
   return (float)((int)byte - 128) * up;

@@ -35,7 +35,7 @@ struct Args {
   const void* positions;
   float* partial;         // backward: [part][block][head_dim] of the gains' gradients
   uint64_t start, tokens, all;  // all: batch * tokens
-  float magnitude, eps;
+  float magnitude, eps, one_over_head;
   uint32_t position_bytes, head, rotary, layout, inverse, gain_dtype;
   uint32_t lanes;         // of a row: a power of two
   uint32_t tile;          // tokens a block takes at once
@@ -107,6 +107,15 @@ __device__ __forceinline__ float row_sum(float v, uint32_t lanes) {
   return v;
 }
 
+// 1 / sqrt(a): the instruction's, within an ulp, and one Newton step.  An inf or
+// NaN, and 0 (a row of zeros without eps), stay what the instruction makes of them.
+__device__ __forceinline__ float inverse_root(float a) {
+  const float r = __builtin_amdgcn_rsqf(a);
+  const float h = __builtin_fmaf(-0.5f * a * r, r, 0.5f);
+  const float n = __builtin_fmaf(r, h, r);
+  return n == n ? n : r;
+}
+
 enum Op { kRope, kNorm, kBack };
 
 constexpr uint32_t kBlock = 256, kWaves = 4;
@@ -150,12 +159,13 @@ struct Raw {
     else
       return __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
   }
-  __device__ __forceinline__ void set(uint32_t i, float f) {
-    if constexpr (DT == ARK_ACT_F32) {
-      w[i] = __float_as_uint(f);
-    } else {
-      const uint32_t b = __builtin_bit_cast(uint16_t, narrow<elem_t<DT>>(f));
-      w[i / 2] = i % 2 ? w[i / 2] | b << 16 : b;
+  __device__ __forceinline__ void set(const float* f) {
+#pragma unroll
+    for (uint32_t i = 0; i < kWords; ++i) {
+      if constexpr (DT == ARK_ACT_F32)
+        w[i] = __float_as_uint(f[i]);
+      else
+        w[i] = narrow2<DT>(f[2 * i], N > 1 ? f[2 * i + 1] : 0.0f);
     }
   }
 };
@@ -258,12 +268,36 @@ struct Row {
         if (r.pairs_v[k]) v[k].store(p + r.ev[k]);
       }
     }
+    // element by element the larger magnitude, inf and NaN above all others
+    __device__ __forceinline__ void larger(const Data& d) {
+#pragma unroll
+      for (uint32_t k = 0; k < K; ++k)
+#pragma unroll
+        for (uint32_t i = 0; i < Raw<DT, V>::kWords; ++i) {
+          u[k].w[i] = larger2(u[k].w[i], d.u[k].w[i]);
+          v[k].w[i] = larger2(v[k].w[i], d.v[k].w[i]);
+        }
+    }
+    template <uint32_t BIT>
+    __device__ __forceinline__ void larger_across() {
+#pragma unroll
+      for (uint32_t k = 0; k < K; ++k)
+#pragma unroll
+        for (uint32_t i = 0; i < Raw<DT, V>::kWords; ++i) {
+          u[k].w[i] = larger2(u[k].w[i], across<BIT>(u[k].w[i]));
+          v[k].w[i] = larger2(v[k].w[i], across<BIT>(v[k].w[i]));
+        }
+    }
+    static __device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) {
+      return DT == ARK_ACT_F32 ? max(a, b & 0x7FFFFFFFu) : max_u16x2(a, b & 0x7FFF7FFFu);
+    }
     // element `second` of the lane's pair e
     __device__ __forceinline__ float get(uint32_t e, bool second) const {
       return second ? v[e / V].get(e % V) : u[e / V].get(e % V);
     }
-    __device__ __forceinline__ void set(uint32_t e, bool second, float f) {
-      second ? v[e / V].set(e % V, f) : u[e / V].set(e % V, f);
+    __device__ __forceinline__ void set(const float* fu, const float* fv) {
+#pragma unroll
+      for (uint32_t k = 0; k < K; ++k) u[k].set(fu + k * V), v[k].set(fv + k * V);
     }
   };
   // where element `second` of pair e lies in the row
@@ -306,15 +340,15 @@ struct Row {
       q = __builtin_fmaf(u[e], u[e], q);
       q = __builtin_fmaf(v[e], v[e], q);
     }
-    if constexpr (OP == kNorm)
-      r = 1.0f / __builtin_sqrtf(row_sum(q, a.lanes) / (float)a.head + a.eps);
+    if constexpr (OP == kNorm) r = inverse_root(row_sum(q, a.lanes) * a.one_over_head + a.eps);
 #pragma unroll
     for (uint32_t e = 0; e < kE; ++e) {
       const float nu = OP == kNorm ? u[e] * (r * gu[e]) : u[e];
       const float nv = OP == kNorm ? v[e] * (r * gv[e]) : v[e];
-      y->set(e, false, __builtin_fmaf(nu, c[e], -(nv * s[e])));
-      y->set(e, true, __builtin_fmaf(nu, s[e], nv * c[e]));
+      u[e] = __builtin_fmaf(nu, c[e], -(nv * s[e]));
+      v[e] = __builtin_fmaf(nu, s[e], nv * c[e]);
     }
+    y->set(u, v);
   }
   // dx from dy and x, and dy rotated back times x r into the gain's sums
   __device__ __forceinline__ void backward(const Args& a, const Data& dy, const float* xu,
@@ -332,16 +366,16 @@ struct Row {
       along = __builtin_fmaf(du[e] * gu[e], xu[e], along);
       along = __builtin_fmaf(dv[e] * gv[e], xv[e], along);
     }
-    const float n = 1.0f / (float)a.head;
-    const float r = 1.0f / __builtin_sqrtf(row_sum(q, a.lanes) * n + a.eps);
-    along = row_sum(along, a.lanes) * n * r * r;
+    const float r = inverse_root(row_sum(q, a.lanes) * a.one_over_head + a.eps);
+    along = row_sum(along, a.lanes) * a.one_over_head * r * r;
 #pragma unroll
     for (uint32_t e = 0; e < kE; ++e) {
       su[e] = __builtin_fmaf(du[e], xu[e] * r, su[e]);
       sv[e] = __builtin_fmaf(dv[e], xv[e] * r, sv[e]);
-      dx->set(e, false, r * __builtin_fmaf(-xu[e], along, du[e] * gu[e]));
-      dx->set(e, true, r * __builtin_fmaf(-xv[e], along, dv[e] * gv[e]));
+      du[e] = r * __builtin_fmaf(-xu[e], along, du[e] * gu[e]);
+      dv[e] = r * __builtin_fmaf(-xv[e], along, dv[e] * gv[e]);
     }
+    dx->set(du, dv);
   }
   // a wave's sums of the gain's gradient, its rows' lanes together, into LDS
   __device__ __forceinline__ void gather(const Args& a, float* su, float* sv, float* out) const {
@@ -367,9 +401,8 @@ struct Tokens {
     at = (uint64_t*)lds;
     turns = (float2*)(lds + a.tile * 24);
   }
-  __device__ __forceinline__ void fill(const Args& a, const Part& p, uint64_t first, uint32_t n,
-                                       bool back) const {
-    const uint32_t half = a.rotary / 2;
+  __device__ __forceinline__ void starts(const Args& a, const Part& p, uint64_t first,
+                                         uint32_t n) const {
     for (uint32_t i = threadIdx.x; i < n * 3; i += kBlock) {
       const uint64_t bt = first + i / 3;
       const Array& r = i % 3 == 0 ? p.x : i % 3 == 1 ? p.dy : p.y;
@@ -377,6 +410,10 @@ struct Tokens {
       if (a.all != a.tokens) b = bt / a.tokens, t = bt % a.tokens;
       at[i] = b * r.sb + t * r.st;
     }
+  }
+  __device__ __forceinline__ void angles(const Args& a, uint64_t first, uint32_t n,
+                                         bool back) const {
+    const uint32_t half = a.rotary / 2;
     for (uint32_t i = threadIdx.x; i < n * half; i += kBlock) {
       float s, c;
       sincos_turns(phase_of(position_at(a, first + i / half), a.turns[i % half]), &s, &c);
@@ -406,25 +443,33 @@ __global__ __launch_bounds__(kBlock) void rows_kernel(Args a) {
        first += (uint64_t)gridDim.x * a.tile) {
     const uint32_t n = (uint32_t)(a.all - first < a.tile ? a.all - first : a.tile);
     __syncthreads();
-    tok.fill(a, P, first, n, OP != kBack && a.inverse);
+    tok.starts(a, P, first, n);
     __syncthreads();
     {
       const uint8_t* exps = P.act + (a.all + ARK_ACT_GROUP - 1) / ARK_ACT_GROUP * columns * ARK_ACT_GROUP;
-      for (uint32_t r0 = wave * at_once; r0 < n * P.heads; r0 += kWaves * at_once * kUnroll) {
-        typename R::Data x[kUnroll], dy[kUnroll];
-        uint32_t t[kUnroll], h[kUnroll];
-        bool in[kUnroll];
+      typename R::Data x[kUnroll], dy[kUnroll];
+      uint32_t t[kUnroll], h[kUnroll];
+      bool in[kUnroll];
+      const auto load = [&](uint32_t r0) {
 #pragma unroll
         for (uint32_t i = 0; i < kUnroll; ++i) {
           const uint32_t r = r0 + i * kWaves * at_once + lane / a.lanes;
           in[i] = r < n * P.heads;
           t[i] = in[i] ? r / P.heads : 0;
           h[i] = in[i] ? r - t[i] * P.heads : 0;
+          if (!in[i]) continue;
           if (OP != kBack || !P.act)
             x[i].load(row, (const T*)P.x.p + tok.at[t[i] * 3] + h[i] * P.x.sh);
           if (OP == kBack)
             dy[i].load(row, (const T*)P.dy.p + tok.at[t[i] * 3 + 1] + h[i] * P.dy.sh);
         }
+      };
+      // the first rows are on their way while the angles are formed
+      load(wave * at_once);
+      tok.angles(a, first, n, OP != kBack && a.inverse);
+      __syncthreads();
+      for (uint32_t r0 = wave * at_once; r0 < n * P.heads; r0 += kWaves * at_once * kUnroll) {
+        if (r0 != wave * at_once) load(r0);
 #pragma unroll
         for (uint32_t i = 0; i < kUnroll; ++i) {
           float c[R::kE], s[R::kE];
@@ -469,6 +514,63 @@ __global__ __launch_bounds__(kBlock) void rows_kernel(Args a) {
   }
 }
 
+// The exponent bytes of a lane's 2V columns: V bytes at u's place, V at v's.
+template <uint32_t V>
+struct Exps {
+  uint32_t u = 0, v = 0;
+  template <typename R>
+  __device__ __forceinline__ void load(const R& row, const uint8_t* p) {
+    if (row.on[0]) u = bytes(p + row.eu[0]);
+    if (row.pairs_v[0]) v = bytes(p + row.ev[0]);
+    if (V > 1 && row.mixed) {  // in order to every other one and those between
+      const uint64_t t = (uint64_t)v << (8 * V) | u;
+      u = v = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < V; ++i) {
+        u |= (uint32_t)(t >> (16 * i) & 255u) << (8 * i);
+        v |= (uint32_t)(t >> (16 * i + 8) & 255u) << (8 * i);
+      }
+    }
+  }
+  template <typename R>
+  __device__ __forceinline__ void store(const R& row, uint8_t* p) const {
+    uint32_t a = u, b = v;
+    if (V > 1 && row.mixed) {
+      uint64_t t = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < V; ++i)
+        t |= (uint64_t)(u >> (8 * i) & 255u) << (16 * i) |
+             (uint64_t)(v >> (8 * i) & 255u) << (16 * i + 8);
+      a = (uint32_t)t;
+      b = (uint32_t)(t >> (8 * V));
+    }
+    if (row.on[0]) put(p + row.eu[0], a);
+    if (row.pairs_v[0]) put(p + row.ev[0], b);
+  }
+  __device__ __forceinline__ uint32_t get(uint32_t i, bool second) const {
+    return (second ? v : u) >> (8 * i) & 255u;
+  }
+  __device__ __forceinline__ void set(uint32_t i, bool second, uint32_t s) {
+    (second ? v : u) |= s << (8 * i);
+  }
+
+ private:
+  typedef uint32_t u32_a1 __attribute__((aligned(1)));
+  typedef uint16_t u16_a1 __attribute__((aligned(1)));
+  static __device__ __forceinline__ uint32_t bytes(const uint8_t* p) {
+    return V == 4 ? *(const ARK_GLOBAL u32_a1*)p : V == 2 ? *(const ARK_GLOBAL u16_a1*)p
+                                                          : *(const ARK_GLOBAL uint8_t*)p;
+  }
+  static __device__ __forceinline__ void put(uint8_t* p, uint32_t x) {
+    if (V == 4)
+      *(ARK_GLOBAL u32_a1*)p = x;
+    else if (V == 2)
+      *(ARK_GLOBAL u16_a1*)p = (uint16_t)x;
+    else
+      *(ARK_GLOBAL uint8_t*)p = (uint8_t)x;
+  }
+};
+
 // The norm of 32 tokens of a head at a time, with the 8-bit form of its input:
 // written by the forward pass, read by the backward pass.  A wave holds the
 // tile, kIt rows a lane, neighbouring tokens, so that a column's largest
@@ -493,70 +595,67 @@ __global__ __launch_bounds__(kBlock) void tiles_kernel(Args a) {
     const uint64_t first = g * ARK_ACT_GROUP;
     const uint32_t n = (uint32_t)(a.all - first < ARK_ACT_GROUP ? a.all - first : ARK_ACT_GROUP);
     __syncthreads();
-    tok.fill(a, P, first, n, false);
+    tok.starts(a, P, first, n);
     __syncthreads();
     {
-      for (uint32_t h = slice * kWaves + wave; h < P.heads; h += a.slices * kWaves) {
-        uint8_t* const q = P.act + (g * columns + h * a.head) * ARK_ACT_GROUP;
-        uint8_t* const exps = P.act + groups * columns * ARK_ACT_GROUP + g * columns + h * a.head;
-        typename R::Data in[kIt];
+      typename R::Data in[kIt];
+      const auto load = [&](uint32_t h) {
+        const Array& from = BACK ? P.dy : P.x;
 #pragma unroll
         for (uint32_t i = 0; i < kIt; ++i) {
-          const uint32_t t = mine + i;
-          const Array& from = BACK ? P.dy : P.x;
-          if (t < n)
-            in[i].load(row, (const T*)from.p + tok.at[t * 3 + BACK] + h * from.sh);
-          else
-            in[i] = typename R::Data();
+          in[i] = typename R::Data();
+          if (mine + i < n)
+            in[i].load(row, (const T*)from.p + tok.at[(mine + i) * 3 + BACK] + h * from.sh);
+        }
+      };
+      // the first head is on its way while the angles are formed
+      const uint32_t first_h = slice * kWaves + wave;
+      if (first_h < P.heads) load(first_h);
+      tok.angles(a, first, n, false);
+      __syncthreads();
+      for (uint32_t h = first_h; h < P.heads; h += a.slices * kWaves) {
+        if (h != first_h) load(h);
+        uint8_t* const q = P.act + (g * columns + h * a.head) * ARK_ACT_GROUP + mine;
+        uint8_t* const exps = P.act + groups * columns * ARK_ACT_GROUP + g * columns + h * a.head;
+        Bytes b[R::kE][2];
+        float up[R::kE][2];
+        if constexpr (BACK) {
+          Exps<V> e;
+          e.load(row, exps);
+#pragma unroll
+          for (uint32_t k = 0; k < 2 * R::kE; ++k) {
+            const bool second = k & 1;
+            b[k / 2][second] = Bytes();
+            if (row.has(k / 2, second))
+              b[k / 2][second] = *(const ARK_GLOBAL Bytes*)(q + row.at(k / 2, second) * ARK_ACT_GROUP);
+            up[k / 2][second] = row.has(k / 2, second) ? act_up(e.get(k / 2, second)) : 0.0f;
+          }
         }
 #pragma unroll
         for (uint32_t i = 0; i < kIt; ++i) in[i].sort(row);
-        Bytes b[R::kE][2];
-        float up[R::kE][2];
-#pragma unroll
-        for (uint32_t e = 0; e < R::kE; ++e)
-#pragma unroll
-          for (uint32_t k = 0; k < 2; ++k) {
-            if (!row.has(e, k)) {
-              b[e][k] = Bytes(), up[e][k] = 0.0f;
-              continue;
-            }
-            uint8_t* const at = q + row.at(e, k) * ARK_ACT_GROUP + mine;
-            if constexpr (BACK) {
-              b[e][k] = *(const ARK_GLOBAL Bytes*)at;
-              up[e][k] = act_up(ld_g<uint8_t>(exps + row.at(e, k)));
-            }
-          }
         if constexpr (!BACK) {
-          uint32_t most[R::kE][2];
+          Exps<V> e;
+          // the largest magnitudes of a lane's columns, as the types' bits order them
+          typename R::Data most = typename R::Data();
 #pragma unroll
-          for (uint32_t e = 0; e < R::kE; ++e)
+          for (uint32_t i = 0; i < kIt; ++i) most.larger(in[i]);
+          if (kLanes <= 8) most.template larger_across<8>();
+          if (kLanes <= 16) most.template larger_across<16>();
+          if (kLanes <= 32) most.template larger_across<32>();
 #pragma unroll
-            for (uint32_t k = 0; k < 2; ++k) {
-              uint32_t m = 0;
+          for (uint32_t k = 0; k < 2 * R::kE; ++k) {
+            const uint32_t p = k / 2;
+            const bool second = k & 1;
+            const ActScale s = act_scale<DT>(__float_as_uint(most.get(p, second)));
+            e.set(p, second, s.s);
+            Bytes w;
 #pragma unroll
-              for (uint32_t i = 0; i < kIt; ++i)
-                m = max(m, __float_as_uint(in[i].get(e, k)) & 0x7FFFFFFFu);
-              if (kLanes <= 8) m = max(m, across<8>(m));
-              if (kLanes <= 16) m = max(m, across<16>(m));
-              if (kLanes <= 32) m = max(m, across<32>(m));
-              most[e][k] = m;
-            }
-#pragma unroll
-          for (uint32_t e = 0; e < R::kE; ++e)
-#pragma unroll
-            for (uint32_t k = 0; k < 2; ++k) {
-              const uint32_t s = act_exponent<DT>(most[e][k]);
-              const float down = act_down(s);
-              Bytes w = Bytes();
-#pragma unroll
-              for (uint32_t i = 0; i < kIt; ++i)
-                w[i / 4] |= act_byte<DT>(in[i].get(e, k), s, down) << (i % 4 * 8);
-              if (row.has(e, k)) {
-                *(ARK_GLOBAL Bytes*)(q + row.at(e, k) * ARK_ACT_GROUP + mine) = w;
-                if (mine == 0) st_g<uint8_t>(exps + row.at(e, k), (uint8_t)s);
-              }
-            }
+            for (uint32_t i = 0; i < kIt; i += 4)
+              w[i / 4] = act_bytes4(s, in[i].get(p, second), in[i + 1].get(p, second),
+                                    in[i + 2].get(p, second), in[i + 3].get(p, second));
+            if (row.has(p, second)) *(ARK_GLOBAL Bytes*)(q + row.at(p, second) * ARK_ACT_GROUP) = w;
+          }
+          if (mine == 0) e.store(row, exps);
         }
 #pragma unroll
         for (uint32_t i = 0; i < kIt; ++i) {
@@ -612,12 +711,11 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(Args a) {
     const uint32_t m = __float_as_uint(v[r]) & 0x7FFFFFFFu;
     most = m > most ? m : most;
   }
-  const uint32_t s = act_exponent<DT>(most);
-  const float down = act_down(s);
+  const ActScale s = act_scale<DT>(most);
 #pragma unroll
-  for (uint32_t r = 0; r < ARK_ACT_GROUP; ++r)
-    P.act[i * ARK_ACT_GROUP + r] = (uint8_t)act_byte<DT>(v[r], s, down);
-  P.act[groups * columns * ARK_ACT_GROUP + i] = (uint8_t)s;
+  for (uint32_t r = 0; r < ARK_ACT_GROUP; r += 4)
+    st_g<uint32_t>(P.act + i * ARK_ACT_GROUP + r, act_bytes4(s, v[r], v[r + 1], v[r + 2], v[r + 3]));
+  P.act[groups * columns * ARK_ACT_GROUP + i] = (uint8_t)s.s;
 }
 
 // The gains' gradients from the blocks' rows, added in order: 64 rows' runs by
@@ -729,9 +827,9 @@ uint32_t launch_tiles(uint32_t dtype, Args* a, hipStream_t s, bool launch = true
   a->tile = ARK_ACT_GROUP;
   const uint64_t groups = ark::act_groups(a->all);
   const uint32_t heads = a->part[0].heads > a->part[1].heads ? a->part[0].heads : a->part[1].heads;
-  // blocks share a group's heads until there are about 1500
+  // blocks share a group's heads until there are about 500 of a part
   uint32_t slices = (heads + kWaves - 1) / kWaves;
-  while (slices > 1 && groups * (slices - 1) >= 1536) --slices;
+  while (slices > 1 && groups * (slices - 1) >= 512) --slices;
   a->slices = slices;
   uint64_t by = groups;
   const uint32_t most = (BACK ? 2048u : 1u << 20) / slices;
@@ -943,6 +1041,7 @@ Args base_args(const ark_rope* r, uint64_t batch, uint64_t tokens, const void* p
   a.all = batch * tokens;
   a.magnitude = r->magnitude;
   a.head = r->head;
+  a.one_over_head = 1.0f / (float)r->head;
   a.rotary = r->rotary;
   a.layout = r->layout;
   return a;

@@ -10,6 +10,8 @@ transposed (batch, heads, tokens, head_dim) arrays are taken as they are.
 """
 import ctypes as C
 
+import torch
+
 from . import _abi
 from ._lib import check, lib, current_stream as _stream
 from .act import Act8, _code
@@ -22,6 +24,7 @@ _SCALINGS = {"linear": (_abi.ROPE_SCALE_LINEAR, ("factor",), {}),
              "bands": (_abi.ROPE_SCALE_BANDS, ("factor", "original", "low", "high"),
                        {"low": 1.0, "high": 4.0})}
 _U64x4 = C.c_uint64 * 4
+_POSITIONS = {torch.int32: 4, torch.int64: 8}
 
 
 def frequencies(rotary_dim, base=10000.0, scaling=None):
@@ -64,7 +67,7 @@ class Rope:
         elif scaling is not None or len(inv_freq) != rotary_dim // 2:
             raise ValueError("inv_freq holds one value a pair and takes no scaling")
         self._h = None
-        import torch
+        self._layouts = {}
         torch.cuda.current_device()
         h = C.c_void_p()
         check(lib().ark_rope_create(head_dim, rotary_dim, _LAYOUTS[layout],
@@ -87,54 +90,70 @@ class Rope:
 
     # ---- arguments --------------------------------------------------------
 
+    def _layout(self, t, what):
+        """The layout of a query or key tensor as the library takes it, one for
+        every shape and strides met."""
+        key = t.shape, t.stride()
+        found = self._layouts.get(key)
+        if found is not None:
+            return found
+        (s, st), n = key, t.dim()
+        if n not in (3, 4):
+            raise ValueError(f"{what} has {n} dimensions: (batch,) tokens, heads, head_dim")
+        if s[-1] != self.head_dim:
+            raise ValueError(f"{what} is {tuple(s)}: its heads must have {self.head_dim} values")
+        if st[-1] != 1 and s[-1] > 1:
+            raise ValueError(f"{what}: the values of a head do not follow one another")
+        if len(self._layouts) >= 256:
+            self._layouts.clear()
+        found = self._layouts[key] = _U64x4(s[-2], st[0] if n == 4 else 0, st[-3], st[-2])
+        return found
+
     def _array(self, t, like, what):
         """(address, layout) of a query or key tensor, whose sizes but the heads
         must be those of ``like``."""
-        n = t.dim()
-        if n != like.dim() or n not in (3, 4):
-            raise ValueError(f"{what} has {n} dimensions: (batch,) tokens, heads, head_dim")
-        if not t.is_cuda or t.device != like.device or t.dtype != like.dtype:
-            raise ValueError(f"{what} is {t.dtype} on {t.device}, not {like.dtype} on "
+        if t is not like and (t.shape[:-2] != like.shape[:-2] or t.dtype != like.dtype
+                              or t.device != like.device):
+            raise ValueError(f"{what} is {tuple(t.shape)} {t.dtype} on {t.device}, not "
+                             f"{tuple(like.shape[:-2])} x heads x {self.head_dim} {like.dtype} on "
                              f"{like.device}")
-        s, st = t.shape, t.stride()
-        if s[-1] != self.head_dim or s[:-2] != like.shape[:-2]:
-            raise ValueError(f"{what} is {tuple(s)}, not {tuple(like.shape[:-2])} x heads x "
-                             f"{self.head_dim}")
-        if st[-1] != 1 and s[-1] > 1:
-            raise ValueError(f"{what}: the values of a head do not follow one another")
-        return t.data_ptr(), _U64x4(s[-2], st[0] if n == 4 else 0, st[-3], st[-2])
+        return t.data_ptr(), self._layout(t, what)
 
     def _call(self, like, positions, start):
         """The arguments every call begins with."""
         code = _code(like, "q")
-        batch = like.shape[0] if like.dim() == 4 else 1
-        tokens = like.shape[-3] if like.dim() >= 3 else 0
+        if not like.is_cuda:
+            raise ValueError(f"q is on {like.device}, not a GPU")
+        s = like.shape
+        if len(s) not in (3, 4):
+            raise ValueError(f"q has {len(s)} dimensions: (batch,) tokens, heads, head_dim")
+        batch, tokens = s[0] if len(s) == 4 else 1, s[-3]
         if positions is None:
-            return (self._h, code, batch, tokens, None, 0, start)
-        if (not positions.is_cuda or not positions.is_contiguous()
-                or positions.is_floating_point() or positions.element_size() not in (4, 8)
-                or positions.numel() != batch * tokens or positions.device != like.device):
+            return self._h, code, batch, tokens, None, 0, start
+        size = _POSITIONS.get(positions.dtype)
+        if (size is None or positions.device != like.device or not positions.is_contiguous()
+                or positions.numel() != batch * tokens):
             raise ValueError(f"positions must be {batch * tokens} contiguous int32 or int64 on "
                              f"{like.device}")
-        return (self._h, code, batch, tokens, positions.data_ptr(), positions.element_size(),
-                start)
+        return self._h, code, batch, tokens, positions.data_ptr(), size, start
 
     def _gains(self, gq, gk, like):
         code = _code(gq, "gain_q")
         for g in (gq, gk):
-            if g is not None and (not g.is_cuda or g.dtype != gq.dtype or not g.is_contiguous()
-                                  or g.numel() != self.head_dim or g.device != like.device):
+            if (g.dtype != gq.dtype or not g.is_contiguous() or g.numel() != self.head_dim
+                    or g.device != like.device):
                 raise ValueError(f"gains must be {self.head_dim} contiguous {gq.dtype} on "
                                  f"{like.device}")
-        return gq.data_ptr(), None if gk is None else gk.data_ptr(), code
+        return gq.data_ptr(), gk.data_ptr(), code
 
     def _out(self, t, out, what):
-        import torch
+        """(the result's tensor, its address, its layout)."""
         if out is None:
-            out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        elif out.shape != t.shape:
+            out = torch.empty_like(t)
+            return out, out.data_ptr(), self._layout(out, what)
+        if out.shape != t.shape:
             raise ValueError(f"{what} is {tuple(out.shape)}, not {tuple(t.shape)}")
-        return out
+        return out, *self._array(out, t, what)
 
     # ---- calls ------------------------------------------------------------
 
@@ -144,20 +163,18 @@ class Rope:
         pair with k; q itself to rotate in place) or new tensors.  inverse
         rotates back, as the gradients of the results are.  Returns the pair, or
         one tensor without k."""
-        oq, ok = (out if k is not None and out is not None else (out, None))
-        oq = self._out(q, oq, "out")
         head = self._call(q, positions, start)
-        qp, ql = self._array(q, q, "q")
-        op, ol = self._array(oq, q, "out")
+        qa = self._array(q, q, "q")
         if k is None:
-            check(lib().ark_rope_apply(*head, qp, ql, op, ol, None, None, None, None,
-                                       int(bool(inverse)), _stream(q)))
+            oq, *oa = self._out(q, out, "out")
+            check(lib().ark_rope_apply(*head, *qa, *oa, None, None, None, None, int(bool(inverse)),
+                                       _stream(q)))
             return oq
-        ok = self._out(k, ok, "out")
-        kp, kl = self._array(k, q, "k")
-        okp, okl = self._array(ok, q, "out")
-        check(lib().ark_rope_apply(*head, qp, ql, op, ol, kp, kl, okp, okl, int(bool(inverse)),
-                                   _stream(q)))
+        oq, ok = (None, None) if out is None else out
+        oq, *oa = self._out(q, oq, "out")
+        ok, *ob = self._out(k, ok, "out")
+        check(lib().ark_rope_apply(*head, *qa, *oa, *self._array(k, q, "k"), *ob,
+                                   int(bool(inverse)), _stream(q)))
         return oq, ok
 
     def norm(self, q, k, gain_q, gain_k, positions=None, start=0, eps=1e-5, out=None,
@@ -167,26 +184,26 @@ class Rope:
         8-bit forms of q and k in the same pass, for norm_backward: True for new
         ones, or a pair of Act8 of batch * tokens rows.  Returns (q, k) or (q,
         k, kept_q, kept_k)."""
-        oq, ok = (None, None) if out is None else out
-        oq, ok = self._out(q, oq, "out"), self._out(k, ok, "out")
         head = self._call(q, positions, start)
-        qp, ql = self._array(q, q, "q")
-        kp, kl = self._array(k, q, "k")
-        oqp, oql = self._array(oq, q, "out")
-        okp, okl = self._array(ok, q, "out")
-        aq = ak = None
-        if keep8:
-            rows, d = head[2] * head[3], self.head_dim
-            if keep8 is True:
-                aq = Act8(rows, q.shape[-2] * d, q.dtype, q.device)
-                ak = Act8(rows, k.shape[-2] * d, q.dtype, q.device)
-            else:
-                aq, ak = keep8
-                self._kept(aq, q, rows, q.shape[-2]), self._kept(ak, q, rows, k.shape[-2])
-        check(lib().ark_rope_norm(*head, eps, *self._gains(gain_q, gain_k, q), qp, ql, oqp, oql,
-                                  aq.data.data_ptr() if keep8 else None, kp, kl, okp, okl,
-                                  ak.data.data_ptr() if keep8 else None, _stream(q)))
-        return (oq, ok, aq, ak) if keep8 else (oq, ok)
+        gains = self._gains(gain_q, gain_k, q)
+        qa, ka = self._array(q, q, "q"), self._array(k, q, "k")
+        oq, ok = (None, None) if out is None else out
+        oq, *oa = self._out(q, oq, "out")
+        ok, *ob = self._out(k, ok, "out")
+        if not keep8:
+            check(lib().ark_rope_norm(*head, eps, *gains, *qa, *oa, None, *ka, *ob, None,
+                                      _stream(q)))
+            return oq, ok
+        rows, d = head[2] * head[3], self.head_dim
+        if keep8 is True:
+            aq = Act8(rows, q.shape[-2] * d, q.dtype, q.device)
+            ak = Act8(rows, k.shape[-2] * d, q.dtype, q.device)
+        else:
+            aq, ak = keep8
+            self._kept(aq, q, rows, q.shape[-2]), self._kept(ak, q, rows, k.shape[-2])
+        check(lib().ark_rope_norm(*head, eps, *gains, *qa, *oa, aq.data.data_ptr(), *ka, *ob,
+                                  ak.data.data_ptr(), _stream(q)))
+        return oq, ok, aq, ak
 
     def _kept(self, a, like, rows, heads):
         if ((a.tokens, a.columns, a.dtype) != (rows, heads * self.head_dim, like.dtype)
@@ -201,12 +218,11 @@ class Rope:
         ``out`` (a pair; dq and dk themselves for in place) or new tensors, and
         of the gains, float32, into dgain_q and dgain_k (added with accumulate)
         or new ones.  Returns (q_grad, k_grad, dgain_q, dgain_k)."""
-        import torch
-        oq, ok = (None, None) if out is None else out
-        oq, ok = self._out(dq, oq, "out"), self._out(dk, ok, "out")
         head = self._call(dq, positions, start)
-        args, grads = [], []
-        for dy, x, o, dgain in ((dq, q, oq, dgain_q), (dk, k, ok, dgain_k)):
+        gains = self._gains(gain_q, gain_k, dq)
+        args, outs, grads = [], [], []
+        for dy, x, o, dgain in ((dq, q, None if out is None else out[0], dgain_q),
+                                (dk, k, None if out is None else out[1], dgain_k)):
             args += self._array(dy, dq, "gradient")
             if isinstance(x, Act8):
                 self._kept(x, dq, head[2] * head[3], dy.shape[-2])
@@ -215,16 +231,17 @@ class Rope:
                 if x.shape != dy.shape:
                     raise ValueError(f"input is {tuple(x.shape)}, its gradient {tuple(dy.shape)}")
                 args += [*self._array(x, dq, "input"), None]
-            args += self._array(o, dq, "out")
+            o, *oa = self._out(dy, o, "out")
             if dgain is None:
                 if accumulate:
                     raise ValueError("accumulate needs dgain_q and dgain_k")
-                dgain = torch.empty(self.head_dim, dtype=torch.float32, device=dq.device)
+                dgain = dq.new_empty(self.head_dim, dtype=torch.float32)
             elif (dgain.dtype != torch.float32 or not dgain.is_contiguous()
                   or dgain.numel() != self.head_dim or dgain.device != dq.device):
                 raise ValueError(f"dgain must be {self.head_dim} contiguous float32")
-            args.append(dgain.data_ptr())
+            args += [*oa, dgain.data_ptr()]
+            outs.append(o)
             grads.append(dgain)
-        check(lib().ark_rope_norm_backward(*head, eps, *self._gains(gain_q, gain_k, dq), *args,
-                                           int(bool(accumulate)), _stream(dq)))
-        return oq, ok, grads[0], grads[1]
+        check(lib().ark_rope_norm_backward(*head, eps, *gains, *args, int(bool(accumulate)),
+                                           _stream(dq)))
+        return outs[0], outs[1], grads[0], grads[1]
