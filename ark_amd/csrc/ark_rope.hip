@@ -213,7 +213,9 @@ __device__ __forceinline__ void mix(Raw<DT, N>& a, Raw<DT, N>& b) {
 // and of long rows with V = 1 the pairs 64 on too, K in all.  Pairs past the
 // rotary ones are made of what is left of the head the same way, and turn by
 // nothing.  A lane's pairs are two stretches of V elements, u and v, in the half
-// layout; in the interleaved one they are one of 2V, sorted once loaded.
+// layout; in the interleaved one they are one of 2V, sorted once loaded.  Lanes
+// past the row's end load its first pairs, add nothing to its sums and store
+// nothing; the last pair of an odd head has no second element.
 template <uint32_t DT, uint32_t V, uint32_t K>
 struct Row {
   static constexpr uint32_t kE = V * K;
@@ -239,17 +241,24 @@ struct Row {
         ev[k] = p < half ? half + p : a.rotary + rest + p - half;
       }
       pairs_v[k] = on[k] && ev[k] < a.head;
+      if (!on[k]) eu[k] = 0;
+      if (!pairs_v[k]) ev[k] = eu[k];
     }
+  }
+  // Places in the row are formed where they are used: kept through a loop they
+  // cost a register an element.
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (uint32_t k = 0; k < K; ++k) asm volatile("" : "+v"(eu[k]), "+v"(ev[k]));
   }
   struct Data {
     Raw<DT, V> u[K], v[K];
     __device__ __forceinline__ void load(const Row& r, const T* p) {
 #pragma unroll
       for (uint32_t k = 0; k < K; ++k) {
-        u[k].clear();
-        v[k].clear();
-        if (r.on[k]) u[k].load(p + r.eu[k]);
-        if (r.pairs_v[k]) v[k].load(p + r.ev[k]);
+        u[k].load(p + r.eu[k]);
+        v[k].load(p + r.ev[k]);
+        if (V == 1 && !r.pairs_v[k]) v[k].clear();
       }
     }
     // what the interleaved layout loaded, e0 e1 ..., to e0 e2 ... and e1 e3 ...
@@ -267,6 +276,13 @@ struct Row {
         if (r.on[k]) u[k].store(p + r.eu[k]);
         if (r.pairs_v[k]) v[k].store(p + r.ev[k]);
       }
+    }
+    __device__ __forceinline__ void opaque() {
+#pragma unroll
+      for (uint32_t k = 0; k < K; ++k)
+#pragma unroll
+        for (uint32_t i = 0; i < Raw<DT, V>::kWords; ++i)
+          asm volatile("" : "+v"(u[k].w[i]), "+v"(v[k].w[i]));
     }
     // element by element the larger magnitude, inf and NaN above all others
     __device__ __forceinline__ void larger(const Data& d) {
@@ -311,8 +327,8 @@ struct Row {
   __device__ __forceinline__ void gains(const Args& a, const void* g, float* gu, float* gv) const {
 #pragma unroll
     for (uint32_t e = 0; e < kE; ++e) {
-      gu[e] = has(e, false) ? gain_at(a, g, at(e, false)) : 0.0f;
-      gv[e] = has(e, true) ? gain_at(a, g, at(e, true)) : 0.0f;
+      gu[e] = gain_at(a, g, at(e, false));
+      gv[e] = gain_at(a, g, has(e, true) ? at(e, true) : 0);
     }
   }
   // the pairs' cosines and sines from a token's line of the block's table
@@ -330,17 +346,22 @@ struct Row {
   }
   // y = the rotation of x, or of x r gain
   template <Op OP>
-  __device__ __forceinline__ void forward(const Args& a, const Data& x, const float* gu,
+  __device__ __forceinline__ void forward(const Args& a, uint32_t lanes, const Data& x, const float* gu,
                                           const float* gv, const float* c, const float* s,
                                           Data* y) const {
     float u[kE], v[kE], r = 1.0f, q = 0.0f;
 #pragma unroll
-    for (uint32_t e = 0; e < kE; ++e) {
-      u[e] = x.get(e, false), v[e] = x.get(e, true);
-      q = __builtin_fmaf(u[e], u[e], q);
-      q = __builtin_fmaf(v[e], v[e], q);
+    for (uint32_t k = 0; k < K; ++k) {
+      float p = 0.0f;
+#pragma unroll
+      for (uint32_t e = k * V; e < k * V + V; ++e) {
+        u[e] = x.get(e, false), v[e] = x.get(e, true);
+        p = __builtin_fmaf(u[e], u[e], p);
+        p = __builtin_fmaf(v[e], v[e], p);
+      }
+      q += on[k] ? p : 0.0f;
     }
-    if constexpr (OP == kNorm) r = inverse_root(row_sum(q, a.lanes) * a.one_over_head + a.eps);
+    if constexpr (OP == kNorm) r = inverse_root(row_sum(q, lanes) * a.one_over_head + a.eps);
 #pragma unroll
     for (uint32_t e = 0; e < kE; ++e) {
       const float nu = OP == kNorm ? u[e] * (r * gu[e]) : u[e];
@@ -351,23 +372,29 @@ struct Row {
     y->set(u, v);
   }
   // dx from dy and x, and dy rotated back times x r into the gain's sums
-  __device__ __forceinline__ void backward(const Args& a, const Data& dy, const float* xu,
+  __device__ __forceinline__ void backward(const Args& a, uint32_t lanes, const Data& dy, const float* xu,
                                            const float* xv, const float* gu, const float* gv,
                                            const float* c, const float* s, float* su, float* sv,
                                            Data* dx) const {
     float du[kE], dv[kE], q = 0.0f, along = 0.0f;
 #pragma unroll
-    for (uint32_t e = 0; e < kE; ++e) {
-      const float u = dy.get(e, false), v = dy.get(e, true);
-      du[e] = __builtin_fmaf(u, c[e], v * s[e]);
-      dv[e] = __builtin_fmaf(v, c[e], -(u * s[e]));
-      q = __builtin_fmaf(xu[e], xu[e], q);
-      q = __builtin_fmaf(xv[e], xv[e], q);
-      along = __builtin_fmaf(du[e] * gu[e], xu[e], along);
-      along = __builtin_fmaf(dv[e] * gv[e], xv[e], along);
+    for (uint32_t k = 0; k < K; ++k) {
+      float p = 0.0f, l = 0.0f;
+#pragma unroll
+      for (uint32_t e = k * V; e < k * V + V; ++e) {
+        const float u = dy.get(e, false), v = dy.get(e, true);
+        du[e] = __builtin_fmaf(u, c[e], v * s[e]);
+        dv[e] = __builtin_fmaf(v, c[e], -(u * s[e]));
+        p = __builtin_fmaf(xu[e], xu[e], p);
+        p = __builtin_fmaf(xv[e], xv[e], p);
+        l = __builtin_fmaf(du[e] * gu[e], xu[e], l);
+        l = __builtin_fmaf(dv[e] * gv[e], xv[e], l);
+      }
+      q += on[k] ? p : 0.0f;
+      along += on[k] ? l : 0.0f;
     }
-    const float r = inverse_root(row_sum(q, a.lanes) * a.one_over_head + a.eps);
-    along = row_sum(along, a.lanes) * a.one_over_head * r * r;
+    const float r = inverse_root(row_sum(q, lanes) * a.one_over_head + a.eps);
+    along = row_sum(along, lanes) * a.one_over_head * r * r;
 #pragma unroll
     for (uint32_t e = 0; e < kE; ++e) {
       su[e] = __builtin_fmaf(du[e], xu[e] * r, su[e]);
@@ -426,13 +453,13 @@ struct Tokens {
 // / lanes rows at once, neighbouring heads of a token, kUnroll times over before
 // it works on the first.
 template <uint32_t DT, Op OP, uint32_t V, uint32_t K>
-__global__ __launch_bounds__(kBlock) void rows_kernel(Args a) {
+__global__ __launch_bounds__(kBlock, 4) void rows_kernel(Args a) {
   typedef Row<DT, V, K> R;
   typedef elem_t<DT> T;
   constexpr uint32_t kUnroll = V == 4 ? 2 : 1;
   extern __shared__ __align__(16) uint8_t lds[];
   const Tokens tok(a, lds);
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const R row(a, lane % a.lanes);
   const uint32_t at_once = 64 / a.lanes;
   const Part& P = a.part[blockIdx.y];
@@ -457,7 +484,6 @@ __global__ __launch_bounds__(kBlock) void rows_kernel(Args a) {
           in[i] = r < n * P.heads;
           t[i] = in[i] ? r / P.heads : 0;
           h[i] = in[i] ? r - t[i] * P.heads : 0;
-          if (!in[i]) continue;
           if (OP != kBack || !P.act)
             x[i].load(row, (const T*)P.x.p + tok.at[t[i] * 3] + h[i] * P.x.sh);
           if (OP == kBack)
@@ -481,7 +507,7 @@ __global__ __launch_bounds__(kBlock) void rows_kernel(Args a) {
             float xu[R::kE], xv[R::kE];
             const uint64_t bt = first + t[i], g = bt / ARK_ACT_GROUP;
             const auto kept = [&](uint32_t e, bool second) {
-              if (!row.has(e, second)) return 0.0f;
+              if (second && !row.has(e, second)) return 0.0f;
               const uint64_t col = g * columns + h[i] * a.head + row.at(e, second);
               return act_value(P.act[col * ARK_ACT_GROUP + bt % ARK_ACT_GROUP], act_up(exps[col]));
             };
@@ -494,11 +520,12 @@ __global__ __launch_bounds__(kBlock) void rows_kernel(Args a) {
 #pragma unroll
               for (uint32_t e = 0; e < R::kE; ++e) xu[e] = xv[e] = 0.0f;
             if (!in[i]) dy[i] = typename R::Data();
-            row.backward(a, dy[i], xu, xv, gu, gv, c, s, su, sv, &y);
+            row.backward(a, a.lanes, dy[i], xu, xv, gu, gv, c, s, su, sv, &y);
           } else {
-            row.template forward<OP>(a, x[i], gu, gv, c, s, &y);
+            row.template forward<OP>(a, a.lanes, x[i], gu, gv, c, s, &y);
           }
           if (in[i]) y.store(row, (T*)P.y.p + tok.at[t[i] * 3 + 2] + h[i] * P.y.sh);
+          if (OP == kBack) __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
@@ -520,8 +547,10 @@ struct Exps {
   uint32_t u = 0, v = 0;
   template <typename R>
   __device__ __forceinline__ void load(const R& row, const uint8_t* p) {
-    if (row.on[0]) u = bytes(p + row.eu[0]);
-    if (row.pairs_v[0]) v = bytes(p + row.ev[0]);
+    uint32_t a = row.eu[0], b = row.ev[0];
+    asm volatile("" : "+v"(a), "+v"(b));
+    u = bytes(p + a);
+    v = bytes(p + b);
     if (V > 1 && row.mixed) {  // in order to every other one and those between
       const uint64_t t = (uint64_t)v << (8 * V) | u;
       u = v = 0;
@@ -576,15 +605,16 @@ struct Exps {
 // tile, kIt rows a lane, neighbouring tokens, so that a column's largest
 // magnitude is its lanes' and its bytes a lane's are neighbours.
 template <uint32_t DT, bool BACK, uint32_t V, uint32_t kIt>
-__global__ __launch_bounds__(kBlock) void tiles_kernel(Args a) {
+__global__ __launch_bounds__(kBlock, V * kIt <= 16 ? (BACK ? 3 : 4) : V * kIt <= 32 && !BACK ? 3 : 2) void tiles_kernel(Args a) {
   typedef Row<DT, V, 1> R;
   typedef elem_t<DT> T;
   constexpr uint32_t kLanes = 2 * kIt;  // of a row: 64 / (32 / kIt)
   typedef uint32_t Bytes __attribute__((ext_vector_type(kIt / 4), aligned(4)));
   extern __shared__ __align__(16) uint8_t lds[];
   const Tokens tok(a, lds);
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, mine = lane / kLanes * kIt;
-  const R row(a, lane % kLanes);
+  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t mine = lane / kLanes * kIt;
+  R row(a, lane % kLanes);
   const uint64_t groups = (a.all + ARK_ACT_GROUP - 1) / ARK_ACT_GROUP;
   const Part& P = a.part[blockIdx.y];
   const uint64_t columns = (uint64_t)P.heads * a.head;
@@ -603,9 +633,9 @@ __global__ __launch_bounds__(kBlock) void tiles_kernel(Args a) {
         const Array& from = BACK ? P.dy : P.x;
 #pragma unroll
         for (uint32_t i = 0; i < kIt; ++i) {
-          in[i] = typename R::Data();
-          if (mine + i < n)
-            in[i].load(row, (const T*)from.p + tok.at[(mine + i) * 3 + BACK] + h * from.sh);
+          uint32_t t = min(mine + i, n - 1);
+          asm volatile("" : "+v"(t));
+          in[i].load(row, (const T*)from.p + tok.at[t * 3 + BACK] + h * from.sh);
         }
       };
       // the first head is on its way while the angles are formed
@@ -615,7 +645,8 @@ __global__ __launch_bounds__(kBlock) void tiles_kernel(Args a) {
       __syncthreads();
       for (uint32_t h = first_h; h < P.heads; h += a.slices * kWaves) {
         if (h != first_h) load(h);
-        uint8_t* const q = P.act + (g * columns + h * a.head) * ARK_ACT_GROUP + mine;
+        row.forget();
+        uint8_t* const q = P.act + (g * columns + h * a.head) * ARK_ACT_GROUP;
         uint8_t* const exps = P.act + groups * columns * ARK_ACT_GROUP + g * columns + h * a.head;
         Bytes b[R::kE][2];
         float up[R::kE][2];
@@ -625,14 +656,24 @@ __global__ __launch_bounds__(kBlock) void tiles_kernel(Args a) {
 #pragma unroll
           for (uint32_t k = 0; k < 2 * R::kE; ++k) {
             const bool second = k & 1;
-            b[k / 2][second] = Bytes();
-            if (row.has(k / 2, second))
-              b[k / 2][second] = *(const ARK_GLOBAL Bytes*)(q + row.at(k / 2, second) * ARK_ACT_GROUP);
-            up[k / 2][second] = row.has(k / 2, second) ? act_up(e.get(k / 2, second)) : 0.0f;
+            uint32_t c = V == 1 && second && !row.pairs_v[0] ? row.eu[0] : row.at(k / 2, second);
+            c = c * ARK_ACT_GROUP + mine;
+            asm volatile("" : "+v"(c));  // an offset from a scalar base, not an address kept
+            b[k / 2][second] = *(const ARK_GLOBAL Bytes*)(q + c);
+          }
+#pragma unroll
+          for (uint32_t k = 0; k < R::kE; ++k) {
+            up[k][0] = act_up(e.get(k, false));
+            up[k][1] = V == 1 && !row.pairs_v[0] ? 0.0f : act_up(e.get(k, true));
           }
         }
+        if (n < ARK_ACT_GROUP)  // tokens past the last: zeros in the 8-bit form and the sums
 #pragma unroll
-        for (uint32_t i = 0; i < kIt; ++i) in[i].sort(row);
+          for (uint32_t i = 0; i < kIt; ++i)
+            if (mine + i >= n) in[i] = typename R::Data();
+        if (row.mixed)
+#pragma unroll
+          for (uint32_t i = 0; i < kIt; ++i) in[i].sort(row);
         if constexpr (!BACK) {
           Exps<V> e;
           // the largest magnitudes of a lane's columns, as the types' bits order them
@@ -653,28 +694,36 @@ __global__ __launch_bounds__(kBlock) void tiles_kernel(Args a) {
             for (uint32_t i = 0; i < kIt; i += 4)
               w[i / 4] = act_bytes4(s, in[i].get(p, second), in[i + 1].get(p, second),
                                     in[i + 2].get(p, second), in[i + 3].get(p, second));
-            if (row.has(p, second)) *(ARK_GLOBAL Bytes*)(q + row.at(p, second) * ARK_ACT_GROUP) = w;
+            uint32_t c = row.at(p, second) * ARK_ACT_GROUP + mine;
+            asm volatile("" : "+v"(c));  // an offset from a scalar base, not an address kept
+            if (V > 1 ? row.on[0] : row.has(p, second)) *(ARK_GLOBAL Bytes*)(q + c) = w;
           }
           if (mine == 0) e.store(row, exps);
         }
 #pragma unroll
         for (uint32_t i = 0; i < kIt; ++i) {
-          const uint32_t t = mine + i;
+          uint32_t t = mine + i;
+          // read from LDS for every head again: kept in registers over all heads the
+          // lines would cost most of them
+          asm volatile("" : "+v"(t));
           float c[R::kE], s[R::kE];
           row.turn(tok.turns + (t < n ? t : 0) * (a.rotary / 2), c, s);
           typename R::Data y;
+          in[i].opaque();  // widened here, not with all the others
           if constexpr (BACK) {
             float xu[R::kE], xv[R::kE];
 #pragma unroll
             for (uint32_t e = 0; e < R::kE; ++e) {
+              asm volatile("" : "+v"(b[e][0][i / 4]), "+v"(b[e][1][i / 4]));
               xu[e] = act_value(b[e][0][i / 4] >> (i % 4 * 8) & 255u, up[e][0]);
               xv[e] = act_value(b[e][1][i / 4] >> (i % 4 * 8) & 255u, up[e][1]);
             }
-            row.backward(a, in[i], xu, xv, gu, gv, c, s, su, sv, &y);
+            row.backward(a, kLanes, in[i], xu, xv, gu, gv, c, s, su, sv, &y);
           } else {
-            row.template forward<kNorm>(a, in[i], gu, gv, c, s, &y);
+            row.template forward<kNorm>(a, kLanes, in[i], gu, gv, c, s, &y);
           }
           if (t < n) y.store(row, (T*)P.y.p + tok.at[t * 3 + 2] + h * P.y.sh);
+          __builtin_amdgcn_sched_barrier(0);  // one row at a time: registers for more waves
         }
       }
     }
