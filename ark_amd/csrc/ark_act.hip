@@ -65,18 +65,32 @@ __global__ __launch_bounds__(kLanes) void pack_kernel(const elem_t<DT>* __restri
   C top;
   top.v = most;
   uint8_t* out = q + (g * columns + c) * ARK_ACT_GROUP;
+  uint32_t s[N];
+  bool at_top = false;
 #pragma unroll
   for (uint32_t k = 0; k < N; ++k) {
-    const ActScale s = act_scale<DT>(__float_as_uint(top.get(k)));
-    u32x4 w[2];
-#pragma unroll
-    for (uint32_t i = 0; i < ARK_ACT_GROUP / 4; ++i)
-      w[i / 4][i % 4] = act_bytes4(s, v[4 * i].get(k), v[4 * i + 1].get(k), v[4 * i + 2].get(k),
-                                   v[4 * i + 3].get(k));
-    st_g<u32x4>(out + k * ARK_ACT_GROUP, w[0]);
-    st_g<u32x4>(out + k * ARK_ACT_GROUP + 16, w[1]);
-    st_g<uint8_t>(e + g * columns + c + k, (uint8_t)s.s);
+    s[k] = act_exponent<DT>(__float_as_uint(top.get(k)));
+    at_top |= s[k] >= kActTop<DT>;
+    st_g<uint8_t>(e + g * columns + c + k, (uint8_t)s[k]);
   }
+  const auto quantise = [&](auto hold) {
+#pragma unroll
+    for (uint32_t k = 0; k < N; ++k) {
+      const auto at = [&](uint32_t i) {
+        return decltype(hold)::value ? act_hold<DT>(s[k], v[i].get(k)) : v[i].get(k);
+      };
+      u32x4 w[2];
+#pragma unroll
+      for (uint32_t i = 0; i < ARK_ACT_GROUP / 4; ++i)
+        w[i / 4][i % 4] = act_bytes4(s[k], at(4 * i), at(4 * i + 1), at(4 * i + 2), at(4 * i + 3));
+      st_g<u32x4>(out + k * ARK_ACT_GROUP, w[0]);
+      st_g<u32x4>(out + k * ARK_ACT_GROUP + 16, w[1]);
+    }
+  };
+  if (__builtin_amdgcn_ballot_w64(at_top))
+    quantise(std::true_type());
+  else
+    quantise(std::false_type());
 }
 
 template <uint32_t DT, uint32_t N>
@@ -107,7 +121,7 @@ __global__ __launch_bounds__(kLanes) void unpack_kernel(const uint8_t* __restric
     float f[N];
 #pragma unroll
     for (uint32_t k = 0; k < N; ++k)
-      f[k] = act_value(w[k][i / 16][i / 4 % 4] >> (i % 4 * 8) & 255u, up[k]);
+      f[k] = act_value(w[k][i / 16][i / 4 % 4], i % 4, up[k]);
     typename C::V v;
 #pragma unroll
     for (uint32_t k = 0; k < C::kWords; ++k) {
@@ -132,10 +146,11 @@ __global__ __launch_bounds__(kLanes) void pack1_kernel(const elem_t<DT>* __restr
   const auto at = [&](uint32_t i) { return t0 + i < tokens ? (float)x[(t0 + i) * stride] : 0.0f; };
   for (uint32_t i = 0; i < ARK_ACT_GROUP; ++i)
     most = max(most, __float_as_uint(at(i)) & 0x7FFFFFFFu);
-  const ActScale s = act_scale<DT>(most);
+  const uint32_t s = act_exponent<DT>(most);
+  const auto held = [&](uint32_t i) { return act_hold<DT>(s, at(i)); };
   for (uint32_t i = 0; i < ARK_ACT_GROUP; i += 4)
-    st_g<uint32_t>(q + t0 + i, act_bytes4(s, at(i), at(i + 1), at(i + 2), at(i + 3)));
-  e[g] = (uint8_t)s.s;
+    st_g<uint32_t>(q + t0 + i, act_bytes4(s, held(i), held(i + 1), held(i + 2), held(i + 3)));
+  e[g] = (uint8_t)s;
 }
 template <uint32_t DT>
 __global__ __launch_bounds__(kLanes) void unpack1_kernel(const uint8_t* __restrict__ q,
@@ -144,7 +159,7 @@ __global__ __launch_bounds__(kLanes) void unpack1_kernel(const uint8_t* __restri
                                                          elem_t<DT>* __restrict__ x,
                                                          uint64_t stride) {
   const uint64_t t = (uint64_t)blockIdx.x * kLanes + threadIdx.x;
-  if (t < tokens) x[t * stride] = (elem_t<DT>)act_value(q[t], act_up(e[t / ARK_ACT_GROUP]));
+  if (t < tokens) x[t * stride] = (elem_t<DT>)act_value(q[t], 0, act_up(e[t / ARK_ACT_GROUP]));
 }
 
 // ---- the weight gradient -----------------------------------------------------

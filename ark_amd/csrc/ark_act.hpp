@@ -57,49 +57,46 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
 // `most` (sign clear): e + 133 for the smallest e with most <= 127 * 2^e, 255
 // when it is inf or NaN.  most = 1.f * 2^(E - 127) asks for e = E - 133 while
 // f <= 0x7E0000 (1.984375 = 127 / 64) and one more above it, which is what the
-// carry of adding 0x1FFFF to the bits does.
+// carry of adding 0x1FFFF to the bits does.  fp16's largest number gives 143, so
+// only there what is not finite needs no test of its own.
 template <uint32_t DT>
 __device__ __forceinline__ uint32_t act_exponent(uint32_t most) {
-  const uint32_t e = (most + 0x1FFFFu) >> 23;
-  constexpr uint32_t lo = DT == ARK_ACT_F16 ? 133u - 24u : 133u - 126u;
-  const uint32_t s = e < lo ? lo : e > 254u ? 254u : e;
+  if constexpr (DT == ARK_ACT_F16) return min(max((most + 0x1FFFFu) >> 23, 133u - 24u), 255u);
+  const uint32_t s = max((min(most, 0x7F7E0000u) + 0x1FFFFu) >> 23, 133u - 126u);
   return most >= 0x7F800000u ? 255u : s;
 }
 
-// 2^-e and 2^e of an exponent byte; NaN for 255.
-__device__ __forceinline__ float act_down(uint32_t s) {
-  return __uint_as_float(s == 255u ? 0x7FC00000u : (260u - s) << 23);
-}
+// 2^e of an exponent byte; NaN for 255.
 __device__ __forceinline__ float act_up(uint32_t s) {
   return __uint_as_float(s == 255u ? 0x7FC00000u : (s - 6u) << 23);
 }
 
-// What quantises a group: x 2^-e rounds to a whole number in the last place of
-// 1.5 * 2^23 + 128, whose low byte then is q + 128.  |x| is held to 127 * 2^e
-// first (63 * 2^10 at fp16's top exponent), which binds only where e is the
-// largest there is.  A group that is NaN gets bytes that mean nothing.
-struct ActScale {
-  uint32_t s;
-  float down, most;
-};
+// The largest exponent of a type, where |x| can pass the largest value there
+// (127 * 2^121, or 63 * 2^10 in fp16) and is held to it.
 template <uint32_t DT>
-__device__ __forceinline__ ActScale act_scale(uint32_t most) {
-  const uint32_t s = act_exponent<DT>(most);
-  return {s, act_down(s), act_up(s) * (DT == ARK_ACT_F16 && s >= 143u ? 63.0f : 127.0f)};
+constexpr uint32_t kActTop = DT == ARK_ACT_F16 ? 143u : 254u;
+template <uint32_t DT>
+__device__ __forceinline__ float act_hold(uint32_t s, float x) {
+  const float most = DT != ARK_ACT_F16 ? 0x1.FCp127f : s >= kActTop<DT> ? 64512.0f : 65536.0f;
+  return __builtin_amdgcn_fmed3f(x, -most, most);
 }
-// Four values' bytes, the first lowest.
-__device__ __forceinline__ uint32_t act_bytes4(const ActScale& a, float x0, float x1, float x2,
-                                               float x3) {
+
+// Four values' bytes under exponent byte s, the first lowest: x 2^-e rounds to a
+// whole number in the last place of 1.5 * 2^23 + 128, whose low byte then is
+// q + 128.  A group that is NaN gets bytes that mean nothing.
+__device__ __forceinline__ uint32_t act_bytes4(uint32_t s, float x0, float x1, float x2, float x3) {
+  const float down = __uint_as_float((260u - s) << 23);
   const auto one = [&](float x) {
-    return __float_as_uint(__builtin_fmaf(__builtin_amdgcn_fmed3f(x, -a.most, a.most), a.down,
-                                          12583040.0f));
+    return __float_as_uint(__builtin_fmaf(x, down, 12583040.0f));
   };
   const uint32_t lo = __builtin_amdgcn_perm(one(x1), one(x0), 0x0C0C0400u);
   const uint32_t hi = __builtin_amdgcn_perm(one(x3), one(x2), 0x04000C0Cu);
   return lo | hi;
 }
-__device__ __forceinline__ float act_value(uint32_t byte, float up) {
-  return (float)((int)byte - 128) * up;
+
+// Value i of a word of bytes: q 2^e.
+__device__ __forceinline__ float act_value(uint32_t word, uint32_t i, float up) {
+  return (float)(int8_t)((word ^ 0x80808080u) >> (8 * i)) * up;
 }
 
 }  // namespace dev

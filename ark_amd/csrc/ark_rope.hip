@@ -3,6 +3,7 @@
 #include <math.h>
 
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "ark_act.hpp"
@@ -38,6 +39,7 @@ struct Args {
   float magnitude, eps, one_over_head;
   uint32_t position_bytes, head, rotary, layout, inverse, gain_dtype;
   uint32_t lanes;         // of a row: a power of two
+  uint32_t line;          // pairs of a head, to a multiple of 4
   uint32_t tile;          // tokens a block takes at once
   uint32_t slices;        // tiles_kernel: blocks that share a group's heads
 };
@@ -107,13 +109,10 @@ __device__ __forceinline__ float row_sum(float v, uint32_t lanes) {
   return v;
 }
 
-// 1 / sqrt(a): the instruction's, within an ulp, and one Newton step.  An inf or
-// NaN, and 0 (a row of zeros without eps), stay what the instruction makes of them.
+// 1 / sqrt(a): the instruction's, within an ulp; it takes no subnormals.
 __device__ __forceinline__ float inverse_root(float a) {
-  const float r = __builtin_amdgcn_rsqf(a);
-  const float h = __builtin_fmaf(-0.5f * a * r, r, 0.5f);
-  const float n = __builtin_fmaf(r, h, r);
-  return n == n ? n : r;
+  const bool small = a < 0x1p-100f;
+  return __builtin_amdgcn_rsqf(small ? a * 0x1p100f : a) * (small ? 0x1p50f : 1.0f);
 }
 
 enum Op { kRope, kNorm, kBack };
@@ -222,10 +221,9 @@ struct Row {
   typedef elem_t<DT> T;
   uint32_t pair[K], eu[K], ev[K];
   bool on[K], pairs_v[K];
-  uint32_t half;
   bool mixed;  // interleaved
   __device__ __forceinline__ Row(const Args& a, uint32_t lane) {
-    half = a.rotary / 2;
+    const uint32_t half = a.rotary / 2;
     mixed = a.layout == ARK_ROPE_INTERLEAVED;
     const uint32_t rest = (a.head - a.rotary + 1) / 2;
 #pragma unroll
@@ -332,17 +330,15 @@ struct Row {
     }
   }
   // the pairs' cosines and sines from a token's line of the block's table
-  __device__ __forceinline__ void turn(const float2* line, float* c, float* s) const {
+  __device__ __forceinline__ void turn(const Args& a, const float* line, float* c, float* s) const {
+    typedef float F __attribute__((ext_vector_type(V)));
 #pragma unroll
-    for (uint32_t e = 0; e < kE; ++e) c[e] = 1.0f, s[e] = 0.0f;
+    for (uint32_t k = 0; k < K; ++k) {
+      const uint32_t p = on[k] ? pair[k] : 0;
+      const F x = *(const F*)(line + p), y = *(const F*)(line + a.line + p);
 #pragma unroll
-    for (uint32_t k = 0; k < K; ++k)
-      if (pair[k] < half)
-#pragma unroll
-        for (uint32_t i = 0; i < V; ++i) {
-          const float2 t = line[pair[k] + i];
-          c[k * V + i] = t.x, s[k * V + i] = t.y;
-        }
+      for (uint32_t i = 0; i < V; ++i) c[k * V + i] = x[i], s[k * V + i] = y[i];
+    }
   }
   // y = the rotation of x, or of x r gain
   template <Op OP>
@@ -405,13 +401,13 @@ struct Row {
     dx->set(du, dv);
   }
   // a wave's sums of the gain's gradient, its rows' lanes together, into LDS
-  __device__ __forceinline__ void gather(const Args& a, float* su, float* sv, float* out) const {
+  __device__ __forceinline__ void gather(const Args& a, uint32_t lanes, float* su, float* sv, float* out) const {
 #pragma unroll
     for (uint32_t e = 0; e < kE; ++e) {
-      if (a.lanes <= 8) su[e] += across<8>(su[e]), sv[e] += across<8>(sv[e]);
-      if (a.lanes <= 16) su[e] += across<16>(su[e]), sv[e] += across<16>(sv[e]);
-      if (a.lanes <= 32) su[e] += across<32>(su[e]), sv[e] += across<32>(sv[e]);
-      if (threadIdx.x % 64 < a.lanes) {
+      if (lanes <= 8) su[e] += across<8>(su[e]), sv[e] += across<8>(sv[e]);
+      if (lanes <= 16) su[e] += across<16>(su[e]), sv[e] += across<16>(sv[e]);
+      if (lanes <= 32) su[e] += across<32>(su[e]), sv[e] += across<32>(sv[e]);
+      if (threadIdx.x % 64 < lanes) {
         if (has(e, false)) out[at(e, false)] = su[e];
         if (has(e, true)) out[at(e, true)] = sv[e];
       }
@@ -419,14 +415,15 @@ struct Row {
   }
 };
 
-// What a block keeps of its tokens in LDS: their cosines and sines, one line of
-// rotary / 2 a token, and where each token starts in the part's x, dy and y.
+// What a block keeps of its tokens in LDS: the cosines and then the sines of a
+// head's pairs, those that do not turn among them, and where each token starts in
+// the part's x, dy and y.
 struct Tokens {
-  float2* turns;
+  float* turns;
   uint64_t* at;  // [token][x, dy, y]
   __device__ __forceinline__ Tokens(const Args& a, uint8_t* lds) {
     at = (uint64_t*)lds;
-    turns = (float2*)(lds + a.tile * 24);
+    turns = (float*)(lds + (a.tile * 24 + 15) / 16 * 16);
   }
   __device__ __forceinline__ void starts(const Args& a, const Part& p, uint64_t first,
                                          uint32_t n) const {
@@ -440,11 +437,16 @@ struct Tokens {
   }
   __device__ __forceinline__ void angles(const Args& a, uint64_t first, uint32_t n,
                                          bool back) const {
-    const uint32_t half = a.rotary / 2;
-    for (uint32_t i = threadIdx.x; i < n * half; i += kBlock) {
-      float s, c;
-      sincos_turns(phase_of(position_at(a, first + i / half), a.turns[i % half]), &s, &c);
-      turns[i] = make_float2(c * a.magnitude, s * (back ? -a.magnitude : a.magnitude));
+    for (uint32_t i = threadIdx.x; i < n * a.line; i += kBlock) {
+      const uint32_t t = i / a.line, p = i % a.line;
+      float s = 0.0f, c = 1.0f;
+      if (p < a.rotary / 2) {
+        sincos_turns(phase_of(position_at(a, first + t), a.turns[p]), &s, &c);
+        c *= a.magnitude;
+        s *= back ? -a.magnitude : a.magnitude;
+      }
+      turns[t * 2 * a.line + p] = c;
+      turns[t * 2 * a.line + a.line + p] = s;
     }
   }
 };
@@ -499,7 +501,7 @@ __global__ __launch_bounds__(kBlock, 4) void rows_kernel(Args a) {
 #pragma unroll
         for (uint32_t i = 0; i < kUnroll; ++i) {
           float c[R::kE], s[R::kE];
-          row.turn(tok.turns + t[i] * (a.rotary / 2), c, s);
+          row.turn(a, tok.turns + t[i] * 2 * a.line, c, s);
           if (OP != kBack || !P.act) x[i].sort(row);
           if (OP == kBack) dy[i].sort(row);
           typename R::Data y;
@@ -509,7 +511,7 @@ __global__ __launch_bounds__(kBlock, 4) void rows_kernel(Args a) {
             const auto kept = [&](uint32_t e, bool second) {
               if (second && !row.has(e, second)) return 0.0f;
               const uint64_t col = g * columns + h[i] * a.head + row.at(e, second);
-              return act_value(P.act[col * ARK_ACT_GROUP + bt % ARK_ACT_GROUP], act_up(exps[col]));
+              return act_value(P.act[col * ARK_ACT_GROUP + bt % ARK_ACT_GROUP], 0, act_up(exps[col]));
             };
 #pragma unroll
             for (uint32_t e = 0; e < R::kE; ++e) {
@@ -533,7 +535,7 @@ __global__ __launch_bounds__(kBlock, 4) void rows_kernel(Args a) {
   if constexpr (OP == kBack) {
     float* sum = (float*)lds;
     __syncthreads();
-    row.gather(a, su, sv, sum + wave * a.head);
+    row.gather(a, a.lanes, su, sv, sum + wave * a.head);
     __syncthreads();
     for (uint32_t j = threadIdx.x; j < a.head; j += kBlock)
       a.partial[((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.head + j] =
@@ -551,7 +553,11 @@ struct Exps {
     asm volatile("" : "+v"(a), "+v"(b));
     u = bytes(p + a);
     v = bytes(p + b);
-    if (V > 1 && row.mixed) {  // in order to every other one and those between
+  }
+  // in order to every other one and those between
+  template <typename R>
+  __device__ __forceinline__ void sort(const R& row) {
+    if (V > 1 && row.mixed) {
       const uint64_t t = (uint64_t)v << (8 * V) | u;
       u = v = 0;
 #pragma unroll
@@ -600,138 +606,176 @@ struct Exps {
   }
 };
 
-// The norm of 32 tokens of a head at a time, with the 8-bit form of its input:
-// written by the forward pass, read by the backward pass.  A wave holds the
-// tile, kIt rows a lane, neighbouring tokens, so that a column's largest
-// magnitude is its lanes' and its bytes a lane's are neighbours.
-template <uint32_t DT, bool BACK, uint32_t V, uint32_t kIt>
-__global__ __launch_bounds__(kBlock, V * kIt <= 16 ? (BACK ? 3 : 4) : V * kIt <= 32 && !BACK ? 3 : 2) void tiles_kernel(Args a) {
+// The norm with the 8-bit form of its input, 32 tokens of a head at a time:
+// written by the forward pass, read by the backward pass.  A lane holds kIt
+// neighbouring tokens of its columns, so that its bytes of a column are
+// neighbours.  In the forward pass a wave holds all 32 tokens, and a column's
+// largest magnitude is its lanes'; the backward pass has no need of that and
+// takes what kIt = 4 leaves of the head.  The next head is loaded while this one
+// is worked on.
+//
+// Waves of a unit's four SIMDs the registers are cut for, by the words a head's
+// share takes of a lane twice over: without spills.
+constexpr int tile_waves(bool back, uint32_t words) {
+  return back ? (words <= 16 ? 3 : 2) : words <= 16 ? 4 : words <= 32 ? 3 : words <= 64 ? 2 : 1;
+}
+template <uint32_t DT, bool BACK, uint32_t V, uint32_t kIt, uint32_t kLanes>
+__global__ __launch_bounds__(kBlock, tile_waves(BACK, V * kIt * (DT == ARK_ACT_F32 ? 2 : 1)))
+void tiles_kernel(Args a) {
   typedef Row<DT, V, 1> R;
   typedef elem_t<DT> T;
-  constexpr uint32_t kLanes = 2 * kIt;  // of a row: 64 / (32 / kIt)
+  constexpr uint32_t kTokens = 64 / kLanes * kIt;           // a wave's of a head
+  constexpr uint32_t kSubs = ARK_ACT_GROUP / kTokens;       // waves' shares of a group
+  static_assert(BACK || kSubs == 1, "the forward pass needs whole columns");
   typedef uint32_t Bytes __attribute__((ext_vector_type(kIt / 4), aligned(4)));
   extern __shared__ __align__(16) uint8_t lds[];
   const Tokens tok(a, lds);
   const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const uint32_t mine = lane / kLanes * kIt;
   R row(a, lane % kLanes);
   const uint64_t groups = (a.all + ARK_ACT_GROUP - 1) / ARK_ACT_GROUP;
   const Part& P = a.part[blockIdx.y];
   const uint64_t columns = (uint64_t)P.heads * a.head;
   float su[R::kE] = {}, sv[R::kE] = {}, gu[R::kE], gv[R::kE];
   if (P.heads) row.gains(a, P.gain, gu, gv);  // no heads: no gain
-  const uint32_t slice = blockIdx.x % a.slices;
+  const uint32_t units = P.heads * kSubs, slice = blockIdx.x % a.slices;
+  const uint32_t first_unit = slice * kWaves + wave, stride = a.slices * kWaves;
   for (uint64_t g = blockIdx.x / a.slices; g < groups; g += gridDim.x / a.slices) {
     const uint64_t first = g * ARK_ACT_GROUP;
     const uint32_t n = (uint32_t)(a.all - first < ARK_ACT_GROUP ? a.all - first : ARK_ACT_GROUP);
+    uint8_t* const values = P.act + g * columns * ARK_ACT_GROUP;
+    uint8_t* const exps = P.act + groups * columns * ARK_ACT_GROUP + g * columns;
+    // a unit as it is loaded
+    struct Held {
+      typename R::Data in[kIt];
+      Bytes b[R::kE][2];
+      Exps<V> e;
+    };
+    const auto mine_of = [&](uint32_t unit) {
+      return unit % kSubs * kTokens + lane / kLanes * kIt;
+    };
+    const auto load = [&](uint32_t unit, Held* held) {
+      const Array& from = BACK ? P.dy : P.x;
+      const uint32_t h = unit / kSubs, mine = mine_of(unit);
+      row.forget();
+#pragma unroll
+      for (uint32_t i = 0; i < kIt; ++i) {
+        uint32_t t = min(mine + i, n - 1);
+        asm volatile("" : "+v"(t));
+        held->in[i].load(row, (const T*)from.p + tok.at[t * 3 + BACK] + h * from.sh);
+      }
+      if constexpr (BACK) {
+        held->e.load(row, exps + h * a.head);
+#pragma unroll
+        for (uint32_t k = 0; k < 2 * R::kE; ++k) {
+          const bool second = k & 1;
+          uint32_t c = V == 1 && second && !row.pairs_v[0] ? row.eu[0] : row.at(k / 2, second);
+          c = c * ARK_ACT_GROUP + mine;
+          asm volatile("" : "+v"(c));  // an offset from a scalar base, not an address kept
+          held->b[k / 2][second] =
+              *(const ARK_GLOBAL Bytes*)(values + (uint64_t)h * a.head * ARK_ACT_GROUP + c);
+        }
+      }
+    };
+    Held now, next;
     __syncthreads();
     tok.starts(a, P, first, n);
     __syncthreads();
-    {
-      typename R::Data in[kIt];
-      const auto load = [&](uint32_t h) {
-        const Array& from = BACK ? P.dy : P.x;
+    // the first head is on its way while the angles are formed
+    if (first_unit < units) load(first_unit, &now);
+    tok.angles(a, first, n, false);
+    __syncthreads();
+    for (uint32_t unit = first_unit; unit < units; unit += stride) {
+      if (unit + stride < units) load(unit + stride, &next);
+      const uint32_t h = unit / kSubs, mine = mine_of(unit);
+      row.forget();
+      if (n < ARK_ACT_GROUP)  // tokens past the last: zeros in the 8-bit form and the sums
 #pragma unroll
-        for (uint32_t i = 0; i < kIt; ++i) {
-          uint32_t t = min(mine + i, n - 1);
-          asm volatile("" : "+v"(t));
-          in[i].load(row, (const T*)from.p + tok.at[t * 3 + BACK] + h * from.sh);
+        for (uint32_t i = 0; i < kIt; ++i)
+          if (mine + i >= n) now.in[i] = typename R::Data();
+      if (row.mixed)
+#pragma unroll
+        for (uint32_t i = 0; i < kIt; ++i) now.in[i].sort(row);
+      float up[R::kE][2];
+      if constexpr (BACK) {
+        now.e.sort(row);
+#pragma unroll
+        for (uint32_t k = 0; k < R::kE; ++k) {
+          up[k][0] = act_up(now.e.get(k, false));
+          up[k][1] = V == 1 && !row.pairs_v[0] ? 0.0f : act_up(now.e.get(k, true));
         }
-      };
-      // the first head is on its way while the angles are formed
-      const uint32_t first_h = slice * kWaves + wave;
-      if (first_h < P.heads) load(first_h);
-      tok.angles(a, first, n, false);
-      __syncthreads();
-      for (uint32_t h = first_h; h < P.heads; h += a.slices * kWaves) {
-        if (h != first_h) load(h);
-        row.forget();
-        uint8_t* const q = P.act + (g * columns + h * a.head) * ARK_ACT_GROUP;
-        uint8_t* const exps = P.act + groups * columns * ARK_ACT_GROUP + g * columns + h * a.head;
-        Bytes b[R::kE][2];
-        float up[R::kE][2];
-        if constexpr (BACK) {
-          Exps<V> e;
-          e.load(row, exps);
+      } else {
+        Exps<V> e;
+        // the largest magnitudes of a lane's columns, as the types' bits order them
+        typename R::Data most = typename R::Data();
 #pragma unroll
-          for (uint32_t k = 0; k < 2 * R::kE; ++k) {
-            const bool second = k & 1;
-            uint32_t c = V == 1 && second && !row.pairs_v[0] ? row.eu[0] : row.at(k / 2, second);
-            c = c * ARK_ACT_GROUP + mine;
-            asm volatile("" : "+v"(c));  // an offset from a scalar base, not an address kept
-            b[k / 2][second] = *(const ARK_GLOBAL Bytes*)(q + c);
-          }
+        for (uint32_t i = 0; i < kIt; ++i) most.larger(now.in[i]);
+        if (kLanes <= 8) most.template larger_across<8>();
+        if (kLanes <= 16) most.template larger_across<16>();
+        if (kLanes <= 32) most.template larger_across<32>();
+        bool at_top = false;
 #pragma unroll
-          for (uint32_t k = 0; k < R::kE; ++k) {
-            up[k][0] = act_up(e.get(k, false));
-            up[k][1] = V == 1 && !row.pairs_v[0] ? 0.0f : act_up(e.get(k, true));
-          }
+        for (uint32_t k = 0; k < 2 * R::kE; ++k) {
+          const uint32_t s = act_exponent<DT>(__float_as_uint(most.get(k / 2, k & 1)));
+          e.set(k / 2, k & 1, s);
+          at_top |= s >= kActTop<DT>;
         }
-        if (n < ARK_ACT_GROUP)  // tokens past the last: zeros in the 8-bit form and the sums
-#pragma unroll
-          for (uint32_t i = 0; i < kIt; ++i)
-            if (mine + i >= n) in[i] = typename R::Data();
-        if (row.mixed)
-#pragma unroll
-          for (uint32_t i = 0; i < kIt; ++i) in[i].sort(row);
-        if constexpr (!BACK) {
-          Exps<V> e;
-          // the largest magnitudes of a lane's columns, as the types' bits order them
-          typename R::Data most = typename R::Data();
-#pragma unroll
-          for (uint32_t i = 0; i < kIt; ++i) most.larger(in[i]);
-          if (kLanes <= 8) most.template larger_across<8>();
-          if (kLanes <= 16) most.template larger_across<16>();
-          if (kLanes <= 32) most.template larger_across<32>();
+        const auto quantise = [&](auto hold) {
 #pragma unroll
           for (uint32_t k = 0; k < 2 * R::kE; ++k) {
             const uint32_t p = k / 2;
             const bool second = k & 1;
-            const ActScale s = act_scale<DT>(__float_as_uint(most.get(p, second)));
-            e.set(p, second, s.s);
+            const auto at = [&](uint32_t i) {
+              const float f = now.in[i].get(p, second);
+              return decltype(hold)::value ? act_hold<DT>(e.get(p, second), f) : f;
+            };
             Bytes w;
 #pragma unroll
             for (uint32_t i = 0; i < kIt; i += 4)
-              w[i / 4] = act_bytes4(s, in[i].get(p, second), in[i + 1].get(p, second),
-                                    in[i + 2].get(p, second), in[i + 3].get(p, second));
+              w[i / 4] = act_bytes4(e.get(p, second), at(i), at(i + 1), at(i + 2), at(i + 3));
             uint32_t c = row.at(p, second) * ARK_ACT_GROUP + mine;
             asm volatile("" : "+v"(c));  // an offset from a scalar base, not an address kept
-            if (V > 1 ? row.on[0] : row.has(p, second)) *(ARK_GLOBAL Bytes*)(q + c) = w;
+            if (V > 1 ? row.on[0] : row.has(p, second))
+              *(ARK_GLOBAL Bytes*)(values + (uint64_t)h * a.head * ARK_ACT_GROUP + c) = w;
           }
-          if (mine == 0) e.store(row, exps);
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < kIt; ++i) {
-          uint32_t t = mine + i;
-          // read from LDS for every head again: kept in registers over all heads the
-          // lines would cost most of them
-          asm volatile("" : "+v"(t));
-          float c[R::kE], s[R::kE];
-          row.turn(tok.turns + (t < n ? t : 0) * (a.rotary / 2), c, s);
-          typename R::Data y;
-          in[i].opaque();  // widened here, not with all the others
-          if constexpr (BACK) {
-            float xu[R::kE], xv[R::kE];
-#pragma unroll
-            for (uint32_t e = 0; e < R::kE; ++e) {
-              asm volatile("" : "+v"(b[e][0][i / 4]), "+v"(b[e][1][i / 4]));
-              xu[e] = act_value(b[e][0][i / 4] >> (i % 4 * 8) & 255u, up[e][0]);
-              xv[e] = act_value(b[e][1][i / 4] >> (i % 4 * 8) & 255u, up[e][1]);
-            }
-            row.backward(a, kLanes, in[i], xu, xv, gu, gv, c, s, su, sv, &y);
-          } else {
-            row.template forward<kNorm>(a, kLanes, in[i], gu, gv, c, s, &y);
-          }
-          if (t < n) y.store(row, (T*)P.y.p + tok.at[t * 3 + 2] + h * P.y.sh);
-          __builtin_amdgcn_sched_barrier(0);  // one row at a time: registers for more waves
-        }
+        };
+        if (__builtin_amdgcn_ballot_w64(at_top))
+          quantise(std::true_type());
+        else
+          quantise(std::false_type());
+        if (mine == 0) e.store(row, exps + h * a.head);
       }
+#pragma unroll
+      for (uint32_t i = 0; i < kIt; ++i) {
+        uint32_t t = mine + i;
+        // read from LDS for every head again: kept in registers over all heads the
+        // lines would cost most of them
+        asm volatile("" : "+v"(t));
+        float c[R::kE], s[R::kE];
+        row.turn(a, tok.turns + min(t, n - 1) * 2 * a.line, c, s);
+        typename R::Data y;
+        now.in[i].opaque();  // widened here, not with all the others
+        if constexpr (BACK) {
+          float xu[R::kE], xv[R::kE];
+#pragma unroll
+          for (uint32_t e = 0; e < R::kE; ++e) {
+            asm volatile("" : "+v"(now.b[e][0][i / 4]), "+v"(now.b[e][1][i / 4]));
+            xu[e] = act_value(now.b[e][0][i / 4], i % 4, up[e][0]);
+            xv[e] = act_value(now.b[e][1][i / 4], i % 4, up[e][1]);
+          }
+          row.backward(a, kLanes, now.in[i], xu, xv, gu, gv, c, s, su, sv, &y);
+        } else {
+          row.template forward<kNorm>(a, kLanes, now.in[i], gu, gv, c, s, &y);
+        }
+        if (t < n) y.store(row, (T*)P.y.p + tok.at[t * 3 + 2] + h * P.y.sh);
+        __builtin_amdgcn_sched_barrier(0);  // one row at a time: registers for more waves
+      }
+      now = next;
     }
   }
   if constexpr (BACK) {
     float* sum = (float*)lds;
     __syncthreads();
-    row.gather(a, su, sv, sum + wave * a.head);
+    row.gather(a, kLanes, su, sv, sum + wave * a.head);
     __syncthreads();
     for (uint32_t j = threadIdx.x; j < a.head; j += kBlock)
       a.partial[((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.head + j] =
@@ -760,11 +804,13 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(Args a) {
     const uint32_t m = __float_as_uint(v[r]) & 0x7FFFFFFFu;
     most = m > most ? m : most;
   }
-  const ActScale s = act_scale<DT>(most);
+  const uint32_t s = act_exponent<DT>(most);
 #pragma unroll
   for (uint32_t r = 0; r < ARK_ACT_GROUP; r += 4)
-    st_g<uint32_t>(P.act + i * ARK_ACT_GROUP + r, act_bytes4(s, v[r], v[r + 1], v[r + 2], v[r + 3]));
-  P.act[groups * columns * ARK_ACT_GROUP + i] = (uint8_t)s.s;
+    st_g<uint32_t>(P.act + i * ARK_ACT_GROUP + r,
+                   act_bytes4(s, act_hold<DT>(s, v[r]), act_hold<DT>(s, v[r + 1]), act_hold<DT>(s, v[r + 2]),
+                              act_hold<DT>(s, v[r + 3])));
+  P.act[groups * columns * ARK_ACT_GROUP + i] = (uint8_t)s;
 }
 
 // The gains' gradients from the blocks' rows, added in order: 64 rows' runs by
@@ -818,30 +864,33 @@ void rows_of(const Shape2& w, dim3 grid, uint32_t lds, hipStream_t s, const Args
 }
 template <uint32_t DT, bool BACK>
 void tiles_of(const Shape2& w, dim3 grid, uint32_t lds, hipStream_t s, const Args& a) {
-#define ARK_TILES(V, L)                                                                  \
-  if (w.v == V && w.lanes == L)                                                          \
-    hipLaunchKernelGGL((tiles_kernel<DT, BACK, V, L / 2>), grid, dim3(kBlock), lds, s, a);
+#define ARK_TILES(V, L)                                                                      \
+  if (w.v == V && w.lanes == L)                                                              \
+    hipLaunchKernelGGL((tiles_kernel<DT, BACK, V, BACK ? 4 : L / 2, L>), grid, dim3(kBlock), lds, s, a);
   ARK_TILES(4, 8)
   ARK_TILES(4, 16)
   ARK_TILES(4, 32)
   ARK_TILES(2, 32)
   ARK_TILES(2, 64)
   ARK_TILES(1, 64)
+  if constexpr (BACK) {
+    ARK_TILES(4, 64)
+  }
 #undef ARK_TILES
 }
 
-// Rows of one line of the table kept small enough for eight blocks a unit.
+// A block's LDS for `tile` tokens, and for the sums of the gain's gradient.
+uint32_t block_lds(const Args& a, uint32_t tile) {
+  const uint32_t t = (tile * 24 + 15) / 16 * 16 + tile * 2 * a.line * 4, sum = kWaves * a.head * 4;
+  return t > sum ? t : sum;
+}
+// Tokens a block of rows_kernel takes: as many as keep its LDS small enough for
+// eight blocks a unit, but a thousand blocks before tokens share one.
 uint32_t rows_tile(const Args& a) {
-  const uint32_t line = 24 + a.rotary / 2 * 8;
-  uint32_t most = 16384 / line;
-  if (most > 32) most = 32;
-  // a thousand blocks before tokens share one
+  uint32_t most = 32;
+  while (most > 1 && block_lds(a, most) > 18 * 1024) --most;
   const uint64_t want = (a.all + 1023) / 1024;
   return want < 1 ? 1 : want < most ? (uint32_t)want : most;
-}
-uint32_t block_lds(const Args& a) {
-  const uint32_t t = a.tile * (24 + a.rotary / 2 * 8), sum = kWaves * a.head * 4;
-  return t > sum ? t : sum;
 }
 
 template <Op OP>
@@ -855,18 +904,19 @@ uint32_t launch_rows(uint32_t dtype, Args* a, hipStream_t s, bool launch = true)
   if (!launch || !blocks) return blocks;
   const dim3 grid(blocks, a->part[1].heads ? 2 : 1);
   if (dtype == ARK_ACT_F16)
-    rows_of<ARK_ACT_F16, OP>(w, grid, block_lds(*a), s, *a);
+    rows_of<ARK_ACT_F16, OP>(w, grid, block_lds(*a, a->tile), s, *a);
   else if (dtype == ARK_ACT_BF16)
-    rows_of<ARK_ACT_BF16, OP>(w, grid, block_lds(*a), s, *a);
+    rows_of<ARK_ACT_BF16, OP>(w, grid, block_lds(*a, a->tile), s, *a);
   else
-    rows_of<ARK_ACT_F32, OP>(w, grid, block_lds(*a), s, *a);
+    rows_of<ARK_ACT_F32, OP>(w, grid, block_lds(*a, a->tile), s, *a);
   return blocks;
 }
 
-// Whether a wave can hold 32 tokens of a head: at most 128 values a lane.
-bool tiles_fit(const Args& a) {
+// Whether a wave can hold 32 tokens of a head, at most 128 values a lane, or for
+// the backward pass four tokens a lane.
+bool tiles_fit(const Args& a, bool back) {
   const Shape2 w = row_shape(a.head, a.rotary);
-  return w.k == 1 && w.v * w.lanes <= 128;
+  return w.k == 1 && (back || w.v * w.lanes <= 128);
 }
 
 template <bool BACK>
@@ -877,7 +927,8 @@ uint32_t launch_tiles(uint32_t dtype, Args* a, hipStream_t s, bool launch = true
   const uint64_t groups = ark::act_groups(a->all);
   const uint32_t heads = a->part[0].heads > a->part[1].heads ? a->part[0].heads : a->part[1].heads;
   // blocks share a group's heads until there are about 500 of a part
-  uint32_t slices = (heads + kWaves - 1) / kWaves;
+  const uint32_t units = BACK ? heads * (w.lanes / 8) : heads;  // of a group
+  uint32_t slices = (units + kWaves - 1) / kWaves;
   while (slices > 1 && groups * (slices - 1) >= 512) --slices;
   a->slices = slices;
   uint64_t by = groups;
@@ -887,11 +938,11 @@ uint32_t launch_tiles(uint32_t dtype, Args* a, hipStream_t s, bool launch = true
   if (!launch || !blocks) return blocks;
   const dim3 grid(blocks, a->part[1].heads ? 2 : 1);
   if (dtype == ARK_ACT_F16)
-    tiles_of<ARK_ACT_F16, BACK>(w, grid, block_lds(*a), s, *a);
+    tiles_of<ARK_ACT_F16, BACK>(w, grid, block_lds(*a, a->tile), s, *a);
   else if (dtype == ARK_ACT_BF16)
-    tiles_of<ARK_ACT_BF16, BACK>(w, grid, block_lds(*a), s, *a);
+    tiles_of<ARK_ACT_BF16, BACK>(w, grid, block_lds(*a, a->tile), s, *a);
   else
-    tiles_of<ARK_ACT_F32, BACK>(w, grid, block_lds(*a), s, *a);
+    tiles_of<ARK_ACT_F32, BACK>(w, grid, block_lds(*a, a->tile), s, *a);
   return blocks;
 }
 
@@ -1091,6 +1142,7 @@ Args base_args(const ark_rope* r, uint64_t batch, uint64_t tokens, const void* p
   a.magnitude = r->magnitude;
   a.head = r->head;
   a.one_over_head = 1.0f / (float)r->head;
+  a.line = ((r->head + 1) / 2 + 3) / 4 * 4;
   a.rotary = r->rotary;
   a.layout = r->layout;
   return a;
@@ -1304,7 +1356,7 @@ int ark_rope_norm(const ark_rope* r, uint32_t dtype, uint64_t batch, uint64_t to
     most = acts[i] && values > most ? values : most;
   }
   // both parts' tiles and 8-bit forms in one pass, or each in its own
-  if (q_act && (k_act || !heads[1]) && tiles_fit(a)) {
+  if (q_act && (k_act || !heads[1]) && tiles_fit(a, false)) {
     launch_tiles<false>(dtype, &a, (hipStream_t)stream);
     ARK_HIP(hipGetLastError());
     return ARK_OPT_OK;
@@ -1391,7 +1443,7 @@ int ark_rope_norm_backward(const ark_rope* r, uint32_t dtype, uint64_t batch, ui
   ark::DeviceGuard guard(r->device);
   if (!guard.ok) return ark::fail(ARK_OPT_EHIP, "cannot select device %d", r->device);
   const hipStream_t st = (hipStream_t)stream;
-  const bool tiled = has[0] && q_act && (k_act || !has[1]) && tiles_fit(a);
+  const bool tiled = has[0] && q_act && (k_act || !has[1]) && tiles_fit(a, true);
   const uint32_t blocks = empty ? 0
                           : tiled ? launch_tiles<true>(dtype, &a, st, false)
                                   : launch_rows<kBack>(dtype, &a, st, false);
