@@ -7,6 +7,7 @@ fp32, written to or added into the gradients an optimizer steps on;
 ``unpack(kept)`` gives the values back.
 """
 import ctypes as C
+import functools
 
 import torch
 
@@ -65,7 +66,9 @@ def pack(x, out=None):
     p, stride = _rows(x, "x")
     t, c = x.shape
     if out is None:
-        out = Act8(t, c, x.dtype, x.device)
+        out = Act8(t, c, x.dtype,
+                   data=x.new_empty(-(-t // _abi.ACT_GROUP) * c * (_abi.ACT_GROUP + 1),
+                                    dtype=torch.uint8))
     elif (out.tokens, out.columns, out.dtype) != (t, c, x.dtype) or out.data.device != x.device:
         raise ValueError(f"out is {out.tokens} x {out.columns} {out.dtype}, x {t} x {c} {x.dtype}")
     check(lib().ark_act_pack(p, stride, code, t, c, out.data.data_ptr(), _stream(x)))
@@ -76,7 +79,7 @@ def unpack(kept, out=None):
     """The values of an Act8, in ``out`` (tokens x columns, rows of any stride)
     or a new tensor of the type they were packed from."""
     if out is None:
-        out = torch.empty((kept.tokens, kept.columns), dtype=kept.dtype, device=kept.data.device)
+        out = kept.data.new_empty((kept.tokens, kept.columns), dtype=kept.dtype)
     elif tuple(out.shape) != (kept.tokens, kept.columns) or out.device != kept.data.device:
         raise ValueError(f"out is {tuple(out.shape)}, the activation {kept.tokens} x "
                          f"{kept.columns}")
@@ -84,6 +87,13 @@ def unpack(kept, out=None):
     check(lib().ark_act_unpack(kept.data.data_ptr(), kept.tokens, kept.columns,
                                _code(out, "out"), p, stride, _stream(out)))
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace(tokens, columns, dy_stride, outputs):
+    need = C.c_uint64()
+    check(lib().ark_act_weight_grad_workspace(tokens, columns, dy_stride, outputs, C.byref(need)))
+    return need.value
 
 
 def weight_grad(kept, dy, dw=None, accumulate=False, layout="in_out"):
@@ -102,19 +112,17 @@ def weight_grad(kept, dy, dw=None, accumulate=False, layout="in_out"):
     if dw is None:
         if accumulate:
             raise ValueError("accumulate needs a dw")
-        dw = torch.empty(shape, dtype=torch.float32, device=dy.device)
+        dw = dy.new_empty(shape, dtype=torch.float32)
     elif tuple(dw.shape) != shape or dw.dtype != torch.float32 or dw.device != dy.device:
         raise ValueError(f"dw is {tuple(dw.shape)} {dw.dtype}, not {shape} float32")
     wp, wstride = _rows(dw, "dw")
     flags = (_abi.ACT_ACCUMULATE if accumulate else 0) | (
         _abi.ACT_TRANSPOSED if layout == "out_in" else 0)
-    need = C.c_uint64()
-    check(lib().ark_act_weight_grad_workspace(kept.tokens, kept.columns, dstride, n,
-                                              C.byref(need)))
+    need = _workspace(kept.tokens, kept.columns, dstride, n)
     # torch's allocator hands a stream's memory back to it without waiting
-    ws = torch.empty(need.value, dtype=torch.uint8, device=dy.device) if need.value else None
+    ws = dy.new_empty(need, dtype=torch.uint8) if need else None
     check(lib().ark_act_weight_grad_noalloc(
         kept.data.data_ptr(), _TYPES[kept.dtype], kept.tokens, kept.columns, dp, dstride,
-        _code(dy, "dy"), n, wp, wstride, flags, ws.data_ptr() if need.value else None, need.value,
+        _code(dy, "dy"), n, wp, wstride, flags, ws.data_ptr() if need else None, need,
         _stream(dy)))
     return dw

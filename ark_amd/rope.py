@@ -25,6 +25,11 @@ _SCALINGS = {"linear": (_abi.ROPE_SCALE_LINEAR, ("factor",), {}),
                        {"low": 1.0, "high": 4.0})}
 _U64x4 = C.c_uint64 * 4
 _POSITIONS = {torch.int32: 4, torch.int64: 8}
+_like = torch.empty_like
+
+
+def _meta(t):
+    return t.shape, t.stride(), t.dtype, t.get_device()
 
 
 def frequencies(rotary_dim, base=10000.0, scaling=None):
@@ -67,7 +72,7 @@ class Rope:
         elif scaling is not None or len(inv_freq) != rotary_dim // 2:
             raise ValueError("inv_freq holds one value a pair and takes no scaling")
         self._h = None
-        self._layouts = {}
+        self._plans = {}
         torch.cuda.current_device()
         h = C.c_void_p()
         check(lib().ark_rope_create(head_dim, rotary_dim, _LAYOUTS[layout],
@@ -91,69 +96,68 @@ class Rope:
     # ---- arguments --------------------------------------------------------
 
     def _layout(self, t, what):
-        """The layout of a query or key tensor as the library takes it, one for
-        every shape and strides met."""
-        key = t.shape, t.stride()
-        found = self._layouts.get(key)
-        if found is not None:
-            return found
-        (s, st), n = key, t.dim()
+        """The layout of a query or key tensor as the library takes it."""
+        s, st, n = t.shape, t.stride(), t.dim()
         if n not in (3, 4):
             raise ValueError(f"{what} has {n} dimensions: (batch,) tokens, heads, head_dim")
         if s[-1] != self.head_dim:
             raise ValueError(f"{what} is {tuple(s)}: its heads must have {self.head_dim} values")
         if st[-1] != 1 and s[-1] > 1:
             raise ValueError(f"{what}: the values of a head do not follow one another")
-        if len(self._layouts) >= 256:
-            self._layouts.clear()
-        found = self._layouts[key] = _U64x4(s[-2], st[0] if n == 4 else 0, st[-3], st[-2])
-        return found
+        return _U64x4(s[-2], st[0] if n == 4 else 0, st[-3], st[-2])
 
-    def _array(self, t, like, what):
-        """(address, layout) of a query or key tensor, whose sizes but the heads
-        must be those of ``like``."""
-        if t is not like and (t.shape[:-2] != like.shape[:-2] or t.dtype != like.dtype
-                              or t.device != like.device):
+    def _beside(self, t, like, what):
+        """The layout of a tensor whose sizes but the heads must be ``like``'s."""
+        if (t.shape[:-2] != like.shape[:-2] or t.dtype != like.dtype
+                or t.device != like.device):
             raise ValueError(f"{what} is {tuple(t.shape)} {t.dtype} on {t.device}, not "
                              f"{tuple(like.shape[:-2])} x heads x {self.head_dim} {like.dtype} on "
                              f"{like.device}")
-        return t.data_ptr(), self._layout(t, what)
+        return self._layout(t, what)
 
-    def _call(self, like, positions, start):
-        """The arguments every call begins with."""
-        code = _code(like, "q")
-        if not like.is_cuda:
-            raise ValueError(f"q is on {like.device}, not a GPU")
-        s = like.shape
-        if len(s) not in (3, 4):
-            raise ValueError(f"q has {len(s)} dimensions: (batch,) tokens, heads, head_dim")
-        batch, tokens = s[0] if len(s) == 4 else 1, s[-3]
-        if positions is None:
-            return self._h, code, batch, tokens, None, 0, start
-        size = _POSITIONS.get(positions.dtype)
-        if (size is None or positions.device != like.device or not positions.is_contiguous()
-                or positions.numel() != batch * tokens):
-            raise ValueError(f"positions must be {batch * tokens} contiguous int32 or int64 on "
-                             f"{like.device}")
-        return self._h, code, batch, tokens, positions.data_ptr(), size, start
-
-    def _gains(self, gq, gk, like):
-        code = _code(gq, "gain_q")
-        for g in (gq, gk):
-            if (g.dtype != gq.dtype or not g.is_contiguous() or g.numel() != self.head_dim
-                    or g.device != like.device):
-                raise ValueError(f"gains must be {self.head_dim} contiguous {gq.dtype} on "
-                                 f"{like.device}")
-        return gq.data_ptr(), gk.data_ptr(), code
-
-    def _out(self, t, out, what):
-        """(the result's tensor, its address, its layout)."""
-        if out is None:
-            out = torch.empty_like(t)
-            return out, out.data_ptr(), self._layout(out, what)
+    def _into(self, out, t, what):
+        """The layout of a result's tensor that the caller gives."""
         if out.shape != t.shape:
             raise ValueError(f"{what} is {tuple(out.shape)}, not {tuple(t.shape)}")
-        return out, *self._array(out, t, what)
+        return self._beside(out, t, what)
+
+    def _plan(self, q, k, positions, gains, key):
+        """What a call's sizes, strides and types come to, checked once for each
+        combination met: the numbers it begins with, the size of a position, the
+        gains' type, and the layouts of q and k and of new results for them."""
+        code = _code(q, "q")
+        if not q.is_cuda:
+            raise ValueError(f"q is on {q.device}, not a GPU")
+        lq = self._layout(q, "q")
+        batch, tokens = q.shape[0] if q.dim() == 4 else 1, q.shape[-3]
+        lk = None if k is None else self._beside(k, q, "k")
+        size = 0
+        if positions is not None:
+            size = _POSITIONS.get(positions.dtype)
+            if (size is None or positions.device != q.device or not positions.is_contiguous()
+                    or positions.numel() != batch * tokens):
+                raise ValueError(f"positions must be {batch * tokens} contiguous int32 or int64 "
+                                 f"on {q.device}")
+        gcode = None
+        if gains is not None:
+            gcode = _code(gains[0], "gain_q")
+            for g in gains:
+                if (g.dtype != gains[0].dtype or not g.is_contiguous()
+                        or g.numel() != self.head_dim or g.device != q.device):
+                    raise ValueError(f"gains must be {self.head_dim} contiguous "
+                                     f"{gains[0].dtype} on {q.device}")
+        if len(self._plans) >= 256:
+            self._plans.clear()
+        found = self._plans[key] = (
+            code, batch, tokens, size, gcode, lq, lk, self._layout(_like(q), "out"),
+            None if k is None else self._layout(_like(k), "out"))
+        return found
+
+    def _kept(self, a, like, rows, heads):
+        if ((a.tokens, a.columns, a.dtype) != (rows, heads * self.head_dim, like.dtype)
+                or a.data.device != like.device):
+            raise ValueError(f"kept is {a.tokens} x {a.columns} {a.dtype}, not {rows} x "
+                             f"{heads * self.head_dim} {like.dtype}")
 
     # ---- calls ------------------------------------------------------------
 
@@ -163,18 +167,33 @@ class Rope:
         pair with k; q itself to rotate in place) or new tensors.  inverse
         rotates back, as the gradients of the results are.  Returns the pair, or
         one tensor without k."""
-        head = self._call(q, positions, start)
-        qa = self._array(q, q, "q")
+        key = _meta(q), k if k is None else _meta(k), positions if positions is None else _meta(
+            positions)
+        code, batch, tokens, size, _, lq, lk, loq, lok = (
+            self._plans.get(key) or self._plan(q, k, positions, None, key))
+        pos = None if positions is None else positions.data_ptr()
+        flag = 1 if inverse else 0
         if k is None:
-            oq, *oa = self._out(q, out, "out")
-            check(lib().ark_rope_apply(*head, *qa, *oa, None, None, None, None, int(bool(inverse)),
-                                       _stream(q)))
-            return oq
+            if out is None:
+                out = _like(q)
+            else:
+                loq = self._into(out, q, "out")
+            check(lib().ark_rope_apply(self._h, code, batch, tokens, pos, size, start,
+                                       q.data_ptr(), lq, out.data_ptr(), loq, None, None, None,
+                                       None, flag, _stream(q)))
+            return out
         oq, ok = (None, None) if out is None else out
-        oq, *oa = self._out(q, oq, "out")
-        ok, *ob = self._out(k, ok, "out")
-        check(lib().ark_rope_apply(*head, *qa, *oa, *self._array(k, q, "k"), *ob,
-                                   int(bool(inverse)), _stream(q)))
+        if oq is None:
+            oq = _like(q)
+        else:
+            loq = self._into(oq, q, "out")
+        if ok is None:
+            ok = _like(k)
+        else:
+            lok = self._into(ok, k, "out")
+        check(lib().ark_rope_apply(self._h, code, batch, tokens, pos, size, start, q.data_ptr(),
+                                   lq, oq.data_ptr(), loq, k.data_ptr(), lk, ok.data_ptr(), lok,
+                                   flag, _stream(q)))
         return oq, ok
 
     def norm(self, q, k, gain_q, gain_k, positions=None, start=0, eps=1e-5, out=None,
@@ -184,32 +203,35 @@ class Rope:
         8-bit forms of q and k in the same pass, for norm_backward: True for new
         ones, or a pair of Act8 of batch * tokens rows.  Returns (q, k) or (q,
         k, kept_q, kept_k)."""
-        head = self._call(q, positions, start)
-        gains = self._gains(gain_q, gain_k, q)
-        qa, ka = self._array(q, q, "q"), self._array(k, q, "k")
+        key = (_meta(q), _meta(k), positions if positions is None else _meta(positions),
+               _meta(gain_q), _meta(gain_k))
+        code, batch, tokens, size, gcode, lq, lk, loq, lok = (
+            self._plans.get(key) or self._plan(q, k, positions, (gain_q, gain_k), key))
         oq, ok = (None, None) if out is None else out
-        oq, *oa = self._out(q, oq, "out")
-        ok, *ob = self._out(k, ok, "out")
-        if not keep8:
-            check(lib().ark_rope_norm(*head, eps, *gains, *qa, *oa, None, *ka, *ob, None,
-                                      _stream(q)))
-            return oq, ok
-        rows, d = head[2] * head[3], self.head_dim
-        if keep8 is True:
-            aq = Act8(rows, q.shape[-2] * d, q.dtype, q.device)
-            ak = Act8(rows, k.shape[-2] * d, q.dtype, q.device)
+        if oq is None:
+            oq = _like(q)
         else:
-            aq, ak = keep8
-            self._kept(aq, q, rows, q.shape[-2]), self._kept(ak, q, rows, k.shape[-2])
-        check(lib().ark_rope_norm(*head, eps, *gains, *qa, *oa, aq.data.data_ptr(), *ka, *ob,
-                                  ak.data.data_ptr(), _stream(q)))
-        return oq, ok, aq, ak
-
-    def _kept(self, a, like, rows, heads):
-        if ((a.tokens, a.columns, a.dtype) != (rows, heads * self.head_dim, like.dtype)
-                or a.data.device != like.device):
-            raise ValueError(f"kept is {a.tokens} x {a.columns} {a.dtype}, not {rows} x "
-                             f"{heads * self.head_dim} {like.dtype}")
+            loq = self._into(oq, q, "out")
+        if ok is None:
+            ok = _like(k)
+        else:
+            lok = self._into(ok, k, "out")
+        aq = ak = dq = dk = None
+        if keep8:
+            rows, d = batch * tokens, self.head_dim
+            if keep8 is True:
+                aq = Act8(rows, q.shape[-2] * d, q.dtype, q.device)
+                ak = Act8(rows, k.shape[-2] * d, q.dtype, q.device)
+            else:
+                aq, ak = keep8
+                self._kept(aq, q, rows, q.shape[-2]), self._kept(ak, q, rows, k.shape[-2])
+            dq, dk = aq.data.data_ptr(), ak.data.data_ptr()
+        check(lib().ark_rope_norm(self._h, code, batch, tokens,
+                                  None if positions is None else positions.data_ptr(), size, start,
+                                  eps, gain_q.data_ptr(), gain_k.data_ptr(), gcode, q.data_ptr(),
+                                  lq, oq.data_ptr(), loq, dq, k.data_ptr(), lk, ok.data_ptr(), lok,
+                                  dk, _stream(q)))
+        return (oq, ok, aq, ak) if keep8 else (oq, ok)
 
     def norm_backward(self, dq, dk, q, k, gain_q, gain_k, positions=None, start=0, eps=1e-5,
                       out=None, dgain_q=None, dgain_k=None, accumulate=False):
@@ -218,20 +240,25 @@ class Rope:
         ``out`` (a pair; dq and dk themselves for in place) or new tensors, and
         of the gains, float32, into dgain_q and dgain_k (added with accumulate)
         or new ones.  Returns (q_grad, k_grad, dgain_q, dgain_k)."""
-        head = self._call(dq, positions, start)
-        gains = self._gains(gain_q, gain_k, dq)
+        key = (_meta(dq), _meta(dk), positions if positions is None else _meta(positions),
+               _meta(gain_q), _meta(gain_k))
+        code, batch, tokens, size, gcode, lq, lk, loq, lok = (
+            self._plans.get(key) or self._plan(dq, dk, positions, (gain_q, gain_k), key))
+        oq, ok = (None, None) if out is None else out
         args, outs, grads = [], [], []
-        for dy, x, o, dgain in ((dq, q, None if out is None else out[0], dgain_q),
-                                (dk, k, None if out is None else out[1], dgain_k)):
-            args += self._array(dy, dq, "gradient")
+        for dy, ldy, x, o, lo, dgain in ((dq, lq, q, oq, loq, dgain_q),
+                                         (dk, lk, k, ok, lok, dgain_k)):
             if isinstance(x, Act8):
-                self._kept(x, dq, head[2] * head[3], dy.shape[-2])
-                args += [None, None, x.data.data_ptr()]
+                self._kept(x, dq, batch * tokens, dy.shape[-2])
+                args += dy.data_ptr(), ldy, None, None, x.data.data_ptr()
             else:
                 if x.shape != dy.shape:
                     raise ValueError(f"input is {tuple(x.shape)}, its gradient {tuple(dy.shape)}")
-                args += [*self._array(x, dq, "input"), None]
-            o, *oa = self._out(dy, o, "out")
+                args += dy.data_ptr(), ldy, x.data_ptr(), self._beside(x, dq, "input"), None
+            if o is None:
+                o = _like(dy)
+            else:
+                lo = self._into(o, dy, "out")
             if dgain is None:
                 if accumulate:
                     raise ValueError("accumulate needs dgain_q and dgain_k")
@@ -239,9 +266,11 @@ class Rope:
             elif (dgain.dtype != torch.float32 or not dgain.is_contiguous()
                   or dgain.numel() != self.head_dim or dgain.device != dq.device):
                 raise ValueError(f"dgain must be {self.head_dim} contiguous float32")
-            args += [*oa, dgain.data_ptr()]
+            args += o.data_ptr(), lo, dgain.data_ptr()
             outs.append(o)
             grads.append(dgain)
-        check(lib().ark_rope_norm_backward(*head, eps, *gains, *args, int(bool(accumulate)),
-                                           _stream(dq)))
+        check(lib().ark_rope_norm_backward(
+            self._h, code, batch, tokens, None if positions is None else positions.data_ptr(), size,
+            start, eps, gain_q.data_ptr(), gain_k.data_ptr(), gcode, *args, 1 if accumulate else 0,
+            _stream(dq)))
         return outs[0], outs[1], grads[0], grads[1]
