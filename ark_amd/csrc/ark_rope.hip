@@ -39,7 +39,6 @@ struct Args {
   float magnitude, eps, one_over_head;
   uint32_t position_bytes, head, rotary, layout, inverse, gain_dtype;
   uint32_t lanes;         // of a row: a power of two
-  uint32_t line;          // pairs of a head, to a multiple of 4
   uint32_t tile;          // tokens a block takes at once
   uint32_t slices;        // tiles_kernel: blocks that share a group's heads
 };
@@ -84,28 +83,39 @@ __device__ __forceinline__ float gain_at(const Args& a, const void* gain, uint32
   return ((const float*)gain)[j];
 }
 
-// The value of the lane that differs in one bit, 1 to 32.
-template <uint32_t BIT>
-__device__ __forceinline__ uint32_t across(uint32_t v) {
-  if constexpr (BIT == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, false);   // quad 1032
-  if constexpr (BIT == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, false);   // quad 2301
-  if constexpr (BIT == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, false);  // row_ror 8
-  if constexpr (BIT == 4 || BIT == 16) return __builtin_amdgcn_ds_swizzle(v, BIT << 10 | 0x1F);
-  return __shfl_xor(v, BIT);
+// op of a lane's value and that of the lane that differs in one bit, 1 to 32, in
+// both lanes; no bit needs LDS.  Bit 4 mirrors eight lanes, so it is for values
+// that already are the same in lanes that differ in bits 1 and 2.
+template <uint32_t BIT, typename F>
+__device__ __forceinline__ uint32_t fold(uint32_t v, F op) {
+  if constexpr (BIT >= 16) {
+    // two rows of 16 lanes (or of 32) change places: both rows then hold both values
+    const auto r = BIT == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false)
+                             : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return op(r[0], r[1]);
+  } else {
+    constexpr int kHow = BIT == 1 ? 0xB1     // quad 1 0 3 2
+                         : BIT == 2 ? 0x4E   // quad 2 3 0 1
+                         : BIT == 4 ? 0x141  // half row mirrored
+                                    : 0x128; // row turned by 8
+    return op(v, __builtin_amdgcn_mov_dpp(v, kHow, 0xF, 0xF, false));
+  }
 }
 template <uint32_t BIT>
-__device__ __forceinline__ float across(float v) {
-  return __uint_as_float(across<BIT>(__float_as_uint(v)));
+__device__ __forceinline__ float fold_sum(float v) {
+  return __uint_as_float(fold<BIT>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
 }
 
 // The sum over the lanes of a row, 8 to 64 of them, in every lane.
 __device__ __forceinline__ float row_sum(float v, uint32_t lanes) {
-  v += across<1>(v);
-  v += across<2>(v);
-  v += across<4>(v);
-  if (lanes >= 16) v += across<8>(v);
-  if (lanes >= 32) v += across<16>(v);
-  if (lanes == 64) v += across<32>(v);
+  v = fold_sum<1>(v);
+  v = fold_sum<2>(v);
+  v = fold_sum<4>(v);
+  if (lanes >= 16) v = fold_sum<8>(v);
+  if (lanes >= 32) v = fold_sum<16>(v);
+  if (lanes == 64) v = fold_sum<32>(v);
   return v;
 }
 
@@ -221,9 +231,10 @@ struct Row {
   typedef elem_t<DT> T;
   uint32_t pair[K], eu[K], ev[K];
   bool on[K], pairs_v[K];
+  uint32_t half;
   bool mixed;  // interleaved
   __device__ __forceinline__ Row(const Args& a, uint32_t lane) {
-    const uint32_t half = a.rotary / 2;
+    half = a.rotary / 2;
     mixed = a.layout == ARK_ROPE_INTERLEAVED;
     const uint32_t rest = (a.head - a.rotary + 1) / 2;
 #pragma unroll
@@ -298,8 +309,8 @@ struct Row {
       for (uint32_t k = 0; k < K; ++k)
 #pragma unroll
         for (uint32_t i = 0; i < Raw<DT, V>::kWords; ++i) {
-          u[k].w[i] = larger2(u[k].w[i], across<BIT>(u[k].w[i]));
-          v[k].w[i] = larger2(v[k].w[i], across<BIT>(v[k].w[i]));
+          u[k].w[i] = fold<BIT>(u[k].w[i], larger2);
+          v[k].w[i] = fold<BIT>(v[k].w[i], larger2);
         }
     }
     static __device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) {
@@ -329,16 +340,19 @@ struct Row {
       gv[e] = gain_at(a, g, has(e, true) ? at(e, true) : 0);
     }
   }
-  // the pairs' cosines and sines from a token's line of the block's table
-  __device__ __forceinline__ void turn(const Args& a, const float* line, float* c, float* s) const {
-    typedef float F __attribute__((ext_vector_type(V)));
+  // the pairs' cosines and sines from a token's line of the block's table; pairs
+  // past the rotary ones do not turn
+  __device__ __forceinline__ void turn(const float2* line, float* c, float* s) const {
 #pragma unroll
-    for (uint32_t k = 0; k < K; ++k) {
-      const uint32_t p = on[k] ? pair[k] : 0;
-      const F x = *(const F*)(line + p), y = *(const F*)(line + a.line + p);
+    for (uint32_t e = 0; e < kE; ++e) c[e] = 1.0f, s[e] = 0.0f;
 #pragma unroll
-      for (uint32_t i = 0; i < V; ++i) c[k * V + i] = x[i], s[k * V + i] = y[i];
-    }
+    for (uint32_t k = 0; k < K; ++k)
+      if (pair[k] < half)
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) {
+          const float2 t = line[pair[k] + i];
+          c[k * V + i] = t.x, s[k * V + i] = t.y;
+        }
   }
   // y = the rotation of x, or of x r gain
   template <Op OP>
@@ -404,9 +418,9 @@ struct Row {
   __device__ __forceinline__ void gather(const Args& a, uint32_t lanes, float* su, float* sv, float* out) const {
 #pragma unroll
     for (uint32_t e = 0; e < kE; ++e) {
-      if (lanes <= 8) su[e] += across<8>(su[e]), sv[e] += across<8>(sv[e]);
-      if (lanes <= 16) su[e] += across<16>(su[e]), sv[e] += across<16>(sv[e]);
-      if (lanes <= 32) su[e] += across<32>(su[e]), sv[e] += across<32>(sv[e]);
+      if (lanes <= 8) su[e] = fold_sum<8>(su[e]), sv[e] = fold_sum<8>(sv[e]);
+      if (lanes <= 16) su[e] = fold_sum<16>(su[e]), sv[e] = fold_sum<16>(sv[e]);
+      if (lanes <= 32) su[e] = fold_sum<32>(su[e]), sv[e] = fold_sum<32>(sv[e]);
       if (threadIdx.x % 64 < lanes) {
         if (has(e, false)) out[at(e, false)] = su[e];
         if (has(e, true)) out[at(e, true)] = sv[e];
@@ -415,15 +429,14 @@ struct Row {
   }
 };
 
-// What a block keeps of its tokens in LDS: the cosines and then the sines of a
-// head's pairs, those that do not turn among them, and where each token starts in
-// the part's x, dy and y.
+// What a block keeps of its tokens in LDS: their cosines and sines, one line of
+// rotary / 2 a token, and where each token starts in the part's x, dy and y.
 struct Tokens {
-  float* turns;
+  float2* turns;
   uint64_t* at;  // [token][x, dy, y]
   __device__ __forceinline__ Tokens(const Args& a, uint8_t* lds) {
     at = (uint64_t*)lds;
-    turns = (float*)(lds + (a.tile * 24 + 15) / 16 * 16);
+    turns = (float2*)(lds + a.tile * 24);
   }
   __device__ __forceinline__ void starts(const Args& a, const Part& p, uint64_t first,
                                          uint32_t n) const {
@@ -437,16 +450,11 @@ struct Tokens {
   }
   __device__ __forceinline__ void angles(const Args& a, uint64_t first, uint32_t n,
                                          bool back) const {
-    for (uint32_t i = threadIdx.x; i < n * a.line; i += kBlock) {
-      const uint32_t t = i / a.line, p = i % a.line;
-      float s = 0.0f, c = 1.0f;
-      if (p < a.rotary / 2) {
-        sincos_turns(phase_of(position_at(a, first + t), a.turns[p]), &s, &c);
-        c *= a.magnitude;
-        s *= back ? -a.magnitude : a.magnitude;
-      }
-      turns[t * 2 * a.line + p] = c;
-      turns[t * 2 * a.line + a.line + p] = s;
+    const uint32_t half = a.rotary / 2;
+    for (uint32_t i = threadIdx.x; i < n * half; i += kBlock) {
+      float s, c;
+      sincos_turns(phase_of(position_at(a, first + i / half), a.turns[i % half]), &s, &c);
+      turns[i] = make_float2(c * a.magnitude, s * (back ? -a.magnitude : a.magnitude));
     }
   }
 };
@@ -501,7 +509,7 @@ __global__ __launch_bounds__(kBlock, 4) void rows_kernel(Args a) {
 #pragma unroll
         for (uint32_t i = 0; i < kUnroll; ++i) {
           float c[R::kE], s[R::kE];
-          row.turn(a, tok.turns + t[i] * 2 * a.line, c, s);
+          row.turn(tok.turns + t[i] * (a.rotary / 2), c, s);
           if (OP != kBack || !P.act) x[i].sort(row);
           if (OP == kBack) dy[i].sort(row);
           typename R::Data y;
@@ -751,7 +759,7 @@ void tiles_kernel(Args a) {
         // lines would cost most of them
         asm volatile("" : "+v"(t));
         float c[R::kE], s[R::kE];
-        row.turn(a, tok.turns + min(t, n - 1) * 2 * a.line, c, s);
+        row.turn(tok.turns + min(t, n - 1) * (a.rotary / 2), c, s);
         typename R::Data y;
         now.in[i].opaque();  // widened here, not with all the others
         if constexpr (BACK) {
@@ -881,14 +889,14 @@ void tiles_of(const Shape2& w, dim3 grid, uint32_t lds, hipStream_t s, const Arg
 
 // A block's LDS for `tile` tokens, and for the sums of the gain's gradient.
 uint32_t block_lds(const Args& a, uint32_t tile) {
-  const uint32_t t = (tile * 24 + 15) / 16 * 16 + tile * 2 * a.line * 4, sum = kWaves * a.head * 4;
+  const uint32_t t = tile * (24 + a.rotary / 2 * 8), sum = kWaves * a.head * 4;
   return t > sum ? t : sum;
 }
-// Tokens a block of rows_kernel takes: as many as keep its LDS small enough for
+// Tokens a block of rows_kernel takes: as many as keep its lines small enough for
 // eight blocks a unit, but a thousand blocks before tokens share one.
 uint32_t rows_tile(const Args& a) {
-  uint32_t most = 32;
-  while (most > 1 && block_lds(a, most) > 18 * 1024) --most;
+  uint32_t most = 16384 / (24 + a.rotary / 2 * 8);
+  if (most > 32) most = 32;
   const uint64_t want = (a.all + 1023) / 1024;
   return want < 1 ? 1 : want < most ? (uint32_t)want : most;
 }
@@ -1142,7 +1150,6 @@ Args base_args(const ark_rope* r, uint64_t batch, uint64_t tokens, const void* p
   a.magnitude = r->magnitude;
   a.head = r->head;
   a.one_over_head = 1.0f / (float)r->head;
-  a.line = ((r->head + 1) / 2 + 3) / 4 * 4;
   a.rotary = r->rotary;
   a.layout = r->layout;
   return a;
