@@ -223,7 +223,7 @@ struct Mat<_Float16> {
   static __device__ __forceinline__ uint32_t shift(uint32_t top) {
     return top >= 143u ? 0u : 142u - top;
   }
-  // what LDS holds of an exponent byte: 2^(e + shift) twice (at least 2^-24)
+  // of an exponent byte: 2^(e + shift) twice (at least 2^-24)
   static __device__ __forceinline__ uint32_t scale(uint32_t s, uint32_t shift) {
     const uint32_t h = __builtin_bit_cast(
         uint16_t, (_Float16)(s == 255u ? act_up(s) : __uint_as_float((s - 6u + shift) << 23)));
@@ -255,16 +255,19 @@ struct Mat<__bf16> {
   static __device__ __forceinline__ uint32_t scale(uint32_t s, uint32_t) {
     return __float_as_uint(act_up(s));
   }
-  // q 2^e has at most 7 significant bits, so fp32's upper half is all of it
+  // q as in fp16's case, then q 2^e in fp32, whose upper half is all of its at
+  // most 7 significant bits
   static __device__ __forceinline__ Frag widen(u32x2 w, uint32_t scale) {
     const float s = __uint_as_float(scale);
+    const f16x2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
     u32x4 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t b = (i < 2 ? w.x : w.y) ^ 0x80808080u;
-      const float lo = (float)(int8_t)(b >> (i % 2 * 16)) * s;
-      const float hi = (float)(int8_t)(b >> (i % 2 * 16 + 8)) * s;
-      r[i] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+      const uint32_t b = i < 2 ? w.x : w.y;
+      const uint32_t u = __builtin_amdgcn_perm(0x64646464u, b, i % 2 ? 0x04030402u : 0x04010400u);
+      const f16x2 q = __builtin_bit_cast(f16x2, u) + off;
+      r[i] = __builtin_amdgcn_perm(__float_as_uint((float)q.y * s), __float_as_uint((float)q.x * s),
+                                   0x07060302u);
     }
     return __builtin_bit_cast(Frag, r);
   }
@@ -315,26 +318,23 @@ struct Tile {
   static constexpr uint32_t kLanes = 256 * WN;
   static constexpr uint32_t kM = 64 * MF, kN = 16 * NF * WN;
   static constexpr uint32_t kRow = kStep * 2;                    // bytes of an output of dy
-  static constexpr uint32_t kB = 0;                              // dy, then act, then scales
-  static constexpr uint32_t kA = kN * kRow;
-  static constexpr uint32_t kS = kA + kStepGroups * kM * ARK_ACT_GROUP;
-  static constexpr uint32_t kBytes = kS + kStepGroups * kM * 4;
-  static_assert(kBytes % kRow == 0, "a buffer starts at a multiple of a row");
+  static constexpr uint32_t kA = kN * kRow;                      // dy, then act, a column a row
+  static constexpr uint32_t kBytes = kA + kM * kRow;
+  static constexpr uint32_t kLds = 2 * kBytes;
   static constexpr uint32_t kWide = NF / 2;                      // outputs a lane stages of 8 tokens
-  static constexpr uint32_t kAAll = kStepGroups * kM * 2;        // 16-byte chunks of act
-  static constexpr uint32_t kAChunks = (kAAll + kLanes - 1) / kLanes;
-  static constexpr uint32_t kScales = kStepGroups * kM;
-  static constexpr uint32_t kSChunks = (kScales + kLanes - 1) / kLanes;
-  static constexpr uint32_t kTop = 2 * kBytes;                   // a column's largest exponent
-  static constexpr uint32_t kLds = kTop + kM * 4;
+  static constexpr uint32_t kAChunks = kM * (kStep / 8) / kLanes;  // of 8 tokens of act
+  static_assert(kAChunks * kLanes == kM * (kStep / 8), "whole chunks");
   static constexpr uint32_t kPhases = 2 * NF;                    // of MF products a step
   static constexpr uint32_t kAhead = NF >= 4 ? 3 : 1;            // dy's reads ahead of them
-  // dy lies in LDS as [output][token], 128 bytes an output, its 16-byte chunks (8
-  // tokens) permuted so that neither the eight lanes that write one chunk of
-  // outputs kWide apart nor the eight that read one chunk of neighbouring
-  // outputs meet in a bank: bits 2-4 of the output, bit 1 on top of bit 4.
+  // dy and act lie in LDS as rows of one output's or column's 64 tokens, a row's
+  // eight 16-byte chunks (8 tokens) permuted by its bits.  LDS takes 16-byte reads
+  // sixteen lanes at a time, of each 32 lanes 0-3, 12-15 and 20-27 and then the
+  // others, and writes eight neighbours at a time (measured: which pairs of lanes
+  // meet).  Reads are of 16 neighbouring rows, the second half of the lanes a chunk
+  // on; writes of one chunk of rows kWide apart, or of four chunks of two
+  // neighbours: with this permutation none of them meet in a bank.
   static __device__ __forceinline__ uint32_t swizzle(uint32_t n) {
-    return (n >> 2 & 7u) ^ (n >> 1 & 1u) << 2;
+    return ((n >> 1 & 3u) ^ (n >> 4 & 1u)) | ((n >> 3 ^ n) & 1u) << 2;
   }
 };
 
@@ -384,32 +384,31 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
   // products are never stored or meet dy's zeros.
   typedef Row<L::kWide> R;
   R rb[8];
-  u32x4 ra[L::kAChunks];
-  uint32_t rs[L::kSChunks], shift[L::kSChunks] = {};
-  uint32_t* top = (uint32_t*)(lds + L::kTop);
+  u32x2 ra[L::kAChunks];
+  uint32_t rs[L::kAChunks], shift[L::kAChunks] = {};
+  // the columns' largest exponents, in the second buffer until it is first used
+  uint32_t* top = (uint32_t*)(lds + L::kBytes);
   constexpr uint32_t kAcross = L::kN / L::kWide;  // lanes of a token
   const uint32_t b_row = tid / kAcross * 8, b_n = tid % kAcross * L::kWide;
   const bool edge = n0 + L::kN > a.outputs && a.outputs % L::kWide;
   const uint32_t b_col = n0 + b_n + L::kWide <= a.outputs ? n0 + b_n : a.outputs - L::kWide;
-  Off oa[L::kAChunks], os[L::kSChunks], ob = ((Off)b_row * (Off)a.dy_stride + b_col) * 2;  // bytes
-  // lanes past the last chunk stage it once more
-  const auto a_chunk = [&](uint32_t i) {
-    return min(tid + i * L::kLanes, L::kAAll - 1);
-  };
-  const auto s_chunk = [&](uint32_t i) { return min(tid + i * L::kLanes, L::kScales - 1); };
+  Off oe[L::kAChunks], ob = ((Off)b_row * (Off)a.dy_stride + b_col) * 2;  // bytes
+  // chunk i: four of a column's group of 32 tokens, the step's first group first
+  const auto a_group = [&](uint32_t i) { return (tid + i * L::kLanes) / (L::kM * 4); };
+  const auto a_col = [&](uint32_t i) { return (tid + i * L::kLanes) / 4 % L::kM; };
   const auto place = [&](uint32_t groups) {  // of the step
-    const auto at = [&](uint32_t g, uint32_t m) {
-      return (Off)(g < groups ? g : groups - 1) * a.columns + (m < a.columns ? m : a.columns - 1);
-    };
 #pragma unroll
     for (uint32_t i = 0; i < L::kAChunks; ++i) {
-      const uint32_t c = a_chunk(i), r = c % (L::kM * 2);
-      oa[i] = at(c / (L::kM * 2), m0 + r / 2) * ARK_ACT_GROUP + r % 2 * 16;
+      const uint32_t m = m0 + a_col(i);
+      oe[i] = (Off)min(a_group(i), groups - 1) * a.columns + min(m, a.columns - 1);
     }
-#pragma unroll
-    for (uint32_t i = 0; i < L::kSChunks; ++i)
-      os[i] = at(s_chunk(i) / L::kM, m0 + s_chunk(i) % L::kM);
   };
+  const auto a_off = [&](Off column) { return column * ARK_ACT_GROUP + tid % 4 * 8; };
+  uint32_t la[L::kAChunks];  // where they go in a buffer
+#pragma unroll
+  for (uint32_t i = 0; i < L::kAChunks; ++i)
+    la[i] = L::kA + a_col(i) * L::kRow +
+            (a_group(i) * 4 + tid % 4 ^ L::swizzle(a_col(i))) * 16;
   const auto load = [&](uint32_t step) {
     const char* dy = (const char*)(a.dy + (uint64_t)step * kStep * a.dy_stride);
     if (step + 1 < a.steps) {
@@ -427,9 +426,10 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
     const uint64_t g0 = (uint64_t)step * kStepGroups * a.columns;
     const char *q = (const char*)a.q + g0 * ARK_ACT_GROUP, *e = (const char*)a.e + g0;
 #pragma unroll
-    for (uint32_t i = 0; i < L::kAChunks; ++i) ra[i] = ld_g<u32x4>(q + oa[i]);
-#pragma unroll
-    for (uint32_t i = 0; i < L::kSChunks; ++i) rs[i] = ld_g<uint8_t>(e + os[i]);
+    for (uint32_t i = 0; i < L::kAChunks; ++i) {
+      ra[i] = ld_g<u32x2>(q + a_off(oe[i]));
+      rs[i] = ld_g<uint8_t>(e + oe[i]);
+    }
   };
   // LDS is addressed in bytes.
   const uint32_t base = (uint32_t)(uintptr_t)(ARK_LDS uint8_t*)lds;
@@ -441,10 +441,7 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
     *lds_at<u32x4>(buf + n * L::kRow + (b_row / 8 ^ L::swizzle(n)) * 16) = v;
   };
   const auto put_a = [&](uint32_t buf, uint32_t i) {
-    *lds_at<u32x4>(buf + L::kA + a_chunk(i) * 16) = ra[i];
-  };
-  const auto put_s = [&](uint32_t buf, uint32_t i) {
-    *lds_at<uint32_t>(buf + L::kS + s_chunk(i) * 4) = M::scale(rs[i], shift[i]);
+    *lds_at<typename M::Frag>(buf + la[i]) = M::widen(ra[i], M::scale(rs[i], shift[i]));
   };
   const auto store = [&](uint32_t buf, uint32_t step) {
     if (edge) {
@@ -462,14 +459,13 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
     for (uint32_t c = 0; c < L::kWide; ++c) put_b(buf, c);
 #pragma unroll
     for (uint32_t i = 0; i < L::kAChunks; ++i) put_a(buf, i);
-#pragma unroll
-    for (uint32_t i = 0; i < L::kSChunks; ++i) put_s(buf, i);
   };
 
   if (s0 < s1) {
     place(kStepGroups);
     load(s0);
   }
+  uint32_t back[MF] = {};  // the shifts of this lane's sums, a byte each
   if constexpr (M::kShift) {
     for (uint32_t i = tid; i < L::kM; i += L::kLanes) top[i] = 109;
     __syncthreads();
@@ -501,7 +497,12 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
     }
     __syncthreads();
 #pragma unroll
-    for (uint32_t i = 0; i < L::kSChunks; ++i) shift[i] = M::shift(top[s_chunk(i) % L::kM]);
+    for (uint32_t i = 0; i < L::kAChunks; ++i) shift[i] = M::shift(top[a_col(i)]);
+#pragma unroll
+    for (uint32_t i = 0; i < MF; ++i)
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k)
+        back[i] |= M::shift(top[(wm * MF + i) * 16 + (SWAP ? li : lg * 4 + k)]) << (8 * k);
   }
 
   f32x4 acc[MF][NF];
@@ -516,28 +517,18 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
   // the step's reads is done, before its last kAhead phases, which then read
   // the next step's first fragments.
   typename M::Frag b[L::kAhead + 1], x[2][MF];
-  u32x4 w[MF];
-  uint32_t sc[MF];
   const uint32_t b_first = wn * NF * 16 + li;
-  const uint32_t b_get = b_first * L::kRow + (lg * 2 ^ L::swizzle(b_first)) * 16;
-  const uint32_t a_m = wm * MF * 16 + li;
-  const uint32_t a_get = L::kA + (lg / 2 * L::kM + a_m) * ARK_ACT_GROUP + lg % 2 * 16;
-  const uint32_t s_get = L::kS + (lg / 2 * L::kM + a_m) * 4;
+  const uint32_t b_get = b_first * L::kRow + (lg ^ L::swizzle(b_first)) * 16;
+  const uint32_t a_first = wm * MF * 16 + li;
+  const uint32_t a_get = L::kA + a_first * L::kRow + (lg ^ L::swizzle(a_first)) * 16;
   const auto read_b = [&](uint32_t buf, uint32_t phase) {
     const uint32_t h = phase / NF, j = phase % NF;
-    // 16 outputs on, bit 4 turns over, and with it the swizzle's bit 2
+    // 16 rows on, bit 4 turns over, and with it the permutation's bit 0
     b[phase % (L::kAhead + 1)] = *lds_at<typename M::Frag>(
-        ((buf + b_get) ^ (h * 16 + j % 2 * 64)) + j * 16 * L::kRow);
+        ((buf + b_get) ^ (h * 64 + j % 2 * 16)) + j * 16 * L::kRow);
   };
-  const auto read_a = [&](uint32_t buf) {
-#pragma unroll
-    for (uint32_t i = 0; i < MF; ++i) {
-      w[i] = *lds_at<u32x4>(buf + a_get + i * 16 * ARK_ACT_GROUP);
-      sc[i] = *lds_at<uint32_t>(buf + s_get + i * 64);
-    }
-  };
-  const auto widen = [&](uint32_t h, uint32_t i) {
-    x[h][i] = M::widen(h ? u32x2{w[i].z, w[i].w} : u32x2{w[i].x, w[i].y}, sc[i]);
+  const auto read_a = [&](uint32_t buf, uint32_t h, uint32_t i) {
+    x[h][i] = *lds_at<typename M::Frag>(((buf + a_get) ^ (h * 64 + i % 2 * 16)) + i * 16 * L::kRow);
   };
   static_assert(L::kPhases % (L::kAhead + 1) == 0, "a step starts at b[0]");
   if (s0 < s1) {
@@ -546,13 +537,12 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
     __syncthreads();
 #pragma unroll
     for (uint32_t p = 0; p < L::kAhead; ++p) read_b(base, p);
-    read_a(base);
 #pragma unroll
-    for (uint32_t i = 0; i < MF; ++i) widen(0, i);
+    for (uint32_t i = 0; i < MF; ++i) read_a(base, 0, i);
   }
   // A plain step's stores and loads one at a time: what the chunk's registers
   // hold goes to the next step's buffer, and the chunk after it is asked for.
-  constexpr uint32_t kItemsB = L::kWide + 8, kItems = kItemsB + L::kAChunks + L::kSChunks;
+  constexpr uint32_t kItemsB = L::kWide + 8, kItems = kItemsB + L::kAChunks;
   const auto pass_on = [&](auto item, uint32_t buf, uint32_t step) {
     constexpr uint32_t k = decltype(item)::value;
     const uint64_t t0 = (uint64_t)step * kStep, g0 = (uint64_t)step * kStepGroups * a.columns;
@@ -563,18 +553,13 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
       Off o = ob;
       asm("" : "+v"(o));  // kept apart from the base, which then stays scalar
       rb[i].load((const char*)(a.dy + (t0 + i) * a.dy_stride) + o);
-    } else if constexpr (k < kItemsB + L::kAChunks) {
-      constexpr uint32_t i = k - kItemsB;
-      Off o = oa[i];
-      asm("" : "+v"(o));
-      put_a(buf, i);
-      ra[i] = ld_g<u32x4>((const char*)a.q + g0 * ARK_ACT_GROUP + o);
     } else {
-      constexpr uint32_t i = k - kItemsB - L::kAChunks;
-      Off o = os[i];
-      asm("" : "+v"(o));
-      put_s(buf, i);
-      rs[i] = ld_g<uint8_t>((const char*)a.e + g0 + o);
+      constexpr uint32_t i = k - kItemsB;
+      Off n = oe[i], o = a_off(n);
+      asm("" : "+v"(o), "+v"(n));
+      put_a(buf, i);
+      ra[i] = ld_g<u32x2>((const char*)a.q + g0 * ARK_ACT_GROUP + o);
+      rs[i] = ld_g<uint8_t>((const char*)a.e + g0 + n);
     }
   };
   const auto multiply = [&](uint32_t s, auto whole) {
@@ -588,7 +573,13 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
         read_b(cur, p + L::kAhead);
       else
         read_b(nxt, p + L::kAhead - L::kPhases);
-      if constexpr (p == kLast) read_a(nxt);
+      // act's fragments of the step's second group over its first phases, of the
+      // next step's first past the barrier
+#pragma unroll
+      for (uint32_t i = 0; i < MF; ++i) {
+        if (p == i * NF / (2 * MF)) read_a(cur, 1, i);
+        if (p == kLast) read_a(nxt, 0, i);
+      }
       if constexpr (kPlain) {
         each<kItems>([&](auto k) __attribute__((always_inline)) {
           if constexpr (p == k * kLast / kItems) pass_on(k, nxt, s + 2);
@@ -597,11 +588,6 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
         if (p == 0 && s + 1 < s1) store(nxt, s + 1);
         if (p == 1 && s + 2 < s1) load(s + 2);
       }
-      // the other half's fragments, over the last phases of this one's
-      constexpr uint32_t kOver = NF < MF ? NF : h == 1 && L::kAhead < MF ? L::kAhead : MF;
-#pragma unroll
-      for (uint32_t i = 0; i < MF; ++i)
-        if (j == NF - kOver + i * kOver / MF) widen(h ^ 1u, i);
 #pragma unroll
       for (uint32_t i = 0; i < MF; ++i)
         acc[i][j] = SWAP ? M::mul(b[p % (L::kAhead + 1)], x[h][i], acc[i][j])
@@ -621,8 +607,7 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
       f32x4 f;
 #pragma unroll
       for (uint32_t k = 0; k < 4; ++k) {
-        const uint32_t m = (wm * MF + i) * 16 + (SWAP ? li : lg * 4 + k);
-        f[k] = __uint_as_float((127u - M::shift(top[m])) << 23);
+        f[k] = __uint_as_float((127u - (back[i] >> (8 * k) & 255u)) << 23);
       }
 #pragma unroll
       for (uint32_t j = 0; j < NF; ++j) acc[i][j] *= f;
