@@ -229,19 +229,14 @@ struct Mat<_Float16> {
         uint16_t, (_Float16)(s == 255u ? act_up(s) : __uint_as_float((s - 6u + shift) << 23)));
     return h | h << 16;
   }
-  // eight bytes q + 128 -> q 2^e: the byte becomes the low mantissa of
-  // 1024 + q + 128, which fp16 holds, and both steps after it are exact
-  static __device__ __forceinline__ Frag widen(u32x2 w, uint32_t scale) {
-    const f16x2 s = __builtin_bit_cast(f16x2, scale);
+  // Two bytes q + 128 of a word, the lower or the upper, to q 2^e: the byte becomes
+  // the low mantissa of 1024 + q + 128, which fp16 holds, and both steps after it
+  // are exact.
+  static __device__ __forceinline__ uint32_t widen(uint32_t w, bool upper, uint32_t scale) {
     const f16x2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-    u32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t b = i < 2 ? w.x : w.y;
-      const uint32_t u = __builtin_amdgcn_perm(0x64646464u, b, i % 2 ? 0x04030402u : 0x04010400u);
-      r[i] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2, u) + off) * s);
-    }
-    return __builtin_bit_cast(Frag, r);
+    const uint32_t u = __builtin_amdgcn_perm(0x64646464u, w, upper ? 0x04030402u : 0x04010400u);
+    return __builtin_bit_cast(
+        uint32_t, (__builtin_bit_cast(f16x2, u) + off) * __builtin_bit_cast(f16x2, scale));
   }
 };
 template <>
@@ -257,19 +252,13 @@ struct Mat<__bf16> {
   }
   // q as in fp16's case, then q 2^e in fp32, whose upper half is all of its at
   // most 7 significant bits
-  static __device__ __forceinline__ Frag widen(u32x2 w, uint32_t scale) {
+  static __device__ __forceinline__ uint32_t widen(uint32_t w, bool upper, uint32_t scale) {
     const float s = __uint_as_float(scale);
     const f16x2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-    u32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t b = i < 2 ? w.x : w.y;
-      const uint32_t u = __builtin_amdgcn_perm(0x64646464u, b, i % 2 ? 0x04030402u : 0x04010400u);
-      const f16x2 q = __builtin_bit_cast(f16x2, u) + off;
-      r[i] = __builtin_amdgcn_perm(__float_as_uint((float)q.y * s), __float_as_uint((float)q.x * s),
-                                   0x07060302u);
-    }
-    return __builtin_bit_cast(Frag, r);
+    const uint32_t u = __builtin_amdgcn_perm(0x64646464u, w, upper ? 0x04030402u : 0x04010400u);
+    const f16x2 q = __builtin_bit_cast(f16x2, u) + off;
+    return __builtin_amdgcn_perm(__float_as_uint((float)q.y * s), __float_as_uint((float)q.x * s),
+                                 0x07060302u);
   }
 };
 
@@ -440,8 +429,13 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
     for (uint32_t k = 0; k < 4; ++k) v[k] = rb[2 * k].pair(rb[2 * k + 1], c);
     *lds_at<u32x4>(buf + n * L::kRow + (b_row / 8 ^ L::swizzle(n)) * 16) = v;
   };
-  const auto put_a = [&](uint32_t buf, uint32_t i) {
-    *lds_at<typename M::Frag>(buf + la[i]) = M::widen(ra[i], M::scale(rs[i], shift[i]));
+  // a chunk of act in five parts: four words widened, then put
+  u32x4 wide;
+  const auto put_a = [&](uint32_t buf, uint32_t i, uint32_t part) {
+    if (part < 4)
+      wide[part] = M::widen(part < 2 ? ra[i].x : ra[i].y, part % 2, M::scale(rs[i], shift[i]));
+    else
+      *lds_at<u32x4>(buf + la[i]) = wide;
   };
   const auto store = [&](uint32_t buf, uint32_t step) {
     if (edge) {
@@ -458,7 +452,7 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
 #pragma unroll
     for (uint32_t c = 0; c < L::kWide; ++c) put_b(buf, c);
 #pragma unroll
-    for (uint32_t i = 0; i < L::kAChunks; ++i) put_a(buf, i);
+    for (uint32_t i = 0; i < 5 * L::kAChunks; ++i) put_a(buf, i / 5, i % 5);
   };
 
   if (s0 < s1) {
@@ -540,24 +534,27 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
 #pragma unroll
     for (uint32_t i = 0; i < MF; ++i) read_a(base, 0, i);
   }
-  // A plain step's stores and loads one at a time: what the chunk's registers
-  // hold goes to the next step's buffer, and the chunk after it is asked for.
-  constexpr uint32_t kItemsB = L::kWide + 8, kItems = kItemsB + L::kAChunks;
-  const auto pass_on = [&](auto item, uint32_t buf, uint32_t step) {
+  // A plain step's staging one piece at a time: what a chunk's registers hold goes
+  // to the next step's buffer, and the chunk after it is asked for.
+  constexpr uint32_t kItemsB = L::kWide + 8, kItemsA = 5 * L::kAChunks;
+  const auto pass_on_b = [&](auto item, uint32_t buf, uint32_t step) {
     constexpr uint32_t k = decltype(item)::value;
-    const uint64_t t0 = (uint64_t)step * kStep, g0 = (uint64_t)step * kStepGroups * a.columns;
     if constexpr (k < L::kWide) {
       put_b(buf, k);
-    } else if constexpr (k < kItemsB) {
+    } else {
       constexpr uint32_t i = k - L::kWide;
       Off o = ob;
       asm("" : "+v"(o));  // kept apart from the base, which then stays scalar
-      rb[i].load((const char*)(a.dy + (t0 + i) * a.dy_stride) + o);
-    } else {
-      constexpr uint32_t i = k - kItemsB;
+      rb[i].load((const char*)(a.dy + ((uint64_t)step * kStep + i) * a.dy_stride) + o);
+    }
+  };
+  const auto pass_on_a = [&](auto item, uint32_t buf, uint32_t step) {
+    constexpr uint32_t i = decltype(item)::value / 5, part = decltype(item)::value % 5;
+    put_a(buf, i, part);
+    if constexpr (part == 4) {
+      const uint64_t g0 = (uint64_t)step * kStepGroups * a.columns;
       Off n = oe[i], o = a_off(n);
       asm("" : "+v"(o), "+v"(n));
-      put_a(buf, i);
       ra[i] = ld_g<u32x2>((const char*)a.q + g0 * ARK_ACT_GROUP + o);
       rs[i] = ld_g<uint8_t>((const char*)a.e + g0 + n);
     }
@@ -581,8 +578,11 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
         if (p == kLast) read_a(nxt, 0, i);
       }
       if constexpr (kPlain) {
-        each<kItems>([&](auto k) __attribute__((always_inline)) {
-          if constexpr (p == k * kLast / kItems) pass_on(k, nxt, s + 2);
+        each<kItemsB>([&](auto k) __attribute__((always_inline)) {
+          if constexpr (p == k * kLast / kItemsB) pass_on_b(k, nxt, s + 2);
+        });
+        each<kItemsA>([&](auto k) __attribute__((always_inline)) {
+          if constexpr (p == k * kLast / kItemsA) pass_on_a(k, nxt, s + 2);
         });
       } else {
         if (p == 0 && s + 1 < s1) store(nxt, s + 1);
@@ -593,6 +593,14 @@ __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
         acc[i][j] = SWAP ? M::mul(b[p % (L::kAhead + 1)], x[h][i], acc[i][j])
                          : M::mul(x[h][i], b[p % (L::kAhead + 1)], acc[i][j]);
       if constexpr (p + 1 == kLast) __syncthreads();
+      if constexpr (kPlain) {
+        // an instruction for the matrix unit, then as many as fit into its time
+#pragma unroll
+        for (uint32_t i = 0; i < MF; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+        }
+      }
       __builtin_amdgcn_sched_barrier(0);
     });
   };
@@ -751,13 +759,14 @@ struct Cut {
 };
 
 // Microseconds a step of 64 tokens takes a tile's block: alone on its compute
-// unit, and its share of a unit full of blocks (MI355X, fp16, 16384 tokens).
+// unit (256 tiles), and its share of a unit full of blocks (2048 tiles), both
+// with every unit busy (MI355X, 8192 tokens, the mean of fp16 and bf16).
 struct Pace {
   uint32_t mf, nf, wn;
   float alone, full;
 };
-constexpr Pace kPaces[] = {{3, 8, 2, 1.24f, 1.40f}, {3, 8, 1, 0.90f, 0.76f},
-                           {2, 4, 1, 0.60f, 0.39f}, {1, 4, 1, 0.47f, 0.25f}};
+constexpr Pace kPaces[] = {{3, 8, 2, 1.60f, 1.60f}, {3, 8, 1, 1.15f, 0.95f},
+                           {2, 4, 1, 0.74f, 0.45f}, {1, 4, 1, 0.59f, 0.27f}};
 
 // The cut expected to end first: the tile's pace times the blocks the fullest
 // of 256 compute units gets, and for splits a launch and the partial tiles'
