@@ -347,7 +347,7 @@ __device__ __forceinline__ void grad_out(const GradArgs& a, uint32_t m, uint32_t
 }
 
 // ANY: any stride and number of outputs; otherwise offsets inside a step fit 32
-// bits and there are eight outputs at least.
+// bits and there are four outputs at least.
 template <typename T, uint32_t MF, uint32_t NF, uint32_t WN, bool SWAP, bool ANY>
 __global__ __launch_bounds__(256 * WN, 2) void grad_kernel(GradArgs a) {
   typedef typename std::conditional<ANY, uint64_t, uint32_t>::type Off;
@@ -796,7 +796,7 @@ Cut cut_of(uint64_t tokens, uint64_t columns, uint64_t outputs, bool any) {
 // Offsets inside a step's rows of dy and act fit 32 bits, and a lane's four
 // outputs are there; other calls take the kernel that asks for neither.
 bool needs_any(uint64_t columns, uint64_t dy_stride, uint64_t outputs) {
-  return outputs < 4 || dy_stride >= (1u << 25) || columns >= (1u << 25);
+  return outputs < 4 || outputs >= (1u << 25) || dy_stride >= (1u << 25) || columns >= (1u << 25);
 }
 
 template <typename T, uint32_t MF, uint32_t NF, uint32_t WN, bool SWAP, bool ANY>
