@@ -12,10 +12,19 @@ import functools
 import torch
 
 from . import _abi
-from ._lib import check, lib, current_stream as _stream
+from ._lib import check, lib
 
 _TYPES = {torch.float16: _abi.ACT_F16, torch.bfloat16: _abi.ACT_BF16,
           torch.float32: _abi.ACT_F32}
+
+
+def _stream(t):
+    """torch's current HIP stream of t's device, as a number (by the call that is
+    not public where this torch has it: a Stream object costs as much as queueing
+    a kernel)."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    dev = t.get_device()
+    return raw(dev) if raw else torch.cuda.current_stream(dev).cuda_stream
 
 
 def _code(t, what):
@@ -54,6 +63,15 @@ class Act8:
             raise ValueError(f"data must be {n} contiguous uint8")
         self.tokens, self.columns, self.dtype, self.data = tokens, columns, dtype, data
 
+    @classmethod
+    def _of(cls, tokens, columns, like):
+        """A new one of the type and on the device of ``like``."""
+        self = cls.__new__(cls)
+        self.tokens, self.columns, self.dtype = tokens, columns, like.dtype
+        self.data = like.new_empty(-(-tokens // _abi.ACT_GROUP) * columns * (_abi.ACT_GROUP + 1),
+                                   dtype=torch.uint8)
+        return self
+
     @property
     def nbytes(self):
         return self.data.numel()
@@ -66,9 +84,7 @@ def pack(x, out=None):
     p, stride = _rows(x, "x")
     t, c = x.shape
     if out is None:
-        out = Act8(t, c, x.dtype,
-                   data=x.new_empty(-(-t // _abi.ACT_GROUP) * c * (_abi.ACT_GROUP + 1),
-                                    dtype=torch.uint8))
+        out = Act8._of(t, c, x)
     elif (out.tokens, out.columns, out.dtype) != (t, c, x.dtype) or out.data.device != x.device:
         raise ValueError(f"out is {out.tokens} x {out.columns} {out.dtype}, x {t} x {c} {x.dtype}")
     check(lib().ark_act_pack(p, stride, code, t, c, out.data.data_ptr(), _stream(x)))

@@ -13,8 +13,8 @@ import ctypes as C
 import torch
 
 from . import _abi
-from ._lib import check, lib, current_stream as _stream
-from .act import Act8, _code
+from ._lib import check, lib
+from .act import Act8, _code, _stream
 
 _LAYOUTS = {"half": _abi.ROPE_HALF, "interleaved": _abi.ROPE_INTERLEAVED}
 _SCALINGS = {"linear": (_abi.ROPE_SCALE_LINEAR, ("factor",), {}),
@@ -220,8 +220,7 @@ class Rope:
         if keep8:
             rows, d = batch * tokens, self.head_dim
             if keep8 is True:
-                aq = Act8(rows, q.shape[-2] * d, q.dtype, q.device)
-                ak = Act8(rows, k.shape[-2] * d, q.dtype, q.device)
+                aq, ak = Act8._of(rows, q.shape[-2] * d, q), Act8._of(rows, k.shape[-2] * d, q)
             else:
                 aq, ak = keep8
                 self._kept(aq, q, rows, q.shape[-2]), self._kept(ak, q, rows, k.shape[-2])
