@@ -957,7 +957,12 @@ uint32_t launch_tiles(uint32_t dtype, Args* a, hipStream_t s, bool launch = true
   while (slices > 1 && groups * (slices - 1) >= 512) --slices;
   a->slices = slices;
   uint64_t by = groups;
-  const uint32_t most = (BACK ? 2048u : 1u << 20) / slices;
+  // Backward, as many blocks as the units hold at once, three each: every block's
+  // row of the gains' gradients is one more to add up, and a last round of a few
+  // blocks would have the chip to itself (237M training pass 34.7 us, 37.6 with a
+  // block a group).
+  const uint32_t parts = a->part[1].heads ? 2 : 1;
+  const uint32_t held = 768 / parts / slices, most = !BACK ? 1u << 20 : held ? held : 1;
   if (by > most) by = most;
   const uint32_t blocks = (uint32_t)by * slices;
   if (!launch || !blocks) return blocks;
