@@ -909,12 +909,21 @@ uint32_t block_lds(const Args& a, uint32_t tile) {
   const uint32_t t = tile * (24 + a.rotary / 2 * 8), sum = kWaves * a.head * 4;
   return t > sum ? t : sum;
 }
-// Tokens a block of rows_kernel takes: as many as keep its lines small enough for
-// eight blocks a unit, but a thousand blocks before tokens share one.
-uint32_t rows_tile(const Args& a) {
+// Tokens a block of rows_kernel takes: a thousand blocks before tokens share one,
+// then as many as `turns` times what its waves take at once, and no more than keep
+// its lines small enough for eight blocks a unit.  More blocks that end sooner
+// keep reads and writes of different blocks side by side (32768 tokens of 16 + 16
+// heads of 128, bf16: rotated by four turns 99 us, by fifteen 120), but the norms'
+// gains and sums are set up once a block (8192 of 64 + 8 of 64: 40 us by four
+// turns, 37 by eight).
+uint32_t rows_tile(const Args& a, const Shape2& w, uint32_t turns) {
   uint32_t most = 16384 / (24 + a.rotary / 2 * 8);
   if (most > 32) most = 32;
+  const uint32_t heads = a.part[0].heads > a.part[1].heads ? a.part[0].heads : a.part[1].heads;
+  const uint32_t rows = 64 / w.lanes * kWaves * (w.v == 4 ? 2 : 1) * turns;
+  const uint32_t fill = rows <= heads ? 1 : rows / (heads ? heads : 1);
   const uint64_t want = (a.all + 1023) / 1024;
+  if (most > fill) most = fill;
   return want < 1 ? 1 : want < most ? (uint32_t)want : most;
 }
 
@@ -922,9 +931,13 @@ template <Op OP>
 uint32_t launch_rows(uint32_t dtype, Args* a, hipStream_t s, bool launch = true) {
   const Shape2 w = row_shape(a->head, a->rotary);
   a->lanes = w.lanes;
-  a->tile = rows_tile(*a);
+  a->tile = rows_tile(*a, w, OP == kRope ? 4 : 8);
   const uint64_t tiles = (a->all + a->tile - 1) / a->tile;
-  const uint32_t most = OP == kBack ? 1024 : 1u << 20;
+  // Backward, the units' fill of a part's blocks, fewer for long heads: their rows
+  // of the gains' gradients then need no memory of the stream's pool, whose host
+  // time is 33 us.
+  const uint32_t rows = 65536 / a->head;
+  const uint32_t most = OP != kBack ? 1u << 20 : rows < 512 ? 512 : rows < 1024 ? rows : 1024;
   const uint32_t blocks = (uint32_t)(tiles < most ? tiles : most);
   if (!launch || !blocks) return blocks;
   const dim3 grid(blocks, a->part[1].heads ? 2 : 1);
