@@ -522,8 +522,9 @@ __global__ __launch_bounds__(kBlock, 4) void rows_kernel(Args a) {
             dy[i].load(row, (const T*)P.dy.p + tok.at[t[i] * 3 + 1] + h[i] * P.dy.sh);
         }
       };
-      // the first rows are on their way while the angles are formed
-      load(wave * at_once);
+      // the first rows are on their way while the angles are formed; a part of no
+      // heads has no array to load from
+      if (P.heads) load(wave * at_once);
       tok.angles<1>(a, first, n, OP != kBack && a.inverse);
       __syncthreads();
       for (uint32_t r0 = wave * at_once; r0 < n * P.heads; r0 += kWaves * at_once * kUnroll) {

@@ -1,0 +1,65 @@
+"""Rotary positions and head norms (include/ark_rope.h) where a part has no
+heads: q or k of zero heads beside one that has some, or both.  A part without
+heads is no work, and its gain's gradient is zero (or stays as it was, when it
+is added to)."""
+import numpy as np
+import pytest
+
+from ark_amd import act
+from ark_amd.rope import Rope
+from tests.test_gpu_act import _f64, _torch
+from tests.test_gpu_rope import Turn, _back64, _gains, _norm64, _qk, _round_to
+
+pytestmark = pytest.mark.gpu
+
+
+def _near(got, want, bound, name="f32"):
+    """Within the bound; a NaN is not."""
+    assert (np.abs(_f64(got) - want) <= _round_to(bound, want, name)).all()
+
+
+@pytest.mark.parametrize("name,d,r", [("f16", 64, 64), ("bf16", 66, 66), ("f32", 256, 128),
+                                      ("f16", 510, 38), ("f32", 5, 4)])
+def test_q_of_no_heads(name, d, r):
+    torch = _torch()
+    rope = Rope(d, r)
+    gains = _gains(d, "f32")
+    for shape in ((1,), (40,), (2, 350)):
+        q, k = _qk(shape, 0, 3, d, name)
+        dq, dk = _qk(shape, 0, 3, d, name, 2)
+        turn = Turn(np.broadcast_to(np.arange(shape[-1]), shape), d, r, "half")
+        x, g = _f64(k), _f64(gains[1])
+        y = rope.apply(q, k)
+        assert y[0].shape == q.shape and torch.equal(y[1], rope.apply(k))
+        assert torch.equal(rope.apply(dq, dk, inverse=True)[1], rope.apply(dk, inverse=True))
+        yq, yk, aq, ak = rope.norm(q, k, *gains, keep8=True)
+        assert aq.nbytes == 0
+        _near(yk, *_norm64(x, g, turn), name)
+        _near(rope.norm(q, k, *gains)[1], *_norm64(x, g, turn), name)
+        for kept in ((q, k), (aq, ak)):
+            if kept[1] is ak:
+                x = _f64(act.unpack(ak)).reshape(k.shape)
+            back = rope.norm_backward(dq, dk, *kept, *gains)
+            dx, b, dg, gb = _back64(_f64(dk), x, g, turn, tuple(range(len(shape) + 1)))
+            _near(back[1], dx, b, name)
+            _near(back[3], dg, gb)
+            assert not back[2].any()
+            a, c = torch.full((d,), 5.0, device="cuda"), torch.zeros(d, device="cuda")
+            rope.norm_backward(dq, dk, *kept, *gains, dgain_q=a, dgain_k=c, accumulate=True)
+            assert (a == 5.0).all() and torch.equal(c, back[3])
+
+
+def test_neither_has_heads():
+    torch = _torch()
+    rope = Rope(64)
+    gains = _gains(64, "f32")
+    for shape in ((1,), (3, 50)):
+        q, k = _qk(shape, 0, 0, 64, "f16")
+        assert rope.apply(q, k)[1].shape == k.shape
+        for kept in ((q, k), rope.norm(q, k, *gains, keep8=True)[2:]):
+            a, b = torch.full((64,), 5.0, device="cuda"), torch.full((64,), 5.0, device="cuda")
+            rope.norm_backward(q, k, *kept, *gains, dgain_q=a, dgain_k=b)
+            assert not a.any() and not b.any()
+            a.fill_(3.0), b.fill_(3.0)
+            rope.norm_backward(q, k, *kept, *gains, dgain_q=a, dgain_k=b, accumulate=True)
+            assert (a == 3.0).all() and (b == 3.0).all()
