@@ -854,17 +854,18 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(Args a) {
   P.act[groups * columns * ARK_ACT_GROUP + i] = (uint8_t)s;
 }
 
-// The gains' gradients from the blocks' rows, added in order: 64 rows' runs by
-// the lanes of a column, then those.  4 us of latency for any number of rows met
+// The gains' gradients from the blocks' rows (none of a part that was not
+// launched), added in order: 64 rows' runs by the lanes of a column, then those.  4 us of latency for any number of rows met
 // here (384 blocks a part at most, or 1024 short heads').
 constexpr uint32_t kGainColumns = 16, kGainRuns = 64;
 __global__ __launch_bounds__(kGainColumns * kGainRuns) void gain_kernel(
-    const float* __restrict__ partial, uint32_t rows, uint32_t head, float* __restrict__ dq,
-    float* __restrict__ dk, uint32_t accumulate) {
+    const float* __restrict__ partial, uint32_t rows_q, uint32_t rows_k, uint32_t head,
+    float* __restrict__ dq, float* __restrict__ dk, uint32_t accumulate) {
   __shared__ float sum[kGainRuns][kGainColumns];
   const uint32_t c = threadIdx.x % kGainColumns, run = threadIdx.x / kGainColumns;
   const uint32_t j = blockIdx.x * kGainColumns + c;
-  const float* p = partial + (uint64_t)blockIdx.y * rows * head + j;
+  const float* p = partial + (blockIdx.y ? (uint64_t)rows_q * head : 0) + j;
+  const uint32_t rows = blockIdx.y ? rows_k : rows_q;
   float s = 0.0f;
   if (j < head)
 #pragma unroll 8
@@ -1518,8 +1519,8 @@ int ark_rope_norm_backward(const ark_rope* r, uint32_t dtype, uint64_t batch, ui
     ARK_HIP(hipGetLastError());
   }
   hipLaunchKernelGGL(gain_kernel, dim3((r->head + kGainColumns - 1) / kGainColumns, dk_layout ? 2 : 1),
-                     dim3(kGainColumns * kGainRuns), 0, st, (const float*)buf.p, blocks, r->head,
-                     dgain_q, dgain_k, accumulate);
+                     dim3(kGainColumns * kGainRuns), 0, st, (const float*)buf.p, blocks,
+                     has[1] ? blocks : 0, r->head, dgain_q, dgain_k, accumulate);
   ARK_HIP(hipGetLastError());
   return ARK_OPT_OK;
 }

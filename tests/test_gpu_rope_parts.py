@@ -63,3 +63,27 @@ def test_neither_has_heads():
             a.fill_(3.0), b.fill_(3.0)
             rope.norm_backward(q, k, *kept, *gains, dgain_q=a, dgain_k=b, accumulate=True)
             assert (a == 3.0).all() and (b == 3.0).all()
+
+
+@pytest.mark.parametrize("keep8", [False, True])
+@pytest.mark.parametrize("d", [64, 66, 256])
+@pytest.mark.parametrize("tokens", [1, 40, 700])
+def test_k_of_no_heads_has_a_gradient_of_zeros(tokens, d, keep8):
+    torch = _torch()
+    rope = Rope(d)
+    gains = _gains(d, "f32")
+    # both parts first: memory used before holds what they left
+    q, k = _qk((tokens,), 4, 2, d, "f16")
+    dq, dk = _qk((tokens,), 4, 2, d, "f16", 2)
+    want = rope.norm_backward(dq, dk, q, k, *gains)
+    none, dnone = k[:, :0], dk[:, :0]
+    kept = rope.norm(q, none, *gains, keep8=True)[2:] if keep8 else (q, none)
+    a, b = (torch.full((d,), 5.0, device="cuda") for _ in range(2))
+    got = rope.norm_backward(dq, dnone, *kept, *gains, dgain_q=a, dgain_k=b)
+    assert got[1].shape == (tokens, 0, d) and not b.any()
+    if not keep8:
+        assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+    b.fill_(5.0)
+    first = a.clone()
+    rope.norm_backward(dq, dnone, *kept, *gains, dgain_q=a, dgain_k=b, accumulate=True)
+    assert (b == 5.0).all() and torch.equal(a, first + first)
