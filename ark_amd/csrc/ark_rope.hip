@@ -381,8 +381,11 @@ struct Row {
     }
     y->set(u, v);
   }
-  // dx from dy and x, and dy rotated back times x r into the gain's sums
-  __device__ __forceinline__ void backward(const Args& a, uint32_t lanes, const Data& dy, const float* xu,
+  // dx from dy and x, and dy rotated back times x r into the gain's sums.  A row that
+  // is not `there` comes as zeros and adds nothing: without eps its 1 / rms is
+  // infinite, and is taken as 0
+  __device__ __forceinline__ void backward(const Args& a, uint32_t lanes, bool there,
+                                           const Data& dy, const float* xu,
                                            const float* xv, const float* gu, const float* gv,
                                            const float* c, const float* s, float* su, float* sv,
                                            Data* dx) const {
@@ -403,7 +406,8 @@ struct Row {
       q += on[k] ? p : 0.0f;
       along += on[k] ? l : 0.0f;
     }
-    const float r = inverse_root(row_sum(q, lanes) * a.one_over_head + a.eps);
+    const float root = inverse_root(row_sum(q, lanes) * a.one_over_head + a.eps);
+    const float r = there ? root : 0.0f;
     along = row_sum(along, lanes) * a.one_over_head * r * r;
 #pragma unroll
     for (uint32_t e = 0; e < kE; ++e) {
@@ -553,7 +557,7 @@ __global__ __launch_bounds__(kBlock, 4) void rows_kernel(Args a) {
 #pragma unroll
               for (uint32_t e = 0; e < R::kE; ++e) xu[e] = xv[e] = 0.0f;
             if (!in[i]) dy[i] = typename R::Data();
-            row.backward(a, a.lanes, dy[i], xu, xv, gu, gv, c, s, su, sv, &y);
+            row.backward(a, a.lanes, in[i], dy[i], xu, xv, gu, gv, c, s, su, sv, &y);
           } else {
             row.template forward<OP>(a, a.lanes, x[i], gu, gv, c, s, &y);
           }
@@ -802,7 +806,7 @@ void tiles_kernel(Args a) {
             xu[e] = act_value(now.b[e][0][i / 4], i % 4, up[e][0]);
             xv[e] = act_value(now.b[e][1][i / 4], i % 4, up[e][1]);
           }
-          row.backward(a, kLanes, now.in[i], xu, xv, gu, gv, c, s, su, sv, &y);
+          row.backward(a, kLanes, t < n, now.in[i], xu, xv, gu, gv, c, s, su, sv, &y);
         } else {
           row.template forward<kNorm>(a, kLanes, now.in[i], gu, gv, c, s, &y);
         }
