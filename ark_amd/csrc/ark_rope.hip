@@ -20,7 +20,8 @@ struct Array {
   uint64_t sb, st, sh;
 };
 
-// One of a call's two tensors, q or k.
+// One of a call's two tensors, q or k; of the two, those that have heads, the
+// first of them first.  Kernels are launched for no others.
 struct Part {
   Array x;           // the input; for the backward pass the norm's input
   Array dy;          // backward: the gradient of the output
@@ -501,7 +502,7 @@ __global__ __launch_bounds__(kBlock, 4) void rows_kernel(Args a) {
   const Part& P = a.part[blockIdx.y];
   const uint64_t columns = (uint64_t)P.heads * a.head;
   float su[R::kE] = {}, sv[R::kE] = {}, gu[R::kE], gv[R::kE];
-  if (OP != kRope && P.heads) row.gains(a, P.gain, gu, gv);  // no heads: no gain
+  if (OP != kRope) row.gains(a, P.gain, gu, gv);
   for (uint64_t first = (uint64_t)blockIdx.x * a.tile; first < a.all;
        first += (uint64_t)gridDim.x * a.tile) {
     const uint32_t n = (uint32_t)(a.all - first < a.tile ? a.all - first : a.tile);
@@ -526,9 +527,8 @@ __global__ __launch_bounds__(kBlock, 4) void rows_kernel(Args a) {
             dy[i].load(row, (const T*)P.dy.p + tok.at[t[i] * 3 + 1] + h[i] * P.dy.sh);
         }
       };
-      // the first rows are on their way while the angles are formed; a part of no
-      // heads has no array to load from
-      if (P.heads) load(wave * at_once);
+      // the first rows are on their way while the angles are formed
+      load(wave * at_once);
       tok.angles<1>(a, first, n, OP != kBack && a.inverse);
       __syncthreads();
       for (uint32_t r0 = wave * at_once; r0 < n * P.heads; r0 += kWaves * at_once * kUnroll) {
@@ -680,7 +680,7 @@ void tiles_kernel(Args a) {
   const Part& P = a.part[blockIdx.y];
   const uint64_t columns = (uint64_t)P.heads * a.head;
   float su[R::kE] = {}, sv[R::kE] = {}, gu[R::kE], gv[R::kE];
-  if (P.heads) row.gains(a, P.gain, gu, gv);  // no heads: no gain
+  row.gains(a, P.gain, gu, gv);
   const uint32_t units = P.heads * kSubs, slice = blockIdx.x % a.slices;
   const uint32_t first_unit = slice * kWaves + wave, stride = a.slices * kWaves;
   for (uint64_t g = blockIdx.x / a.slices; g < groups; g += gridDim.x / a.slices) {
@@ -858,9 +858,9 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(Args a) {
   P.act[groups * columns * ARK_ACT_GROUP + i] = (uint8_t)s;
 }
 
-// The gains' gradients from the blocks' rows (none of a part that was not
-// launched), added in order: 64 rows' runs by the lanes of a column, then those.  4 us of latency for any number of rows met
-// here (384 blocks a part at most, or 1024 short heads').
+// The gains' gradients from the blocks' rows (none of a part of no heads), added in
+// order: 64 rows' runs by the lanes of a column, then those.  4 us of latency for
+// any number of rows met here (384 blocks a part at most, or 1024 short heads').
 constexpr uint32_t kGainColumns = 16, kGainRuns = 64;
 __global__ __launch_bounds__(kGainColumns * kGainRuns) void gain_kernel(
     const float* __restrict__ partial, uint32_t rows_q, uint32_t rows_k, uint32_t head,
@@ -1356,11 +1356,13 @@ int ark_rope_apply(const ark_rope* r, uint32_t dtype, uint64_t batch, uint64_t t
   if ((rc = check_apart(g, 4, in_place, f, 1, s)) || (rc = check_memory(g, 4, f, 1))) return rc;
   Args a = base_args(r, batch, tokens, positions, position_bytes, start);
   a.inverse = inverse != 0;
+  Part* part = a.part;
   for (int i = 0; i < 2; ++i) {
     if (!heads[i]) continue;
-    a.part[i].x = array_of(g[2 * i + 1]);
-    a.part[i].y = array_of(g[2 * i]);
-    a.part[i].heads = heads[i];
+    part->x = array_of(g[2 * i + 1]);
+    part->y = array_of(g[2 * i]);
+    part->heads = heads[i];
+    ++part;
   }
   ark::DeviceGuard guard(r->device);
   if (!guard.ok) return ark::fail(ARK_OPT_EHIP, "cannot select device %d", r->device);
@@ -1411,24 +1413,28 @@ int ark_rope_norm(const ark_rope* r, uint32_t dtype, uint64_t batch, uint64_t to
   uint64_t most = 0;
   ark::DeviceGuard guard(r->device);
   if (!guard.ok) return ark::fail(ARK_OPT_EHIP, "cannot select device %d", r->device);
+  bool all_kept = true;
+  Part* part = a.part;
   for (int i = 0; i < 2; ++i) {
     if (!heads[i]) continue;
-    a.part[i].x = array_of(g[2 * i + 1]);
-    a.part[i].y = array_of(g[2 * i]);
-    a.part[i].heads = heads[i];
-    a.part[i].gain = gains[i];
-    a.part[i].act = (uint8_t*)acts[i];
+    part->x = array_of(g[2 * i + 1]);
+    part->y = array_of(g[2 * i]);
+    part->heads = heads[i];
+    part->gain = gains[i];
+    part->act = (uint8_t*)acts[i];
+    all_kept = all_kept && acts[i];
     const uint64_t values = ark::act_groups(n) * heads[i] * r->head;
     most = acts[i] && values > most ? values : most;
+    ++part;
   }
   // both parts' tiles and 8-bit forms in one pass, or each in its own
-  if (q_act && (k_act || !heads[1]) && tiles_fit(a, false)) {
+  if (all_kept && tiles_fit(a, false)) {
     launch_tiles<false>(dtype, &a, (hipStream_t)stream);
     ARK_HIP(hipGetLastError());
     return ARK_OPT_OK;
   }
   if (most) {
-    const dim3 grid((uint32_t)((most + kBlock - 1) / kBlock), 1, heads[1] ? 2 : 1);
+    const dim3 grid((uint32_t)((most + kBlock - 1) / kBlock), 1, a.part[1].heads ? 2 : 1);
     if (dtype == ARK_ACT_F16)
       hipLaunchKernelGGL(keep_kernel<ARK_ACT_F16>, grid, dim3(kBlock), 0, (hipStream_t)stream, a);
     else if (dtype == ARK_ACT_BF16)
@@ -1497,20 +1503,24 @@ int ark_rope_norm_backward(const ark_rope* r, uint32_t dtype, uint64_t batch, ui
   a.gain_dtype = gain_dtype;
   const void* gains[2] = {gain_q, gain_k};
   const void* acts[2] = {q_act, k_act};
+  bool all_kept = true;
+  Part* part = a.part;
   for (int i = 0; i < 2; ++i) {
     if (!has[i]) continue;
-    if (!acts[i]) a.part[i].x = array_of(g[3 * i + 2]);
-    a.part[i].dy = array_of(g[3 * i + 1]);
-    a.part[i].y = array_of(g[3 * i]);
-    a.part[i].heads = heads[i];
-    a.part[i].gain = gains[i];
-    a.part[i].act = (uint8_t*)acts[i];
+    if (!acts[i]) part->x = array_of(g[3 * i + 2]);
+    part->dy = array_of(g[3 * i + 1]);
+    part->y = array_of(g[3 * i]);
+    part->heads = heads[i];
+    part->gain = gains[i];
+    part->act = (uint8_t*)acts[i];
+    all_kept = all_kept && acts[i];
+    ++part;
   }
   ark::DeviceGuard guard(r->device);
   if (!guard.ok) return ark::fail(ARK_OPT_EHIP, "cannot select device %d", r->device);
   const hipStream_t st = (hipStream_t)stream;
-  const bool tiled = has[0] && q_act && (k_act || !has[1]) && tiles_fit(a, true);
-  const uint32_t blocks = empty ? 0
+  const bool tiled = all_kept && tiles_fit(a, true);
+  const uint32_t blocks = part == a.part ? 0
                           : tiled ? launch_tiles<true>(dtype, &a, st, false)
                                   : launch_rows<kBack>(dtype, &a, st, false);
   ark::StreamBuf buf;
@@ -1523,8 +1533,9 @@ int ark_rope_norm_backward(const ark_rope* r, uint32_t dtype, uint64_t batch, ui
     ARK_HIP(hipGetLastError());
   }
   hipLaunchKernelGGL(gain_kernel, dim3((r->head + kGainColumns - 1) / kGainColumns, dk_layout ? 2 : 1),
-                     dim3(kGainColumns * kGainRuns), 0, st, (const float*)buf.p, blocks,
-                     has[1] ? blocks : 0, r->head, dgain_q, dgain_k, accumulate);
+                     dim3(kGainColumns * kGainRuns), 0, st, (const float*)buf.p,
+                     has[0] ? blocks : 0, has[1] ? blocks : 0, r->head, dgain_q, dgain_k,
+                     accumulate);
   ARK_HIP(hipGetLastError());
   return ARK_OPT_OK;
 }
