@@ -502,7 +502,10 @@ __global__ __launch_bounds__(kBlock, 4) void rows_kernel(Args a) {
   const Part& P = a.part[blockIdx.y];
   const uint64_t columns = (uint64_t)P.heads * a.head;
   float su[R::kE] = {}, sv[R::kE] = {}, gu[R::kE], gv[R::kE];
-  if (OP != kRope) row.gains(a, P.gain, gu, gv);
+  // the condition always holds, and leaves the gains a block of their own: backward,
+  // 32768 tokens of 16 + 16 heads of 128, bf16, with it 285 us of both passes, 289
+  // without (fences for the scheduler or the values do not do the same)
+  if (OP != kRope && P.heads) row.gains(a, P.gain, gu, gv);
   for (uint64_t first = (uint64_t)blockIdx.x * a.tile; first < a.all;
        first += (uint64_t)gridDim.x * a.tile) {
     const uint32_t n = (uint32_t)(a.all - first < a.tile ? a.all - first : a.tile);
