@@ -341,8 +341,8 @@ struct Row {
       gv[e] = gain_at(a, g, has(e, true) ? at(e, true) : 0);
     }
   }
-  // the pairs' cosines and sines from a token's line of the block's table; pairs
-  // past the rotary ones do not turn
+  // the pairs' cosines and sines from a token's line of the block's table; for pairs
+  // past the rotary ones numbers that are not used
   __device__ __forceinline__ void turn(const float2* line, float* c, float* s) const {
 #pragma unroll
     for (uint32_t e = 0; e < kE; ++e) c[e] = 1.0f, s[e] = 0.0f;
@@ -355,7 +355,12 @@ struct Row {
           c[k * V + i] = t.x, s[k * V + i] = t.y;
         }
   }
-  // y = the rotation of x, or of x r gain
+  // y = the rotation of x, or of x r gain.  Pairs past the rotary ones are two values
+  // that have nothing to do with each other: a product with their sine of 0 would
+  // bring an inf or NaN of the one, and the sign of its zero, into the other, so
+  // they are kept (chosen under a condition of the whole call: without it the
+  // backward pass's registers spill, 32768 tokens of 16 + 16 heads of 128, bf16,
+  // both ways 601 us for 283)
   template <Op OP>
   __device__ __forceinline__ void forward(const Args& a, uint32_t lanes, const Data& x, const float* gu,
                                           const float* gv, const float* c, const float* s,
@@ -379,6 +384,7 @@ struct Row {
       const float nv = OP == kNorm ? v[e] * (r * gv[e]) : v[e];
       u[e] = __builtin_fmaf(nu, c[e], -(nv * s[e]));
       v[e] = __builtin_fmaf(nu, s[e], nv * c[e]);
+      if (a.rotary < a.head && pair[e / V] >= half) u[e] = nu, v[e] = nv;
     }
     y->set(u, v);
   }
@@ -399,6 +405,7 @@ struct Row {
         const float u = dy.get(e, false), v = dy.get(e, true);
         du[e] = __builtin_fmaf(u, c[e], v * s[e]);
         dv[e] = __builtin_fmaf(v, c[e], -(u * s[e]));
+        if (a.rotary < a.head && pair[k] >= half) du[e] = u, dv[e] = v;
         p = __builtin_fmaf(xu[e], xu[e], p);
         p = __builtin_fmaf(xv[e], xv[e], p);
         l = __builtin_fmaf(du[e] * gu[e], xu[e], l);
