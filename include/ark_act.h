@@ -69,7 +69,12 @@ int ark_act_unpack(const void *act, uint64_t tokens, uint64_t columns, uint32_t 
  * order of the reference's weights, proyecto_ark/ark01/src/memory.rs:227-255)
  * or transposed.  act_dtype is the type act was
  * packed from; dy is fp16 (act packed from fp16) or bf16 (from any): every
- * product is then exact in fp32.  tokens = 0 writes zeros, or leaves an
+ * product is then exact in fp32.  A sum of T products is within (T + 1) 2^-23 of
+ * the sum of their magnitudes, in which, with fp16 dy, a dy below 2^-14 (but not
+ * 0) counts as 2^-14 and an act more than 2^23 below its column's largest 2^e as
+ * 2^-23 of that: additions align by the factors' exponent fields, and a
+ * subnormal's is that of 2^-14.  (Such a dy is itself given to half a place of
+ * 2^-25, 2^12 times as much.)  tokens = 0 writes zeros, or leaves an
  * accumulated dw as it is.  dw must not overlap act or dy; a dw that is a
  * gradient of an optimizer is one the step may read at once, on the same
  * stream. */
