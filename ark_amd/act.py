@@ -27,6 +27,17 @@ def _stream(t):
     return raw(dev) if raw else torch.cuda.current_stream(dev).cuda_stream
 
 
+def _queue(t, call, *args):
+    """call(*args, the current stream of t's device) on that device: the library
+    launches on the current one, and a default stream is any device's."""
+    dev = t.get_device()
+    if dev == torch.cuda.current_device():
+        check(call(*args, _stream(t)))
+    else:
+        with torch.cuda.device(dev):
+            check(call(*args, _stream(t)))
+
+
 def _code(t, what):
     code = _TYPES.get(t.dtype)
     if code is None:
@@ -87,7 +98,7 @@ def pack(x, out=None):
         out = Act8._of(t, c, x)
     elif (out.tokens, out.columns, out.dtype) != (t, c, x.dtype) or out.data.device != x.device:
         raise ValueError(f"out is {out.tokens} x {out.columns} {out.dtype}, x {t} x {c} {x.dtype}")
-    check(lib().ark_act_pack(p, stride, code, t, c, out.data.data_ptr(), _stream(x)))
+    _queue(x, lib().ark_act_pack, p, stride, code, t, c, out.data.data_ptr())
     return out
 
 
@@ -100,8 +111,8 @@ def unpack(kept, out=None):
         raise ValueError(f"out is {tuple(out.shape)}, the activation {kept.tokens} x "
                          f"{kept.columns}")
     p, stride = _rows(out, "out")
-    check(lib().ark_act_unpack(kept.data.data_ptr(), kept.tokens, kept.columns,
-                               _code(out, "out"), p, stride, _stream(out)))
+    _queue(out, lib().ark_act_unpack, kept.data.data_ptr(), kept.tokens, kept.columns,
+           _code(out, "out"), p, stride)
     return out
 
 
@@ -137,8 +148,7 @@ def weight_grad(kept, dy, dw=None, accumulate=False, layout="in_out"):
     need = _workspace(kept.tokens, kept.columns, dstride, n)
     # torch's allocator hands a stream's memory back to it without waiting
     ws = dy.new_empty(need, dtype=torch.uint8) if need else None
-    check(lib().ark_act_weight_grad_noalloc(
-        kept.data.data_ptr(), _TYPES[kept.dtype], kept.tokens, kept.columns, dp, dstride,
-        _code(dy, "dy"), n, wp, wstride, flags, ws.data_ptr() if need else None, need,
-        _stream(dy)))
+    _queue(dy, lib().ark_act_weight_grad_noalloc, kept.data.data_ptr(), _TYPES[kept.dtype],
+           kept.tokens, kept.columns, dp, dstride, _code(dy, "dy"), n, wp, wstride, flags,
+           ws.data_ptr() if need else None, need)
     return dw

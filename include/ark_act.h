@@ -27,7 +27,8 @@
  *
  * Every function is stream ordered and returns an ARK_OPT_* status code
  * (include/ark_opt.h), with the message in ark_opt_last_error().  Pointers
- * are device pointers.  Row strides are in elements.
+ * are device pointers of the current device, and stream is one of its streams.
+ * Row strides are in elements.
  */
 #ifndef ARK_ACT_H
 #define ARK_ACT_H

@@ -1,0 +1,82 @@
+"""The host side of act.py and rope.py without a GPU: a recorded library and
+stand-ins for device tensors."""
+import contextlib
+import types
+
+import pytest
+import torch
+
+from ark_amd import act
+
+
+class Fake:
+    """A contiguous device tensor as far as act.py and rope.py look at one."""
+
+    def __init__(self, shape, dtype=torch.float16, device=1, requires_grad=False):
+        self.shape, self.dtype = torch.Size(shape), dtype
+        self.device = torch.device("cuda", device)
+        self.is_cuda, self.requires_grad = True, requires_grad
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return self.shape.numel()
+
+    def stride(self, i=None):
+        st = [1] * len(self.shape)
+        for j in range(len(st) - 2, -1, -1):
+            st[j] = st[j + 1] * self.shape[j + 1]
+        return tuple(st) if i is None else st[i]
+
+    def is_contiguous(self):
+        return True
+
+    def get_device(self):
+        return self.device.index
+
+    def data_ptr(self):
+        return 4096
+
+    def new_empty(self, shape, dtype=None):
+        return Fake((shape,) if isinstance(shape, int) else shape, dtype or self.dtype,
+                    self.device.index)
+
+
+@pytest.fixture
+def gpus(monkeypatch):
+    """Two devices, the first of them current, and a library that notes, call by
+    call, its name, the current device and the stream."""
+    calls, current = [], [0]
+
+    @contextlib.contextmanager
+    def device(dev):
+        before, current[0] = current[0], torch.device("cuda", dev).index
+        yield
+        current[0] = before
+
+    class Lib:
+        def __getattr__(self, name):
+            def call(*args):
+                calls.append((name, current[0], args[-1]))
+                return 0
+            return call
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: 700 + dev,
+                        raising=False)
+    monkeypatch.setattr(act, "lib", Lib)
+    monkeypatch.setattr(act, "_workspace", lambda *a: 0)
+    return types.SimpleNamespace(calls=calls, current=current)
+
+
+@pytest.mark.parametrize("dev", [0, 1])
+def test_act_runs_on_its_tensors_device(gpus, dev):
+    x, dy = Fake((64, 8), device=dev), Fake((64, 16), device=dev)
+    kept = act.pack(x)
+    act.unpack(kept)
+    act.weight_grad(kept, dy)
+    assert gpus.calls == [(name, dev, 700 + dev) for name in
+                          ("ark_act_pack", "ark_act_unpack", "ark_act_weight_grad_noalloc")]
+    assert gpus.current == [0]
