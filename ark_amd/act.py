@@ -69,7 +69,7 @@ class Act8:
             raise ValueError(f"sizes {tokens} x {columns}")
         n = -(-tokens // _abi.ACT_GROUP) * columns * (_abi.ACT_GROUP + 1)
         if data is None:
-            data = torch.empty(n, dtype=torch.uint8, device=device or "cuda")
+            data = torch.empty(n, dtype=torch.uint8, device="cuda" if device is None else device)
         elif data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() != n:
             raise ValueError(f"data must be {n} contiguous uint8")
         self.tokens, self.columns, self.dtype, self.data = tokens, columns, dtype, data

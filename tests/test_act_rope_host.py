@@ -80,3 +80,11 @@ def test_act_runs_on_its_tensors_device(gpus, dev):
     assert gpus.calls == [(name, dev, 700 + dev) for name in
                           ("ark_act_pack", "ark_act_unpack", "ark_act_weight_grad_noalloc")]
     assert gpus.current == [0]
+
+
+def test_act8_on_a_device_by_number(monkeypatch):
+    where = []
+    monkeypatch.setattr(torch, "empty", lambda n, dtype, device: where.append(device))
+    for given in (None, 0, 1, "cuda:1"):
+        act.Act8(32, 4, torch.float16, device=given)
+    assert where == ["cuda", 0, 1, "cuda:1"]
