@@ -73,7 +73,7 @@ class Rope:
             raise ValueError("inv_freq holds one value a pair and takes no scaling")
         self._h = None
         self._plans = {}
-        torch.cuda.current_device()
+        self.device = torch.device("cuda", torch.cuda.current_device())
         h = C.c_void_p()
         check(lib().ark_rope_create(head_dim, rotary_dim, _LAYOUTS[layout],
                                     (C.c_double * max(1, len(inv_freq)))(*inv_freq), magnitude,
@@ -128,6 +128,9 @@ class Rope:
         code = _code(q, "q")
         if not q.is_cuda:
             raise ValueError(f"q is on {q.device}, not a GPU")
+        if q.device != self.device:
+            raise ValueError(f"q is on {q.device}, the rotation on {self.device}: make a Rope "
+                             f"there")
         lq = self._layout(q, "q")
         batch, tokens = q.shape[0] if q.dim() == 4 else 1, q.shape[-3]
         lk = None if k is None else self._beside(k, q, "k")

@@ -25,9 +25,11 @@
  * in turns: at any position it is as exact as inv_freq itself (no tables).
  *
  * Every function is stream ordered and returns an ARK_OPT_* status code
- * (include/ark_opt.h), with the message in ark_opt_last_error().  Element
- * types are ARK_ACT_F16, ARK_ACT_BF16 and ARK_ACT_F32 (include/ark_act.h);
- * all arithmetic is fp32, rounded once where a result is stored.
+ * (include/ark_opt.h), with the message in ark_opt_last_error().  Pointers are
+ * device pointers of the rotation's device, and stream is one of its streams.
+ * Element types are ARK_ACT_F16, ARK_ACT_BF16 and ARK_ACT_F32
+ * (include/ark_act.h); all arithmetic is fp32, rounded once where a result is
+ * stored.
  */
 #ifndef ARK_ROPE_H
 #define ARK_ROPE_H

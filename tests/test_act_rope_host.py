@@ -88,3 +88,31 @@ def test_act8_on_a_device_by_number(monkeypatch):
     for given in (None, 0, 1, "cuda:1"):
         act.Act8(32, 4, torch.float16, device=given)
     assert where == ["cuda", 0, 1, "cuda:1"]
+
+
+@pytest.fixture
+def rope(gpus, monkeypatch):
+    """A Rope of heads of 8 made on device 0."""
+    from ark_amd import rope
+    monkeypatch.setattr(rope, "lib", act.lib)
+    monkeypatch.setattr(rope, "_like", lambda t: t.new_empty(t.shape))
+    r = rope.Rope(8)
+    gpus.calls.clear()
+    return r
+
+
+def test_rope_refuses_another_device_than_its_own(gpus, rope):
+    q = [Fake((5, 2, 8), device=d) for d in (0, 1)]
+    k = [Fake((5, 1, 8), device=d) for d in (0, 1)]
+    g = [Fake((8,), torch.float32, d) for d in (0, 1)]
+    for call in (lambda i: rope.apply(q[i], k[i]), lambda i: rope.apply(q[i]),
+                 lambda i: rope.norm(q[i], k[i], g[i], g[i]),
+                 lambda i: rope.norm_backward(q[i], k[i], q[i], k[i], g[i], g[i])):
+        call(0)
+        assert gpus.calls.pop()[1:] == (0, 700) and not gpus.calls
+        for current in (0, 1):
+            gpus.current[0] = current
+            with pytest.raises(ValueError, match="cuda:1.*cuda:0"):
+                call(1)
+        gpus.current[0] = 0
+        assert not gpus.calls
