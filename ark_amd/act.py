@@ -4,7 +4,9 @@ torch tensors, and the weight gradient that reads them.
 ``pack(x)`` keeps a layer's input as an ``Act8`` of half the bytes (a quarter
 of fp32's); ``weight_grad(kept, dy)`` is the weight gradient x^T dy from it, in
 fp32, written to or added into the gradients an optimizer steps on;
-``unpack(kept)`` gives the values back.
+``unpack(kept)`` gives the values back.  No call records an autograd graph: they
+take the values of tensors that require grad, and their results are the parts
+of a backward pass that its caller writes (an ``autograd.Function``, say).
 """
 import ctypes as C
 import functools

@@ -7,6 +7,11 @@ rotation in the same pass (include/ark_rope.h), for torch tensors.
 head_dim) or (batch, tokens, heads, head_dim) tensors of any strides whose
 head_dim values follow one another: slices of a fused projection and
 transposed (batch, heads, tokens, head_dim) arrays are taken as they are.
+
+No call records an autograd graph.  ``apply`` and ``norm`` refuse inputs that
+require grad while one is recorded: call them under ``torch.no_grad()``, or from
+an ``autograd.Function`` whose backward calls ``apply(inverse=True)`` or
+``norm_backward``.
 """
 import ctypes as C
 
@@ -30,6 +35,14 @@ _like = torch.empty_like
 
 def _meta(t):
     return t.shape, t.stride(), t.dtype, t.get_device()
+
+
+def _no_graph(what):
+    """For inputs of which some require grad."""
+    if torch.is_grad_enabled():
+        raise ValueError(f"an input of {what} requires grad, and its result would have no graph: "
+                         "use torch.no_grad(), or an autograd.Function over it and its backward "
+                         "call")
 
 
 def frequencies(rotary_dim, base=10000.0, scaling=None):
@@ -170,6 +183,8 @@ class Rope:
         pair with k; q itself to rotate in place) or new tensors.  inverse
         rotates back, as the gradients of the results are.  Returns the pair, or
         one tensor without k."""
+        if q.requires_grad or (k is not None and k.requires_grad):
+            _no_graph("apply")
         key = _meta(q), k if k is None else _meta(k), positions if positions is None else _meta(
             positions)
         code, batch, tokens, size, _, lq, lk, loq, lok = (
@@ -206,6 +221,9 @@ class Rope:
         8-bit forms of q and k in the same pass, for norm_backward: True for new
         ones, or a pair of Act8 of batch * tokens rows.  Returns (q, k) or (q,
         k, kept_q, kept_k)."""
+        if (q.requires_grad or k.requires_grad or gain_q.requires_grad
+                or gain_k.requires_grad):
+            _no_graph("norm")
         key = (_meta(q), _meta(k), positions if positions is None else _meta(positions),
                _meta(gain_q), _meta(gain_k))
         code, batch, tokens, size, gcode, lq, lk, loq, lok = (

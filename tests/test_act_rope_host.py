@@ -116,3 +116,24 @@ def test_rope_refuses_another_device_than_its_own(gpus, rope):
                 call(1)
         gpus.current[0] = 0
         assert not gpus.calls
+
+
+def test_rope_refuses_what_would_lose_a_graph(gpus, rope):
+    """Results carry no graph: an input that requires grad is refused while one
+    is recorded, and taken under no_grad (as inside an autograd.Function)."""
+    q, k, g = Fake((5, 2, 8)), Fake((5, 1, 8)), Fake((8,), torch.float32)
+    for t in (q, k, g):
+        t.device = torch.device("cuda", 0)
+    calls = (lambda: rope.apply(q), lambda: rope.apply(q, k), lambda: rope.norm(q, k, g, g))
+    for which, needs in ((q, (1, 1, 1)), (k, (0, 1, 1)), (g, (0, 0, 1))):
+        which.requires_grad = True
+        for call, need in zip(calls, needs):
+            if need:
+                with pytest.raises(ValueError, match="requires grad"):
+                    call()
+            else:
+                call()
+            with torch.no_grad():
+                call()
+        which.requires_grad = False
+    assert len(gpus.calls) == 9 + 3
