@@ -20,24 +20,27 @@ _TYPES = {torch.float16: _abi.ACT_F16, torch.bfloat16: _abi.ACT_BF16,
           torch.float32: _abi.ACT_F32}
 
 
+# By the calls that are not public where this torch has them: a Stream object costs
+# as much as queueing a kernel, the public current_device twice as much as this.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _stream(t):
-    """torch's current HIP stream of t's device, as a number (by the call that is
-    not public where this torch has it: a Stream object costs as much as queueing
-    a kernel)."""
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    dev = t.get_device()
-    return raw(dev) if raw else torch.cuda.current_stream(dev).cuda_stream
+    """torch's current HIP stream of t's device, as a number."""
+    return _raw_stream(t.get_device())
 
 
 def _queue(t, call, *args):
     """call(*args, the current stream of t's device) on that device: the library
     launches on the current one, and a default stream is any device's."""
     dev = t.get_device()
-    if dev == torch.cuda.current_device():
-        check(call(*args, _stream(t)))
+    if dev == _device():
+        check(call(*args, _raw_stream(dev)))
     else:
         with torch.cuda.device(dev):
-            check(call(*args, _stream(t)))
+            check(call(*args, _raw_stream(dev)))
 
 
 def _code(t, what):
@@ -53,9 +56,10 @@ def _rows(t, what):
         raise ValueError(f"{what} has {t.dim()} dimensions, not 2")
     if not t.is_cuda:
         raise ValueError(f"{what} is not a device tensor")
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    stride, one = t.stride()
+    if one != 1 and t.shape[1] > 1:
         raise ValueError(f"{what}: the values of a row do not follow one another")
-    return t.data_ptr(), t.stride(0)
+    return t.data_ptr(), stride
 
 
 class Act8:

@@ -64,8 +64,8 @@ def gpus(monkeypatch):
 
     monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
     monkeypatch.setattr(torch.cuda, "device", device)
-    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: 700 + dev,
-                        raising=False)
+    monkeypatch.setattr(act, "_device", lambda: current[0])
+    monkeypatch.setattr(act, "_raw_stream", lambda dev: 700 + dev)
     monkeypatch.setattr(act, "lib", Lib)
     monkeypatch.setattr(act, "_workspace", lambda *a: 0)
     return types.SimpleNamespace(calls=calls, current=current)
