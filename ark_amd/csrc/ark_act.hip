@@ -140,23 +140,28 @@ __global__ __launch_bounds__(kLanes) void unpack_kernel(const uint8_t* __restric
   }
 }
 
-// The same for a single column.
+// The same for a single column, a group or a token a lane, and the ones a grid on:
+// a column may be longer than a launch (2^32 lanes).
 template <uint32_t DT>
 __global__ __launch_bounds__(kLanes) void pack1_kernel(const elem_t<DT>* __restrict__ x,
                                                        uint64_t stride, uint64_t tokens,
                                                        uint8_t* __restrict__ q,
                                                        uint8_t* __restrict__ e) {
-  const uint64_t g = (uint64_t)blockIdx.x * kLanes + threadIdx.x, t0 = g * ARK_ACT_GROUP;
-  if (t0 >= tokens) return;
-  uint32_t most = 0;
-  const auto at = [&](uint32_t i) { return t0 + i < tokens ? (float)x[(t0 + i) * stride] : 0.0f; };
-  for (uint32_t i = 0; i < ARK_ACT_GROUP; ++i)
-    most = max(most, __float_as_uint(at(i)) & 0x7FFFFFFFu);
-  const uint32_t s = act_exponent<DT>(most);
-  const auto held = [&](uint32_t i) { return act_hold<DT>(s, at(i)); };
-  for (uint32_t i = 0; i < ARK_ACT_GROUP; i += 4)
-    st_g<uint32_t>(q + t0 + i, act_bytes4(s, held(i), held(i + 1), held(i + 2), held(i + 3)));
-  e[g] = (uint8_t)s;
+  for (uint64_t g = (uint64_t)blockIdx.x * kLanes + threadIdx.x; g * ARK_ACT_GROUP < tokens;
+       g += (uint64_t)gridDim.x * kLanes) {
+    const uint64_t t0 = g * ARK_ACT_GROUP;
+    uint32_t most = 0;
+    const auto at = [&](uint32_t i) {
+      return t0 + i < tokens ? (float)x[(t0 + i) * stride] : 0.0f;
+    };
+    for (uint32_t i = 0; i < ARK_ACT_GROUP; ++i)
+      most = max(most, __float_as_uint(at(i)) & 0x7FFFFFFFu);
+    const uint32_t s = act_exponent<DT>(most);
+    const auto held = [&](uint32_t i) { return act_hold<DT>(s, at(i)); };
+    for (uint32_t i = 0; i < ARK_ACT_GROUP; i += 4)
+      st_g<uint32_t>(q + t0 + i, act_bytes4(s, held(i), held(i + 1), held(i + 2), held(i + 3)));
+    e[g] = (uint8_t)s;
+  }
 }
 template <uint32_t DT>
 __global__ __launch_bounds__(kLanes) void unpack1_kernel(const uint8_t* __restrict__ q,
@@ -164,8 +169,9 @@ __global__ __launch_bounds__(kLanes) void unpack1_kernel(const uint8_t* __restri
                                                          uint64_t tokens,
                                                          elem_t<DT>* __restrict__ x,
                                                          uint64_t stride) {
-  const uint64_t t = (uint64_t)blockIdx.x * kLanes + threadIdx.x;
-  if (t < tokens) x[t * stride] = (elem_t<DT>)act_value(q[t], 0, act_up(e[t / ARK_ACT_GROUP]));
+  for (uint64_t t = (uint64_t)blockIdx.x * kLanes + threadIdx.x; t < tokens;
+       t += (uint64_t)gridDim.x * kLanes)
+    x[t * stride] = (elem_t<DT>)act_value(q[t], 0, act_up(e[t / ARK_ACT_GROUP]));
 }
 
 // ---- the weight gradient -----------------------------------------------------
@@ -678,8 +684,8 @@ int check_dtype(uint32_t dtype, const char* what) {
   return ARK_OPT_OK;
 }
 
-// Sizes for which no address below wraps: at most 2^32 - 1 columns and 2^47
-// values, so any byte offset fits 64 bits with room to spare.
+// Sizes for which no address below wraps: fewer than 2^31 columns and 2^40 tokens,
+// and 2^47 values at most, so any byte offset fits 64 bits with room to spare.
 int check_sizes(uint64_t tokens, uint64_t columns) {
   if (columns >= (1ull << 31))
     return ark::fail(ARK_OPT_EINVAL, "columns = %llu too large", (unsigned long long)columns);
@@ -733,6 +739,12 @@ int check_copy(const void* x, uint64_t x_stride, uint32_t dtype, uint64_t tokens
   return checker.check(x, *x_bytes, "x", 0);
 }
 
+// Blocks for n lanes' work of a single column's kernels.
+dim3 column_grid(uint64_t n) {
+  const uint64_t blocks = (n + kLanes - 1) / kLanes;
+  return dim3((uint32_t)(blocks < (1u << 20) ? blocks : 1u << 20));
+}
+
 // Columns a lane takes: two (4 bytes of 16-bit rows); four take twice the
 // registers and leave half the waves (16384 x 2048 fp16, both ways: 37.5 us by
 // two, 44.6 by four).
@@ -745,8 +757,8 @@ void launch_pack(const void* x, uint64_t stride, uint64_t tokens, uint64_t colum
   uint8_t* e = act + groups * columns * ARK_ACT_GROUP;
   const elem_t<DT>* p = (const elem_t<DT>*)x;
   if (columns < kWide)
-    hipLaunchKernelGGL(pack1_kernel<DT>, dim3((uint32_t)((groups + kLanes - 1) / kLanes)),
-                       dim3(kLanes), 0, s, p, stride, tokens, act, e);
+    hipLaunchKernelGGL(pack1_kernel<DT>, column_grid(groups), dim3(kLanes), 0, s, p, stride,
+                       tokens, act, e);
   else
     hipLaunchKernelGGL((pack_kernel<DT, kWide>),
                        group_grid((columns + kLanes * kWide - 1) / (kLanes * kWide), groups),
@@ -760,8 +772,8 @@ void launch_unpack(const uint8_t* act, uint64_t tokens, uint64_t columns, void* 
   const uint8_t* e = act + groups * columns * ARK_ACT_GROUP;
   elem_t<DT>* p = (elem_t<DT>*)x;
   if (columns < kWide)
-    hipLaunchKernelGGL(unpack1_kernel<DT>, dim3((uint32_t)((tokens + kLanes - 1) / kLanes)),
-                       dim3(kLanes), 0, s, act, e, tokens, p, stride);
+    hipLaunchKernelGGL(unpack1_kernel<DT>, column_grid(tokens), dim3(kLanes), 0, s, act, e,
+                       tokens, p, stride);
   else
     hipLaunchKernelGGL((unpack_kernel<DT, kWide>),
                        group_grid((columns + kLanes * kWide - 1) / (kLanes * kWide), groups),
