@@ -715,7 +715,8 @@ int check_act(const void* act, uint64_t tokens, uint64_t columns, ark::BufferChe
   return checker->check(act, 33 * ark::act_groups(tokens) * columns, "act", 0);
 }
 
-// Blocks over groups in y and z: y stays within a launch's 65535.
+// Blocks over groups in y and z, each within a launch's 65535.
+constexpr uint64_t kMaxGroups = 65535ull * 32768;
 dim3 group_grid(uint64_t x, uint64_t groups) {
   const uint64_t y = groups < 32768 ? groups : 32768;
   return dim3((uint32_t)x, (uint32_t)y, (uint32_t)((groups + y - 1) / y));
@@ -729,6 +730,8 @@ int check_copy(const void* x, uint64_t x_stride, uint32_t dtype, uint64_t tokens
   if ((rc = check_dtype(dtype, "dtype"))) return rc;
   if ((rc = check_sizes(tokens, columns))) return rc;
   if (*skip) return ARK_OPT_OK;
+  if (columns > 1 && ark::act_groups(tokens) > kMaxGroups)
+    return ark::fail(ARK_OPT_EINVAL, "tokens = %llu too large", (unsigned long long)tokens);
   const uint32_t es = ark::act_elem_size(dtype);
   if ((uintptr_t)x % es) return ark::fail(ARK_OPT_EINVAL, "x not aligned to its element");
   if ((rc = rows_bytes(tokens, columns, x_stride, es, unpack, "x", x_bytes))) return rc;
@@ -901,7 +904,11 @@ int weight_grad(const void* act, uint32_t act_dtype, uint64_t tokens, uint64_t c
   const bool any = needs_any(columns, dy_stride, outputs);
   const Cut c = cut_of(tokens, columns, outputs, any);
   const uint64_t steps = (tokens + kStep - 1) / kStep;
-  if (steps >= (1ull << 31) || c.tiles >= (1ull << 31) / 32 || c.tiles * c.mf * c.nf >= (1ull << 31))
+  // a launch holds fewer than 2^32 lanes, 256 wn a block (the sum of splits has
+  // mf * nf blocks a tile)
+  const uint64_t blocks = c.splits > 1 ? c.tiles * (c.splits > c.mf * c.nf ? c.splits : c.mf * c.nf)
+                                       : c.tiles;
+  if (steps >= (1ull << 31) || blocks >= (1ull << 32) / (256 * c.wn))
     return ark::fail(ARK_OPT_EINVAL, "tokens, columns or outputs too large");
   ark::BufferChecker checker;
   if (given && c.bytes()) {

@@ -1,12 +1,13 @@
 """The host side of act.py and rope.py without a GPU: a recorded library and
-stand-ins for device tensors."""
+stand-ins for device tensors; and the library's own refusals before any device
+call."""
 import contextlib
 import types
 
 import pytest
 import torch
 
-from ark_amd import act
+from ark_amd import _abi, _lib, act
 
 
 class Fake:
@@ -137,3 +138,24 @@ def test_rope_refuses_what_would_lose_a_graph(gpus, rope):
                 call()
         which.requires_grad = False
     assert len(gpus.calls) == 9 + 3
+
+
+@pytest.mark.parametrize("columns,outputs,flags", [(1 << 30, 1, 0), (1, 1 << 30, 2),
+                                                   ((1 << 30) + 7, 3, 0), (1 << 20, 1 << 24, 0)])
+def test_weight_grad_refuses_more_blocks_than_a_launch_holds(columns, outputs, flags):
+    """A launch holds fewer than 2^32 lanes: 64 x 64 outputs' blocks have 512."""
+    L = _lib.lib()
+    gb = 1 << 40
+    rc = L.ark_act_weight_grad(gb, _abi.ACT_F16, 32, columns, 100 * gb, outputs, _abi.ACT_F16,
+                               outputs, 200 * gb, columns if flags else outputs, flags, None)
+    assert rc == _abi.EINVAL and "too large" in L.ark_opt_last_error().decode()
+
+
+@pytest.mark.parametrize("columns", [2, 700])
+def test_packing_refuses_more_groups_than_a_launch_holds(columns):
+    """65535 x 32768 groups of 32 tokens."""
+    L = _lib.lib()
+    gb, t = 1 << 50, (65535 * 32768 + 1) * 32
+    for rc in (L.ark_act_pack(gb, 0, _abi.ACT_F16, t, columns, 3 * gb, None),
+               L.ark_act_unpack(3 * gb, t, columns, _abi.ACT_F16, gb, columns, None)):
+        assert rc == _abi.EINVAL and "too large" in L.ark_opt_last_error().decode()
