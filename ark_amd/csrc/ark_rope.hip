@@ -870,7 +870,8 @@ __global__ __launch_bounds__(kBlock) void keep_kernel(Args a) {
 
 // The gains' gradients from the blocks' rows (none of a part of no heads), added in
 // order: 64 rows' runs by the lanes of a column, then those.  4 us of latency for
-// any number of rows met here (384 blocks a part at most, or 1024 short heads').
+// any number of rows met here (about 768 in all of tiles, up to 1024 a part of
+// rows).
 constexpr uint32_t kGainColumns = 16, kGainRuns = 64;
 __global__ __launch_bounds__(kGainColumns * kGainRuns) void gain_kernel(
     const float* __restrict__ partial, uint32_t rows_q, uint32_t rows_k, uint32_t head,
@@ -965,8 +966,9 @@ uint32_t launch_rows(uint32_t dtype, Args* a, hipStream_t s, bool launch = true)
   a->lanes = w.lanes;
   a->tile = rows_tile(*a, w, OP == kRope ? 4 : 8);
   const uint64_t tiles = (a->all + a->tile - 1) / a->tile;
-  // Backward, the units' fill of a part's blocks, fewer for long heads: their rows
-  // of the gains' gradients then need no memory of the stream's pool, whose host
+  // Backward, the units' fill of a part's blocks, fewer for long heads: up to 128
+  // values the rows of both gains' gradients then fit a kept slot of 512 KiB.
+  // Longer heads keep 512 blocks a part and take the stream's pool, whose host
   // time is 33 us.
   const uint32_t rows = 65536 / a->head;
   const uint32_t most = OP != kBack ? 1u << 20 : rows < 512 ? 512 : rows < 1024 ? rows : 1024;
@@ -1007,7 +1009,7 @@ uint32_t launch_tiles(uint32_t dtype, Args* a, hipStream_t s, bool launch = true
   // Backward, as many blocks as the units hold at once, three each: every block's
   // row of the gains' gradients is one more to add up, and a last round of a few
   // blocks would have the chip to itself (237M training pass 34.7 us, 37.6 with a
-  // block a group).
+  // block a group).  Their rows fit a kept slot up to heads of 170 values.
   const uint32_t parts = a->part[1].heads ? 2 : 1;
   const uint32_t held = 768 / parts / slices, most = !BACK ? 1u << 20 : held ? held : 1;
   if (by > most) by = most;
@@ -1535,7 +1537,7 @@ int ark_rope_norm_backward(const ark_rope* r, uint32_t dtype, uint64_t batch, ui
                                   : launch_rows<kBack>(dtype, &a, st, false);
   ark::StreamBuf buf;
   if (blocks) {
-    const hipError_t e = buf.alloc((uint64_t)2 * blocks * r->head * 4, st);
+    const hipError_t e = buf.alloc((uint64_t)(part - a.part) * blocks * r->head * 4, st);
     if (e != hipSuccess) return ark::hip_fail(e, "workspace of ark_rope_norm_backward");
     a.partial = (float*)buf.p;
     tiled ? launch_tiles<true>(dtype, &a, st)

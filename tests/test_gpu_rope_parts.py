@@ -67,7 +67,7 @@ def test_neither_has_heads():
 
 @pytest.mark.parametrize("keep8", [False, True])
 @pytest.mark.parametrize("d", [64, 66, 256])
-@pytest.mark.parametrize("tokens", [1, 40, 700])
+@pytest.mark.parametrize("tokens", [1, 40, 700, 30000])
 def test_k_of_no_heads_has_a_gradient_of_zeros(tokens, d, keep8):
     torch = _torch()
     rope = Rope(d)
