@@ -1,7 +1,7 @@
-"""Rotary positions and head norms (include/ark_rope.h) where a part has no
-heads: q or k of zero heads beside one that has some, or both.  A part without
-heads is no work, and its gain's gradient is zero (or stays as it was, when it
-is added to)."""
+"""Rotary positions and head norms (include/ark_rope.h) where q and k differ: one of
+zero heads beside one that has some, or both of none, or one kept in 8 bits and the
+other a tensor.  A part without heads is no work, and its gain's gradient is zero
+(or stays as it was, when it is added to)."""
 import numpy as np
 import pytest
 
@@ -87,3 +87,46 @@ def test_k_of_no_heads_has_a_gradient_of_zeros(tokens, d, keep8):
     first = a.clone()
     rope.norm_backward(dq, dnone, *kept, *gains, dgain_q=a, dgain_k=b, accumulate=True)
     assert (b == 5.0).all() and torch.equal(a, first + first)
+
+
+@pytest.mark.parametrize("name,d", [("f16", 64), ("bf16", 128), ("f32", 66)])
+@pytest.mark.parametrize("which", [0, 1])
+def test_one_input_kept_and_the_other_a_tensor(name, d, which):
+    torch = _torch()
+    rope = Rope(d)
+    gains = _gains(d, "f32")
+    for shape in ((1,), (2, 70)):
+        xs, dys = _qk(shape, 4, 2, d, name), _qk(shape, 4, 2, d, name, 2)
+        kept = list(xs)
+        kept[which] = rope.norm(*xs, *gains, keep8=True)[2 + which]
+        back = rope.norm_backward(*dys, *kept, *gains)
+        turn = Turn(np.broadcast_to(np.arange(shape[-1]), shape), d, d, "half")
+        for i in range(2):
+            x = _f64(act.unpack(kept[i])).reshape(xs[i].shape) if i == which else _f64(xs[i])
+            dx, b, dg, gb = _back64(_f64(dys[i]), x, _f64(gains[i]), turn,
+                                    tuple(range(len(shape) + 1)))
+            _near(back[i], dx, b, name)
+            _near(back[2 + i], dg, gb)
+
+
+def test_one_input_kept_by_the_c_entry():
+    """ark_rope_norm with a q_act or a k_act alone writes what pack gives."""
+    torch = _torch()
+    import ctypes as C
+    from ark_amd import _abi, _lib
+    rope = Rope(64)
+    g = _gains(64, "f32")
+    q, k = _qk((2, 45), 3, 2, 64, "f16")
+    want = rope.norm(q, k, *g)
+    lay = [(C.c_uint64 * 4)(x.shape[2], x.stride(0), x.stride(1), x.stride(2)) for x in (q, k)]
+    for which in (0, 1):
+        out = [torch.empty_like(x) for x in (q, k)]
+        kept = act.Act8(90, 64 * (3, 2)[which], torch.float16)
+        kept.data.fill_(1)
+        acts = [kept.data.data_ptr() if i == which else None for i in range(2)]
+        _lib.check(_lib.lib().ark_rope_norm(
+            rope._h, _abi.ACT_F16, 2, 45, None, 0, 0, 1e-5, g[0].data_ptr(), g[1].data_ptr(),
+            _abi.ACT_F32, q.data_ptr(), lay[0], out[0].data_ptr(), lay[0], acts[0], k.data_ptr(),
+            lay[1], out[1].data_ptr(), lay[1], acts[1], _lib.current_stream(q)))
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        assert torch.equal(kept.data, act.pack((q, k)[which].reshape(90, -1)).data)
