@@ -27,11 +27,6 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 _device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _stream(t):
-    """torch's current HIP stream of t's device, as a number."""
-    return _raw_stream(t.get_device())
-
-
 def _queue(t, call, *args):
     """call(*args, the current stream of t's device) on that device: the library
     launches on the current one, and a default stream is any device's."""

@@ -19,7 +19,7 @@ import torch
 
 from . import _abi
 from ._lib import check, lib
-from .act import Act8, _code, _stream
+from .act import Act8, _code, _raw_stream
 
 _LAYOUTS = {"half": _abi.ROPE_HALF, "interleaved": _abi.ROPE_INTERLEAVED}
 _SCALINGS = {"linear": (_abi.ROPE_SCALE_LINEAR, ("factor",), {}),
@@ -34,6 +34,7 @@ _like = torch.empty_like
 
 
 def _meta(t):
+    """What a plan depends on; the last is the device's number."""
     return t.shape, t.stride(), t.dtype, t.get_device()
 
 
@@ -198,7 +199,7 @@ class Rope:
                 loq = self._into(out, q, "out")
             check(lib().ark_rope_apply(self._h, code, batch, tokens, pos, size, start,
                                        q.data_ptr(), lq, out.data_ptr(), loq, None, None, None,
-                                       None, flag, _stream(q)))
+                                       None, flag, _raw_stream(key[0][-1])))
             return out
         oq, ok = (None, None) if out is None else out
         if oq is None:
@@ -211,7 +212,7 @@ class Rope:
             lok = self._into(ok, k, "out")
         check(lib().ark_rope_apply(self._h, code, batch, tokens, pos, size, start, q.data_ptr(),
                                    lq, oq.data_ptr(), loq, k.data_ptr(), lk, ok.data_ptr(), lok,
-                                   flag, _stream(q)))
+                                   flag, _raw_stream(key[0][-1])))
         return oq, ok
 
     def norm(self, q, k, gain_q, gain_k, positions=None, start=0, eps=1e-5, out=None,
@@ -250,7 +251,7 @@ class Rope:
                                   None if positions is None else positions.data_ptr(), size, start,
                                   eps, gain_q.data_ptr(), gain_k.data_ptr(), gcode, q.data_ptr(),
                                   lq, oq.data_ptr(), loq, dq, k.data_ptr(), lk, ok.data_ptr(), lok,
-                                  dk, _stream(q)))
+                                  dk, _raw_stream(key[0][-1])))
         return (oq, ok, aq, ak) if keep8 else (oq, ok)
 
     def norm_backward(self, dq, dk, q, k, gain_q, gain_k, positions=None, start=0, eps=1e-5,
@@ -292,5 +293,5 @@ class Rope:
         check(lib().ark_rope_norm_backward(
             self._h, code, batch, tokens, None if positions is None else positions.data_ptr(), size,
             start, eps, gain_q.data_ptr(), gain_k.data_ptr(), gcode, *args, 1 if accumulate else 0,
-            _stream(dq)))
+            _raw_stream(key[0][-1])))
         return outs[0], outs[1], grads[0], grads[1]

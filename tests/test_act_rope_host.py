@@ -96,6 +96,7 @@ def rope(gpus, monkeypatch):
     """A Rope of heads of 8 made on device 0."""
     from ark_amd import rope
     monkeypatch.setattr(rope, "lib", act.lib)
+    monkeypatch.setattr(rope, "_raw_stream", act._raw_stream)
     monkeypatch.setattr(rope, "_like", lambda t: t.new_empty(t.shape))
     r = rope.Rope(8)
     gpus.calls.clear()
