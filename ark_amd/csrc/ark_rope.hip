@@ -494,8 +494,10 @@ struct Tokens {
 // heads; a row's sum of squares stays in its lanes.  One pass over the data,
 // bound by HBM when long: 16384 tokens of 16 + 16 heads of 128, bf16, rotated, 268
 // MB in 46 us, 5.8 TB/s; 5003 tokens of 12 + 12 heads of 64, fp32, 61 MB in 11 us,
-// 5.5 TB/s.  4099 tokens of 12 + 12 of 64 normed and rotated, fp16, 25 MB, take
+// 5.6 TB/s.  4099 tokens of 12 + 12 of 64 normed and rotated, fp16, 25 MB, take
 // 10 us, mostly the way through one round of blocks: angles, loads, sums, stores.
+// Backward from tensors, 32768 tokens of 16 + 16 heads of 128, bf16, 805 MB take 176
+// us, 4.6 TB/s; in fp32, four pairs a lane, its registers spill 72 bytes a lane.
 template <uint32_t DT, Op OP, uint32_t V, uint32_t K>
 __global__ __launch_bounds__(kBlock, 4) void rows_kernel(Args a) {
   typedef Row<DT, V, K> R;
@@ -667,7 +669,7 @@ struct Exps {
 // and the vector units' (17) overlap only in part.
 //
 // Waves of a SIMD the registers are cut for, by the words a head's share takes of a
-// lane twice over: the most without spills (but for 36 bytes at V = 1 forward).
+// lane twice over: the most without spills (but for 28 bytes at V = 1 forward, of 16-bit types).
 // Backward at four waves instead of three spills 88 bytes and takes 50 us for 38
 // (237M training pass).
 constexpr int tile_waves(bool back, uint32_t words) {

@@ -55,7 +55,8 @@ extern "C" {
  *   YARN    { factor, original length L, fast turns, slow turns }: pairs that
  *           turn more often than `fast` over L keep f_i, those below `slow`
  *           take f_i / factor, linear in i between floor and ceil of
- *           R ln(L / (2 pi turns)) / (2 ln base); magnitude 0.1 ln(factor) + 1
+ *           R ln(L / (2 pi turns)) / (2 ln base), held to 0 and R - 1;
+ *           magnitude 0.1 ln(factor) + 1, and 1 for a factor up to 1
  *   BANDS   { factor, original length L, low, high }: with n = L f_i / (2 pi)
  *           turns, f_i where n > high, f_i / factor where n < low, and between
  *           them linear in n
