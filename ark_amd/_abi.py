@@ -154,5 +154,20 @@ ROPE_SCALE_YARN = 3
 ROPE_SCALE_BANDS = 4
 
 
+# include/ark_head.h
+HEAD_F16 = 0
+HEAD_BF16 = 1
+HEAD_F32 = 2
+HEAD_MAX_TOP = 256
+HEAD_ACCUMULATE = 1
+
+
+# include/ark_embed.h
+EMBED_F16 = 0
+EMBED_BF16 = 1
+EMBED_F32 = 2
+EMBED_ACCUMULATE = 1
+
+
 # every struct whose size ark_opt_struct_sizes reports, in its order
 ALL_STRUCTS = STRUCTS + (CodecSpan, CkptRecord, CkptInfo, GradSpan)

@@ -99,6 +99,19 @@ def _declare(L):
                           C.c_int),
         "ark_rope_norm_backward": ([H, u32, u64, u64, P, u32, u64, f32, P, P, u32] + [P] * 16
                                    + [u32, P], C.c_int),
+        "ark_head_workspace": ([P, u64, u64, u64, u64, u64, u32, u32, C.POINTER(u64)], C.c_int),
+        "ark_head_cross_entropy": ([P, u64, P, u64, u32, u64, u64, u64, P, u32, i32, f32, P, P, u64,
+                                    P], C.c_int),
+        "ark_head_cross_entropy_grad": ([P, u64, P, u64, u32, u64, u64, u64, P, u32, i32, f32, f32,
+                                         P, P, P, u64, P, u32, u64, u32, P, u64, P], C.c_int),
+        "ark_head_distill": ([P, u64, P, u64, u32, u64, u64, u64, P, u32, u64, P, u32, u64, u64, f32,
+                              P, P, u64, P], C.c_int),
+        "ark_head_distill_grad": ([P, u64, P, u64, u32, u64, u64, u64, P, u32, u64, P, u32, u64, u64,
+                                   f32, f32, P, P, P, u64, P, u32, u64, u32, P, u64, P], C.c_int),
+        "ark_embed_lookup": ([P, u64, u32, u64, u64, P, u32, u64, f32, P, u64, u32, P], C.c_int),
+        "ark_embed_grad_workspace": ([u64, u64, u64, C.POINTER(u64)], C.c_int),
+        "ark_embed_grad": ([P, u64, u32, P, u32, u64, u64, u64, f32, P, u64, u32, P, u64, P],
+                           C.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)

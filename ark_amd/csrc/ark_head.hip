@@ -1,0 +1,1104 @@
+// ark_head.hip -- the loss over a vocabulary and its gradients, and distillation
+// from a teacher's top logits (include/ark_head.h).
+//
+// With live rows X (the tokens that have a loss, copied together), the output
+// layer W and sparse targets p, a piece of the tokens takes these steps:
+//
+//   gather_kernel   X, padded to whole steps of the products, and where its rows
+//                   come from; zeros for the tokens without a loss
+//   dots_kernel     z at the targets, in fp32: X_t . W_index
+//   logits_kernel   z = scale X W^T in tiles that stay in registers; of every row
+//                   and span of the vocabulary its largest z and its sum of
+//                   exp(z - largest), and with gradients the exponentials
+//                   themselves, in 16 bits: 2^-9 or 2^-12 of each
+//   loss_kernel     the spans' sums joined: log(sum exp z), the loss
+//   dz_kernel       the same, and the exponentials turned into dz where they lie
+//   product_kernel  dx = dz W and dw = dz^T X
+//
+// The sums over spans make one pass over the vocabulary do: a span's exponentials
+// are relative to its own largest logit, as a row's is not known yet, and take the
+// row's scale when dz is formed.
+#include <math.h>
+
+#include <atomic>
+
+#include "ark_act.hpp"
+#include "ark_common.hpp"
+#include "ark_head.h"
+#include "ark_product.hpp"
+
+namespace {
+
+using namespace ark::dev;
+using ark::fail;
+
+constexpr uint32_t kLanes = 256;
+constexpr uint32_t kRowPad = 256;   // rows of a piece are laid out for whole tiles
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr uint32_t kGatherRows = 32;  // tokens a block of gather_kernel takes
+
+// What a piece's kernels leave for each other.
+struct Meta {
+  uint32_t live;  // rows with a loss
+  float alpha;    // dz is dz * 1 / alpha
+};
+
+template <typename T>
+constexpr uint32_t kTypeOf = sizeof(T) == 4 ? ARK_HEAD_F32 : ARK_HEAD_F16;
+template <>
+constexpr uint32_t kTypeOf<__bf16> = ARK_HEAD_BF16;
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+  return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+__device__ __forceinline__ int64_t ld_int(const void* p, uint32_t bytes, uint64_t i) {
+  return bytes == 8 ? ld_g<int64_t>((const int64_t*)p + i) : ld_g<int32_t>((const int32_t*)p + i);
+}
+__device__ __forceinline__ float ld_float(const void* p, uint32_t dtype, uint64_t i) {
+  if (dtype == ARK_HEAD_F32) return ld_g<float>((const float*)p + i);
+  const uint32_t h = ld_g<uint16_t>((const uint16_t*)p + i);
+  return dtype == ARK_HEAD_BF16 ? __uint_as_float(h << 16) : h2f(h);
+}
+
+// Where a token's targets are: one each (cross entropy), or what teacher_kernel
+// left of a teacher's entries.
+struct Targets {
+  const void* targets;  // NULL: a teacher's
+  uint32_t bytes;
+  int64_t ignore;
+  const uint32_t* index;  // [tokens][top], ~0: left out
+  const float* p;         // [tokens][top]
+  const float* self;      // [tokens] sum of p log p
+  const uint32_t* there;  // [tokens]
+  uint32_t top, vocab;
+
+  __device__ __forceinline__ bool live(uint32_t t) const {
+    if (!targets) return ld_g<uint32_t>(there + t) != 0;
+    const int64_t y = ld_int(targets, bytes, t);
+    return y != ignore && y >= 0 && y < (int64_t)vocab;
+  }
+  __device__ __forceinline__ uint32_t at(uint32_t t, uint32_t k) const {
+    return targets ? (uint32_t)ld_int(targets, bytes, t) : ld_g<uint32_t>(index + (uint64_t)t * top + k);
+  }
+  __device__ __forceinline__ float weight(uint32_t t, uint32_t k) const {
+    return targets ? 1.0f : ld_g<float>(p + (uint64_t)t * top + k);
+  }
+};
+
+// A teacher's distribution, a wave a token.
+__global__ __launch_bounds__(kLanes) void teacher_kernel(
+    const void* __restrict__ index, uint32_t index_bytes, uint64_t index_stride,
+    const void* __restrict__ logits, uint32_t dtype, uint64_t logits_stride, uint32_t tokens,
+    uint32_t top, uint32_t vocab, float scale, uint32_t* __restrict__ out, float* __restrict__ p,
+    float* __restrict__ self, uint32_t* __restrict__ there) {
+  const uint32_t t = blockIdx.x * (kLanes / 64) + threadIdx.x / 64, lane = threadIdx.x % 64;
+  if (t >= tokens) return;
+  constexpr uint32_t kEach = ARK_HEAD_MAX_TOP / 64;
+  float a[kEach], most = -INFINITY;
+  uint32_t id[kEach];
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i) {
+    const uint32_t k = i * 64 + lane;
+    id[i] = ~0u, a[i] = -INFINITY;
+    if (k < top) {
+      const int64_t v = ld_int(index, index_bytes, t * index_stride + k);
+      const float l = ld_float(logits, dtype, t * logits_stride + k) * scale;
+      if (v >= 0 && v < (int64_t)vocab && l != -INFINITY) id[i] = (uint32_t)v, a[i] = l;
+    }
+    most = fmaxf(most, a[i]);
+  }
+  most = wave_max(most);
+  float sum = 0.0f;
+  bool any = false;
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i)
+    if (id[i] != ~0u) a[i] -= most, sum += expf(a[i]), any = true;
+  sum = wave_sum(sum);
+  const float log_sum = logf(sum);
+  float own = 0.0f;
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i) {
+    const uint32_t k = i * 64 + lane;
+    float q = 0.0f;
+    if (id[i] != ~0u) {
+      q = expf(a[i]) / sum;
+      if (q != 0.0f) own += q * (a[i] - log_sum);
+    }
+    if (k < top) {
+      out[(uint64_t)t * top + k] = id[i];
+      p[(uint64_t)t * top + k] = q;
+    }
+  }
+  own = wave_sum(own);
+  const bool live = __ballot(any) != 0;
+  if (lane == 0) self[t] = own, there[t] = live ? 1u : 0u;
+}
+
+struct GatherArgs {
+  Targets targets;
+  const uint16_t* x;
+  uint64_t x_stride;
+  uint32_t tokens, columns, padded;  // padded: columns of out
+  uint32_t vec;                      // x takes 16-byte loads
+  uint16_t* out;
+  uint32_t* rows;
+  Meta* meta;
+  const float* grads;  // or NULL
+  float* largest;      // [blocks]: of |grads| over live tokens
+  float* loss;
+  uint16_t* dx;  // or NULL
+  uint64_t dx_stride;
+};
+
+// The live tokens' rows, in order.  A block counts the live tokens before its own
+// (a token's target is 4 or 8 bytes, its row thousands).
+__global__ __launch_bounds__(kLanes) void gather_kernel(GatherArgs a) {
+  __shared__ uint32_t s_count[kLanes / 64], s_live;
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const uint32_t t0 = blockIdx.x * kGatherRows;
+  uint32_t before = 0;
+  for (uint32_t t = threadIdx.x; t < t0; t += kLanes) before += a.targets.live(t) ? 1u : 0u;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) before += __shfl_xor(before, o);
+  if (lane == 0) s_count[wave] = before;
+  if (wave == 0) {
+    const uint32_t t = t0 + lane;
+    const bool live = lane < kGatherRows && t < a.tokens && a.targets.live(t);
+    const uint64_t mask = __ballot(live);
+    if (lane == 0) s_live = (uint32_t)mask;
+    if (a.grads) {
+      // as whole numbers, so that a NaN is the largest
+      uint32_t g = live ? __float_as_uint(a.grads[t]) & 0x7FFFFFFFu : 0u;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) g = max(g, (uint32_t)__shfl_xor(g, o));
+      if (lane == 0) a.largest[blockIdx.x] = __uint_as_float(g);
+    }
+  }
+  __syncthreads();
+  uint32_t base = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < kLanes / 64; ++w) base += s_count[w];
+  const uint32_t mask = s_live, n = base + __popc(mask);
+  for (uint32_t r = wave; r < kGatherRows && t0 + r < a.tokens; r += kLanes / 64) {
+    const uint32_t t = t0 + r;
+    if (!(mask >> r & 1u)) {
+      if (lane == 0) a.loss[t] = 0.0f;
+      if (a.dx)
+        for (uint32_t c = lane; c < a.columns; c += 64) a.dx[t * a.dx_stride + c] = 0;
+      continue;
+    }
+    const uint32_t to = base + __popc(mask & ((1u << r) - 1u));
+    if (lane == 0) a.rows[to] = t;
+    const uint16_t* src = a.x + t * a.x_stride;
+    uint16_t* dst = a.out + (uint64_t)to * a.padded;
+    if (a.vec) {
+      for (uint32_t c = lane * 8; c < a.columns; c += 512)
+        *(u32x4*)(dst + c) = ld_g<u32x4>(src + c);
+      for (uint32_t c = a.columns + lane; c < a.padded; c += 64) dst[c] = 0;
+    } else {
+      for (uint32_t c = lane; c < a.padded; c += 64) dst[c] = c < a.columns ? src[c] : 0;
+    }
+  }
+  if (blockIdx.x + 1 == gridDim.x) {
+    const uint32_t end = (n + kProductStep - 1) / kProductStep * kProductStep;
+    for (uint32_t r = n + wave; r < end; r += kLanes / 64)
+      for (uint32_t c = lane * 8; c < a.padded; c += 512)
+        *(u32x4*)(a.out + (uint64_t)r * a.padded + c) = u32x4{0, 0, 0, 0};
+    if (threadIdx.x == 0) a.meta->live = n;
+  }
+}
+
+// W's rows padded to whole steps, where its own cannot be read 16 bytes at a time.
+__global__ __launch_bounds__(kLanes) void pad_kernel(const uint16_t* __restrict__ w,
+                                                     uint64_t stride, uint32_t vocab,
+                                                     uint32_t columns, uint32_t padded,
+                                                     uint16_t* __restrict__ out) {
+  const uint32_t per = padded / 8;
+  const uint64_t all = (uint64_t)vocab * per;
+  for (uint64_t i = (uint64_t)blockIdx.x * kLanes + threadIdx.x; i < all;
+       i += (uint64_t)gridDim.x * kLanes) {
+    const uint64_t row = i / per;
+    const uint32_t c = (uint32_t)(i % per) * 8;
+    uint32_t v[8];
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k) v[k] = c + k < columns ? w[row * stride + c + k] : 0u;
+    *(u32x4*)(out + row * padded + c) =
+        u32x4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+  }
+}
+
+// z at the targets: a wave takes up to four of a row's.
+constexpr uint32_t kDots = 4;
+template <typename T>
+__global__ __launch_bounds__(kLanes) void dots_kernel(Targets targets,
+                                                      const uint16_t* __restrict__ x,
+                                                      uint32_t padded,
+                                                      const uint16_t* __restrict__ w,
+                                                      uint64_t w_stride,
+                                                      const uint32_t* __restrict__ rows,
+                                                      const Meta* __restrict__ meta, float scale,
+                                                      float* __restrict__ z) {
+  typedef T V __attribute__((ext_vector_type(8)));
+  const uint32_t lane = threadIdx.x % 64;
+  const uint32_t per = (targets.top + kDots - 1) / kDots;
+  const uint64_t id = (uint64_t)blockIdx.x * (kLanes / 64) + threadIdx.x / 64;
+  const uint32_t row = (uint32_t)(id / per), k0 = (uint32_t)(id % per) * kDots;
+  if (row >= meta->live) return;
+  const uint32_t t = rows[row], n = min(targets.top - k0, kDots);
+  const uint16_t* xr = x + (uint64_t)row * padded;
+  const uint16_t* wr[kDots];
+  bool there[kDots];
+#pragma unroll
+  for (uint32_t k = 0; k < kDots; ++k) {
+    const uint32_t v = k < n ? targets.at(t, k0 + k) : ~0u;
+    there[k] = v != ~0u;
+    wr[k] = w + (uint64_t)(there[k] ? v : 0u) * w_stride;
+  }
+  float s[kDots] = {};
+  for (uint32_t c = lane * 8; c < padded; c += 512) {
+    const V a = *(const V*)(xr + c);
+#pragma unroll
+    for (uint32_t k = 0; k < kDots; ++k) {
+      if (!there[k]) continue;
+      const V b = *(const V*)(wr[k] + c);
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) s[k] = __builtin_fmaf((float)a[i], (float)b[i], s[k]);
+    }
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < kDots; ++k) {
+    const float v = wave_sum(s[k]) * scale;
+    if (lane == 0 && k < n) z[(uint64_t)row * targets.top + k0 + k] = v;
+  }
+}
+
+// The tile of a block: blocks of one XCD (every eighth) take neighbouring tiles,
+// and these go through eight tiles of rows for every tile of columns, so that the
+// operands of those that run together are few.
+struct Tiles {
+  uint32_t m, n;
+  __device__ __forceinline__ void find(uint32_t block, uint32_t blocks, uint32_t* tm,
+                                       uint32_t* tn, uint32_t* split) const {
+    const uint32_t per = blocks / 8, rest = blocks % 8, xcd = block % 8;
+    const uint32_t id = xcd * per + min(xcd, rest) + block / 8, tiles = m * n;
+    *split = id / tiles;
+    const uint32_t tile = id % tiles, group = tile / (8 * m);
+    const uint32_t wide = min(n - group * 8, 8u), in = tile - group * 8 * m;
+    *tm = in / wide;
+    *tn = group * 8 + in % wide;
+  }
+};
+
+struct LogitsArgs {
+  const uint16_t *x, *w;
+  uint64_t w_stride;
+  uint32_t padded, vocab, spans;
+  uint64_t e_stride;
+  float scale;
+  Tiles tiles;
+  const Meta* meta;
+  float* stats;  // [row][span] of (largest, sum)
+  uint16_t* e;   // [row][e_stride], or NULL
+};
+
+template <typename P>
+__global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {
+  extern __shared__ __align__(1024) uint8_t lds[];
+  uint32_t tm, tn, split;
+  a.tiles.find(blockIdx.x, gridDim.x, &tm, &tn, &split);
+  const uint32_t live = a.meta->live, m0 = tm * P::BM, n0 = tn * P::BN;
+  if (n0 >= live) return;
+  P p;
+  const Operand ow = {a.w + m0 * a.w_stride, a.w_stride, a.vocab - m0, 0};
+  const Operand ox = {a.x + (uint64_t)n0 * a.padded, a.padded, P::BN, 0};
+  p.run(ow, ox, 0, a.padded / kProductStep, (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds);
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const uint32_t v0 = m0 + wave % P::WM * 16 * P::MF + lane / 16 * 4;
+  const uint32_t span = tm * P::WM + wave % P::WM;
+#pragma unroll
+  for (uint32_t j = 0; j < P::NF; ++j) {
+    const uint32_t t = n0 + wave / P::WM * 16 * P::NF + j * 16 + lane % 16;
+    float most = -INFINITY;
+#pragma unroll
+    for (uint32_t i = 0; i < P::MF; ++i)
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) {
+        float z = p.acc[i][j][k] * a.scale;
+        if (v0 + i * 16 + k >= a.vocab) z = -INFINITY;
+        p.acc[i][j][k] = z;
+        most = fmaxf(most, z);
+      }
+    most = fmaxf(most, __shfl_xor(most, 16));
+    most = fmaxf(most, __shfl_xor(most, 32));
+    const float from = most == -INFINITY ? 0.0f : most;
+    float sum = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < P::MF; ++i)
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) {
+        const float e = exp_of(p.acc[i][j][k] - from);
+        p.acc[i][j][k] = e;
+        sum += e;
+      }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (t >= live) continue;
+    if (lane < 16) {
+      float* s = a.stats + ((uint64_t)t * a.spans + span) * 2;
+      s[0] = most, s[1] = sum;
+    }
+    if (a.e) {
+      uint16_t* e = a.e + t * a.e_stride + v0;
+#pragma unroll
+      for (uint32_t i = 0; i < P::MF; ++i) {
+        const f32x4 v = p.acc[i][j];
+        st_g<u32x2>(e + i * 16, u32x2{narrow2<kTypeOf<typename P::T>>(v[0], v[1]),
+                                      narrow2<kTypeOf<typename P::T>>(v[2], v[3])});
+      }
+    }
+  }
+}
+
+// log of the sum of a row's exponentials, from its spans, by `lanes` lanes of a
+// block (a wave or all of it; red: a value a wave).
+template <uint32_t LANES>
+__device__ __forceinline__ float join_spans(const float* stats, uint32_t spans, uint32_t lane,
+                                            float* red) {
+  float most = -INFINITY;
+  for (uint32_t i = lane; i < spans; i += LANES) most = fmaxf(most, stats[2 * i]);
+  most = wave_max(most);
+  if constexpr (LANES > 64) {
+    if (lane % 64 == 0) red[lane / 64] = most;
+    __syncthreads();
+    for (uint32_t w = 0; w < LANES / 64; ++w) most = fmaxf(most, red[w]);
+    __syncthreads();
+  }
+  float sum = 0.0f;
+  for (uint32_t i = lane; i < spans; i += LANES) sum += stats[2 * i + 1] * expf(stats[2 * i] - most);
+  sum = wave_sum(sum);
+  if constexpr (LANES > 64) {
+    if (lane % 64 == 0) red[lane / 64] = sum;
+    __syncthreads();
+    sum = 0.0f;
+    for (uint32_t w = 0; w < LANES / 64; ++w) sum += red[w];
+    __syncthreads();
+  }
+  return most + logf(sum);
+}
+
+// A token's loss: sum of p (log p - log q), by a wave.
+__device__ __forceinline__ float row_loss(const Targets& g, uint32_t t, const float* z, float lse,
+                                          uint32_t lane) {
+  float s = 0.0f;
+  for (uint32_t k = lane; k < g.top; k += 64) {
+    const float p = g.weight(t, k);
+    if (p != 0.0f) s += p * (lse - z[k]);
+  }
+  s = wave_sum(s);
+  return g.targets ? s : s + g.self[t];
+}
+
+struct LossArgs {
+  Targets targets;
+  const uint32_t* rows;
+  const Meta* meta;
+  const float* stats;
+  uint32_t spans;
+  const float* z;
+  float* loss;
+};
+
+__global__ __launch_bounds__(kLanes) void loss_kernel(LossArgs a) {
+  const uint32_t row = blockIdx.x * (kLanes / 64) + threadIdx.x / 64, lane = threadIdx.x % 64;
+  if (row >= a.meta->live) return;
+  const uint32_t t = a.rows[row];
+  const float lse = join_spans<64>(a.stats + (uint64_t)row * a.spans * 2, a.spans, lane, nullptr);
+  const float loss = row_loss(a.targets, t, a.z + (uint64_t)row * a.targets.top, lse, lane);
+  if (lane == 0) a.loss[t] = loss;
+}
+
+struct DzArgs {
+  LossArgs loss;
+  Meta* meta;
+  const float* grads;    // or NULL
+  const float* largest;  // [parts]
+  uint32_t parts;
+  float grad, scale;
+  uint16_t* e;
+  uint64_t e_stride;
+  uint32_t span;  // values a span covers
+};
+
+// A row's exponentials to dz, a block a row; rows past the live ones, up to a
+// whole step of the products, to zeros.
+template <typename T>
+__global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
+  typedef T V __attribute__((ext_vector_type(8)));
+  constexpr uint32_t DT = kTypeOf<T>;
+  __shared__ float red[kLanes / 64];
+  __shared__ uint32_t s_index[ARK_HEAD_MAX_TOP];
+  __shared__ float s_p[ARK_HEAD_MAX_TOP];
+  const LossArgs& l = a.loss;
+  const uint32_t row = blockIdx.x, live = l.meta->live, tid = threadIdx.x;
+  // the largest |grad * scale| times 2^shift lies in [2^13, 2^14)
+  float largest = fabsf(a.grad);
+  if (a.grads) {
+    uint32_t m = 0;
+    for (uint32_t i = tid % 64; i < a.parts; i += 64) m = max(m, __float_as_uint(a.largest[i]));
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = max(m, (uint32_t)__shfl_xor(m, o));
+    largest = __uint_as_float(m);
+  }
+  largest *= fabsf(a.scale);
+  int shift = 0;
+  if (largest > 0.0f && largest < INFINITY) shift = min(max(14 - ilogbf(largest) - 1, -100), 100);
+  if (row == 0 && tid == 0) a.meta->alpha = ldexpf(1.0f, -shift);
+  if (row >= (live + kProductStep - 1) / kProductStep * kProductStep) return;
+  uint16_t* e = a.e + row * a.e_stride;
+  if (row >= live) {
+    for (uint32_t c = tid * 8; c < a.e_stride; c += kLanes * 8) *(u32x4*)(e + c) = u32x4{0, 0, 0, 0};
+    return;
+  }
+  const uint32_t t = l.rows[row], top = l.targets.top;
+  const float* stats = l.stats + (uint64_t)row * l.spans * 2;
+  const float* z = l.z + (uint64_t)row * top;
+  const float lse = join_spans<kLanes>(stats, l.spans, tid, red);
+  if (tid < 64) {
+    const float loss = row_loss(l.targets, t, z, lse, tid);
+    if (tid == 0) l.loss[t] = loss;
+  }
+  const float f = ldexpf((a.grads ? a.grads[t] : a.grad) * a.scale, shift);
+  for (uint32_t k = tid; k < top; k += kLanes) {
+    s_index[k] = l.targets.at(t, k);
+    s_p[k] = l.targets.weight(t, k);
+  }
+  for (uint32_t c = tid * 8; c < a.e_stride; c += kLanes * 8) {
+    const float s = expf(stats[c / a.span * 2] - lse) * f;
+    const V v = *(const V*)(e + c);
+    u32x4 o;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+      o[i] = narrow2<DT>((float)v[2 * i] * s, (float)v[2 * i + 1] * s);
+    *(u32x4*)(e + c) = o;
+  }
+  __syncthreads();
+  // the targets' own entries, from fp32 (an index that comes twice writes the same
+  // value twice)
+  for (uint32_t k = tid; k < top; k += kLanes) {
+    const uint32_t v = s_index[k];
+    if (v == ~0u) continue;
+    float p = 0.0f;
+    for (uint32_t i = 0; i < top; ++i) p += s_index[i] == v ? s_p[i] : 0.0f;
+    // q - p without the difference of two numbers near 1
+    const float d = (expm1f(z[k] - lse) + (1.0f - p)) * f;
+    e[v] = (uint16_t)narrow2<DT>(d, 0.0f);
+  }
+}
+
+// Where a product goes.
+struct Out {
+  void* p;         // fp32 or 16 bits
+  uint64_t stride;
+  uint32_t dtype, vec;      // vec: takes four values at a time
+  const float* add;         // fp32 to add, of `add_stride`, or NULL
+  uint64_t add_stride;
+  const uint32_t* rows;     // row n goes to rows[n], or NULL
+  uint32_t width, height;   // m and n that are stored
+  const Meta* meta;
+
+  __device__ __forceinline__ void put(uint32_t n, uint32_t m, f32x4 v) const {
+    v *= meta->alpha;
+    const uint64_t row = rows ? rows[n] : n;
+    const uint32_t c = min(width - m, 4u);
+    if (add) {
+      const float* q = add + row * add_stride + m;
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k)
+        if (k < c) v[k] += q[k];
+    }
+    if (dtype == ARK_HEAD_F32) {
+      float* q = (float*)p + row * stride + m;
+      if (vec && c == 4) {
+        *(f32x4*)q = v;
+        return;
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k)
+        if (k < c) q[k] = v[k];
+      return;
+    }
+    const u32x2 h = dtype == ARK_HEAD_F16
+                        ? u32x2{narrow2<ARK_ACT_F16>(v[0], v[1]), narrow2<ARK_ACT_F16>(v[2], v[3])}
+                        : u32x2{narrow2<ARK_ACT_BF16>(v[0], v[1]), narrow2<ARK_ACT_BF16>(v[2], v[3])};
+    uint16_t* q = (uint16_t*)p + row * stride + m;
+    if (vec && c == 4) {
+      *(u32x2*)q = h;
+      return;
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+      if (k < c) q[k] = (uint16_t)(h[k / 2] >> (k % 2 * 16));
+  }
+};
+
+// dx (DX: a = W across its rows, b = dz along them) or dw (a = X, b = dz, both
+// across).
+struct ProductArgs {
+  const uint16_t *a, *b;
+  uint64_t a_stride, b_stride;
+  uint32_t a_width;   // values of a row of a
+  uint32_t b_width;   // dw: of a row of b
+  uint32_t a_rows;    // dx: rows of W
+  Tiles tiles;
+  uint32_t splits;
+  float* partial;     // [split][height][width up to 4], or NULL
+  const Meta* meta;
+  Out out;
+};
+
+template <typename P, bool DX>
+__global__ __launch_bounds__(P::kLanes, 2) void product_kernel(ProductArgs g) {
+  extern __shared__ __align__(1024) uint8_t lds[];
+  uint32_t tm, tn, split;
+  g.tiles.find(blockIdx.x, gridDim.x, &tm, &tn, &split);
+  const uint32_t live = g.meta->live, m0 = tm * P::BM, n0 = tn * P::BN;
+  if (DX && n0 >= live) return;
+  const uint32_t ks = DX ? g.a_rows : (live + kProductStep - 1) / kProductStep * kProductStep;
+  const uint32_t steps = (ks + kProductStep - 1) / kProductStep;
+  const uint32_t s0 = (uint32_t)((uint64_t)steps * split / g.splits);
+  const uint32_t s1 = (uint32_t)((uint64_t)steps * (split + 1) / g.splits);
+  P p;
+  const Operand oa = {g.a + m0, g.a_stride, g.a_width - m0, ks};
+  const Operand ob = DX ? Operand{g.b + n0 * g.b_stride, g.b_stride, P::BN, 0}
+                        : Operand{g.b + n0, g.b_stride, g.b_width - n0, ks};
+  p.run(oa, ob, s0, s1, (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds);
+  const uint32_t height = DX ? min(live, g.out.height) : g.out.height;
+  const uint64_t w4 = (g.out.width + 3) / 4 * 4;
+  p.each([&](uint32_t m, uint32_t n, f32x4 v) __attribute__((always_inline)) {
+    m += m0, n += n0;
+    if (m >= g.out.width || n >= height) return;
+    if (g.partial)
+      *(f32x4*)(g.partial + ((uint64_t)split * g.out.height + n) * w4 + m) = v;
+    else
+      g.out.put(n, m, v);
+  });
+}
+
+// The splits' partial products, added in order.
+__global__ __launch_bounds__(kLanes) void join_kernel(const float* __restrict__ partial,
+                                                      uint32_t splits, uint32_t live_rows, Out out) {
+  const uint32_t per = (out.width + 3) / 4;
+  const uint32_t height = live_rows ? min(out.meta->live, out.height) : out.height;
+  const uint64_t all = (uint64_t)height * per, step = (uint64_t)out.height * per;
+  for (uint64_t i = (uint64_t)blockIdx.x * kLanes + threadIdx.x; i < all;
+       i += (uint64_t)gridDim.x * kLanes) {
+    const f32x4* p = (const f32x4*)partial + i;
+    f32x4 v = p[0];
+    for (uint32_t s = 1; s < splits; ++s) v += p[s * step];
+    out.put((uint32_t)(i / per), (uint32_t)(i % per) * 4, v);
+  }
+}
+
+// ---- host -------------------------------------------------------------------
+
+constexpr uint64_t kDzBytes = 1ull << 30;  // of a piece's dz, at most
+
+struct Big {
+  template <typename T, bool AMC, bool BMC>
+  using P = Product<T, AMC, BMC, 8, 4, 2, 4>;
+};
+struct Small {
+  template <typename T, bool AMC, bool BMC>
+  using P = Product<T, AMC, BMC, 4, 2, 2, 2>;
+};
+
+constexpr uint32_t kMaxSplits = 32;
+
+// How a call is cut, and where things lie in its workspace (offsets of 256).
+struct Plan {
+  bool small;                   // tiles
+  uint32_t piece;               // tokens
+  uint32_t pieces;
+  uint32_t padded;              // columns
+  bool copy_w;
+  uint32_t bm, bn, span, spans;
+  uint64_t e_stride;
+  uint32_t dx_splits, dw_splits;
+  uint64_t meta, rows, largest, index, p, self, there, z, x, w, stats, e, partial, dw, bytes;
+};
+
+uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
+
+uint32_t splits_of(uint64_t tiles, uint64_t steps) {
+  uint64_t s = 1;
+  while (s < kMaxSplits && tiles * s < 256 && steps >= s * 8) s *= 2;
+  return (uint32_t)s;
+}
+
+Plan plan_of(const void* w, uint64_t w_stride, uint64_t tokens, uint64_t columns, uint64_t vocab,
+             uint64_t top, uint32_t dw_dtype, bool grad) {
+  Plan p = {};
+  p.small = tokens <= 64;
+  p.bm = p.small ? 128 : 256, p.bn = p.small ? 64 : 256;
+  p.span = p.small ? 64 : 128;
+  p.e_stride = up(vocab, p.bm);
+  p.spans = (uint32_t)(up(vocab, p.bm) / p.span);
+  p.padded = (uint32_t)up(columns, kProductStep);
+  p.copy_w = columns % kProductStep || w_stride % 8 || (uintptr_t)w % 16;
+  // pieces of equal sizes, whole tiles
+  uint64_t most = grad ? kDzBytes / (p.e_stride * 2) / kRowPad * kRowPad : 16384;
+  if (most < kRowPad) most = kRowPad;
+  if (most > 16384) most = 16384;
+  p.pieces = (uint32_t)((tokens + most - 1) / most);
+  if (p.pieces == 0) p.pieces = 1;
+  p.piece = (uint32_t)(p.pieces == 1 ? tokens : up((tokens + p.pieces - 1) / p.pieces, kRowPad));
+  const uint64_t rows = up(p.piece ? p.piece : 1, kRowPad);
+  uint64_t at = 0;
+  const auto take = [&](uint64_t bytes) {
+    const uint64_t here = at;
+    at += up(bytes, 256);
+    return here;
+  };
+  p.meta = take(sizeof(Meta));
+  p.rows = take(rows * 4);
+  p.largest = take((rows / kGatherRows) * 4);
+  p.index = take(rows * top * 4);
+  p.p = take(rows * top * 4);
+  p.self = take(rows * 4);
+  p.there = take(rows * 4);
+  p.z = take(rows * top * 4);
+  p.x = take(rows * p.padded * 2);
+  p.w = take(p.copy_w ? vocab * p.padded * 2 : 0);
+  p.stats = take(rows * p.spans * 8);
+  if (grad) {
+    p.e = take(rows * p.e_stride * 2);
+    const uint64_t mt = (columns + p.bm - 1) / p.bm, w4 = up(columns, 4);
+    p.dx_splits = splits_of(mt * ((p.piece + p.bn - 1) / p.bn), (vocab + 63) / 64);
+    p.dw_splits = splits_of(mt * ((vocab + p.bn - 1) / p.bn), rows / 64);
+    const uint64_t a = p.dx_splits > 1 ? p.dx_splits * p.piece * w4 * 4 : 0;
+    const uint64_t b = p.dw_splits > 1 ? p.dw_splits * vocab * w4 * 4 : 0;
+    p.partial = take(a > b ? a : b);
+    p.dw = take(dw_dtype != ARK_HEAD_F32 && p.pieces > 1 ? vocab * columns * 4 : 0);
+  }
+  p.bytes = at;
+  return p;
+}
+
+struct Call {
+  const void* x;
+  uint64_t x_stride;
+  const void* w;
+  uint64_t w_stride;
+  uint32_t dtype;
+  uint64_t tokens, columns, vocab;
+  const void* targets;  // NULL: a teacher's entries
+  uint32_t target_bytes;
+  int64_t ignore;
+  const void* index;
+  uint32_t index_bytes;
+  uint64_t index_stride;
+  const void* logits;
+  uint32_t logits_dtype;
+  uint64_t logits_stride, top;
+  float scale;
+  bool with_grad;
+  float grad;
+  const float* grads;
+  float* loss;
+  void* dx;
+  uint64_t dx_stride;
+  void* dw;
+  uint32_t dw_dtype;
+  uint64_t dw_stride;
+  uint32_t flags;
+  char* ws;
+  uint64_t ws_bytes;
+  hipStream_t stream;
+  bool teacher;
+};
+
+template <typename K>
+int with_lds(K kernel, uint32_t bytes, std::atomic<uint64_t>* ready) {
+  int dev = 0;
+  ARK_HIP(hipGetDevice(&dev));
+  if (dev >= 64 || !(ready->load(std::memory_order_relaxed) >> dev & 1u)) {
+    ARK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)bytes));
+    if (dev < 64) ready->fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  return ARK_OPT_OK;
+}
+
+template <typename P>
+int launch_logits(const LogitsArgs& a, hipStream_t s) {
+  static std::atomic<uint64_t> ready{0};
+  if (int rc = with_lds(logits_kernel<P>, P::kLds, &ready)) return rc;
+  hipLaunchKernelGGL(logits_kernel<P>, dim3(a.tiles.m * a.tiles.n), dim3(P::kLanes), P::kLds, s, a);
+  ARK_HIP(hipGetLastError());
+  return ARK_OPT_OK;
+}
+
+template <typename P, bool DX>
+int launch_product(const ProductArgs& g, hipStream_t s) {
+  static std::atomic<uint64_t> ready{0};
+  if (int rc = with_lds(product_kernel<P, DX>, P::kLds, &ready)) return rc;
+  hipLaunchKernelGGL((product_kernel<P, DX>), dim3(g.tiles.m * g.tiles.n * g.splits),
+                     dim3(P::kLanes), P::kLds, s, g);
+  ARK_HIP(hipGetLastError());
+  if (g.splits > 1) {
+    const uint64_t n = (uint64_t)g.out.height * ((g.out.width + 3) / 4);
+    const uint64_t blocks = (n + kLanes - 1) / kLanes;
+    hipLaunchKernelGGL(join_kernel, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(kLanes),
+                       0, s, (const float*)g.partial, g.splits, DX ? 1u : 0u, g.out);
+    ARK_HIP(hipGetLastError());
+  }
+  return ARK_OPT_OK;
+}
+
+template <typename T, typename Size>
+int run_piece(const Call& c, const Plan& p, uint32_t piece) {
+  const hipStream_t s = c.stream;
+  const uint64_t t0 = (uint64_t)piece * p.piece;
+  const uint32_t tokens = (uint32_t)(c.tokens - t0 < p.piece ? c.tokens - t0 : p.piece);
+  const uint32_t top = (uint32_t)c.top;
+  char* ws = c.ws;
+  Meta* meta = (Meta*)(ws + p.meta);
+  uint32_t* rows = (uint32_t*)(ws + p.rows);
+  uint16_t* x = (uint16_t*)(ws + p.x);
+  float* z = (float*)(ws + p.z);
+  Targets g = {};
+  g.top = top;
+  g.vocab = (uint32_t)c.vocab;
+  if (c.teacher) {
+    uint32_t* index = (uint32_t*)(ws + p.index);
+    float *q = (float*)(ws + p.p), *self = (float*)(ws + p.self);
+    uint32_t* there = (uint32_t*)(ws + p.there);
+    if (tokens) {
+      hipLaunchKernelGGL(teacher_kernel, dim3((tokens + 3) / 4), dim3(kLanes), 0, s,
+                         (const char*)c.index + t0 * c.index_stride * c.index_bytes,
+                         c.index_bytes, c.index_stride,
+                         (const char*)c.logits +
+                             t0 * c.logits_stride * ark::act_elem_size(c.logits_dtype),
+                         c.logits_dtype, c.logits_stride, tokens, top, (uint32_t)c.vocab, c.scale,
+                         index, q, self, there);
+      ARK_HIP(hipGetLastError());
+    }
+    g.index = index, g.p = q, g.self = self, g.there = there;
+  } else {
+    g.targets = (const char*)c.targets + t0 * c.target_bytes;
+    g.bytes = c.target_bytes;
+    g.ignore = c.ignore;
+  }
+  // one block of these runs also without a token, for dw's zeros
+  const uint32_t gather_blocks = tokens ? (tokens + kGatherRows - 1) / kGatherRows : 1;
+  GatherArgs ga = {};
+  ga.targets = g;
+  ga.x = (const uint16_t*)c.x + t0 * c.x_stride;
+  ga.x_stride = c.x_stride;
+  ga.tokens = tokens;
+  ga.columns = (uint32_t)c.columns;
+  ga.padded = p.padded;
+  ga.vec = c.x_stride % 8 == 0 && (uintptr_t)c.x % 16 == 0 && c.columns % 8 == 0;
+  ga.out = x;
+  ga.rows = rows;
+  ga.meta = meta;
+  ga.grads = c.grads ? c.grads + t0 : nullptr;
+  ga.largest = (float*)(ws + p.largest);
+  ga.loss = c.loss + t0;
+  ga.dx = c.dx ? (uint16_t*)c.dx + t0 * c.dx_stride : nullptr;
+  ga.dx_stride = c.dx_stride;
+  hipLaunchKernelGGL(gather_kernel, dim3(gather_blocks), dim3(kLanes), 0, s, ga);
+  ARK_HIP(hipGetLastError());
+  const uint16_t* w = p.copy_w ? (const uint16_t*)(ws + p.w) : (const uint16_t*)c.w;
+  const uint64_t w_stride = p.copy_w ? p.padded : c.w_stride;
+  const uint64_t waves = (uint64_t)tokens * ((top + kDots - 1) / kDots);
+  if (tokens) {
+    hipLaunchKernelGGL(dots_kernel<T>, dim3((uint32_t)((waves + 3) / 4)), dim3(kLanes), 0, s, g,
+                       (const uint16_t*)x, p.padded, w, w_stride, (const uint32_t*)rows,
+                       (const Meta*)meta, c.scale, z);
+    ARK_HIP(hipGetLastError());
+  }
+  LogitsArgs la = {};
+  la.x = x, la.w = w, la.w_stride = w_stride;
+  la.padded = p.padded, la.vocab = (uint32_t)c.vocab, la.spans = p.spans;
+  la.e_stride = p.e_stride;
+  la.scale = c.scale;
+  la.tiles = {(uint32_t)((c.vocab + p.bm - 1) / p.bm), (tokens + p.bn - 1) / p.bn};
+  la.meta = meta;
+  la.stats = (float*)(ws + p.stats);
+  la.e = c.with_grad ? (uint16_t*)(ws + p.e) : nullptr;
+  int rc;
+  if (tokens && (rc = launch_logits<typename Size::template P<T, false, false>>(la, s))) return rc;
+  LossArgs lo = {g, rows, meta, la.stats, p.spans, z, ga.loss};
+  if (!c.with_grad) {  // with tokens, or run() ends before
+    hipLaunchKernelGGL(loss_kernel, dim3((tokens + 3) / 4), dim3(kLanes), 0, s, lo);
+    ARK_HIP(hipGetLastError());
+    return ARK_OPT_OK;
+  }
+  DzArgs da = {};
+  da.loss = lo, da.meta = meta, da.grads = ga.grads, da.largest = ga.largest;
+  da.parts = gather_blocks;
+  da.grad = c.grad, da.scale = c.scale;
+  da.e = la.e, da.e_stride = p.e_stride, da.span = p.span;
+  hipLaunchKernelGGL(dz_kernel<T>, dim3(tokens ? (uint32_t)up(tokens, kProductStep) : 1u), dim3(kLanes),
+                     0, s, da);
+  ARK_HIP(hipGetLastError());
+  ProductArgs pa = {};
+  pa.b = la.e, pa.b_stride = p.e_stride, pa.b_width = (uint32_t)p.e_stride;
+  pa.partial = nullptr;
+  pa.meta = meta;
+  Out& o = pa.out;
+  o.meta = meta;
+  o.width = (uint32_t)c.columns;
+  if (c.dx && tokens) {
+    pa.a = w, pa.a_stride = w_stride, pa.a_width = p.padded, pa.a_rows = (uint32_t)c.vocab;
+    pa.tiles = {(uint32_t)((c.columns + p.bm - 1) / p.bm), (tokens + p.bn - 1) / p.bn};
+    pa.splits = p.dx_splits;
+    pa.partial = pa.splits > 1 ? (float*)(ws + p.partial) : nullptr;
+    o.p = ga.dx, o.stride = c.dx_stride, o.dtype = c.dtype, o.rows = rows, o.height = tokens;
+    o.vec = c.dx_stride % 4 == 0 && (uintptr_t)c.dx % 8 == 0;
+    if ((rc = launch_product<typename Size::template P<T, true, false>, true>(pa, s))) return rc;
+  }
+  if (c.dw) {
+    pa.a = x, pa.a_stride = p.padded, pa.a_width = p.padded, pa.a_rows = 0;
+    pa.tiles = {(uint32_t)((c.columns + p.bm - 1) / p.bm), (uint32_t)((c.vocab + p.bn - 1) / p.bn)};
+    pa.splits = p.dw_splits;
+    pa.partial = pa.splits > 1 ? (float*)(ws + p.partial) : nullptr;
+    o.rows = nullptr, o.height = (uint32_t)c.vocab;
+    // fp32 sums over the pieces, in dw itself or beside it
+    const bool last = piece + 1 == p.pieces, wide = c.dw_dtype == ARK_HEAD_F32;
+    float* sums = wide ? (float*)c.dw : (float*)(ws + p.dw);
+    const uint64_t sums_stride = wide ? c.dw_stride : c.columns;
+    const bool add = piece > 0 || (c.flags & ARK_HEAD_ACCUMULATE);
+    o.add = add ? sums : nullptr, o.add_stride = sums_stride;
+    const bool final = wide || last;
+    o.p = final ? c.dw : (void*)sums;
+    o.stride = final ? c.dw_stride : sums_stride;
+    o.dtype = final ? c.dw_dtype : ARK_HEAD_F32;
+    o.vec = o.stride % 4 == 0 && (uintptr_t)o.p % 16 == 0;
+    if ((rc = launch_product<typename Size::template P<T, true, true>, false>(pa, s))) return rc;
+  }
+  return ARK_OPT_OK;
+}
+
+template <typename T>
+int run_call(const Call& c, const Plan& p) {
+  if (p.copy_w) {
+    const uint64_t n = c.vocab * (p.padded / 8), blocks = (n + kLanes - 1) / kLanes;
+    hipLaunchKernelGGL(pad_kernel, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(kLanes),
+                       0, c.stream, (const uint16_t*)c.w, c.w_stride, (uint32_t)c.vocab,
+                       (uint32_t)c.columns, p.padded, (uint16_t*)(c.ws + p.w));
+    ARK_HIP(hipGetLastError());
+  }
+  for (uint32_t i = 0; i < p.pieces; ++i) {
+    const int rc = p.small ? run_piece<T, Small>(c, p, i) : run_piece<T, Big>(c, p, i);
+    if (rc) return rc;
+  }
+  return ARK_OPT_OK;
+}
+
+// Bytes that rows x row elements at a row stride span; 0 for none.  Strides are
+// below 2^22 for what the products read themselves, 2^40 otherwise.
+int rows_bytes(uint64_t rows, uint64_t row, uint64_t stride, uint32_t es, bool written,
+               const char* what, uint64_t* bytes) {
+  *bytes = 0;
+  if (rows == 0 || row == 0) return ARK_OPT_OK;
+  if (rows > 1 && stride >= (1ull << 32))
+    return fail(ARK_OPT_EINVAL, "%s: stride %llu too large", what, (unsigned long long)stride);
+  if (written && rows > 1 && stride < row)
+    return fail(ARK_OPT_EINVAL, "%s: rows of %llu elements overlap at stride %llu", what,
+                (unsigned long long)row, (unsigned long long)stride);
+  *bytes = ((rows - 1) * stride + row) * es;
+  return ARK_OPT_OK;
+}
+
+int check_sizes(uint64_t tokens, uint64_t columns, uint64_t vocab, uint64_t top, uint32_t dw_dtype) {
+  if (dw_dtype > ARK_HEAD_F32) return fail(ARK_OPT_EINVAL, "dw_dtype %u unknown", dw_dtype);
+  if (tokens >= (1ull << 31))
+    return fail(ARK_OPT_EINVAL, "tokens = %llu too large", (unsigned long long)tokens);
+  if (columns == 0 || columns > 65536)
+    return fail(ARK_OPT_EINVAL, "columns = %llu: 1 to 65536", (unsigned long long)columns);
+  if (vocab == 0 || vocab > (1ull << 21))
+    return fail(ARK_OPT_EINVAL, "vocab = %llu: 1 to 2097152", (unsigned long long)vocab);
+  if (top == 0 || top > ARK_HEAD_MAX_TOP)
+    return fail(ARK_OPT_EINVAL, "top = %llu: 1 to %d", (unsigned long long)top, ARK_HEAD_MAX_TOP);
+  return ARK_OPT_OK;
+}
+
+struct Range {
+  const void* p;
+  uint64_t bytes;
+  const char* what;
+};
+
+int run(Call c) {
+  int rc;
+  if (c.dtype != ARK_HEAD_F16 && c.dtype != ARK_HEAD_BF16)
+    return fail(ARK_OPT_EINVAL, "dtype %u: x and w are fp16 or bf16", c.dtype);
+  if ((rc = check_sizes(c.tokens, c.columns, c.vocab, c.top, c.dw ? c.dw_dtype : c.dtype)))
+    return rc;
+  if (c.dw && c.dw_dtype != ARK_HEAD_F32 && c.dw_dtype != c.dtype)
+    return fail(ARK_OPT_EINVAL, "dw_dtype %u: fp32, or that of w", c.dw_dtype);
+  if (c.flags & ~ARK_HEAD_ACCUMULATE) return fail(ARK_OPT_EINVAL, "flags %#x unknown", c.flags);
+  if ((c.flags & ARK_HEAD_ACCUMULATE) && c.dw && c.dw_dtype != ARK_HEAD_F32)
+    return fail(ARK_OPT_EINVAL, "only an fp32 dw can be added to");
+  const uint32_t ib = c.teacher ? c.index_bytes : c.target_bytes;
+  if (ib != 4 && ib != 8)
+    return fail(ARK_OPT_EINVAL, "%s of %u bytes: 4 or 8", c.teacher ? "indices" : "targets", ib);
+  if (c.teacher && c.logits_dtype > ARK_HEAD_F32)
+    return fail(ARK_OPT_EINVAL, "logits_dtype %u unknown", c.logits_dtype);
+  if (!(c.scale > 0.0f) || !(c.scale < INFINITY))
+    return fail(ARK_OPT_EINVAL, "%s", c.teacher ? "temperature must be positive and finite, and so "
+                                                  "must its reciprocal"
+                                                : "scale must be positive and finite");
+  if (c.w_stride >= (1u << 22))
+    return fail(ARK_OPT_EINVAL, "w: stride %llu too large", (unsigned long long)c.w_stride);
+  const uint32_t les = c.teacher ? ark::act_elem_size(c.logits_dtype) : 1;
+  uint64_t xb, wb, tb = 0, ixb = 0, lgb = 0, dxb = 0, dwb = 0;
+  const uint32_t dwes = c.dw_dtype == ARK_HEAD_F32 ? 4 : 2;
+  if ((rc = rows_bytes(c.tokens, c.columns, c.x_stride, 2, false, "x", &xb)) ||
+      (rc = rows_bytes(c.vocab, c.columns, c.w_stride, 2, false, "w", &wb)))
+    return rc;
+  if (c.teacher) {
+    if ((rc = rows_bytes(c.tokens, c.top, c.index_stride, ib, false, "index", &ixb)) ||
+        (rc = rows_bytes(c.tokens, c.top, c.logits_stride, les, false, "logits", &lgb)))
+      return rc;
+  } else {
+    tb = c.tokens * ib;
+  }
+  if (c.dx && (rc = rows_bytes(c.tokens, c.columns, c.dx_stride, 2, true, "dx", &dxb))) return rc;
+  if (c.dw && (rc = rows_bytes(c.vocab, c.columns, c.dw_stride, dwes, true, "dw", &dwb))) return rc;
+  if ((uintptr_t)c.x % 2 || (uintptr_t)c.w % 2 || (uintptr_t)c.dx % 2 || (uintptr_t)c.dw % dwes ||
+      (uintptr_t)c.targets % ib || (uintptr_t)c.index % ib || (uintptr_t)c.logits % les ||
+      (uintptr_t)c.loss % 4 || (uintptr_t)c.grads % 4)
+    return fail(ARK_OPT_EINVAL, "an array is not aligned to its elements");
+  const Plan p = plan_of(c.w, c.w_stride, c.tokens, c.columns, c.vocab, c.top,
+                         c.dw ? c.dw_dtype : ARK_HEAD_F32, c.with_grad);
+  if (c.tokens == 0 && (!c.dw || (c.flags & ARK_HEAD_ACCUMULATE))) return ARK_OPT_OK;
+  if (c.ws_bytes < p.bytes)
+    return fail(ARK_OPT_EINVAL, "workspace of %llu B, %llu B needed",
+                (unsigned long long)c.ws_bytes, (unsigned long long)p.bytes);
+  if ((uintptr_t)c.ws % 16)
+    return fail(ARK_OPT_EINVAL, "workspace %p is not 16-byte aligned", (void*)c.ws);
+  const Range written[] = {{c.loss, c.tokens * 4, "loss"},
+                           {c.dx, dxb, "dx"},
+                           {c.dw, dwb, "dw"},
+                           {c.ws, p.bytes, "workspace"}};
+  const Range read[] = {{c.x, xb, "x"},           {c.w, wb, "w"},
+                        {c.targets, tb, "targets"}, {c.index, ixb, "index"},
+                        {c.logits, lgb, "logits"},  {c.grads, c.grads ? c.tokens * 4 : 0, "grads"}};
+  for (int i = 0; i < 4; ++i) {
+    if (!written[i].bytes) continue;
+    for (int k = 0; k < i; ++k)
+      if (ark::overlaps(written[i].p, written[i].bytes, written[k].p, written[k].bytes))
+        return fail(ARK_OPT_EINVAL, "%s overlaps %s", written[i].what, written[k].what);
+    for (const Range& r : read)
+      if (r.bytes && ark::overlaps(written[i].p, written[i].bytes, r.p, r.bytes))
+        return fail(ARK_OPT_EINVAL, "%s overlaps %s", written[i].what, r.what);
+  }
+  ark::BufferChecker checker;
+  for (const Range& r : read)
+    if ((rc = checker.check(r.p, r.bytes, r.what, 0))) return rc;
+  for (const Range& r : written)
+    if ((rc = checker.check(r.p, r.bytes, r.what, 0))) return rc;
+  {
+    const void* d[4];
+    uint64_t b[4];
+    for (int i = 0; i < 4; ++i) d[i] = written[i].p, b[i] = written[i].bytes;
+    ark::opt_units_invalidate(d, b, 4);
+  }
+  return c.dtype == ARK_HEAD_F16 ? run_call<_Float16>(c, p) : run_call<__bf16>(c, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int ark_head_workspace(const void* w, uint64_t w_stride, uint64_t tokens, uint64_t columns,
+                       uint64_t vocab, uint64_t top, uint32_t dw_dtype, uint32_t grad,
+                       uint64_t* bytes) {
+  if (!bytes) return fail(ARK_OPT_EINVAL, "bytes is NULL");
+  *bytes = 0;
+  if (int rc = check_sizes(tokens, columns, vocab, top, dw_dtype)) return rc;
+  *bytes = plan_of(w, w_stride, tokens, columns, vocab, top, dw_dtype, grad != 0).bytes;
+  return ARK_OPT_OK;
+}
+
+int ark_head_cross_entropy(const void* x, uint64_t x_stride, const void* w, uint64_t w_stride,
+                           uint32_t dtype, uint64_t tokens, uint64_t columns, uint64_t vocab,
+                           const void* targets, uint32_t target_bytes, int32_t ignore, float scale,
+                           float* loss, void* workspace, uint64_t workspace_bytes, void* stream) {
+  Call c = {};
+  c.x = x, c.x_stride = x_stride, c.w = w, c.w_stride = w_stride, c.dtype = dtype;
+  c.tokens = tokens, c.columns = columns, c.vocab = vocab;
+  c.targets = targets, c.target_bytes = target_bytes, c.ignore = ignore, c.top = 1;
+  c.scale = scale, c.loss = loss;
+  c.ws = (char*)workspace, c.ws_bytes = workspace_bytes, c.stream = (hipStream_t)stream;
+  return run(c);
+}
+
+int ark_head_cross_entropy_grad(const void* x, uint64_t x_stride, const void* w, uint64_t w_stride,
+                                uint32_t dtype, uint64_t tokens, uint64_t columns, uint64_t vocab,
+                                const void* targets, uint32_t target_bytes, int32_t ignore,
+                                float scale, float grad, const float* grads, float* loss, void* dx,
+                                uint64_t dx_stride, void* dw, uint32_t dw_dtype,
+                                uint64_t dw_stride, uint32_t flags, void* workspace,
+                                uint64_t workspace_bytes, void* stream) {
+  Call c = {};
+  c.x = x, c.x_stride = x_stride, c.w = w, c.w_stride = w_stride, c.dtype = dtype;
+  c.tokens = tokens, c.columns = columns, c.vocab = vocab;
+  c.targets = targets, c.target_bytes = target_bytes, c.ignore = ignore, c.top = 1;
+  c.scale = scale, c.with_grad = true, c.grad = grad, c.grads = grads, c.loss = loss;
+  c.dx = dx, c.dx_stride = dx_stride, c.dw = dw, c.dw_dtype = dw_dtype, c.dw_stride = dw_stride;
+  c.flags = flags;
+  c.ws = (char*)workspace, c.ws_bytes = workspace_bytes, c.stream = (hipStream_t)stream;
+  return run(c);
+}
+
+int ark_head_distill(const void* x, uint64_t x_stride, const void* w, uint64_t w_stride,
+                     uint32_t dtype, uint64_t tokens, uint64_t columns, uint64_t vocab,
+                     const void* index, uint32_t index_bytes, uint64_t index_stride,
+                     const void* logits, uint32_t logits_dtype, uint64_t logits_stride,
+                     uint64_t top, float temperature, float* loss, void* workspace,
+                     uint64_t workspace_bytes, void* stream) {
+  Call c = {};
+  c.x = x, c.x_stride = x_stride, c.w = w, c.w_stride = w_stride, c.dtype = dtype;
+  c.tokens = tokens, c.columns = columns, c.vocab = vocab;
+  c.teacher = true, c.index = index, c.index_bytes = index_bytes, c.index_stride = index_stride;
+  c.logits = logits, c.logits_dtype = logits_dtype, c.logits_stride = logits_stride, c.top = top;
+  c.scale = temperature < INFINITY ? 1.0f / temperature : 0.0f, c.loss = loss;
+  c.ws = (char*)workspace, c.ws_bytes = workspace_bytes, c.stream = (hipStream_t)stream;
+  return run(c);
+}
+
+int ark_head_distill_grad(const void* x, uint64_t x_stride, const void* w, uint64_t w_stride,
+                          uint32_t dtype, uint64_t tokens, uint64_t columns, uint64_t vocab,
+                          const void* index, uint32_t index_bytes, uint64_t index_stride,
+                          const void* logits, uint32_t logits_dtype, uint64_t logits_stride,
+                          uint64_t top, float temperature, float grad, const float* grads,
+                          float* loss, void* dx, uint64_t dx_stride, void* dw, uint32_t dw_dtype,
+                          uint64_t dw_stride, uint32_t flags, void* workspace,
+                          uint64_t workspace_bytes, void* stream) {
+  Call c = {};
+  c.x = x, c.x_stride = x_stride, c.w = w, c.w_stride = w_stride, c.dtype = dtype;
+  c.tokens = tokens, c.columns = columns, c.vocab = vocab;
+  c.teacher = true, c.index = index, c.index_bytes = index_bytes, c.index_stride = index_stride;
+  c.logits = logits, c.logits_dtype = logits_dtype, c.logits_stride = logits_stride, c.top = top;
+  c.scale = temperature < INFINITY ? 1.0f / temperature : 0.0f;
+  c.with_grad = true, c.grad = grad, c.grads = grads, c.loss = loss;
+  c.dx = dx, c.dx_stride = dx_stride, c.dw = dw, c.dw_dtype = dw_dtype, c.dw_stride = dw_stride;
+  c.flags = flags;
+  c.ws = (char*)workspace, c.ws_bytes = workspace_bytes, c.stream = (hipStream_t)stream;
+  return run(c);
+}
+
+}  // extern "C"

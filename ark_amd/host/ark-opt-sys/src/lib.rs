@@ -370,6 +370,72 @@ extern "C" {
                                   stream: *mut c_void) -> c_int;
 }
 
+// ---- include/ark_head.h (the logits and loss of `objc/bridge.m:414-503`, `:954-976`
+// as this library's own operators) ------------------------------------------------
+
+pub const ARK_HEAD_F16: u32 = 0;
+pub const ARK_HEAD_BF16: u32 = 1;
+pub const ARK_HEAD_F32: u32 = 2;
+pub const ARK_HEAD_MAX_TOP: u64 = 256;
+pub const ARK_HEAD_ACCUMULATE: u32 = 1;
+
+extern "C" {
+    pub fn ark_head_workspace(w: *const c_void, w_stride: u64, tokens: u64, columns: u64,
+                              vocab: u64, top: u64, dw_dtype: u32, grad: u32,
+                              bytes: *mut u64) -> c_int;
+    /// The loss of every token over the vocabulary, without the logits in memory.
+    pub fn ark_head_cross_entropy(x: *const c_void, x_stride: u64, w: *const c_void,
+                                  w_stride: u64, dtype: u32, tokens: u64, columns: u64,
+                                  vocab: u64, targets: *const c_void, target_bytes: u32,
+                                  ignore: i32, scale: f32, loss: *mut f32,
+                                  workspace: *mut c_void, workspace_bytes: u64,
+                                  stream: *mut c_void) -> c_int;
+    /// The same with the gradients of x and w.
+    pub fn ark_head_cross_entropy_grad(x: *const c_void, x_stride: u64, w: *const c_void,
+                                       w_stride: u64, dtype: u32, tokens: u64, columns: u64,
+                                       vocab: u64, targets: *const c_void, target_bytes: u32,
+                                       ignore: i32, scale: f32, grad: f32, grads: *const f32,
+                                       loss: *mut f32, dx: *mut c_void, dx_stride: u64,
+                                       dw: *mut c_void, dw_dtype: u32, dw_stride: u64, flags: u32,
+                                       workspace: *mut c_void, workspace_bytes: u64,
+                                       stream: *mut c_void) -> c_int;
+    /// The divergence from a teacher's distribution over its top logits.
+    pub fn ark_head_distill(x: *const c_void, x_stride: u64, w: *const c_void, w_stride: u64,
+                            dtype: u32, tokens: u64, columns: u64, vocab: u64,
+                            index: *const c_void, index_bytes: u32, index_stride: u64,
+                            logits: *const c_void, logits_dtype: u32, logits_stride: u64,
+                            top: u64, temperature: f32, loss: *mut f32, workspace: *mut c_void,
+                            workspace_bytes: u64, stream: *mut c_void) -> c_int;
+    pub fn ark_head_distill_grad(x: *const c_void, x_stride: u64, w: *const c_void, w_stride: u64,
+                                 dtype: u32, tokens: u64, columns: u64, vocab: u64,
+                                 index: *const c_void, index_bytes: u32, index_stride: u64,
+                                 logits: *const c_void, logits_dtype: u32, logits_stride: u64,
+                                 top: u64, temperature: f32, grad: f32, grads: *const f32,
+                                 loss: *mut f32, dx: *mut c_void, dx_stride: u64,
+                                 dw: *mut c_void, dw_dtype: u32, dw_stride: u64, flags: u32,
+                                 workspace: *mut c_void, workspace_bytes: u64,
+                                 stream: *mut c_void) -> c_int;
+}
+
+// ---- include/ark_embed.h (lookup and gradient of the embedding, scaled, any type) ---
+
+pub const ARK_EMBED_F16: u32 = 0;
+pub const ARK_EMBED_BF16: u32 = 1;
+pub const ARK_EMBED_F32: u32 = 2;
+pub const ARK_EMBED_ACCUMULATE: u32 = 1;
+
+extern "C" {
+    pub fn ark_embed_lookup(table: *const c_void, table_stride: u64, table_dtype: u32, vocab: u64,
+                            columns: u64, tokens: *const c_void, token_bytes: u32, n: u64,
+                            scale: f32, out: *mut c_void, out_stride: u64, out_dtype: u32,
+                            stream: *mut c_void) -> c_int;
+    pub fn ark_embed_grad_workspace(n: u64, vocab: u64, columns: u64, bytes: *mut u64) -> c_int;
+    pub fn ark_embed_grad(dy: *const c_void, dy_stride: u64, dy_dtype: u32, tokens: *const c_void,
+                          token_bytes: u32, n: u64, vocab: u64, columns: u64, scale: f32,
+                          dw: *mut f32, dw_stride: u64, flags: u32, workspace: *mut c_void,
+                          workspace_bytes: u64, stream: *mut c_void) -> c_int;
+}
+
 // ---- include/ark_synth.h (no reference counterpart: test and bench inputs) ---
 
 extern "C" {

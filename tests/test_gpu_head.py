@@ -1,0 +1,595 @@
+"""The loss over a vocabulary, its gradients, and distillation
+(include/ark_head.h), against their formulas in 64 bits.
+
+Tolerances, from the arithmetic alone (u: half a step of the 16-bit type):
+* A logit is a sum of d products in fp32: within bz = (d + 4) 2^-23 of the sum of
+  magnitudes, and 2^-23 of itself for the scale.
+* log(sum exp): every exponential's argument is off by bz and by 2^-22 of its
+  distance from the row's largest, the exponential by 2^-21, a sum of V terms in
+  stretches by (64 + V / 4096) 2^-24; weighted by the exponentials' shares q.
+* dz = g (q - p): q is rounded twice, and an entry at a target once; in fp16, a
+  q below 2^-14 of its span's largest loses up to 2^-25 of that, and dz 2^-38 of
+  the largest gradient; in bf16 both vanish below fp32's smallest normal number,
+  2^-126 (an exponential's result and a matrix instruction's factor there may be
+  taken for 0), which is at most 2^-126 of a q and of the largest gradient.
+* dx and dw: the products of what dz is off by, (terms + 4) 2^-23 of the sum of
+  magnitudes (in which fp16 factors count as 2^-14 at least), and one rounding.
+"""
+import math
+
+import pytest
+
+from ark_amd import _abi, head
+from ark_amd._lib import ArkOptError
+
+pytestmark = pytest.mark.gpu
+
+TYPES = ["f16", "bf16"]
+SIZES = [(1, 1, 1), (1, 64, 300), (3, 8, 5), (64, 64, 256), (65, 96, 257), (63, 129, 1000),
+         (257, 72, 513), (300, 100, 33), (130, 256, 2049), (513, 65, 640), (16, 1030, 70)]
+
+
+def _torch():
+    import torch
+    assert torch.cuda.is_available(), "GPU test run without a GPU"
+    return torch
+
+
+def _dt(name):
+    torch = _torch()
+    return {"f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+def _half(dtype):
+    return _torch().finfo(dtype).eps / 2
+
+
+def make(t, d, v, name, masked=0.2, seed=0):
+    """x, w and targets, some of them without a token (outside the vocabulary)."""
+    torch = _torch()
+    gen = torch.Generator(device="cuda").manual_seed(seed + 1000 * t + v)
+    w = torch.randn((v, d), generator=gen, device="cuda") * (2.0 / d ** 0.5)
+    y = torch.randint(0, v, (t,), generator=gen, device="cuda")
+    x = torch.randn((t, d), generator=gen, device="cuda")
+    x += 3.0 * torch.rand((t, 1), generator=gen, device="cuda") * w[y]
+    off = torch.rand((t,), generator=gen, device="cuda") < masked
+    y = torch.where(off, torch.where(torch.rand((t,), generator=gen, device="cuda") < 0.5, -100,
+                                     v + 7), y)
+    return x.to(_dt(name)), w.to(_dt(name)), y
+
+
+class Want:
+    """Loss and gradients in 64 bits of a wanted distribution p (t x v; rows of
+    zeros have no loss), and how far the kernels' may be off."""
+
+    def __init__(self, x, w, p, live, scale, g, own=0.0):
+        torch = _torch()
+        f16 = x.dtype == torch.float16
+        u = _half(x.dtype)
+        x = torch.where(live[:, None], x.double(), 0.0)
+        w = w.double()
+        t, d = x.shape
+        v = len(w)
+        z = (x @ w.t()) * scale
+        lse = torch.logsumexp(z, 1, keepdim=True)
+        q = (z - lse).exp()
+        self.loss = torch.where(live, own + (p * (lse - z)).sum(1), 0.0)
+        bz = (d + 4) * 2.0 ** -23 * scale * (x.abs() @ w.abs().t()) + 2.0 ** -23 * z.abs()
+        r = lse - z
+        b_lse = (q * (bz + 2.0 ** -22 * r + 2.0 ** -21)).sum(1, keepdim=True)
+        b_lse += (64 + v / 4096) * 2.0 ** -24 + 2.0 ** -23 * lse.abs()
+        size = (p * (lse.abs() + z.abs() + r.abs())).sum(1)
+        self.b_loss = live * (b_lse[:, 0] + (p * bz).sum(1)
+                              + 2.0 ** -20 * (size + abs(own)) + 1e-30)
+        gs = (live * g).double()[:, None] * scale
+        most = gs.abs().max() if t else 0.0
+        dz = gs * (q - p)
+        delta = bz + b_lse + 2.0 ** -22 * r + 2.0 ** -21
+        e = gs.abs() * (q * (2.1 * u + delta) + p * (1.05 * u + 2.0 ** -22))
+        if f16:
+            e = e + gs.abs() * 2.0 ** -24 + (gs != 0) * most * 2.0 ** -37
+        else:
+            e = e + (gs.abs() + (gs != 0) * most) * 2.0 ** -125
+        least = 2.0 ** -14 if f16 else 0.0
+        dz_size = dz.abs() + e + (2.0 ** -27 * most if f16 else 0.0)
+        tiny = 2.0 ** -24 if f16 else 2.0 ** -133
+
+        def out(value, err, sizes, n):
+            b = err + (n + 4) * 2.0 ** -23 * sizes
+            return b + u * (value.abs() + b) + tiny
+        self.dx = dz @ w
+        aw = w.abs().clamp_min(least)
+        self.b_dx = out(self.dx, e @ w.abs(), dz_size @ aw, v)
+        self.dw = dz.t() @ x
+        ax = torch.where(live[:, None], x.abs().clamp_min(least), 0.0)
+        self.b_dw = out(self.dw, e.t() @ x.abs(), dz_size.t() @ ax, t)
+
+    def check(self, loss, dx, dw):
+        for name, got in (("loss", loss), ("dx", dx), ("dw", dw)):
+            if got is None:
+                continue
+            want, b = getattr(self, name), getattr(self, "b_" + name)
+            off = (got.double() - want).abs()
+            assert (off <= b).all(), (name, (off / b).max().item())
+
+
+def one_hot(y, live, v):
+    torch = _torch()
+    p = torch.zeros((len(y), v), dtype=torch.float64, device="cuda")
+    rows = live.nonzero()[:, 0]
+    p[rows, y[rows].long()] = 1.0
+    return p
+
+
+def ce(x, w, y, scale=1.0, g=1.0, ignore=-100):
+    torch = _torch()
+    live = (y >= 0) & (y < len(w)) & (y != ignore)
+    g = torch.as_tensor(g, device="cuda").double().expand(len(x))
+    return Want(x, w, one_hot(y, live, len(w)), live, scale, g)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("t,d,v", SIZES)
+def test_cross_entropy(t, d, v, name):
+    torch = _torch()
+    x, w, y = make(t, d, v, name)
+    want = ce(x, w, y, g=8.0 / t)
+    want.check(head.cross_entropy(x, w, y), None, None)
+    loss, dx, dw = head.cross_entropy_grad(x, w, y, grad=8.0 / t)
+    assert dx.dtype == x.dtype and dw.dtype == w.dtype and loss.dtype == torch.float32
+    want.check(loss, dx, dw)
+    live = (y >= 0) & (y < v)
+    assert (dx[~live] == 0).all() and (loss[~live] == 0).all()
+    # a number for each token, int32 targets, fp32 dw
+    g = torch.rand(t, device="cuda") * torch.exp2(torch.randint(-12, 6, (t,), device="cuda"))
+    loss, dx, dw = head.cross_entropy_grad(x, w, y.int(), grad=g,
+                                           dw=torch.empty((v, d), device="cuda"))
+    ce(x, w, y, g=g).check(loss, dx, dw)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("scale", [0.125, 30.0])
+def test_scale(scale, name):
+    x, w, y = make(100, 48, 301, name)
+    want = ce(x, w, y, scale=scale, g=0.5)
+    want.check(*head.cross_entropy_grad(x, w, y, grad=0.5, scale=scale))
+    want.check(head.cross_entropy(x, w, y, scale=scale), None, None)
+
+
+@pytest.mark.parametrize("name", TYPES)
+def test_strides_and_what_lies_beside(name):
+    """Rows of any stride and alignment; nothing beside a written row changes."""
+    torch = _torch()
+    t, d, v = 150, 40, 290
+    x, w, y = make(t, d, v, name)
+    want = ce(x, w, y, g=0.25)
+    for off, wide in ((0, 64), (3, 47), (8, 56)):
+        def beside(a, fill):
+            b = torch.full((len(a), wide + d), fill, dtype=a.dtype, device="cuda")
+            b[:, off:off + d] = a
+            return b, b[:, off:off + d]
+        bx, xs = beside(x, float("nan"))
+        bw, ws = beside(w, float("nan"))
+        bdx, dx = beside(torch.empty_like(x), 7.0)
+        for dt in (w.dtype, torch.float32):
+            bdw, dw = beside(torch.empty((v, d), dtype=dt, device="cuda"), 7.0)
+            loss, a, b = head.cross_entropy_grad(xs, ws, y, grad=0.25, dx=dx, dw=dw)
+            assert a is dx and b is dw
+            want.check(loss, dx, dw)
+            for full in (bdx, bdw):
+                assert (full[:, :off] == 7).all() and (full[:, off + d:] == 7).all()
+        want.check(head.cross_entropy(xs, ws, y), None, None)
+
+
+@pytest.mark.parametrize("name", TYPES)
+def test_accumulate_and_parts(name):
+    torch = _torch()
+    x, w, y = make(200, 64, 700, name)
+    want = ce(x, w, y, g=0.1)
+    before = torch.randn((700, 64), device="cuda")
+    dw = before.clone()
+    loss, dx, out = head.cross_entropy_grad(x, w, y, grad=0.1, dw=dw, accumulate=True)
+    assert out is dw
+    want.check(loss, dx, None)
+    off = (dw.double() - before.double() - want.dw).abs()
+    assert (off <= want.b_dw + 2.0 ** -23 * (before.abs().double() + want.dw.abs())).all()
+    fresh = head.cross_entropy_grad(x, w, y, grad=0.1, dw=torch.empty_like(before))[2]
+    assert torch.equal(dw, fresh + before)
+    a = head.cross_entropy_grad(x, w, y, grad=0.1, dx=False)
+    b = head.cross_entropy_grad(x, w, y, grad=0.1, dw=False)
+    c = head.cross_entropy_grad(x, w, y, grad=0.1)
+    assert a[1] is None and b[2] is None
+    assert torch.equal(a[2], c[2]) and torch.equal(b[1], c[1]) and torch.equal(a[0], b[0])
+    assert head.cross_entropy_grad(x, w, y, dx=False, dw=False)[1:] == (None, None)
+
+
+@pytest.mark.parametrize("name", TYPES)
+def test_tokens_without_a_loss_reach_nothing(name):
+    """NaN and inf in their rows and numbers, whole blocks of them, and no others."""
+    torch = _torch()
+    t, d, v = 600, 32, 100
+    x, w, y = make(t, d, v, name, masked=0.0)
+    off = torch.zeros(t, dtype=torch.bool, device="cuda")
+    off[:70] = off[200:300] = off[599] = True
+    off[400::3] = True
+    y[off] = -100
+    clean = head.cross_entropy_grad(x, w, y, grad=0.5)
+    ce(x, w, y, g=0.5).check(*clean)
+    bad = x.clone()
+    bad[off] = float("nan")
+    bad[:35] = float("inf")
+    for a, b in zip(clean, head.cross_entropy_grad(bad, w, y, grad=0.5)):
+        assert torch.equal(a, b)
+    g = torch.full((t,), 0.5, device="cuda")
+    g[off] = float("nan")
+    for a, b in zip(clean, head.cross_entropy_grad(bad, w, y, grad=g)):
+        assert torch.equal(a, b)
+    y[:] = -100
+    loss, dx, dw = head.cross_entropy_grad(bad, w, y, grad=g)
+    assert not loss.any() and not dx.any() and not dw.any()
+    assert not head.cross_entropy(bad, w, y).any()
+    dw = torch.ones((v, d), device="cuda")
+    head.cross_entropy_grad(bad, w, y, grad=g, dw=dw, accumulate=True)
+    assert (dw == 1).all()
+
+
+def test_ignored_index_in_the_vocabulary():
+    torch = _torch()
+    x, w, y = make(90, 24, 12, "f16", masked=0.0)
+    want = ce(x, w, y, ignore=3, g=1.0)
+    want.check(*head.cross_entropy_grad(x, w, y, ignore=3))
+    assert (head.cross_entropy(x, w, y, ignore=3)[y == 3] == 0).all()
+    far = torch.where(y == 3, torch.tensor(2 ** 40 + 5, device="cuda"), y)
+    assert torch.equal(head.cross_entropy(x, w, far), head.cross_entropy(x, w, y, ignore=3))
+
+
+@pytest.mark.parametrize("name", TYPES)
+def test_what_is_not_finite_shows(name):
+    torch = _torch()
+    x, w, y = make(120, 64, 500, name, masked=0.1)
+    good = head.cross_entropy(x, w, y)
+    live = ((y >= 0) & (y < 500)).nonzero()[:, 0]
+    for value in (float("nan"), float("inf")):
+        bad = x.clone()
+        bad[live[5], 3] = value
+        loss, dx, dw = head.cross_entropy_grad(bad, w, y)
+        others = torch.arange(120, device="cuda") != live[5]
+        assert not torch.isfinite(loss[live[5]]) and torch.equal(loss[others], good[others])
+        assert not torch.isfinite(dx[live[5]]).any() and torch.isfinite(dx[others]).all()
+        assert not torch.isfinite(dw).all(1).any()
+    g = torch.ones(120, device="cuda")
+    g[live[2]] = float("inf")
+    loss, dx, dw = head.cross_entropy_grad(x, w, y, grad=g)
+    assert torch.equal(loss, good) and not torch.isfinite(dw).all()
+    assert not torch.isfinite(dx[live[2]]).all()
+
+
+@pytest.mark.parametrize("name", TYPES)
+def test_far_logits(name):
+    """Logits in the thousands, rows that are sure of a token, rows without any
+    difference."""
+    torch = _torch()
+    x, w, y = make(80, 64, 400, name, masked=0.0)
+    x = x * 64
+    x[10:20] = 0
+    want = ce(x, w, y, scale=16.0)
+    want.check(*head.cross_entropy_grad(x, w, y, scale=16.0))
+    # all but one logit -inf
+    w2 = torch.full((7, 8), -60000.0, device="cuda").to(_dt(name))
+    w2[3] = 0
+    x2 = torch.full((5, 8), 60000.0, device="cuda").to(_dt(name))
+    y2 = torch.tensor([3, 3, 2, -1, 3], device="cuda")
+    loss, dx, dw = head.cross_entropy_grad(x2, w2, y2, scale=3e38 / 2 ** 34)
+    assert loss[0] == loss[1] == loss[3] == loss[4] == 0 and loss[2] > 1e30
+    assert (dx[0] == 0).all() and (dx[4] == 0).all()
+
+
+def test_pieces():
+    """More tokens than a piece, by tokens and by the vocabulary's size."""
+    torch = _torch()
+    for t, d, v in ((16384 * 2 + 77, 8, 40), (700, 8, (1 << 20) + 3)):
+        x, w, y = make(t, d, v, "bf16")
+        g = torch.rand(t, device="cuda")
+        for dt in (torch.bfloat16, torch.float32):
+            got = head.cross_entropy_grad(x, w, y, grad=g, dw=torch.empty((v, d), dtype=dt,
+                                                                          device="cuda"))
+            ce(x, w, y, g=g).check(*got)
+        ce(x, w, y).check(head.cross_entropy(x, w, y), None, None)
+
+
+def test_no_tokens():
+    torch = _torch()
+    x, w, y = (torch.empty((0, 16), device="cuda").half(), torch.ones((9, 16), device="cuda").half(),
+               torch.empty(0, dtype=torch.long, device="cuda"))
+    assert head.cross_entropy(x, w, y).numel() == 0
+    loss, dx, dw = head.cross_entropy_grad(x, w, y)
+    assert loss.numel() == dx.numel() == 0 and (dw == 0).all() and dw.shape == (9, 16)
+    g = torch.empty(0, device="cuda")
+    dw = torch.ones((9, 16), device="cuda")
+    head.cross_entropy_grad(x, w, y, grad=g, dw=dw, accumulate=True)
+    assert (dw == 1).all()
+    head.cross_entropy_grad(x, w, y, grad=g, dw=dw)
+    assert (dw == 0).all()
+
+
+@pytest.mark.parametrize("grad", [0.0, 1e-30, 3e30, -2.0])
+def test_sizes_of_the_gradient(grad):
+    """Gradients far from 1, in bf16, whose range holds them."""
+    torch = _torch()
+    x, w, y = make(70, 32, 90, "bf16")
+    g = torch.full((70,), grad, device="cuda")
+    want = ce(x, w, y, g=g)
+    want.check(*head.cross_entropy_grad(x, w, y, grad=grad))
+    want.check(*head.cross_entropy_grad(x, w, y, grad=g))
+
+
+def test_loss_by_differences():
+    """The sum of the losses along a line, by central differences of step h: off by
+    h^2 / 6 of the third derivative, at most twice the cube of the largest range of
+    a logit's slope, and by the losses' own tolerance over h."""
+    torch = _torch()
+    x, w, y = make(40, 32, 200, "f16")
+    x = (x * 64).round() / 64
+    x = x.clamp(-7, 7)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    line = torch.randint(-1, 2, x.shape, generator=gen, device="cuda").to(x.dtype)
+    h = 2.0 ** -5
+    want = ce(x, w, y)
+    up, down = (head.cross_entropy(x + s * h * line, w, y).double().sum() for s in (1, -1))
+    slope = line.double() @ w.double().t()
+    reach = 2 * (slope.max(1).values - slope.min(1).values) ** 3
+    limit = h * h / 6 * reach.sum() + 2.1 * want.b_loss.sum() / (2 * h)
+    dx = head.cross_entropy_grad(x, w, y)[1].double()
+    limit = limit + (want.b_dx * line.abs().double()).sum()
+    assert ((up - down) / (2 * h) - (dx * line.double()).sum()).abs() <= limit
+    # and along w
+    line = torch.randint(-1, 2, w.shape, generator=gen, device="cuda").to(w.dtype)
+    w = (w * 256).round() / 256
+    want = ce(x, w, y)
+    h = 2.0 ** -6
+    up, down = (head.cross_entropy(x, w + s * h * line, y).double().sum() for s in (1, -1))
+    slope = x.double() @ line.double().t()
+    reach = 2 * (slope.max(1).values - slope.min(1).values) ** 3
+    dw = head.cross_entropy_grad(x, w, y)[2].double()
+    limit = (h * h / 6 * reach.sum() + 2.1 * want.b_loss.sum() / (2 * h)
+             + (want.b_dw * line.abs().double()).sum())
+    assert ((up - down) / (2 * h) - (dw * line.double()).sum()).abs() <= limit
+
+
+# ---- distillation -----------------------------------------------------------------
+
+def teacher(t, v, k, seed=0, dtype=None):
+    """index (repeats and entries outside the vocabulary among them) and logits,
+    garbage where left out, -inf here and there."""
+    torch = _torch()
+    gen = torch.Generator(device="cuda").manual_seed(seed + 31 * t + k)
+    index = torch.randint(0, v, (t, k), generator=gen, device="cuda")
+    logits = 4.0 * torch.randn((t, k), generator=gen, device="cuda")
+    lot = torch.rand((t, k), generator=gen, device="cuda")
+    logits = torch.where(lot < 0.1, -float("inf"), logits)
+    index = torch.where(lot > 0.85, torch.where(lot > 0.93, -1, v), index)
+    logits = torch.where(lot > 0.9, float("nan"), logits)
+    index = torch.where((lot > 0.9) & (index < v), -1, index)
+    index[0] = -1
+    if t > 2:
+        logits[1] = -float("inf")
+    return index, logits.to(dtype or torch.float32)
+
+
+def kl(x, w, index, logits, tau, g):
+    torch = _torch()
+    v = len(w)
+    ok = (index >= 0) & (index < v) & (logits != -float("inf"))
+    live = ok.any(1)
+    a = torch.where(ok, logits.double() / tau, -float("inf"))
+    a = torch.where(live[:, None], a, 0.0)
+    log_p = torch.log_softmax(a, 1)
+    p = torch.where(ok, log_p.exp(), 0.0)
+    own = torch.where(ok, p * log_p, 0.0).sum(1)
+    dense = torch.zeros((len(x), v), dtype=torch.float64, device="cuda")
+    dense.scatter_add_(1, torch.where(ok, index, 0).long(), p)
+    g = torch.as_tensor(g, device="cuda").double().expand(len(x))
+    return Want(x, w, dense, live, 1.0 / tau, g, own)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("t,d,v,k", [(1, 8, 3, 1), (5, 64, 40, 256), (33, 72, 300, 7),
+                                     (130, 40, 1000, 64), (300, 128, 513, 65), (64, 64, 256, 130)])
+def test_distill(t, d, v, k, name):
+    torch = _torch()
+    x, w, _ = make(t, d, v, name)
+    index, logits = teacher(t, v, k)
+    for tau in (1.0, 2.5):
+        want = kl(x, w, index, logits, tau, 4.0 / t)
+        want.check(head.distill(x, w, index, logits, tau), None, None)
+        want.check(*head.distill_grad(x, w, index, logits, grad=4.0 / t, temperature=tau))
+    g = torch.rand(t, device="cuda")
+    for dt in (torch.float16, torch.bfloat16):
+        narrow = logits.to(dt)
+        wide = torch.full((t, k + 5), 3, device="cuda", dtype=torch.int32)
+        wide[:, 2:2 + k] = index
+        want = kl(x, w, index, narrow, 1.0, g)
+        want.check(*head.distill_grad(x, w, wide[:, 2:2 + k], narrow, grad=g,
+                                      dw=torch.empty((v, d), device="cuda")))
+
+
+def test_distill_without_entries():
+    torch = _torch()
+    x, w, _ = make(70, 16, 50, "f16")
+    x[:] = float("nan")
+    index = torch.full((70, 4), -1, device="cuda")
+    logits = torch.full((70, 4), float("nan"), device="cuda")
+    loss, dx, dw = head.distill_grad(x, w, index, logits)
+    assert not loss.any() and not dx.any() and not dw.any()
+    index[:] = 3
+    logits[:] = -float("inf")
+    assert not head.distill(x, w, index, logits).any()
+
+
+def test_distill_of_one_certain_entry_is_cross_entropy():
+    torch = _torch()
+    x, w, y = make(99, 64, 333, "bf16")
+    live = (y >= 0) & (y < 333)
+    a = head.cross_entropy_grad(x, w, y, grad=0.5)
+    b = head.distill_grad(x, w, y[:, None], torch.zeros((99, 1), device="cuda"), grad=0.5)
+    for one, other in zip(a, b):
+        assert torch.equal(one, other)
+    # the same token three times over
+    c = head.distill_grad(x, w, y[:, None].expand(99, 4).contiguous(),
+                          torch.zeros((99, 4), device="cuda"), grad=0.5)
+    want = Want(x, w, one_hot(y, live, 333), live, 1.0,
+                torch.full((99,), 0.5, device="cuda"), torch.where(live, -math.log(4.0), 0.0))
+    want.check(*c)  # four entries of 1/4 each: sum of p log p = -log 4
+
+
+def test_distill_shows_what_is_not_finite():
+    torch = _torch()
+    x, w, _ = make(10, 16, 50, "f16")
+    index = torch.arange(4, device="cuda").expand(10, 4).contiguous()
+    logits = torch.zeros((10, 4), device="cuda")
+    good = head.distill(x, w, index, logits)
+    for value in (float("nan"), float("inf")):
+        bad = logits.clone()
+        bad[6, 2] = value
+        loss, dx, dw = head.distill_grad(x, w, index, bad)
+        keep = torch.arange(10, device="cuda") != 6
+        assert torch.isnan(loss[6]) and torch.equal(loss[keep], good[keep])
+        assert not torch.isfinite(dw).all()
+
+
+# ---- how it runs --------------------------------------------------------------------
+
+def _calls(x, w, y, index, logits):
+    return [head.cross_entropy(x, w, y), *head.cross_entropy_grad(x, w, y, grad=0.5),
+            head.distill(x, w, index, logits, 2.0),
+            *head.distill_grad(x, w, index, logits, temperature=2.0)]
+
+
+@pytest.mark.parametrize("t,d,v", [(40, 64, 700), (300, 72, 1500)])
+def test_equal_calls_give_equal_bits_also_side_by_side(t, d, v):
+    torch = _torch()
+    x, w, y = make(t, d, v, "f16")
+    index, logits = teacher(t, v, 9)
+    first = _calls(x, w, y, index, logits)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(_calls(x, w, y, index, logits))
+    torch.cuda.synchronize()
+    for g in got:
+        for a, b in zip(first, g):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+@pytest.mark.parametrize("t,d,v", [(8, 64, 500), (200, 100, 900)])
+def test_in_a_graph(t, d, v):
+    torch = _torch()
+    x, w, y = make(t, d, v, "bf16")
+    index, logits = teacher(t, v, 5)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        _calls(x, w, y, index, logits)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        out = _calls(x, w, y, index, logits)
+    for k in range(4):
+        x.normal_()
+        y.random_(-5, v)
+        torch.cuda.synchronize()
+        for o in out:
+            o.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, _calls(x, w, y, index, logits)):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16)), k
+
+
+def test_a_training_loop_of_the_two_ends():
+    """Lookup, loss and both gradients of a tied embedding into an optimizer's fp32
+    gradients: the step sees their sum."""
+    torch = _torch()
+    from ark_amd import embed
+    from ark_amd.eko import TensorSpec
+    from ark_amd.optimizer import AdamConfig, AmpConfig, Optimizer, ParamSet
+    t, d, v = 130, 64, 600
+    ps = ParamSet([TensorSpec("embed", (v, d), True, False)], 0.0, grad_dtype=_abi.GRAD_F32)
+    table = ps.w(0).view(v, d)
+    table.normal_(0.0, 0.3)
+    opt = Optimizer(AdamConfig(), ps, AmpConfig(loss_scale_init=1024.0))
+    tokens = torch.randint(0, v, (t,), device="cuda")
+    targets = torch.randint(0, v, (t,), device="cuda")
+    x = embed.lookup(table, tokens, scale=4.0)
+    grad = ps.g(0).view(v, d)
+    g = opt.loss_scale / t
+    loss, dx, _ = head.cross_entropy_grad(x, table, targets, grad=g, dw=grad)
+    embed.lookup_grad(dx, tokens, v, scale=4.0, dw=grad, accumulate=True)
+    want = ce(x, table, targets, g=g)
+    want.check(loss, dx, None)
+    both = want.dw.clone().index_add_(0, tokens, 4.0 * dx.double())
+    size = torch.zeros_like(both).index_add_(0, tokens, 4.0 * dx.double().abs())
+    assert ((grad.double() - both).abs() <= want.b_dw + t * 2.0 ** -23 * (size + both.abs())).all()
+    info = opt.step_all(1e-3, info=True)[1]
+    norm = grad.double().norm().item() / 1024.0
+    assert info.applied == 1 and abs(info.grad_norm - norm) <= 1e-6 * norm
+    opt.close()
+
+
+def test_refusals():
+    torch = _torch()
+    x, w, y = make(20, 16, 30, "f16")
+    index, logits = teacher(20, 30, 4)
+    bad = pytest.raises(ValueError)
+    with bad:
+        head.cross_entropy(x.float(), w.float(), y)
+    with bad:
+        head.cross_entropy(x, w.bfloat16(), y)
+    with bad:
+        head.cross_entropy(x.t(), w, y)
+    with bad:
+        head.cross_entropy(x, w[:, :15], y)
+    with bad:
+        head.cross_entropy(x, w, y[:19])
+    with bad:
+        head.cross_entropy(x, w, y.float())
+    with bad:
+        head.cross_entropy(x, w, y, ignore=2 ** 31)
+    with bad:
+        head.cross_entropy(x.cpu(), w.cpu(), y.cpu())
+    with bad:
+        head.cross_entropy_grad(x, w, y, grad=torch.ones(19, device="cuda"))
+    with bad:
+        head.cross_entropy_grad(x, w, y, accumulate=True)
+    with bad:
+        head.cross_entropy_grad(x, w, y, dw=torch.empty((30, 16), device="cuda").bfloat16())
+    with bad:
+        head.cross_entropy_grad(x, w, y, dx=torch.empty((20, 16), device="cuda"))
+    with bad:
+        head.distill(x, w, index[:, :3], logits)
+    with bad:
+        head.distill(x, w, index.float(), logits)
+    with pytest.raises(ArkOptError, match="fp32 dw"):
+        head.cross_entropy_grad(x, w, y, dw=torch.empty_like(w), accumulate=True)
+    with pytest.raises(ArkOptError, match="overlap"):
+        head.cross_entropy_grad(x, w, y, dx=x)
+    with pytest.raises(ArkOptError, match="overlap"):
+        head.cross_entropy_grad(x, w, y, dw=w)
+    with pytest.raises(ArkOptError, match="scale"):
+        head.cross_entropy(x, w, y, scale=0.0)
+    for tau in (0.0, -1.0, float("inf"), float("nan"), 1e-45):
+        with pytest.raises(ArkOptError, match="temperature"):
+            head.distill(x, w, index, logits, temperature=tau)
+    with pytest.raises(ArkOptError, match="top"):
+        many = torch.zeros((20, 257), device="cuda")
+        head.distill(x, w, many.long(), many)
+    for t in (x, w, logits):
+        t.requires_grad_()
+        with pytest.raises(ValueError, match="requires grad"):
+            head.distill(x, w, index, logits)
+        with torch.no_grad():
+            head.distill(x, w, index, logits)
+        head.distill_grad(x, w, index, logits)
+        t.requires_grad_(False)
