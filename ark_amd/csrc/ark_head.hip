@@ -614,11 +614,11 @@ constexpr uint64_t kDzBytes = 1ull << 30;  // of a piece's dz, at most
 
 struct Big {
   template <typename T, bool AMC, bool BMC>
-  using P = Product<T, AMC, BMC, 8, 4, 2, 4>;
+  using P = Product<T, AMC, BMC, 8, 4, 2, 4, 4>;
 };
 struct Small {
   template <typename T, bool AMC, bool BMC>
-  using P = Product<T, AMC, BMC, 4, 2, 2, 2>;
+  using P = Product<T, AMC, BMC, 4, 2, 2, 2, 4>;
 };
 
 constexpr uint32_t kMaxSplits = 32;

@@ -6,10 +6,10 @@
 // An operand lies in memory with k along its rows (KC: a row is an m or n, its k
 // follow one another) or across them (MC: a row is a k).  A block forms BM x BN
 // outputs, a wave 16 MF x 16 NF of them; a lane ends up with four neighbouring m
-// of one n.  A step is 64 k of both operands, which go from memory into LDS
-// without passing through registers (global_load_lds), into one of two buffers.
+// of one n.  A step is 32 k of both operands, which go from memory into LDS
+// without passing through registers (global_load_lds), into one of BUFS buffers.
 //
-// LDS holds a KC operand as rows of 64 k, eight 16-byte chunks each, permuted by
+// LDS holds a KC operand as rows of 32 k, four 16-byte chunks each, permuted by
 // the row's bits so that a fragment's 16-byte reads meet in no bank, and an MC
 // operand as it comes, rows of BM or BN values; its fragments are read through
 // the transposing read, which gives lane i of sixteen the values of column i in
@@ -20,6 +20,8 @@
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "ark_device.hpp"
 
@@ -50,7 +52,7 @@ struct Frag<__bf16> {
   }
 };
 
-constexpr uint32_t kProductStep = 64;  // k a step
+constexpr uint32_t kProductStep = 32;  // k a step
 
 // An operand of one block: `at` is its first value (of the tile's first row and
 // first k when KC, of the first k's row and the tile's first column when MC).
@@ -72,8 +74,11 @@ struct Staged {
 
   static __device__ __forceinline__ uint32_t swizzle(uint32_t row) {
     if constexpr (MC) return ((row & 3u) | (row >> 3 & 1u) << 2) & (B / 16 - 1);
-    // 16-byte reads of 16 neighbouring rows, the second half of the lanes a chunk on
-    return ((row >> 1 & 3u) ^ (row >> 4 & 1u)) | ((row >> 3 ^ row) & 1u) << 2;
+    // LDS takes 16-byte reads sixteen lanes at a time, of each 32 lanes 0-3, 12-15 and
+    // 20-27 and then the others (measured: which pairs meet); lanes 16 on are a chunk
+    // on.  Four rows are 256 bytes, a row of all banks: of rows 4 apart the four that
+    // are read together get four different places.
+    return ((row >> 2 ^ row >> 3) & 1u) << 1 | (row >> 3 & 1u);
   }
   // The offsets; of an MC operand's rows past `ks` from the step's first, the
   // last one's again.
@@ -89,9 +94,11 @@ struct Staged {
       }
     }
   }
-  // Sixty-four k from `step` on, into LDS at byte `to`.  The load writes LDS at m0
-  // plus 16 bytes a lane; nothing returns to registers, and multiply() waits for
-  // it by count.
+  // The k of `step`, into LDS at byte `to`.  The load writes LDS at m0
+  // plus 16 bytes a lane; nothing returns to registers, and meet() waits for it by
+  // count.  (The wait states are those between a vector instruction that writes an
+  // address's scalar register and a load that reads it, which the compiler does not
+  // see inside the block; one would do between m0 and the load.)
   __device__ __forceinline__ void load(const Operand& o, uint32_t step, uint32_t to) {
     const uint16_t* p = o.at + (uint64_t)step * kProductStep * (MC ? o.stride : 1);
     if constexpr (MC) {
@@ -102,15 +109,14 @@ struct Staged {
 #pragma unroll
     for (uint32_t i = 0; i < kLoads; ++i) {
       const uint32_t at = to + (i * LANES + wave * 64) * 16;
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
                    :
                    : "s"(at), "v"(off[i]), "s"(p));
     }
   }
 };
 
-// Where a lane reads fragment f (16 rows or columns) of a wave's part, for the
-// step's first (h = 0) or second 32 k.
+// Where a lane reads fragment f (16 rows or columns) of a wave's part.
 template <typename T, uint32_t B, bool MC>
 struct Reader {
   uint32_t at;
@@ -126,38 +132,47 @@ struct Reader {
       at = (first + i) * S::kRow + (g ^ S::swizzle(first + i)) * 16;
     }
   }
-  __device__ __forceinline__ typename Frag<T>::V get(uint32_t buf, uint32_t h, uint32_t f) const {
+  __device__ __forceinline__ typename Frag<T>::V get(uint32_t buf, uint32_t f) const {
     typedef typename Frag<T>::V V;
     typedef Staged<B, MC, 64> S;
     if constexpr (MC) {
-      const uint32_t a = buf + (at ^ (f * 32)) + h * 32 * S::kRow;
+      const uint32_t a = buf + (at ^ (f * 32));
       typedef __attribute__((address_space(3))) s16x4 L;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(uintptr_t)a);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(uintptr_t)(a + 4 * S::kRow));
       return __builtin_bit_cast(V, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
-    // 16 rows on, bit 4 of the row turns over, and with it the permutation's bit 0
-    return ARK_LDS_AT(V, buf + (at ^ (h * 64 + f % 2 * 16)) + f * 16 * S::kRow);
+    return ARK_LDS_AT(V, buf + at + f * 16 * S::kRow);
   }
 };
 
-// A block's shape: WM x WN waves of MF x NF fragments.
-template <typename T_, bool AMC_, bool BMC_, uint32_t MF_, uint32_t NF_, uint32_t WM_, uint32_t WN_>
+// A block's shape: WM x WN waves of MF x NF fragments, BUFS steps in LDS.
+template <typename T_, bool AMC_, bool BMC_, uint32_t MF_, uint32_t NF_, uint32_t WM_, uint32_t WN_,
+          uint32_t BUFS_>
 struct Product {
   typedef T_ T;
-  static constexpr uint32_t MF = MF_, NF = NF_, WM = WM_, WN = WN_;
+  static constexpr uint32_t MF = MF_, NF = NF_, WM = WM_, WN = WN_, BUFS = BUFS_;
   static constexpr bool AMC = AMC_, BMC = BMC_;
   static constexpr uint32_t kLanes = 64 * WM * WN;
   static constexpr uint32_t BM = 16 * MF * WM, BN = 16 * NF * WN;
   typedef Staged<BM, AMC, kLanes> A;
   typedef Staged<BN, BMC, kLanes> B;
   static constexpr uint32_t kBuffer = A::kBytes + B::kBytes;
-  static constexpr uint32_t kLds = 2 * kBuffer;
+  static constexpr uint32_t kLds = BUFS * kBuffer;
+  static constexpr uint32_t kLoads = A::kLoads + B::kLoads;
+  static_assert(BUFS >= 3, "one read, one arriving, one asked for");
 
   f32x4 acc[MF][NF];
 
-  // acc = the product over steps [s0, s1).  lds: kLds bytes, aligned to 1024, free
-  // again when every wave has come back.
+  // All but the newest `left` loads of this wave have arrived, and so have every
+  // other wave's.
+  template <uint32_t LEFT>
+  static __device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"(LEFT) : "memory");
+  }
+
+  // acc = the product over steps [s0, s1).  lds: kLds bytes, aligned to 1024; the
+  // caller's to use again after a barrier.
   __device__ __forceinline__ void run(const Operand& oa, const Operand& ob, uint32_t s0,
                                       uint32_t s1, uint32_t lds) {
 #pragma unroll
@@ -172,42 +187,66 @@ struct Product {
     b.place(ob, kProductStep);
     const Reader<T, BM, AMC> ra(wave % WM * 16 * MF);
     const Reader<T, BN, BMC> rb(wave / WM * 16 * NF);
-    typename Frag<T>::V fa[2][MF], fb[2][NF];
-    const auto load = [&](uint32_t s, uint32_t buf) {
+    typename Frag<T>::V fa[MF], fb[2][NF];
+    const auto load = [&](uint32_t s, uint32_t buf) __attribute__((always_inline)) {
       a.load(oa, s, buf);
       b.load(ob, s, buf + A::kBytes);
     };
-    const auto read = [&](uint32_t buf, uint32_t h) {
+    const uint32_t end = lds + kLds;
+    uint32_t to = lds;  // the buffer of the next load
+    const auto next = [&](uint32_t buf) { return buf + kBuffer == end ? lds : buf + kBuffer; };
+    uint32_t s = s0;
+    for (; s < s1 && s < s0 + BUFS - 1; ++s) load(s, to), to = next(to);
+    if (s1 - s0 >= BUFS - 1)
+      meet<(BUFS - 2) * kLoads>();
+    else
+      meet<0>();
+    uint32_t from = lds;  // the buffer of the next fragments
+    const auto read_b = [&](auto set) __attribute__((always_inline)) {
 #pragma unroll
-      for (uint32_t j = 0; j < NF; ++j) fb[h][j] = rb.get(buf + A::kBytes, h, j);
-#pragma unroll
-      for (uint32_t i = 0; i < MF; ++i) fa[h][i] = ra.get(buf, h, i);
+      for (uint32_t j = 0; j < NF; ++j) fb[decltype(set)::value][j] = rb.get(from + A::kBytes, j);
     };
-    const auto mul = [&](uint32_t h) {
+    // A step is multiplied from registers while the next one's fragments take their
+    // places: b's into the other set, each of a's when its products are done.  The
+    // barrier before says that the next step is there, and that the buffer of the one
+    // before is free: its fragments have been multiplied.  (The last step reads what
+    // is in the buffer after its own and does not use it.)
+    s = s0;
+    const auto step = [&](auto set) __attribute__((always_inline)) {
+      constexpr uint32_t p = decltype(set)::value;
+      if (s + BUFS - 1 <= s1)
+        meet<(BUFS - 3) * kLoads>();
+      else
+        meet<0>();
+      if (s + BUFS - 1 < s1) load(s + BUFS - 1, to), to = next(to);
+      read_b(std::integral_constant<uint32_t, p ^ 1>());
 #pragma unroll
-      for (uint32_t i = 0; i < MF; ++i)
+      for (uint32_t i = 0; i < MF; ++i) {
 #pragma unroll
-        for (uint32_t j = 0; j < NF; ++j) acc[i][j] = Frag<T>::mul(fa[h][i], fb[h][j], acc[i][j]);
+        for (uint32_t j = 0; j < NF; ++j) acc[i][j] = Frag<T>::mul(fa[i], fb[p][j], acc[i][j]);
+        fa[i] = ra.get(from, i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      from = next(from);
+      ++s;
     };
-    // every wave's loads into LDS and reads of it have ended
-    const auto meet = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-    load(s0, lds);
-    meet();
-    if (s0 + 1 < s1) load(s0 + 1, lds + kBuffer);
-    read(lds, 0);
-    // A step's first half is multiplied while its second is read; when the barrier
-    // then says that the step has been read and the next one has come, the next
-    // one's first half is read and the one after asked for, behind the products of
-    // the second half.
-    for (uint32_t s = s0; s < s1; ++s) {
-      const uint32_t odd = (s - s0) % 2;
-      const uint32_t cur = lds + odd * kBuffer, nxt = lds + (odd ^ 1u) * kBuffer;
-      read(cur, 1);
-      mul(0);
-      meet();
-      if (s + 2 < s1) load(s + 2, cur);
-      if (s + 1 < s1) read(nxt, 0);
-      mul(1);
+    const auto first = [&](auto set) __attribute__((always_inline)) {
+      read_b(set);
+#pragma unroll
+      for (uint32_t i = 0; i < MF; ++i) fa[i] = ra.get(from, i);
+      from = next(from);
+    };
+    typedef std::integral_constant<uint32_t, 0> S0;
+    typedef std::integral_constant<uint32_t, 1> S1;
+    if ((s1 - s0) % 2) {
+      first(S1());
+      step(S1());
+    } else {
+      first(S0());
+    }
+    while (s < s1) {
+      step(S0());
+      step(S1());
     }
   }
 
