@@ -10,46 +10,40 @@ using ark::fail;
 
 constexpr uint32_t kLanes = 256;
 
-// Eight neighbouring values, in fp32.
-struct Eight {
-  float v[8];
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// N neighbouring values of a row, in fp32, at any element's alignment (gfx950 takes
+// unaligned global accesses).
+template <uint32_t N>
+struct Some {
+  float v[N];
   template <uint32_t DT>
-  __device__ __forceinline__ void load(const void* row, uint64_t c, uint32_t n, bool vec) {
+  __device__ __forceinline__ void load(const void* row, uint64_t c) {
     typedef elem_t<DT> T;
-    const T* p = (const T*)row + c;
-    if (vec && n >= 8) {
-      if constexpr (DT == ARK_EMBED_F32) {
-        const f32x4 a = ld_g<f32x4>(p), b = ld_g<f32x4>(p + 4);
+    typedef T V __attribute__((ext_vector_type(N < 8 || DT != ARK_EMBED_F32 ? N : 4),
+                               aligned(sizeof(T))));
+    constexpr uint32_t kEach = sizeof(V) / sizeof(T);
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
-      } else {
-        typedef T V __attribute__((ext_vector_type(8)));
-        const V a = ld_g<V>(p);
+    for (uint32_t i = 0; i < N; i += kEach) {
+      const V a = *(const ARK_GLOBAL V*)((const T*)row + c + i);
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) v[i] = (float)a[i];
-      }
-      return;
+      for (uint32_t k = 0; k < kEach; ++k) v[i + k] = (float)a[k];
     }
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.0f;
   }
   template <uint32_t DT>
-  __device__ __forceinline__ void store(void* row, uint64_t c, uint32_t n, bool vec) const {
+  __device__ __forceinline__ void store(void* row, uint64_t c) const {
     typedef elem_t<DT> T;
-    T* p = (T*)row + c;
-    if (vec && n >= 8) {
-      if constexpr (DT == ARK_EMBED_F32) {
-        st_g<f32x4>(p, f32x4{v[0], v[1], v[2], v[3]});
-        st_g<f32x4>(p + 4, f32x4{v[4], v[5], v[6], v[7]});
-      } else {
-        st_g<u32x4>(p, u32x4{narrow2<DT>(v[0], v[1]), narrow2<DT>(v[2], v[3]),
-                             narrow2<DT>(v[4], v[5]), narrow2<DT>(v[6], v[7])});
-      }
-      return;
-    }
+    if constexpr (DT == ARK_EMBED_F32) {
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i)
-      if (i < n) p[i] = (T)v[i];
+      for (uint32_t i = 0; i < N; i += 4)
+        st_g<f32x4_a4>((T*)row + c + i, f32x4_a4{v[i], v[i + 1], v[i + 2], v[i + 3]});
+    } else {
+      typedef uint32_t V __attribute__((ext_vector_type(N / 2), aligned(2)));
+      V a;
+#pragma unroll
+      for (uint32_t i = 0; i < N / 2; ++i) a[i] = narrow2<DT>(v[2 * i], v[2 * i + 1]);
+      *(ARK_GLOBAL V*)((T*)row + c) = a;
+    }
   }
 };
 
@@ -69,10 +63,13 @@ struct LookupArgs {
   const void* table;
   void* out;
   uint64_t table_stride, out_stride, n;
-  uint32_t columns, vec_in, vec_out;
+  uint32_t columns;
   float scale;
 };
 
+// A lane takes eight values of a row; those past the last whole eight are the last
+// eight again, written twice alike.  Bound by HBM: 16384 rows of 2048 bf16, 18 us
+// with the call, 7.3 TB/s (rows that occur twice come from cache).
 template <uint32_t IN, uint32_t OUT>
 __global__ __launch_bounds__(kLanes) void lookup_kernel(LookupArgs a) {
   const uint32_t per = (a.columns + 7) / 8;
@@ -80,15 +77,28 @@ __global__ __launch_bounds__(kLanes) void lookup_kernel(LookupArgs a) {
   for (uint64_t i = (uint64_t)blockIdx.x * kLanes + threadIdx.x; i < all;
        i += (uint64_t)gridDim.x * kLanes) {
     const uint64_t t = i / per;
-    const uint32_t c = (uint32_t)(i % per) * 8, n = min(a.columns - c, 8u);
+    const uint32_t c = min((uint32_t)(i % per) * 8, a.columns - 8);
     const uint32_t v = a.tokens.at(t);
-    Eight e = {};
+    Some<8> e = {};
     if (v != ~0u) {
-      e.load<IN>((const elem_t<IN>*)a.table + v * a.table_stride, c, n, a.vec_in);
+      e.load<IN>((const elem_t<IN>*)a.table + v * a.table_stride, c);
 #pragma unroll
       for (uint32_t k = 0; k < 8; ++k) e.v[k] *= a.scale;
     }
-    e.store<OUT>((elem_t<OUT>*)a.out + t * a.out_stride, c, n, a.vec_out);
+    e.store<OUT>((elem_t<OUT>*)a.out + t * a.out_stride, c);
+  }
+}
+// Rows of fewer than eight values, a lane a value.
+template <uint32_t IN, uint32_t OUT>
+__global__ __launch_bounds__(kLanes) void lookup_short_kernel(LookupArgs a) {
+  const uint64_t all = a.n * a.columns;
+  for (uint64_t i = (uint64_t)blockIdx.x * kLanes + threadIdx.x; i < all;
+       i += (uint64_t)gridDim.x * kLanes) {
+    const uint64_t t = i / a.columns;
+    const uint32_t c = (uint32_t)(i % a.columns), v = a.tokens.at(t);
+    const float x =
+        v != ~0u ? (float)((const elem_t<IN>*)a.table)[v * a.table_stride + c] * a.scale : 0.0f;
+    ((elem_t<OUT>*)a.out)[t * a.out_stride + c] = (elem_t<OUT>)x;
   }
 }
 
@@ -97,77 +107,97 @@ __global__ __launch_bounds__(kLanes) void lookup_kernel(LookupArgs a) {
 // Positions sorted by token: a block takes kGroup rows of the table, goes through
 // the tokens twice, first counting its own rows' and those of rows before its own,
 // then placing the positions of its rows, each wave a stretch of the tokens, so
-// that a token's positions stay in order.  Then sums of whole windows of 64 sorted
-// positions of one token (frequent ones: text's most frequent token takes a tenth
-// of all), and a row's sum from its windows' and the positions beside them.
+// that a token's positions stay in order.  Then sums of whole windows of sixteen
+// sorted positions of one token (text's most frequent token takes a tenth of all:
+// its rows are added by many waves at once), and a row's sum from its windows' and
+// the positions beside them.
 
 constexpr uint32_t kGroup = 128;
 constexpr uint32_t kSortLanes = 1024;
 constexpr uint32_t kSortWaves = kSortLanes / 64;
-constexpr uint32_t kWindow = 64;
+constexpr uint32_t kKept = 16;  // tokens a lane asks for at once
+constexpr uint32_t kWindow = 16;
 
+// KEEP: each lane has kKept tokens at most, which stay in registers for the second
+// time (16384 tokens into 250 groups: 16 us without).
+template <bool KEEP>
 __global__ __launch_bounds__(kSortLanes) void sort_kernel(Tokens tokens, uint32_t n,
                                                           uint32_t* __restrict__ start,
                                                           uint32_t* __restrict__ pos) {
-  __shared__ uint32_t s_at[kSortWaves][kGroup], s_below[kSortWaves];
+  __shared__ uint32_t s_at[kSortWaves][kGroup], s_below[kSortWaves], s_first;
+  static_assert(kGroup == 128, "two waves' rows");
   const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const uint32_t v0 = blockIdx.x * kGroup;
   const uint32_t per = (n + kSortLanes - 1) / kSortLanes * 64;  // tokens a wave takes
   const uint32_t lo = min(n, wave * per), hi = min(n, lo + per);
   for (uint32_t i = lane; i < kGroup; i += 64) s_at[wave][i] = 0;
-  uint32_t below = 0;
-  for (uint32_t t = lo + lane; t < hi; t += 64) {
-    const uint32_t v = tokens.at(t);
-    if (v < v0)
-      ++below;
-    else if (v - v0 < kGroup)
-      atomicAdd(&s_at[wave][v - v0], 1u);
+  uint32_t below = 0, v[kKept];
+  const auto ask = [&](uint32_t t0) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t k = 0; k < kKept; ++k) {
+      const uint32_t t = t0 + k * 64 + lane;
+      v[k] = tokens.at(min(t, n - 1));
+      if (t >= hi) v[k] = ~0u;
+    }
+  };
+  if (KEEP && n) ask(lo);
+  for (uint32_t t0 = lo; t0 < hi; t0 += 64 * kKept) {
+    if (!KEEP) ask(t0);
+#pragma unroll
+    for (uint32_t k = 0; k < kKept; ++k) {
+      if (v[k] < v0)
+        ++below;
+      else if (v[k] - v0 < kGroup)
+        atomicAdd(&s_at[wave][v[k] - v0], 1u);
+    }
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) below += __shfl_xor(below, o);
   if (lane == 0) s_below[wave] = below;
   __syncthreads();
-  // starts: of the group's rows, and of each wave's positions in them
-  if (wave == 0) {
-    uint32_t at = 0;
-    for (uint32_t w = 0; w < kSortWaves; ++w) at += s_below[w];
-    uint32_t mine[2] = {0, 0};  // rows 2 lane, 2 lane + 1
+  // starts: of the group's rows, and of each wave's positions in them, a lane a row
+  const uint32_t row = threadIdx.x;
+  uint32_t count[kSortWaves], total = 0, incl = 0;
+  if (row < kGroup) {
 #pragma unroll
-    for (uint32_t k = 0; k < 2; ++k)
-      for (uint32_t w = 0; w < kSortWaves; ++w) mine[k] += s_at[w][2 * lane + k];
-    uint32_t incl = mine[0] + mine[1];
+    for (uint32_t w = 0; w < kSortWaves; ++w) count[w] = s_at[w][row];
+#pragma unroll
+    for (uint32_t w = 0; w < kSortWaves; ++w) total += count[w];
+    incl = total;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const uint32_t y = __shfl_up(incl, o);
       if (lane >= (uint32_t)o) incl += y;
     }
-    uint32_t from = at + incl - mine[0] - mine[1];
-#pragma unroll
-    for (uint32_t k = 0; k < 2; ++k) {
-      const uint32_t v = v0 + 2 * lane + k;
-      if (v <= tokens.vocab) start[v] = from;
-      for (uint32_t w = 0; w < kSortWaves; ++w) {
-        const uint32_t c = s_at[w][2 * lane + k];
-        s_at[w][2 * lane + k] = from;
-        from += c;
-      }
-    }
-    if (lane == 63 && v0 + kGroup == tokens.vocab) start[tokens.vocab] = from;
+    if (row == 63) s_first = incl;
   }
   __syncthreads();
-  for (uint32_t t0 = lo; t0 < hi; t0 += 64) {
-    const uint32_t t = t0 + lane;
-    const uint32_t v = t < hi ? tokens.at(t) : ~0u;
-    const uint32_t r = v - v0;
-    uint64_t left = __ballot(v != ~0u && v >= v0 && r < kGroup);
-    while (left) {
-      const uint32_t first = (uint32_t)__ffsll((unsigned long long)left) - 1u;
-      const uint32_t row = __builtin_amdgcn_readlane(r, first);
-      const uint64_t same = __ballot(r == row) & left;
-      const uint32_t at = s_at[wave][row];
-      if (same >> lane & 1u) pos[at + __popcll(same & ((1ull << lane) - 1ull))] = t;
-      if (lane == first) s_at[wave][row] = at + (uint32_t)__popcll(same);
-      left &= ~same;
+  if (row < kGroup) {
+    uint32_t from = incl - total + (row < 64 ? 0u : s_first);
+#pragma unroll
+    for (uint32_t w = 0; w < kSortWaves; ++w) from += s_below[w];
+    if (v0 + row <= tokens.vocab) start[v0 + row] = from;
+    if (row + 1 == kGroup && v0 + kGroup == tokens.vocab) start[tokens.vocab] = from + total;
+#pragma unroll
+    for (uint32_t w = 0; w < kSortWaves; ++w) s_at[w][row] = from, from += count[w];
+  }
+  __syncthreads();
+  for (uint32_t t0 = lo; t0 < hi; t0 += 64 * kKept) {
+    if (!KEEP) ask(t0);
+#pragma unroll
+    for (uint32_t k = 0; k < kKept; ++k) {
+      const uint32_t r = v[k] - v0;
+      uint64_t left = __ballot(v[k] != ~0u && v[k] >= v0 && r < kGroup);
+      while (left) {
+        const uint32_t first = (uint32_t)__ffsll((unsigned long long)left) - 1u;
+        const uint32_t row = __builtin_amdgcn_readlane(r, first);
+        const uint64_t same = __ballot(r == row) & left;
+        const uint32_t at = s_at[wave][row];
+        if (same >> lane & 1u)
+          pos[at + __popcll(same & ((1ull << lane) - 1ull))] = t0 + k * 64 + lane;
+        if (lane == first) s_at[wave][row] = at + (uint32_t)__popcll(same);
+        left &= ~same;
+      }
     }
   }
 }
@@ -177,89 +207,167 @@ struct SumArgs {
   const void* dy;
   uint64_t dy_stride;
   const uint32_t *start, *pos;
-  float* windows;  // [n / 64][columns up to 8]
+  float* windows;  // [n / 16][columns up to 4]
   float* dw;
   uint64_t dw_stride;
-  uint32_t n, columns, vec_in, vec_out, accumulate;
+  uint32_t n, columns, accumulate;
   float scale;
 };
 
-constexpr uint32_t kBatch = 8;  // rows in flight
+// A wave takes 256 columns, a lane four; those past the last whole four are the
+// last four again.  Rows of fewer than four values: a lane one of them (WIDE false).
+template <bool WIDE>
+struct Column {
+  static constexpr uint32_t kEach = WIDE ? 4 : 1, kWave = WIDE ? 256 : 64;
+  uint32_t own, c;  // the first that is the lane's alone, and that it loads (lanes
+                    // past the last column load with the others and store nothing)
+  __device__ __forceinline__ Column(uint32_t tile, uint32_t columns) {
+    own = (tile * 64 + threadIdx.x % 64) * kEach;
+    c = min(own, columns - kEach);
+  }
+};
 
-// e = the rows at sorted positions [lo, hi), added in order, columns [c, c + n).
-template <uint32_t DT>
-__device__ __forceinline__ void add_rows(const SumArgs& a, Eight* e, uint32_t lo, uint32_t hi,
-                                         uint32_t c, uint32_t n) {
+// e = e + the rows at sorted positions [lo, hi), in order, kBatch in flight.
+template <uint32_t DT, bool WIDE, uint32_t kBatch>
+__device__ __forceinline__ void add_rows(const SumArgs& a, const Column<WIDE>& col,
+                                         float (&e)[Column<WIDE>::kEach], uint32_t lo,
+                                         uint32_t hi) {
+  constexpr uint32_t E = Column<WIDE>::kEach;
   for (uint32_t i = lo; i < hi; i += kBatch) {
-    Eight v[kBatch];
+    // the positions of the rows, a lane one
+    const uint32_t k = i + threadIdx.x % kBatch;
+    const uint32_t p = ld_g<uint32_t>(a.pos + min(k, hi - 1));
+    float v[kBatch][E];
 #pragma unroll
-    for (uint32_t k = 0; k < kBatch; ++k)
-      if (i + k < hi)
-        v[k].load<DT>((const elem_t<DT>*)a.dy + a.pos[i + k] * a.dy_stride, c, n, a.vec_in);
+    for (uint32_t k = 0; k < kBatch; ++k) {
+      const uint32_t t = __builtin_amdgcn_readlane(p, k);
+      const elem_t<DT>* row = (const elem_t<DT>*)a.dy + t * a.dy_stride;
+      if (i + k < hi) {
+        if constexpr (WIDE) {
+          Some<4> s;
+          s.load<DT>(row, col.c);
+#pragma unroll
+          for (uint32_t j = 0; j < E; ++j) v[k][j] = s.v[j];
+        } else {
+          v[k][0] = (float)row[col.c];
+        }
+      }
+    }
 #pragma unroll
     for (uint32_t k = 0; k < kBatch; ++k)
       if (i + k < hi) {
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) e->v[j] += v[k].v[j];
+        for (uint32_t j = 0; j < E; ++j) e[j] += v[k][j];
       }
   }
 }
 
-// Columns a wave takes: 512.
-__device__ __forceinline__ uint32_t wave_tiles(uint32_t columns) { return (columns + 511) / 512; }
+__device__ __forceinline__ uint64_t window_width(uint32_t columns) {
+  return (columns + 3) / 4 * 4;
+}
 
-template <uint32_t DT>
+template <uint32_t DT, bool WIDE>
 __global__ __launch_bounds__(kLanes) void window_kernel(SumArgs a) {
-  const uint32_t tiles = wave_tiles(a.columns);
-  const uint64_t id = (uint64_t)blockIdx.x * (kLanes / 64) + threadIdx.x / 64;
+  typedef Column<WIDE> C;
+  const uint32_t tiles = (a.columns + C::kWave - 1) / C::kWave;
+  const uint64_t id = (uint64_t)blockIdx.x * (kLanes / 64) +
+                      __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint64_t w = id / tiles;
-  const uint32_t c = ((uint32_t)(id % tiles) * 64 + threadIdx.x % 64) * 8;
   if ((w + 1) * kWindow > a.start[a.tokens.vocab]) return;
   const uint32_t lo = (uint32_t)w * kWindow;
   if (a.tokens.at(a.pos[lo]) != a.tokens.at(a.pos[lo + kWindow - 1])) return;
-  if (c >= a.columns) return;
-  Eight e = {};
-  add_rows<DT>(a, &e, lo, lo + kWindow, c, min(a.columns - c, 8u));
-  const uint64_t width = (a.columns + 7) / 8 * 8;
-  e.store<ARK_EMBED_F32>(a.windows + w * width, c, 8, true);
+  const C col((uint32_t)(id % tiles), a.columns);
+  float e[C::kEach] = {};
+  add_rows<DT, WIDE, kWindow>(a, col, e, lo, lo + kWindow);
+  float* out = a.windows + w * window_width(a.columns) + col.c;
+  // a lane's last four may be another's too: written twice alike
+#pragma unroll
+  for (uint32_t j = 0; j < C::kEach; ++j) out[j] = e[j];
 }
 
-template <uint32_t DT>
+constexpr uint32_t kBatch = 8;  // half the registers of sixteen, twice the waves
+
+constexpr uint32_t kRows = 4;     // rows of the table a wave takes, their starts read at once
+
+template <uint32_t DT, bool WIDE>
+__device__ __forceinline__ void sum_row(const SumArgs& a, const Column<WIDE>& col, uint32_t v,
+                                        uint32_t lo, uint32_t hi) {
+  typedef Column<WIDE> C;
+  float e[C::kEach] = {};
+  const uint32_t w0 = (lo + kWindow - 1) / kWindow, w1 = hi / kWindow;  // whole windows
+  const bool windows = w0 < w1;
+  add_rows<DT, WIDE, kBatch>(a, col, e, lo, windows ? w0 * kWindow : hi);
+  if (windows) {
+    const uint64_t width = window_width(a.columns);
+    for (uint32_t w = w0; w < w1; w += kBatch) {
+      float s[kBatch][C::kEach];
+#pragma unroll
+      for (uint32_t k = 0; k < kBatch; ++k)
+        if (w + k < w1) {
+          const float* in = a.windows + (w + k) * width + col.c;
+#pragma unroll
+          for (uint32_t j = 0; j < C::kEach; ++j) s[k][j] = in[j];
+        }
+#pragma unroll
+      for (uint32_t k = 0; k < kBatch; ++k)
+        if (w + k < w1) {
+#pragma unroll
+          for (uint32_t j = 0; j < C::kEach; ++j) e[j] += s[k][j];
+        }
+    }
+    add_rows<DT, WIDE, kBatch>(a, col, e, w1 * kWindow, hi);
+  }
+  float* row = a.dw + v * a.dw_stride;
+#pragma unroll
+  for (uint32_t j = 0; j < C::kEach; ++j) e[j] *= a.scale;
+  if constexpr (WIDE) {
+    if (col.c == col.own) {
+      Some<4> out;
+      if (a.accumulate) out.load<ARK_EMBED_F32>(row, col.c);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) out.v[j] = a.accumulate ? out.v[j] + e[j] : e[j];
+      out.store<ARK_EMBED_F32>(row, col.c);
+      return;
+    }
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < C::kEach; ++j)
+    if (col.c + j >= col.own) row[col.c + j] = a.accumulate ? row[col.c + j] + e[j] : e[j];
+}
+
+// Every row of the table, or those of tokens that occur.  Most rows have no token
+// (a vocabulary is larger than a batch's words), so what counts is the zeros'
+// way to memory: 16384 tokens into 32000 x 768, 98 MB.
+template <uint32_t DT, bool WIDE>
 __global__ __launch_bounds__(kLanes) void sum_kernel(SumArgs a) {
-  const uint32_t tiles = wave_tiles(a.columns);
-  const uint64_t all = (uint64_t)a.tokens.vocab * tiles;
-  for (uint64_t id = (uint64_t)blockIdx.x * (kLanes / 64) + threadIdx.x / 64; id < all;
-       id += (uint64_t)gridDim.x * (kLanes / 64)) {
-    const uint32_t v = (uint32_t)(id / tiles);
-    const uint32_t c = ((uint32_t)(id % tiles) * 64 + threadIdx.x % 64) * 8;
-    const uint32_t lo = a.start[v], hi = a.start[v + 1];
-    if ((a.accumulate && lo == hi) || c >= a.columns) continue;
-    const uint32_t n = min(a.columns - c, 8u);
-    Eight e = {};
-    const uint32_t w0 = (lo + kWindow - 1) / kWindow, w1 = hi / kWindow;  // whole windows
-    if (w0 < w1) {
-      const uint64_t width = (a.columns + 7) / 8 * 8;
-      add_rows<DT>(a, &e, lo, w0 * kWindow, c, n);
-      for (uint32_t w = w0; w < w1; ++w) {
-        Eight s;
-        s.load<ARK_EMBED_F32>(a.windows + w * width, c, 8, true);
+  typedef Column<WIDE> C;
+  const uint32_t tiles = (a.columns + C::kWave - 1) / C::kWave, vocab = a.tokens.vocab;
+  const uint64_t all = (uint64_t)((vocab + kRows - 1) / kRows) * tiles;
+  for (uint64_t id = (uint64_t)blockIdx.x * (kLanes / 64) +
+                     __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+       id < all; id += (uint64_t)gridDim.x * (kLanes / 64)) {
+    const uint32_t v0 = (uint32_t)(id / tiles) * kRows;
+    const C col((uint32_t)(id % tiles), a.columns);
+    uint32_t at[kRows + 1];
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) e.v[j] += s.v[j];
+    for (uint32_t k = 0; k <= kRows; ++k) at[k] = a.start[min(v0 + k, vocab)];
+    if (!a.accumulate) {
+#pragma unroll
+      for (uint32_t k = 0; k < kRows; ++k) {
+        if (at[k] != at[k + 1] || v0 + k >= vocab) continue;
+        float* row = a.dw + (v0 + k) * a.dw_stride;
+        if (WIDE && col.c == col.own) {
+          const Some<4> none = {};
+          none.store<ARK_EMBED_F32>(row, col.c);
+        } else {
+#pragma unroll
+          for (uint32_t j = 0; j < C::kEach; ++j)
+            if (col.c + j >= col.own) row[col.c + j] = 0.0f;
+        }
       }
-      add_rows<DT>(a, &e, w1 * kWindow, hi, c, n);
-    } else {
-      add_rows<DT>(a, &e, lo, hi, c, n);
     }
-    float* row = a.dw + v * a.dw_stride;
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) e.v[j] *= a.scale;
-    if (a.accumulate) {
-      Eight old;
-      old.load<ARK_EMBED_F32>(row, c, n, a.vec_out);
-#pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) e.v[j] += old.v[j];
-    }
-    e.store<ARK_EMBED_F32>(row, c, n, a.vec_out);
+    for (uint32_t k = 0; k < kRows; ++k)
+      if (at[k] != at[k + 1]) sum_row<DT, WIDE>(a, col, v0 + k, at[k], at[k + 1]);
   }
 }
 
@@ -273,7 +381,7 @@ Layout layout_of(uint64_t n, uint64_t vocab, uint64_t columns) {
   l.start = 0;
   l.pos = ark::align_up((vocab + 1) * 4, 256);
   l.windows = l.pos + ark::align_up(n * 4, 256);
-  l.bytes = l.windows + n / kWindow * ((columns + 7) / 8 * 8) * 4;
+  l.bytes = l.windows + n / kWindow * ((columns + 3) / 4 * 4) * 4;
   return l;
 }
 
@@ -299,10 +407,6 @@ int rows_bytes(uint64_t rows, uint64_t row, uint64_t stride, uint32_t es, bool w
   return ARK_OPT_OK;
 }
 
-bool vec16(const void* p, uint64_t stride, uint32_t es) {
-  return (uintptr_t)p % 16 == 0 && stride * es % 16 == 0;
-}
-
 int check_types(uint32_t a, uint32_t b, uint32_t token_bytes) {
   if (a > ARK_EMBED_F32 || b > ARK_EMBED_F32)
     return fail(ARK_OPT_EINVAL, "dtype %u unknown", a > ARK_EMBED_F32 ? a : b);
@@ -311,28 +415,42 @@ int check_types(uint32_t a, uint32_t b, uint32_t token_bytes) {
   return ARK_OPT_OK;
 }
 
+template <uint32_t IN, uint32_t OUT>
+void launch_lookup(const LookupArgs& a, dim3 grid, hipStream_t s) {
+  if (a.columns < 8)
+    hipLaunchKernelGGL((lookup_short_kernel<IN, OUT>), grid, dim3(kLanes), 0, s, a);
+  else
+    hipLaunchKernelGGL((lookup_kernel<IN, OUT>), grid, dim3(kLanes), 0, s, a);
+}
 template <uint32_t IN>
 void launch_lookup(const LookupArgs& a, uint32_t out, dim3 grid, hipStream_t s) {
   if (out == ARK_EMBED_F16)
-    hipLaunchKernelGGL((lookup_kernel<IN, ARK_EMBED_F16>), grid, dim3(kLanes), 0, s, a);
+    launch_lookup<IN, ARK_EMBED_F16>(a, grid, s);
   else if (out == ARK_EMBED_BF16)
-    hipLaunchKernelGGL((lookup_kernel<IN, ARK_EMBED_BF16>), grid, dim3(kLanes), 0, s, a);
+    launch_lookup<IN, ARK_EMBED_BF16>(a, grid, s);
   else
-    hipLaunchKernelGGL((lookup_kernel<IN, ARK_EMBED_F32>), grid, dim3(kLanes), 0, s, a);
+    launch_lookup<IN, ARK_EMBED_F32>(a, grid, s);
 }
 
-template <uint32_t DT>
+template <uint32_t DT, bool WIDE>
 int launch_sums(const SumArgs& a, hipStream_t s) {
-  const uint64_t tiles = (a.columns + 511) / 512, windows = a.n / kWindow * tiles;
+  const uint64_t tiles = (a.columns + Column<WIDE>::kWave - 1) / Column<WIDE>::kWave;
+  const uint64_t windows = a.n / kWindow * tiles;
   if (windows) {
-    hipLaunchKernelGGL(window_kernel<DT>, dim3((uint32_t)((windows + 3) / 4)), dim3(kLanes), 0, s, a);
+    hipLaunchKernelGGL((window_kernel<DT, WIDE>), dim3((uint32_t)((windows + 3) / 4)), dim3(kLanes),
+                       0, s, a);
     ARK_HIP(hipGetLastError());
   }
-  const uint64_t blocks = ((uint64_t)a.tokens.vocab * tiles + 3) / 4;
-  hipLaunchKernelGGL(sum_kernel<DT>, dim3((uint32_t)(blocks < (1u << 23) ? blocks : 1u << 23)),
-                     dim3(kLanes), 0, s, a);
+  const uint64_t blocks = (((uint64_t)a.tokens.vocab + kRows - 1) / kRows * tiles + 3) / 4;
+  hipLaunchKernelGGL((sum_kernel<DT, WIDE>),
+                     dim3((uint32_t)(blocks < (1u << 23) ? blocks : 1u << 23)), dim3(kLanes), 0, s,
+                     a);
   ARK_HIP(hipGetLastError());
   return ARK_OPT_OK;
+}
+template <uint32_t DT>
+int launch_sums(const SumArgs& a, hipStream_t s) {
+  return a.columns < 4 ? launch_sums<DT, false>(a, s) : launch_sums<DT, true>(a, s);
 }
 
 }  // namespace
@@ -369,7 +487,6 @@ int ark_embed_lookup(const void* table, uint64_t table_stride, uint32_t table_dt
   a.table = table, a.out = out;
   a.table_stride = table_stride, a.out_stride = out_stride, a.n = n;
   a.columns = (uint32_t)columns;
-  a.vec_in = vec16(table, table_stride, es), a.vec_out = vec16(out, out_stride, eo);
   a.scale = scale;
   const uint64_t blocks = (n * ((columns + 7) / 8) + kLanes - 1) / kLanes;
   const dim3 grid((uint32_t)(blocks < (1u << 20) ? blocks : 1u << 20));
@@ -439,11 +556,15 @@ int ark_embed_grad(const void* dy, uint64_t dy_stride, uint32_t dy_dtype, const 
   a.windows = (float*)(ws + l.windows);
   a.dw = dw, a.dw_stride = dw_stride;
   a.n = (uint32_t)n, a.columns = (uint32_t)columns;
-  a.vec_in = vec16(dy, dy_stride, es), a.vec_out = vec16(dw, dw_stride, 4);
   a.accumulate = flags & ARK_EMBED_ACCUMULATE ? 1u : 0u;
   a.scale = scale;
-  hipLaunchKernelGGL(sort_kernel, dim3((uint32_t)((vocab + kGroup - 1) / kGroup)), dim3(kSortLanes),
-                     0, s, a.tokens, a.n, (uint32_t*)a.start, (uint32_t*)a.pos);
+  const dim3 groups((uint32_t)((vocab + kGroup - 1) / kGroup));
+  if (n <= kSortLanes * kKept)
+    hipLaunchKernelGGL(sort_kernel<true>, groups, dim3(kSortLanes), 0, s, a.tokens, a.n,
+                       (uint32_t*)a.start, (uint32_t*)a.pos);
+  else
+    hipLaunchKernelGGL(sort_kernel<false>, groups, dim3(kSortLanes), 0, s, a.tokens, a.n,
+                       (uint32_t*)a.start, (uint32_t*)a.pos);
   ARK_HIP(hipGetLastError());
   if (dy_dtype == ARK_EMBED_F16) return launch_sums<ARK_EMBED_F16>(a, s);
   if (dy_dtype == ARK_EMBED_BF16) return launch_sums<ARK_EMBED_BF16>(a, s);

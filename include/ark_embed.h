@@ -11,8 +11,8 @@
  * A token outside [0, vocab) has no row: its out is zeros, and its dy is not read.
  *
  * The gradient's sums are of fp32: positions of a token in increasing order, by
- * groups of 64 whose sums are added in order, so equal calls give equal bits, and
- * a sum of n rows is within (min(n, 128) + n / 64 + 2) 2^-24 of the sum of their
+ * groups of 16 whose sums are added in order, so equal calls give equal bits, and
+ * a sum of n rows is within (min(n, 64) + n / 16 + 2) 2^-24 of the sum of their
  * magnitudes.
  *
  * Every function is stream ordered and returns an ARK_OPT_* status code

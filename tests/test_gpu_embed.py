@@ -2,8 +2,8 @@
 64 bits.
 
 A row is one product and one rounding: within 2^-24 and half a step of the output's
-type.  A gradient is a sum of n rows in fp32, by groups of 64: within
-(min(n, 128) + n / 64 + 2) 2^-24 of the sum of their magnitudes, 2^-24 of it for the
+type.  A gradient is a sum of n rows in fp32, by groups of 16: within
+(min(n, 64) + n / 16 + 2) 2^-24 of the sum of their magnitudes, 2^-24 of it for the
 scale and, accumulated, another of the result; whole numbers are exact."""
 import pytest
 
@@ -82,7 +82,7 @@ def _check(dw, dy, tokens, v, scale=1.0, before=None):
     size.index_add_(0, at, rows.abs())
     n.index_add_(0, at, torch.ones_like(at, dtype=torch.float64))
     s = torch.tensor(scale, dtype=torch.float32).double().item()
-    limit = ((n.clamp_max(128) + n / 64 + 3) * 2.0 ** -24)[:, None] * size * abs(s)
+    limit = ((n.clamp_max(64) + n / 16 + 3) * 2.0 ** -24)[:, None] * size * abs(s)
     want = want * s
     if before is not None:
         want = want + before.double()
