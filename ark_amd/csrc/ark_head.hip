@@ -166,6 +166,7 @@ __global__ __launch_bounds__(kLanes) void gather_kernel(GatherArgs a) {
   const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const uint32_t t0 = blockIdx.x * kGatherRows;
   uint32_t before = 0;
+#pragma unroll 8
   for (uint32_t t = threadIdx.x; t < t0; t += kLanes) before += a.targets.live(t) ? 1u : 0u;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) before += __shfl_xor(before, o);
@@ -321,50 +322,70 @@ __global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {
   const Operand ow = {a.w + m0 * a.w_stride, a.w_stride, a.vocab - m0, 0};
   const Operand ox = {a.x + (uint64_t)n0 * a.padded, a.padded, P::BN, 0};
   p.run(ow, ox, 0, a.padded / kProductStep, (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds);
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const uint32_t v0 = m0 + wave % P::WM * 16 * P::MF + lane / 16 * 4;
+  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t w0 = m0 + wave % P::WM * 16 * P::MF;  // the wave's first of the vocabulary
   const uint32_t span = tm * P::WM + wave % P::WM;
+  if (m0 + P::BM > a.vocab) {
+#pragma unroll
+    for (uint32_t i = 0; i < P::MF; ++i)
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k)
+        if (w0 + lane / 16 * 4 + i * 16 + k >= a.vocab) {
+#pragma unroll
+          for (uint32_t j = 0; j < P::NF; ++j) p.acc[i][j][k] = -INFINITY;
+        }
+  }
+  if (a.e) __syncthreads();  // LDS is the exponentials' now
+  // A wave's exponentials of 16 rows pass through LDS of its own, so that a row's
+  // leave as whole lines: chunks of 16 bytes, permuted by the row against conflicts.
+  constexpr uint32_t kRow = P::MF * 32, kChunks = kRow / 16;  // bytes of a row
+  static_assert(16 * kRow * P::WM * P::WN <= P::kLds, "a part of LDS for each wave");
+  uint8_t* mine = lds + wave * 16 * kRow;
+  const float to2 = a.scale * kLog2e;
 #pragma unroll
   for (uint32_t j = 0; j < P::NF; ++j) {
-    const uint32_t t = n0 + wave / P::WM * 16 * P::NF + j * 16 + lane % 16;
+    const uint32_t t0 = n0 + wave / P::WM * 16 * P::NF + j * 16, t = t0 + lane % 16;
     float most = -INFINITY;
 #pragma unroll
     for (uint32_t i = 0; i < P::MF; ++i)
 #pragma unroll
-      for (uint32_t k = 0; k < 4; ++k) {
-        float z = p.acc[i][j][k] * a.scale;
-        if (v0 + i * 16 + k >= a.vocab) z = -INFINITY;
-        p.acc[i][j][k] = z;
-        most = fmaxf(most, z);
-      }
+      for (uint32_t k = 0; k < 4; ++k) most = fmaxf(most, p.acc[i][j][k]);
     most = fmaxf(most, __shfl_xor(most, 16));
     most = fmaxf(most, __shfl_xor(most, 32));
-    const float from = most == -INFINITY ? 0.0f : most;
+    const float from = most == -INFINITY ? 0.0f : -most * to2;
     float sum = 0.0f;
 #pragma unroll
     for (uint32_t i = 0; i < P::MF; ++i)
 #pragma unroll
       for (uint32_t k = 0; k < 4; ++k) {
-        const float e = exp_of(p.acc[i][j][k] - from);
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(p.acc[i][j][k], to2, from));
         p.acc[i][j][k] = e;
         sum += e;
       }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    if (t >= live) continue;
-    if (lane < 16) {
+    if (lane < 16 && t < live) {
       float* s = a.stats + ((uint64_t)t * a.spans + span) * 2;
-      s[0] = most, s[1] = sum;
+      s[0] = most * a.scale, s[1] = sum;
     }
-    if (a.e) {
-      uint16_t* e = a.e + t * a.e_stride + v0;
+    if (!a.e) continue;
+    const uint32_t row = lane % 16;
 #pragma unroll
-      for (uint32_t i = 0; i < P::MF; ++i) {
-        const f32x4 v = p.acc[i][j];
-        st_g<u32x2>(e + i * 16, u32x2{narrow2<kTypeOf<typename P::T>>(v[0], v[1]),
-                                      narrow2<kTypeOf<typename P::T>>(v[2], v[3])});
-      }
+    for (uint32_t i = 0; i < P::MF; ++i) {
+      const f32x4 v = p.acc[i][j];
+      const uint32_t chunk = (i * 2 + lane / 32) ^ (row % kChunks);
+      *(u32x2*)(mine + row * kRow + chunk * 16 + lane / 16 % 2 * 8) =
+          u32x2{narrow2<kTypeOf<typename P::T>>(v[0], v[1]),
+                narrow2<kTypeOf<typename P::T>>(v[2], v[3])};
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (uint32_t i = 0; i < kRow / 64; ++i) {
+      const uint32_t q = i * 64 + lane, r = q / kChunks, c = q % kChunks;
+      const u32x4 v = *(const u32x4*)(mine + r * kRow + (c ^ (r % kChunks)) * 16);
+      if (t0 + r < live) st_g<u32x4>(a.e + (t0 + r) * a.e_stride + w0 + c * 8, v);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
@@ -956,10 +977,9 @@ int run(Call c) {
     return fail(ARK_OPT_EINVAL, "%s of %u bytes: 4 or 8", c.teacher ? "indices" : "targets", ib);
   if (c.teacher && c.logits_dtype > ARK_HEAD_F32)
     return fail(ARK_OPT_EINVAL, "logits_dtype %u unknown", c.logits_dtype);
-  if (!(c.scale > 0.0f) || !(c.scale < INFINITY))
-    return fail(ARK_OPT_EINVAL, "%s", c.teacher ? "temperature must be positive and finite, and so "
-                                                  "must its reciprocal"
-                                                : "scale must be positive and finite");
+  if (!(c.scale > 0.0f) || !(c.scale < 0x1p126f))
+    return fail(ARK_OPT_EINVAL, "%s must be positive, and %s below 2^126",
+                c.teacher ? "temperature" : "scale", c.teacher ? "finite, its reciprocal" : "it");
   if (c.w_stride >= (1u << 22))
     return fail(ARK_OPT_EINVAL, "w: stride %llu too large", (unsigned long long)c.w_stride);
   const uint32_t les = c.teacher ? ark::act_elem_size(c.logits_dtype) : 1;
