@@ -4,9 +4,10 @@
 // With live rows X (the tokens that have a loss, copied together), the output
 // layer W and sparse targets p, a piece of the tokens takes these steps:
 //
-//   gather_kernel   X, padded to whole steps of the products, and where its rows
-//                   come from; zeros for the tokens without a loss
-//   dots_kernel     z at the targets, in fp32: X_t . W_index
+//   rank_kernel     which tokens are live, and what follows from how many there are
+//   gather_kernel   X, padded to whole steps of the products, and z at its targets in
+//                   fp32 (X_t . W_target; a teacher's entries: dots_kernel); zeros
+//                   for the tokens without a loss
 //   logits_kernel   z = scale X W^T in tiles that stay in registers; of every row
 //                   and span of the vocabulary its largest z and its sum of
 //                   exp(z - largest), and with gradients the exponentials
@@ -35,13 +36,33 @@ using ark::fail;
 constexpr uint32_t kLanes = 256;
 constexpr uint32_t kRowPad = 256;   // rows of a piece are laid out for whole tiles
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr uint32_t kGatherRows = 32;  // tokens a block of gather_kernel takes
+constexpr uint32_t kMaxPiece = 16384;  // tokens: what rank_kernel's block ranks
+constexpr uint32_t kFew = 64;          // tokens that a wave ranks by itself
 
 // What a piece's kernels leave for each other.
 struct Meta {
-  uint32_t live;  // rows with a loss
-  float alpha;    // dz is dz * 1 / alpha
+  uint32_t live;                  // rows with a loss
+  uint32_t dx_splits, dw_splits;  // parts that the products' sums are cut into
+  float up, down;                 // dz is formed times up, a power of two, and taken down after
 };
+
+// How a product is cut, decided where the number of live rows is known: whole
+// tiles over `tiles` blocks, or each tile's sum in parts that join_kernel adds.
+struct Cut {
+  uint32_t tiles_m, bn;  // tiles across, rows of a tile
+  float step, part, row; // microseconds: a step of 32, a block, a part's row of partial sums
+  uint32_t most;         // parts of n tiles down: most * bn rows of partial sums fit
+  // What s parts of every tile take on 256 compute units.
+  __host__ __device__ float cost(uint32_t s, uint32_t tiles_n, uint32_t steps) const {
+    const uint32_t rounds = (tiles_m * tiles_n * s + 255) / 256;
+    return (float)rounds * ((float)((steps + s - 1) / s) * step + part) +
+           (s > 1 ? 4.0f + (float)(s * tiles_n * bn) * row : 0.0f);
+  }
+  __host__ __device__ bool may(uint32_t s, uint32_t tiles_n, uint32_t steps) const {
+    return s == 1 || (s * tiles_n <= most && s * 8 <= steps);
+  }
+};
+constexpr uint32_t kMaxSplits = 64;
 
 template <typename T>
 constexpr uint32_t kTypeOf = sizeof(T) == 4 ? ARK_HEAD_F32 : ARK_HEAD_F16;
@@ -58,7 +79,6 @@ __device__ __forceinline__ float wave_max(float v) {
   for (int o = 1; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
   return v;
 }
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 __device__ __forceinline__ int64_t ld_int(const void* p, uint32_t bytes, uint64_t i) {
   return bytes == 8 ? ld_g<int64_t>((const int64_t*)p + i) : ld_g<int32_t>((const int32_t*)p + i);
@@ -143,78 +163,189 @@ __global__ __launch_bounds__(kLanes) void teacher_kernel(
   if (lane == 0) self[t] = own, there[t] = live ? 1u : 0u;
 }
 
-struct GatherArgs {
+// The cheapest of 1 to 64 parts, a lane each.
+__device__ __forceinline__ uint32_t cut_parts(const Cut& c, uint32_t tiles_n, uint32_t steps) {
+  const uint32_t lane = threadIdx.x % 64;
+  float cost = c.may(lane + 1, tiles_n, steps) ? c.cost(lane + 1, tiles_n, steps) : INFINITY;
+  float best = cost;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) best = fminf(best, __shfl_xor(best, o));
+  return (uint32_t)__ffsll((unsigned long long)__ballot(cost == best));
+}
+
+struct RankArgs {
   Targets targets;
+  uint32_t tokens;
+  uint32_t* rank;      // [tokens]: a live token's row of X, ~0
+  uint32_t* rows;      // and back
+  Meta* meta;
+  const float* grads;  // or NULL: grad
+  float grad, scale;
+  uint32_t with_grad;
+  Cut dx, dw;
+  uint32_t vocab;
+};
+
+// By one wave, with the number of live tokens and the largest |grad| over them.
+__device__ __forceinline__ void write_meta(const RankArgs& a, uint32_t live, float largest) {
+  Meta m = {live, 1, 1, 1.0f, 1.0f};
+  if (a.with_grad) {
+    // the largest |grad * scale| times `up` lies in [2^13, 2^14)
+    largest *= fabsf(a.scale);
+    if (largest > 0.0f && largest < INFINITY) {
+      const int shift = min(max(13 - ilogbf(largest), -100), 100);
+      m.up = ldexpf(1.0f, shift), m.down = ldexpf(1.0f, -shift);
+    }
+    const uint32_t v = (a.vocab + kProductStep - 1) / kProductStep;
+    const uint32_t t = (live + kProductStep - 1) / kProductStep;
+    m.dx_splits = cut_parts(a.dx, (live + a.dx.bn - 1) / a.dx.bn, v);
+    m.dw_splits = cut_parts(a.dw, (a.vocab + a.dw.bn - 1) / a.dw.bn, t);
+  }
+  if (threadIdx.x % 64 == 0) *a.meta = m;
+}
+
+// |grad| as a whole number, so that a NaN is the largest.
+__device__ __forceinline__ uint32_t grad_size(const RankArgs& a, uint32_t t) {
+  return __float_as_uint(a.grads[t]) & 0x7FFFFFFFu;
+}
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t g) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) g = max(g, (uint32_t)__shfl_xor(g, o));
+  return g;
+}
+
+// The live tokens' order, by one block: 1024 tokens at a time side by side, their
+// numbers of live ones summed in the tokens' order.
+constexpr uint32_t kRankLanes = 1024, kRankWaves = kRankLanes / 64;
+constexpr uint32_t kRankEach = kMaxPiece / kRankLanes;
+__global__ __launch_bounds__(kRankLanes) void rank_kernel(RankArgs a) {
+  __shared__ uint32_t s_count[kRankEach * kRankWaves + 1], s_most[kRankWaves];
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  uint64_t mask[kRankEach];
+  uint32_t most = 0;
+#pragma unroll
+  for (uint32_t k = 0; k < kRankEach; ++k) {
+    const uint32_t t = k * kRankLanes + threadIdx.x;
+    const bool live = t < a.tokens && a.targets.live(min(t, a.tokens - 1));
+    mask[k] = __ballot(live);
+    if (live && a.grads) most = max(most, grad_size(a, t));
+  }
+  most = wave_max_bits(most);
+  if (lane == 0) {
+#pragma unroll
+    for (uint32_t k = 0; k < kRankEach; ++k) s_count[k * kRankWaves + wave] = __popcll(mask[k]);
+    s_most[wave] = most;
+  }
+  __syncthreads();
+  static_assert(kRankEach * kRankWaves == 256, "four counts a lane");
+  if (wave == 0) {
+    uint32_t c[4], sum = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) c[k] = s_count[4 * lane + k], sum += c[k];
+    uint32_t incl = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t y = __shfl_up(incl, o);
+      if (lane >= (uint32_t)o) incl += y;
+    }
+    uint32_t from = incl - sum;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) s_count[4 * lane + k] = from, from += c[k];
+    const float largest = a.grads ? __uint_as_float(wave_max_bits(s_most[lane % kRankWaves]))
+                                  : fabsf(a.grad);
+    write_meta(a, (uint32_t)__builtin_amdgcn_readlane(incl, 63), largest);
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t k = 0; k < kRankEach; ++k) {
+    const uint32_t t = k * kRankLanes + threadIdx.x;
+    if (t >= a.tokens) break;
+    const uint32_t row = s_count[k * kRankWaves + wave] + __popcll(mask[k] & ((1ull << lane) - 1));
+    const bool live = mask[k] >> lane & 1;
+    a.rank[t] = live ? row : ~0u;
+    if (live) a.rows[row] = t;
+  }
+}
+
+struct GatherArgs {
+  RankArgs rank;
   const uint16_t* x;
   uint64_t x_stride;
-  uint32_t tokens, columns, padded;  // padded: columns of out
-  uint32_t vec;                      // x takes 16-byte loads
+  uint32_t columns, padded;  // padded: columns of out
   uint16_t* out;
-  uint32_t* rows;
-  Meta* meta;
-  const float* grads;  // or NULL
-  float* largest;      // [blocks]: of |grads| over live tokens
   float* loss;
   uint16_t* dx;  // or NULL
   uint64_t dx_stride;
+  const uint16_t* w;
+  uint64_t w_stride;
+  float* z;
 };
 
-// The live tokens' rows, in order.  A block counts the live tokens before its own
-// (a token's target is 4 or 8 bytes, its row thousands).
+// Eight neighbouring 16-bit values at any element's alignment (gfx950 takes
+// unaligned global accesses), those past n as zeros.
+__device__ __forceinline__ u32x4 load8(const uint16_t* p, uint32_t n) {
+  typedef uint32_t V __attribute__((ext_vector_type(4), aligned(2)));
+  if (n >= 8) return *(const ARK_GLOBAL V*)p;
+  uint32_t v[8];
+#pragma unroll
+  for (uint32_t k = 0; k < 8; ++k) v[k] = k < n ? p[k] : 0u;
+  return u32x4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+}
+
+// A wave a token: its row of x, and with one target z there.  The waves past the
+// last token fill X up to a whole step of the products.  FEW: at most 64 tokens,
+// which every wave ranks for itself, without rank_kernel before.
+template <typename T, bool FEW>
 __global__ __launch_bounds__(kLanes) void gather_kernel(GatherArgs a) {
-  __shared__ uint32_t s_count[kLanes / 64], s_live;
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const uint32_t t0 = blockIdx.x * kGatherRows;
-  uint32_t before = 0;
-#pragma unroll 8
-  for (uint32_t t = threadIdx.x; t < t0; t += kLanes) before += a.targets.live(t) ? 1u : 0u;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) before += __shfl_xor(before, o);
-  if (lane == 0) s_count[wave] = before;
-  if (wave == 0) {
-    const uint32_t t = t0 + lane;
-    const bool live = lane < kGatherRows && t < a.tokens && a.targets.live(t);
-    const uint64_t mask = __ballot(live);
-    if (lane == 0) s_live = (uint32_t)mask;
-    if (a.grads) {
-      // as whole numbers, so that a NaN is the largest
-      uint32_t g = live ? __float_as_uint(a.grads[t]) & 0x7FFFFFFFu : 0u;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) g = max(g, (uint32_t)__shfl_xor(g, o));
-      if (lane == 0) a.largest[blockIdx.x] = __uint_as_float(g);
+  typedef T V __attribute__((ext_vector_type(8)));
+  const uint32_t lane = threadIdx.x % 64;
+  const uint32_t t = __builtin_amdgcn_readfirstlane(blockIdx.x * (kLanes / 64) + threadIdx.x / 64);
+  const RankArgs& r = a.rank;
+  uint32_t row, live;
+  if constexpr (FEW) {
+    const bool mine = lane < r.tokens && r.targets.live(min(lane, r.tokens - 1));
+    const uint64_t mask = __ballot(mine);
+    live = __popcll(mask);
+    row = t < r.tokens && (mask >> t & 1) ? __popcll(mask & ((1ull << t) - 1)) : ~0u;
+    if (t == 0) {
+      const uint32_t g = mine && r.grads ? grad_size(r, lane) : 0u;
+      write_meta(r, live, r.grads ? __uint_as_float(wave_max_bits(g)) : fabsf(r.grad));
+      if (mine) r.rows[__popcll(mask & ((1ull << lane) - 1))] = lane;
     }
+  } else {
+    row = t < r.tokens ? r.rank[t] : ~0u;
+    live = r.meta->live;
   }
-  __syncthreads();
-  uint32_t base = 0;
-#pragma unroll
-  for (uint32_t w = 0; w < kLanes / 64; ++w) base += s_count[w];
-  const uint32_t mask = s_live, n = base + __popc(mask);
-  for (uint32_t r = wave; r < kGatherRows && t0 + r < a.tokens; r += kLanes / 64) {
-    const uint32_t t = t0 + r;
-    if (!(mask >> r & 1u)) {
-      if (lane == 0) a.loss[t] = 0.0f;
-      if (a.dx)
-        for (uint32_t c = lane; c < a.columns; c += 64) a.dx[t * a.dx_stride + c] = 0;
-      continue;
-    }
-    const uint32_t to = base + __popc(mask & ((1u << r) - 1u));
-    if (lane == 0) a.rows[to] = t;
-    const uint16_t* src = a.x + t * a.x_stride;
-    uint16_t* dst = a.out + (uint64_t)to * a.padded;
-    if (a.vec) {
-      for (uint32_t c = lane * 8; c < a.columns; c += 512)
-        *(u32x4*)(dst + c) = ld_g<u32x4>(src + c);
-      for (uint32_t c = a.columns + lane; c < a.padded; c += 64) dst[c] = 0;
-    } else {
-      for (uint32_t c = lane; c < a.padded; c += 64) dst[c] = c < a.columns ? src[c] : 0;
-    }
-  }
-  if (blockIdx.x + 1 == gridDim.x) {
-    const uint32_t end = (n + kProductStep - 1) / kProductStep * kProductStep;
-    for (uint32_t r = n + wave; r < end; r += kLanes / 64)
+  if (t >= r.tokens) {
+    row = live + (t - r.tokens);
+    if (row < (live + kProductStep - 1) / kProductStep * kProductStep)
       for (uint32_t c = lane * 8; c < a.padded; c += 512)
-        *(u32x4*)(a.out + (uint64_t)r * a.padded + c) = u32x4{0, 0, 0, 0};
-    if (threadIdx.x == 0) a.meta->live = n;
+        *(u32x4*)(a.out + (uint64_t)row * a.padded + c) = u32x4{0, 0, 0, 0};
+    return;
+  }
+  if (row == ~0u) {
+    if (lane == 0) a.loss[t] = 0.0f;
+    if (a.dx)
+      for (uint32_t c = lane; c < a.columns; c += 64) a.dx[t * a.dx_stride + c] = 0;
+    return;
+  }
+  const uint16_t* src = a.x + t * a.x_stride;
+  uint16_t* dst = a.out + (uint64_t)row * a.padded;
+  const bool dot = r.targets.targets != nullptr;
+  const uint16_t* w = a.w + (dot ? r.targets.at(t, 0) : 0u) * a.w_stride;
+  float sum = 0.0f;
+  for (uint32_t c = lane * 8; c < a.padded; c += 512) {
+    const u32x4 v = load8(src + c, c < a.columns ? a.columns - c : 0u);
+    *(u32x4*)(dst + c) = v;
+    if (dot) {
+      const V x = __builtin_bit_cast(V, v), y = *(const V*)(w + c);
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) sum = __builtin_fmaf((float)x[i], (float)y[i], sum);
+    }
+  }
+  if (dot) {
+    sum = wave_sum(sum) * r.scale;
+    if (lane == 0) a.z[row] = sum;
   }
 }
 
@@ -229,15 +360,12 @@ __global__ __launch_bounds__(kLanes) void pad_kernel(const uint16_t* __restrict_
        i += (uint64_t)gridDim.x * kLanes) {
     const uint64_t row = i / per;
     const uint32_t c = (uint32_t)(i % per) * 8;
-    uint32_t v[8];
-#pragma unroll
-    for (uint32_t k = 0; k < 8; ++k) v[k] = c + k < columns ? w[row * stride + c + k] : 0u;
     *(u32x4*)(out + row * padded + c) =
-        u32x4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+        load8(w + row * stride + c, c < columns ? columns - c : 0u);
   }
 }
 
-// z at the targets: a wave takes up to four of a row's.
+// z at a teacher's entries: a wave takes up to four of a row's.
 constexpr uint32_t kDots = 4;
 template <typename T>
 __global__ __launch_bounds__(kLanes) void dots_kernel(Targets targets,
@@ -284,7 +412,8 @@ __global__ __launch_bounds__(kLanes) void dots_kernel(Targets targets,
 
 // The tile of a block: blocks of one XCD (every eighth) take neighbouring tiles,
 // and these go through eight tiles of rows for every tile of columns, so that the
-// operands of those that run together are few.
+// operands of those that run together are few.  Only tiles that have live rows
+// count (tiles left out in the middle would leave whole XCDs idle).
 struct Tiles {
   uint32_t m, n;
   __device__ __forceinline__ void find(uint32_t block, uint32_t blocks, uint32_t* tm,
@@ -305,7 +434,7 @@ struct LogitsArgs {
   uint32_t padded, vocab, spans;
   uint64_t e_stride;
   float scale;
-  Tiles tiles;
+  uint32_t tiles_m;
   const Meta* meta;
   float* stats;  // [row][span] of (largest, sum)
   uint16_t* e;   // [row][e_stride], or NULL
@@ -315,9 +444,11 @@ template <typename P>
 __global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {
   extern __shared__ __align__(1024) uint8_t lds[];
   uint32_t tm, tn, split;
-  a.tiles.find(blockIdx.x, gridDim.x, &tm, &tn, &split);
-  const uint32_t live = a.meta->live, m0 = tm * P::BM, n0 = tn * P::BN;
-  if (n0 >= live) return;
+  const uint32_t live = a.meta->live;
+  const Tiles tiles = {a.tiles_m, (live + P::BN - 1) / P::BN};
+  if (blockIdx.x >= tiles.m * tiles.n) return;
+  tiles.find(blockIdx.x, tiles.m * tiles.n, &tm, &tn, &split);
+  const uint32_t m0 = tm * P::BM, n0 = tn * P::BN;
   P p;
   const Operand ow = {a.w + m0 * a.w_stride, a.w_stride, a.vocab - m0, 0};
   const Operand ox = {a.x + (uint64_t)n0 * a.padded, a.padded, P::BN, 0};
@@ -449,10 +580,7 @@ __global__ __launch_bounds__(kLanes) void loss_kernel(LossArgs a) {
 
 struct DzArgs {
   LossArgs loss;
-  Meta* meta;
-  const float* grads;    // or NULL
-  const float* largest;  // [parts]
-  uint32_t parts;
+  const float* grads;  // or NULL
   float grad, scale;
   uint16_t* e;
   uint64_t e_stride;
@@ -470,19 +598,6 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
   __shared__ float s_p[ARK_HEAD_MAX_TOP];
   const LossArgs& l = a.loss;
   const uint32_t row = blockIdx.x, live = l.meta->live, tid = threadIdx.x;
-  // the largest |grad * scale| times 2^shift lies in [2^13, 2^14)
-  float largest = fabsf(a.grad);
-  if (a.grads) {
-    uint32_t m = 0;
-    for (uint32_t i = tid % 64; i < a.parts; i += 64) m = max(m, __float_as_uint(a.largest[i]));
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) m = max(m, (uint32_t)__shfl_xor(m, o));
-    largest = __uint_as_float(m);
-  }
-  largest *= fabsf(a.scale);
-  int shift = 0;
-  if (largest > 0.0f && largest < INFINITY) shift = min(max(14 - ilogbf(largest) - 1, -100), 100);
-  if (row == 0 && tid == 0) a.meta->alpha = ldexpf(1.0f, -shift);
   if (row >= (live + kProductStep - 1) / kProductStep * kProductStep) return;
   uint16_t* e = a.e + row * a.e_stride;
   if (row >= live) {
@@ -497,7 +612,7 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
     const float loss = row_loss(l.targets, t, z, lse, tid);
     if (tid == 0) l.loss[t] = loss;
   }
-  const float f = ldexpf((a.grads ? a.grads[t] : a.grad) * a.scale, shift);
+  const float f = (a.grads ? a.grads[t] : a.grad) * a.scale * l.meta->up;
   for (uint32_t k = tid; k < top; k += kLanes) {
     s_index[k] = l.targets.at(t, k);
     s_p[k] = l.targets.weight(t, k);
@@ -537,7 +652,7 @@ struct Out {
   const Meta* meta;
 
   __device__ __forceinline__ void put(uint32_t n, uint32_t m, f32x4 v) const {
-    v *= meta->alpha;
+    v *= meta->down;
     const uint64_t row = rows ? rows[n] : n;
     const uint32_t c = min(width - m, 4u);
     if (add) {
@@ -579,9 +694,8 @@ struct ProductArgs {
   uint32_t a_width;   // values of a row of a
   uint32_t b_width;   // dw: of a row of b
   uint32_t a_rows;    // dx: rows of W
-  Tiles tiles;
-  uint32_t splits;
-  float* partial;     // [split][height][width up to 4], or NULL
+  uint32_t tiles_m;
+  float* partial;     // [part][rows of tiles][width up to 4]
   const Meta* meta;
   Out out;
 };
@@ -590,41 +704,45 @@ template <typename P, bool DX>
 __global__ __launch_bounds__(P::kLanes, 2) void product_kernel(ProductArgs g) {
   extern __shared__ __align__(1024) uint8_t lds[];
   uint32_t tm, tn, split;
-  g.tiles.find(blockIdx.x, gridDim.x, &tm, &tn, &split);
-  const uint32_t live = g.meta->live, m0 = tm * P::BM, n0 = tn * P::BN;
-  if (DX && n0 >= live) return;
+  const uint32_t live = g.meta->live, height = DX ? live : g.out.height;
+  const uint32_t splits = DX ? g.meta->dx_splits : g.meta->dw_splits;
+  const Tiles tiles = {g.tiles_m, (height + P::BN - 1) / P::BN};
+  if (blockIdx.x >= tiles.m * tiles.n * splits) return;
+  tiles.find(blockIdx.x, tiles.m * tiles.n * splits, &tm, &tn, &split);
+  const uint32_t m0 = tm * P::BM, n0 = tn * P::BN;
   const uint32_t ks = DX ? g.a_rows : (live + kProductStep - 1) / kProductStep * kProductStep;
   const uint32_t steps = (ks + kProductStep - 1) / kProductStep;
-  const uint32_t s0 = (uint32_t)((uint64_t)steps * split / g.splits);
-  const uint32_t s1 = (uint32_t)((uint64_t)steps * (split + 1) / g.splits);
+  const uint32_t s0 = (uint32_t)((uint64_t)steps * split / splits);
+  const uint32_t s1 = (uint32_t)((uint64_t)steps * (split + 1) / splits);
   P p;
   const Operand oa = {g.a + m0, g.a_stride, g.a_width - m0, ks};
   const Operand ob = DX ? Operand{g.b + n0 * g.b_stride, g.b_stride, P::BN, 0}
                         : Operand{g.b + n0, g.b_stride, g.b_width - n0, ks};
   p.run(oa, ob, s0, s1, (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds);
-  const uint32_t height = DX ? min(live, g.out.height) : g.out.height;
   const uint64_t w4 = (g.out.width + 3) / 4 * 4;
+  float* partial = g.partial + (uint64_t)split * height * w4;
   p.each([&](uint32_t m, uint32_t n, f32x4 v) __attribute__((always_inline)) {
     m += m0, n += n0;
     if (m >= g.out.width || n >= height) return;
-    if (g.partial)
-      *(f32x4*)(g.partial + ((uint64_t)split * g.out.height + n) * w4 + m) = v;
+    if (splits > 1)
+      *(f32x4*)(partial + n * w4 + m) = v;
     else
       g.out.put(n, m, v);
   });
 }
 
-// The splits' partial products, added in order.
-__global__ __launch_bounds__(kLanes) void join_kernel(const float* __restrict__ partial,
-                                                      uint32_t splits, uint32_t live_rows, Out out) {
-  const uint32_t per = (out.width + 3) / 4;
-  const uint32_t height = live_rows ? min(out.meta->live, out.height) : out.height;
-  const uint64_t all = (uint64_t)height * per, step = (uint64_t)out.height * per;
+// The parts of a product, added in order.
+template <bool DX>
+__global__ __launch_bounds__(kLanes) void join_kernel(const float* __restrict__ partial, Out out) {
+  const uint32_t splits = DX ? out.meta->dx_splits : out.meta->dw_splits;
+  if (splits == 1) return;
+  const uint32_t per = (out.width + 3) / 4, height = DX ? out.meta->live : out.height;
+  const uint64_t all = (uint64_t)height * per;
   for (uint64_t i = (uint64_t)blockIdx.x * kLanes + threadIdx.x; i < all;
        i += (uint64_t)gridDim.x * kLanes) {
     const f32x4* p = (const f32x4*)partial + i;
     f32x4 v = p[0];
-    for (uint32_t s = 1; s < splits; ++s) v += p[s * step];
+    for (uint32_t s = 1; s < splits; ++s) v += p[s * all];
     out.put((uint32_t)(i / per), (uint32_t)(i % per) * 4, v);
   }
 }
@@ -636,13 +754,15 @@ constexpr uint64_t kDzBytes = 1ull << 30;  // of a piece's dz, at most
 struct Big {
   template <typename T, bool AMC, bool BMC>
   using P = Product<T, AMC, BMC, 8, 4, 2, 4, 4>;
+  template <typename T>
+  using L = P<T, false, false>;
 };
 struct Small {
   template <typename T, bool AMC, bool BMC>
   using P = Product<T, AMC, BMC, 4, 2, 2, 2, 4>;
+  template <typename T>
+  using L = P<T, false, false>;
 };
-
-constexpr uint32_t kMaxSplits = 32;
 
 // How a call is cut, and where things lie in its workspace (offsets of 256).
 struct Plan {
@@ -653,16 +773,28 @@ struct Plan {
   bool copy_w;
   uint32_t bm, bn, span, spans;
   uint64_t e_stride;
-  uint32_t dx_splits, dw_splits;
-  uint64_t meta, rows, largest, index, p, self, there, z, x, w, stats, e, partial, dw, bytes;
+  Cut dx, dw;
+  uint64_t meta, rank, rows, index, p, self, there, z, x, w, stats, e, partial, sums, bytes;
 };
 
 uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
-uint32_t splits_of(uint64_t tiles, uint64_t steps) {
-  uint64_t s = 1;
-  while (s < kMaxSplits && tiles * s < 256 && steps >= s * 8) s *= 2;
-  return (uint32_t)s;
+// The rows of partial sums that a product's parts may take: as many as it asks for
+// with every token live, and at least what keeps every compute unit busy twice.
+Cut cut_of(uint32_t tiles_m, uint32_t bn, uint64_t width, uint64_t height, uint32_t steps,
+           bool small) {
+  // measured on MI355X: a step's share of a full unit, and what a block takes
+  // besides; partial sums out and back at 5 TB/s
+  Cut c = {tiles_m, bn, small ? 0.11f : 0.87f, small ? 2.0f : 5.0f,
+           (float)up(width, 4) * 8.0f / 5e6f, ~0u};
+  const uint32_t n = (uint32_t)((height + bn - 1) / bn);
+  uint32_t best = 1;
+  for (uint32_t s = 2; s <= kMaxSplits; ++s)
+    if (c.may(s, n, steps) && c.cost(s, n, steps) < c.cost(best, n, steps)) best = s;
+  c.most = best * n;
+  const uint32_t twice = (512 + tiles_m - 1) / tiles_m;
+  if (best > 1 && c.most < twice) c.most = twice;
+  return c;
 }
 
 Plan plan_of(const void* w, uint64_t w_stride, uint64_t tokens, uint64_t columns, uint64_t vocab,
@@ -676,9 +808,9 @@ Plan plan_of(const void* w, uint64_t w_stride, uint64_t tokens, uint64_t columns
   p.padded = (uint32_t)up(columns, kProductStep);
   p.copy_w = columns % kProductStep || w_stride % 8 || (uintptr_t)w % 16;
   // pieces of equal sizes, whole tiles
-  uint64_t most = grad ? kDzBytes / (p.e_stride * 2) / kRowPad * kRowPad : 16384;
+  uint64_t most = grad ? kDzBytes / (p.e_stride * 2) / kRowPad * kRowPad : kMaxPiece;
   if (most < kRowPad) most = kRowPad;
-  if (most > 16384) most = 16384;
+  if (most > kMaxPiece) most = kMaxPiece;
   p.pieces = (uint32_t)((tokens + most - 1) / most);
   if (p.pieces == 0) p.pieces = 1;
   p.piece = (uint32_t)(p.pieces == 1 ? tokens : up((tokens + p.pieces - 1) / p.pieces, kRowPad));
@@ -690,8 +822,8 @@ Plan plan_of(const void* w, uint64_t w_stride, uint64_t tokens, uint64_t columns
     return here;
   };
   p.meta = take(sizeof(Meta));
+  p.rank = take(rows * 4);
   p.rows = take(rows * 4);
-  p.largest = take((rows / kGatherRows) * 4);
   p.index = take(rows * top * 4);
   p.p = take(rows * top * 4);
   p.self = take(rows * 4);
@@ -702,13 +834,13 @@ Plan plan_of(const void* w, uint64_t w_stride, uint64_t tokens, uint64_t columns
   p.stats = take(rows * p.spans * 8);
   if (grad) {
     p.e = take(rows * p.e_stride * 2);
-    const uint64_t mt = (columns + p.bm - 1) / p.bm, w4 = up(columns, 4);
-    p.dx_splits = splits_of(mt * ((p.piece + p.bn - 1) / p.bn), (vocab + 63) / 64);
-    p.dw_splits = splits_of(mt * ((vocab + p.bn - 1) / p.bn), rows / 64);
-    const uint64_t a = p.dx_splits > 1 ? p.dx_splits * p.piece * w4 * 4 : 0;
-    const uint64_t b = p.dw_splits > 1 ? p.dw_splits * vocab * w4 * 4 : 0;
+    const uint32_t mt = (uint32_t)((columns + p.bm - 1) / p.bm);
+    p.dx = cut_of(mt, p.bn, columns, p.piece ? p.piece : 1, (uint32_t)((vocab + 31) / 32), p.small);
+    p.dw = cut_of(mt, p.bn, columns, vocab, (uint32_t)(rows / 32), p.small);
+    const uint64_t w4 = up(columns, 4) * 4 * p.bn, none = up(vocab, p.bn) / p.bn;
+    const uint64_t a = p.dx.most * w4, b = p.dw.most > none ? p.dw.most * w4 : 0;
     p.partial = take(a > b ? a : b);
-    p.dw = take(dw_dtype != ARK_HEAD_F32 && p.pieces > 1 ? vocab * columns * 4 : 0);
+    p.sums = take(dw_dtype != ARK_HEAD_F32 && p.pieces > 1 ? vocab * columns * 4 : 0);
   }
   p.bytes = at;
   return p;
@@ -760,26 +892,26 @@ int with_lds(K kernel, uint32_t bytes, std::atomic<uint64_t>* ready) {
 }
 
 template <typename P>
-int launch_logits(const LogitsArgs& a, hipStream_t s) {
+int launch_logits(const LogitsArgs& a, uint32_t blocks, hipStream_t s) {
   static std::atomic<uint64_t> ready{0};
   if (int rc = with_lds(logits_kernel<P>, P::kLds, &ready)) return rc;
-  hipLaunchKernelGGL(logits_kernel<P>, dim3(a.tiles.m * a.tiles.n), dim3(P::kLanes), P::kLds, s, a);
+  hipLaunchKernelGGL(logits_kernel<P>, dim3(blocks), dim3(P::kLanes), P::kLds, s, a);
   ARK_HIP(hipGetLastError());
   return ARK_OPT_OK;
 }
 
 template <typename P, bool DX>
-int launch_product(const ProductArgs& g, hipStream_t s) {
+int launch_product(const ProductArgs& g, const Cut& cut, uint32_t height, hipStream_t s) {
   static std::atomic<uint64_t> ready{0};
   if (int rc = with_lds(product_kernel<P, DX>, P::kLds, &ready)) return rc;
-  hipLaunchKernelGGL((product_kernel<P, DX>), dim3(g.tiles.m * g.tiles.n * g.splits),
-                     dim3(P::kLanes), P::kLds, s, g);
+  const uint32_t n = (height + P::BN - 1) / P::BN;  // blocks without a part leave at once
+  const uint32_t blocks = g.tiles_m * (cut.most > n ? cut.most : n);
+  hipLaunchKernelGGL((product_kernel<P, DX>), dim3(blocks), dim3(P::kLanes), P::kLds, s, g);
   ARK_HIP(hipGetLastError());
-  if (g.splits > 1) {
-    const uint64_t n = (uint64_t)g.out.height * ((g.out.width + 3) / 4);
-    const uint64_t blocks = (n + kLanes - 1) / kLanes;
-    hipLaunchKernelGGL(join_kernel, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(kLanes),
-                       0, s, (const float*)g.partial, g.splits, DX ? 1u : 0u, g.out);
+  if (DX ? cut.most > 1 : cut.most >= 2 * n) {
+    const uint64_t each = ((uint64_t)height * ((g.out.width + 3) / 4) + kLanes - 1) / kLanes;
+    hipLaunchKernelGGL(join_kernel<DX>, dim3((uint32_t)(each < 65536 ? each : 65536)), dim3(kLanes),
+                       0, s, (const float*)g.partial, g.out);
     ARK_HIP(hipGetLastError());
   }
   return ARK_OPT_OK;
@@ -819,30 +951,42 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
     g.bytes = c.target_bytes;
     g.ignore = c.ignore;
   }
-  // one block of these runs also without a token, for dw's zeros
-  const uint32_t gather_blocks = tokens ? (tokens + kGatherRows - 1) / kGatherRows : 1;
+  const uint16_t* w = p.copy_w ? (const uint16_t*)(ws + p.w) : (const uint16_t*)c.w;
+  const uint64_t w_stride = p.copy_w ? p.padded : c.w_stride;
   GatherArgs ga = {};
-  ga.targets = g;
+  RankArgs& ra = ga.rank;
+  ra.targets = g;
+  ra.tokens = tokens;
+  ra.rank = (uint32_t*)(ws + p.rank), ra.rows = rows;
+  ra.meta = meta;
+  ra.grads = c.grads ? c.grads + t0 : nullptr;
+  ra.grad = c.grad, ra.scale = c.scale;
+  ra.with_grad = c.with_grad;
+  ra.dx = p.dx, ra.dw = p.dw;
+  ra.vocab = (uint32_t)c.vocab;
   ga.x = (const uint16_t*)c.x + t0 * c.x_stride;
   ga.x_stride = c.x_stride;
-  ga.tokens = tokens;
   ga.columns = (uint32_t)c.columns;
   ga.padded = p.padded;
-  ga.vec = c.x_stride % 8 == 0 && (uintptr_t)c.x % 16 == 0 && c.columns % 8 == 0;
   ga.out = x;
-  ga.rows = rows;
-  ga.meta = meta;
-  ga.grads = c.grads ? c.grads + t0 : nullptr;
-  ga.largest = (float*)(ws + p.largest);
   ga.loss = c.loss + t0;
   ga.dx = c.dx ? (uint16_t*)c.dx + t0 * c.dx_stride : nullptr;
   ga.dx_stride = c.dx_stride;
-  hipLaunchKernelGGL(gather_kernel, dim3(gather_blocks), dim3(kLanes), 0, s, ga);
-  ARK_HIP(hipGetLastError());
-  const uint16_t* w = p.copy_w ? (const uint16_t*)(ws + p.w) : (const uint16_t*)c.w;
-  const uint64_t w_stride = p.copy_w ? p.padded : c.w_stride;
-  const uint64_t waves = (uint64_t)tokens * ((top + kDots - 1) / kDots);
+  ga.w = w, ga.w_stride = w_stride, ga.z = z;
+  if (!tokens || tokens > kFew) {  // without tokens for what dw's zeros need
+    hipLaunchKernelGGL(rank_kernel, dim3(1), dim3(kRankLanes), 0, s, ra);
+    ARK_HIP(hipGetLastError());
+  }
   if (tokens) {
+    const dim3 grid((tokens + kProductStep - 1 + 3) / 4);
+    if (tokens <= kFew)
+      hipLaunchKernelGGL((gather_kernel<T, true>), grid, dim3(kLanes), 0, s, ga);
+    else
+      hipLaunchKernelGGL((gather_kernel<T, false>), grid, dim3(kLanes), 0, s, ga);
+    ARK_HIP(hipGetLastError());
+  }
+  if (tokens && c.teacher) {
+    const uint64_t waves = (uint64_t)tokens * ((top + kDots - 1) / kDots);
     hipLaunchKernelGGL(dots_kernel<T>, dim3((uint32_t)((waves + 3) / 4)), dim3(kLanes), 0, s, g,
                        (const uint16_t*)x, p.padded, w, w_stride, (const uint32_t*)rows,
                        (const Meta*)meta, c.scale, z);
@@ -853,12 +997,13 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
   la.padded = p.padded, la.vocab = (uint32_t)c.vocab, la.spans = p.spans;
   la.e_stride = p.e_stride;
   la.scale = c.scale;
-  la.tiles = {(uint32_t)((c.vocab + p.bm - 1) / p.bm), (tokens + p.bn - 1) / p.bn};
+  typedef typename Size::template L<T> L;
+  la.tiles_m = (uint32_t)((c.vocab + L::BM - 1) / L::BM);
   la.meta = meta;
   la.stats = (float*)(ws + p.stats);
   la.e = c.with_grad ? (uint16_t*)(ws + p.e) : nullptr;
   int rc;
-  if (tokens && (rc = launch_logits<typename Size::template P<T, false, false>>(la, s))) return rc;
+  if (tokens && (rc = launch_logits<L>(la, la.tiles_m * ((tokens + L::BN - 1) / L::BN), s))) return rc;
   LossArgs lo = {g, rows, meta, la.stats, p.spans, z, ga.loss};
   if (!c.with_grad) {  // with tokens, or run() ends before
     hipLaunchKernelGGL(loss_kernel, dim3((tokens + 3) / 4), dim3(kLanes), 0, s, lo);
@@ -866,38 +1011,36 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
     return ARK_OPT_OK;
   }
   DzArgs da = {};
-  da.loss = lo, da.meta = meta, da.grads = ga.grads, da.largest = ga.largest;
-  da.parts = gather_blocks;
+  da.loss = lo, da.grads = ra.grads;
   da.grad = c.grad, da.scale = c.scale;
   da.e = la.e, da.e_stride = p.e_stride, da.span = p.span;
-  hipLaunchKernelGGL(dz_kernel<T>, dim3(tokens ? (uint32_t)up(tokens, kProductStep) : 1u), dim3(kLanes),
-                     0, s, da);
-  ARK_HIP(hipGetLastError());
+  if (tokens) {
+    hipLaunchKernelGGL(dz_kernel<T>, dim3((uint32_t)up(tokens, kProductStep)), dim3(kLanes), 0, s,
+                       da);
+    ARK_HIP(hipGetLastError());
+  }
   ProductArgs pa = {};
   pa.b = la.e, pa.b_stride = p.e_stride, pa.b_width = (uint32_t)p.e_stride;
-  pa.partial = nullptr;
+  pa.partial = (float*)(ws + p.partial);
   pa.meta = meta;
   Out& o = pa.out;
   o.meta = meta;
   o.width = (uint32_t)c.columns;
   if (c.dx && tokens) {
     pa.a = w, pa.a_stride = w_stride, pa.a_width = p.padded, pa.a_rows = (uint32_t)c.vocab;
-    pa.tiles = {(uint32_t)((c.columns + p.bm - 1) / p.bm), (tokens + p.bn - 1) / p.bn};
-    pa.splits = p.dx_splits;
-    pa.partial = pa.splits > 1 ? (float*)(ws + p.partial) : nullptr;
+    pa.tiles_m = p.dx.tiles_m;
     o.p = ga.dx, o.stride = c.dx_stride, o.dtype = c.dtype, o.rows = rows, o.height = tokens;
     o.vec = c.dx_stride % 4 == 0 && (uintptr_t)c.dx % 8 == 0;
-    if ((rc = launch_product<typename Size::template P<T, true, false>, true>(pa, s))) return rc;
+    if ((rc = launch_product<typename Size::template P<T, true, false>, true>(pa, p.dx, tokens, s)))
+      return rc;
   }
   if (c.dw) {
     pa.a = x, pa.a_stride = p.padded, pa.a_width = p.padded, pa.a_rows = 0;
-    pa.tiles = {(uint32_t)((c.columns + p.bm - 1) / p.bm), (uint32_t)((c.vocab + p.bn - 1) / p.bn)};
-    pa.splits = p.dw_splits;
-    pa.partial = pa.splits > 1 ? (float*)(ws + p.partial) : nullptr;
+    pa.tiles_m = p.dw.tiles_m;
     o.rows = nullptr, o.height = (uint32_t)c.vocab;
     // fp32 sums over the pieces, in dw itself or beside it
     const bool last = piece + 1 == p.pieces, wide = c.dw_dtype == ARK_HEAD_F32;
-    float* sums = wide ? (float*)c.dw : (float*)(ws + p.dw);
+    float* sums = wide ? (float*)c.dw : (float*)(ws + p.sums);
     const uint64_t sums_stride = wide ? c.dw_stride : c.columns;
     const bool add = piece > 0 || (c.flags & ARK_HEAD_ACCUMULATE);
     o.add = add ? sums : nullptr, o.add_stride = sums_stride;
@@ -906,7 +1049,8 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
     o.stride = final ? c.dw_stride : sums_stride;
     o.dtype = final ? c.dw_dtype : ARK_HEAD_F32;
     o.vec = o.stride % 4 == 0 && (uintptr_t)o.p % 16 == 0;
-    if ((rc = launch_product<typename Size::template P<T, true, true>, false>(pa, s))) return rc;
+    if ((rc = launch_product<typename Size::template P<T, true, true>, false>(pa, p.dw, o.height, s)))
+      return rc;
   }
   return ARK_OPT_OK;
 }
