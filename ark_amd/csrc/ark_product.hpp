@@ -96,9 +96,9 @@ struct Staged {
   }
   // The k of `step`, into LDS at byte `to`.  The load writes LDS at m0
   // plus 16 bytes a lane; nothing returns to registers, and meet() waits for it by
-  // count.  (The wait states are those between a vector instruction that writes an
-  // address's scalar register and a load that reads it, which the compiler does not
-  // see inside the block; one would do between m0 and the load.)
+  // count.  (One wait state between m0 and a load; the first load's others are those
+  // between a vector instruction that writes an address's scalar registers and a load
+  // that reads them, which the compiler does not see inside the block.)
   __device__ __forceinline__ void load(const Operand& o, uint32_t step, uint32_t to) {
     const uint16_t* p = o.at + (uint64_t)step * kProductStep * (MC ? o.stride : 1);
     if constexpr (MC) {
@@ -109,9 +109,14 @@ struct Staged {
 #pragma unroll
     for (uint32_t i = 0; i < kLoads; ++i) {
       const uint32_t at = to + (i * LANES + wave * 64) * 16;
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
-                   :
-                   : "s"(at), "v"(off[i]), "s"(p));
+      if (i == 0)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :
+                     : "s"(at), "v"(off[i]), "s"(p));
+      else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :
+                     : "s"(at), "v"(off[i]), "s"(p));
     }
   }
 };
@@ -218,13 +223,15 @@ struct Product {
         meet<(BUFS - 3) * kLoads>();
       else
         meet<0>();
-      if (s + BUFS - 1 < s1) load(s + BUFS - 1, to), to = next(to);
-      read_b(std::integral_constant<uint32_t, p ^ 1>());
 #pragma unroll
       for (uint32_t i = 0; i < MF; ++i) {
 #pragma unroll
         for (uint32_t j = 0; j < NF; ++j) acc[i][j] = Frag<T>::mul(fa[i], fb[p][j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+        // between the products, so that they start right behind the barrier
+        if (i == 0) read_b(std::integral_constant<uint32_t, p ^ 1>());
         fa[i] = ra.get(from, i);
+        if (i == 1 && s + BUFS - 1 < s1) load(s + BUFS - 1, to), to = next(to);
         __builtin_amdgcn_sched_barrier(0);
       }
       from = next(from);
@@ -244,6 +251,8 @@ struct Product {
     } else {
       first(S0());
     }
+    // nothing on its way from LDS that the compiler would wait for in the loop
+    __builtin_amdgcn_s_waitcnt(0xC07F);
     while (s < s1) {
       step(S0());
       step(S1());
