@@ -514,7 +514,7 @@ __global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {
     for (uint32_t i = 0; i < kRow / 64; ++i) {
       const uint32_t q = i * 64 + lane, r = q / kChunks, c = q % kChunks;
       const u32x4 v = *(const u32x4*)(mine + r * kRow + (c ^ (r % kChunks)) * 16);
-      if (t0 + r < live) st_g<u32x4>(a.e + (t0 + r) * a.e_stride + w0 + c * 8, v);
+      if (t0 + r < live) st_nt<u32x4>(a.e + (t0 + r) * a.e_stride + w0 + c * 8, v);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
@@ -619,7 +619,7 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
   }
   for (uint32_t c = tid * 8; c < a.e_stride; c += kLanes * 8) {
     const float s = expf(stats[c / a.span * 2] - lse) * f;
-    const V v = *(const V*)(e + c);
+    const V v = ld_nt<V>(e + c);
     u32x4 o;
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i)
