@@ -160,6 +160,9 @@ HEAD_BF16 = 1
 HEAD_F32 = 2
 HEAD_MAX_TOP = 256
 HEAD_ACCUMULATE = 1
+HEAD_DX = 1
+HEAD_DW = 2
+HEAD_GRAD = 4
 
 
 # include/ark_embed.h

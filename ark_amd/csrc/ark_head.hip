@@ -14,7 +14,8 @@
 //                   themselves, in 16 bits: 2^-9 or 2^-12 of each
 //   loss_kernel     the spans' sums joined: log(sum exp z), the loss
 //   dz_kernel       the same, and the exponentials turned into dz where they lie
-//   product_kernel  dx = dz W and dw = dz^T X
+//   grad_kernel     dx = dz W and dw = dz^T X, in one launch
+//   join_kernel     sums that were formed in parts
 //
 // The sums over spans make one pass over the vocabulary do: a span's exponentials
 // are relative to its own largest logit, as a row's is not known yet, and take the
@@ -42,27 +43,67 @@ constexpr uint32_t kFew = 64;          // tokens that a wave ranks by itself
 // What a piece's kernels leave for each other.
 struct Meta {
   uint32_t live;                  // rows with a loss
-  uint32_t dx_splits, dw_splits;  // parts that the products' sums are cut into
+  uint32_t dx_parts, dw_parts;    // that the products' sums are cut into
+  uint32_t dw_first;              // dw's blocks are the longer ones
   float up, down;                 // dz is formed times up, a power of two, and taken down after
 };
 
-// How a product is cut, decided where the number of live rows is known: whole
-// tiles over `tiles` blocks, or each tile's sum in parts that join_kernel adds.
+// How both products' work is cut, decided where the number of live rows is known:
+// a tile's sum whole, or in parts that join_kernel adds.  Blocks of both are in one
+// launch, the longer ones first, so that the shorter ones fill what those leave.
 struct Cut {
-  uint32_t tiles_m, bn;  // tiles across, rows of a tile
-  float step, part, row; // microseconds: a step of 32, a block, a part's row of partial sums
-  uint32_t most;         // parts of n tiles down: most * bn rows of partial sums fit
-  // What s parts of every tile take on 256 compute units.
-  __host__ __device__ float cost(uint32_t s, uint32_t tiles_n, uint32_t steps) const {
-    const uint32_t rounds = (tiles_m * tiles_n * s + 255) / 256;
-    return (float)rounds * ((float)((steps + s - 1) / s) * step + part) +
-           (s > 1 ? 4.0f + (float)(s * tiles_n * bn) * row : 0.0f);
+  uint32_t tiles_m, bn, units;       // tiles across, rows of a tile, blocks that run at once
+  float step, part, row;             // microseconds: a step of 32 k, a block besides, a row of
+                                     // partial sums out and back
+  uint32_t vocab, has_dx, has_dw;
+  uint32_t dx_most, dw_most;         // parts times tiles down that have room
+
+  struct Parts {
+    uint32_t dx, dw;
+  };
+  // Candidate i of 64.
+  static __host__ __device__ Parts candidate(uint32_t i) {
+    const uint64_t dx = 0x18100C0804030201ull, dw = 0x4020100804030201ull;
+    return {(uint32_t)(dx >> (i % 8 * 8)) & 255u, (uint32_t)(dw >> (i / 8 * 8)) & 255u};
   }
-  __host__ __device__ bool may(uint32_t s, uint32_t tiles_n, uint32_t steps) const {
-    return s == 1 || (s * tiles_n <= most && s * 8 <= steps);
+  __host__ __device__ uint32_t tiles_of(uint32_t rows) const { return (rows + bn - 1) / bn; }
+  static __host__ __device__ uint32_t steps_of(uint32_t k) {
+    return (k + kProductStep - 1) / kProductStep;
+  }
+  __host__ __device__ float length(uint32_t k, uint32_t parts) const {
+    return (float)((steps_of(k) + parts - 1) / parts) * step + part;
+  }
+  // When the last of n1 blocks of length l1 and then n2 of l2 <= l1 ends.
+  __host__ __device__ float end(uint32_t n1, float l1, uint32_t n2, float l2) const {
+    const uint32_t q = n1 / units, r = n1 % units, left = units - r;
+    const float a = (float)q * l1, b = r ? a + l1 : a;
+    if (!n2) return b;
+    // those that start at a end turns after it, or the others turns after b
+    const uint32_t later = (uint32_t)ceilf(l1 / l2), sooner = (uint32_t)(l1 / l2);
+    uint32_t k = (n2 + left - 1) / left;
+    if (r && k > later) k = (n2 + r * later + units - 1) / units;
+    float t = a + (float)k * l2;
+    if (r) {
+      const uint32_t m = n2 > left * sooner ? (n2 - left * sooner + units - 1) / units : 0;
+      t = fmaxf(fminf(t, b + (float)m * l2), b);
+    }
+    return t;
+  }
+  __host__ __device__ float cost(Parts p, uint32_t live) const {
+    const uint32_t n = has_dx ? tiles_m * tiles_of(live) * p.dx : 0;
+    const uint32_t m = has_dw ? tiles_m * tiles_of(vocab) * p.dw : 0;
+    const float ln = length(vocab, p.dx), lm = length(live, p.dw);
+    float t = ln >= lm ? end(n, ln, m, lm) : end(m, lm, n, ln);
+    if (has_dx && p.dx > 1) t += 3.0f + (float)(p.dx * live) * row;
+    if (has_dw && p.dw > 1) t += 3.0f + (float)p.dw * (float)vocab * row;
+    return t;
+  }
+  // A part has four steps at least.
+  __host__ __device__ bool may(Parts p, uint32_t live) const {
+    return (p.dx == 1 || (p.dx * 4 <= steps_of(vocab) && p.dx * tiles_of(live) <= dx_most)) &&
+           (p.dw == 1 || (p.dw * 4 <= steps_of(live) && p.dw * tiles_of(vocab) <= dw_most));
   }
 };
-constexpr uint32_t kMaxSplits = 64;
 
 template <typename T>
 constexpr uint32_t kTypeOf = sizeof(T) == 4 ? ARK_HEAD_F32 : ARK_HEAD_F16;
@@ -163,16 +204,6 @@ __global__ __launch_bounds__(kLanes) void teacher_kernel(
   if (lane == 0) self[t] = own, there[t] = live ? 1u : 0u;
 }
 
-// The cheapest of 1 to 64 parts, a lane each.
-__device__ __forceinline__ uint32_t cut_parts(const Cut& c, uint32_t tiles_n, uint32_t steps) {
-  const uint32_t lane = threadIdx.x % 64;
-  float cost = c.may(lane + 1, tiles_n, steps) ? c.cost(lane + 1, tiles_n, steps) : INFINITY;
-  float best = cost;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) best = fminf(best, __shfl_xor(best, o));
-  return (uint32_t)__ffsll((unsigned long long)__ballot(cost == best));
-}
-
 struct RankArgs {
   Targets targets;
   uint32_t tokens;
@@ -182,13 +213,12 @@ struct RankArgs {
   const float* grads;  // or NULL: grad
   float grad, scale;
   uint32_t with_grad;
-  Cut dx, dw;
-  uint32_t vocab;
+  Cut cut;
 };
 
 // By one wave, with the number of live tokens and the largest |grad| over them.
 __device__ __forceinline__ void write_meta(const RankArgs& a, uint32_t live, float largest) {
-  Meta m = {live, 1, 1, 1.0f, 1.0f};
+  Meta m = {live, 1, 1, 0, 1.0f, 1.0f};
   if (a.with_grad) {
     // the largest |grad * scale| times `up` lies in [2^13, 2^14)
     largest *= fabsf(a.scale);
@@ -196,10 +226,16 @@ __device__ __forceinline__ void write_meta(const RankArgs& a, uint32_t live, flo
       const int shift = min(max(13 - ilogbf(largest), -100), 100);
       m.up = ldexpf(1.0f, shift), m.down = ldexpf(1.0f, -shift);
     }
-    const uint32_t v = (a.vocab + kProductStep - 1) / kProductStep;
-    const uint32_t t = (live + kProductStep - 1) / kProductStep;
-    m.dx_splits = cut_parts(a.dx, (live + a.dx.bn - 1) / a.dx.bn, v);
-    m.dw_splits = cut_parts(a.dw, (a.vocab + a.dw.bn - 1) / a.dw.bn, t);
+    // the cheapest of the 64 candidates, a lane each
+    const Cut::Parts mine = Cut::candidate(threadIdx.x % 64);
+    const float cost = a.cut.may(mine, live) ? a.cut.cost(mine, live) : INFINITY;
+    float best = cost;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) best = fminf(best, __shfl_xor(best, o));
+    const Cut::Parts p =
+        Cut::candidate((uint32_t)__ffsll((unsigned long long)__ballot(cost == best)) - 1u);
+    m.dx_parts = p.dx, m.dw_parts = p.dw;
+    m.dw_first = a.cut.length(live, p.dw) > a.cut.length(a.cut.vocab, p.dx) ? 1 : 0;
   }
   if (threadIdx.x % 64 == 0) *a.meta = m;
 }
@@ -694,57 +730,82 @@ struct ProductArgs {
   uint32_t a_width;   // values of a row of a
   uint32_t b_width;   // dw: of a row of b
   uint32_t a_rows;    // dx: rows of W
+  float* partial;     // [part][rows][width up to 4]
+  Out out;            // p NULL: not formed
+};
+struct GradArgs {
+  ProductArgs dx, dw;
   uint32_t tiles_m;
-  float* partial;     // [part][rows of tiles][width up to 4]
   const Meta* meta;
-  Out out;
 };
 
+// One block of dx or dw: `block` of the blocks of its kind.
 template <typename P, bool DX>
-__global__ __launch_bounds__(P::kLanes, 2) void product_kernel(ProductArgs g) {
-  extern __shared__ __align__(1024) uint8_t lds[];
-  uint32_t tm, tn, split;
-  const uint32_t live = g.meta->live, height = DX ? live : g.out.height;
-  const uint32_t splits = DX ? g.meta->dx_splits : g.meta->dw_splits;
-  const Tiles tiles = {g.tiles_m, (height + P::BN - 1) / P::BN};
-  if (blockIdx.x >= tiles.m * tiles.n * splits) return;
-  tiles.find(blockIdx.x, tiles.m * tiles.n * splits, &tm, &tn, &split);
+__device__ __forceinline__ void product_block(const ProductArgs& g, const Meta& meta,
+                                              const Tiles& tiles, uint32_t block, uint8_t* lds) {
+  const uint32_t parts = DX ? meta.dx_parts : meta.dw_parts;
+  const uint32_t height = DX ? meta.live : g.out.height;
+  uint32_t tm, tn, part;
+  tiles.find(block, tiles.m * tiles.n * parts, &tm, &tn, &part);
   const uint32_t m0 = tm * P::BM, n0 = tn * P::BN;
-  const uint32_t ks = DX ? g.a_rows : (live + kProductStep - 1) / kProductStep * kProductStep;
+  const uint32_t ks = DX ? g.a_rows : (meta.live + kProductStep - 1) / kProductStep * kProductStep;
   const uint32_t steps = (ks + kProductStep - 1) / kProductStep;
-  const uint32_t s0 = (uint32_t)((uint64_t)steps * split / splits);
-  const uint32_t s1 = (uint32_t)((uint64_t)steps * (split + 1) / splits);
+  const uint32_t s0 = (uint32_t)((uint64_t)steps * part / parts);
+  const uint32_t s1 = (uint32_t)((uint64_t)steps * (part + 1) / parts);
   P p;
   const Operand oa = {g.a + m0, g.a_stride, g.a_width - m0, ks};
   const Operand ob = DX ? Operand{g.b + n0 * g.b_stride, g.b_stride, P::BN, 0}
                         : Operand{g.b + n0, g.b_stride, g.b_width - n0, ks};
   p.run(oa, ob, s0, s1, (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds);
   const uint64_t w4 = (g.out.width + 3) / 4 * 4;
-  float* partial = g.partial + (uint64_t)split * height * w4;
+  float* partial = g.partial + (uint64_t)part * height * w4;
   p.each([&](uint32_t m, uint32_t n, f32x4 v) __attribute__((always_inline)) {
     m += m0, n += n0;
     if (m >= g.out.width || n >= height) return;
-    if (splits > 1)
+    if (parts > 1)
       *(f32x4*)(partial + n * w4 + m) = v;
     else
       g.out.put(n, m, v);
   });
 }
 
-// The parts of a product, added in order.
-template <bool DX>
-__global__ __launch_bounds__(kLanes) void join_kernel(const float* __restrict__ partial, Out out) {
-  const uint32_t splits = DX ? out.meta->dx_splits : out.meta->dw_splits;
-  if (splits == 1) return;
-  const uint32_t per = (out.width + 3) / 4, height = DX ? out.meta->live : out.height;
+template <typename X, typename W>
+__global__ __launch_bounds__(X::kLanes, 2) void grad_kernel(GradArgs g) {
+  extern __shared__ __align__(1024) uint8_t lds[];
+  const Meta meta = *g.meta;
+  const Tiles x = {g.tiles_m, g.dx.out.p ? (meta.live + X::BN - 1) / X::BN : 0u};
+  const Tiles w = {g.tiles_m, g.dw.out.p ? (g.dw.out.height + W::BN - 1) / W::BN : 0u};
+  const uint32_t nx = x.m * x.n * meta.dx_parts, nw = w.m * w.n * meta.dw_parts;
+  // the second kind starts at a multiple of the XCDs
+  const uint32_t first = meta.dw_first ? nw : nx, up = (first + 7) / 8 * 8;
+  const bool second = blockIdx.x >= up;
+  const uint32_t block = second ? blockIdx.x - up : blockIdx.x;
+  if ((meta.dw_first != 0) != second) {
+    if (block < nw) product_block<W, false>(g.dw, meta, w, block, lds);
+  } else {
+    if (block < nx) product_block<X, true>(g.dx, meta, x, block, lds);
+  }
+}
+
+// The parts of both products, added in order.
+__device__ __forceinline__ void join(const float* partial, uint32_t parts, uint32_t height,
+                                     const Out& out, uint64_t i, uint64_t step) {
+  const uint32_t per = (out.width + 3) / 4;
   const uint64_t all = (uint64_t)height * per;
-  for (uint64_t i = (uint64_t)blockIdx.x * kLanes + threadIdx.x; i < all;
-       i += (uint64_t)gridDim.x * kLanes) {
+  for (; i < all; i += step) {
     const f32x4* p = (const f32x4*)partial + i;
     f32x4 v = p[0];
-    for (uint32_t s = 1; s < splits; ++s) v += p[s * all];
+    for (uint32_t s = 1; s < parts; ++s) v += p[s * all];
     out.put((uint32_t)(i / per), (uint32_t)(i % per) * 4, v);
   }
+}
+__global__ __launch_bounds__(kLanes) void join_kernel(GradArgs g) {
+  const Meta meta = *g.meta;
+  const uint64_t i = (uint64_t)blockIdx.x * kLanes + threadIdx.x, step = (uint64_t)gridDim.x * kLanes;
+  if (g.dx.out.p && meta.dx_parts > 1)
+    join(g.dx.partial, meta.dx_parts, meta.live, g.dx.out, i, step);
+  if (g.dw.out.p && meta.dw_parts > 1)
+    join(g.dw.partial, meta.dw_parts, g.dw.out.height, g.dw.out, i, step);
 }
 
 // ---- host -------------------------------------------------------------------
@@ -773,32 +834,43 @@ struct Plan {
   bool copy_w;
   uint32_t bm, bn, span, spans;
   uint64_t e_stride;
-  Cut dx, dw;
-  uint64_t meta, rank, rows, index, p, self, there, z, x, w, stats, e, partial, sums, bytes;
+  Cut cut;
+  uint64_t meta, rank, rows, index, p, self, there, z, x, w, stats, e, dx_parts, dw_parts, sums, bytes;
 };
 
 uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
-// The rows of partial sums that a product's parts may take: as many as it asks for
-// with every token live, and at least what keeps every compute unit busy twice.
-Cut cut_of(uint32_t tiles_m, uint32_t bn, uint64_t width, uint64_t height, uint32_t steps,
-           bool small) {
-  // measured on MI355X: a step's share of a full unit, and what a block takes
-  // besides; partial sums out and back at 5 TB/s
-  Cut c = {tiles_m, bn, small ? 0.11f : 0.87f, small ? 2.0f : 5.0f,
-           (float)up(width, 4) * 8.0f / 5e6f, ~0u};
-  const uint32_t n = (uint32_t)((height + bn - 1) / bn);
-  uint32_t best = 1;
-  for (uint32_t s = 2; s <= kMaxSplits; ++s)
-    if (c.may(s, n, steps) && c.cost(s, n, steps) < c.cost(best, n, steps)) best = s;
-  c.most = best * n;
-  const uint32_t twice = (512 + tiles_m - 1) / tiles_m;
-  if (best > 1 && c.most < twice) c.most = twice;
+// The cut of a piece of `rows` tokens, with room for the parts that it asks for with
+// every token live, and for some more of dx's when few are.
+Cut cut_of(bool small, uint32_t columns, uint32_t rows, uint32_t vocab, bool has_dx, bool has_dw) {
+  Cut c = {};
+  // measured on MI355X: a large tile has a unit to itself, of small ones three share it;
+  // partial sums go out and come back at 5 TB/s
+  c.tiles_m = small ? (columns + 127) / 128 : (columns + 255) / 256;
+  c.bn = small ? 64 : 256;
+  c.units = small ? 768 : 256;
+  c.step = small ? 0.33f : 0.85f;
+  c.part = small ? 3.0f : 6.0f;
+  c.row = (float)up(columns, 4) * 8.0f / 5e6f;
+  c.vocab = vocab, c.has_dx = has_dx, c.has_dw = has_dw;
+  c.dx_most = c.dw_most = ~0u;
+  Cut::Parts best = Cut::candidate(0);
+  float cost = c.cost(best, rows);
+  for (uint32_t i = 1; i < 64; ++i) {
+    const Cut::Parts p = Cut::candidate(i);
+    if (!c.may(p, rows)) continue;
+    const float t = c.cost(p, rows);
+    if (t < cost) best = p, cost = t;
+  }
+  const uint32_t n = c.tiles_of(rows), some = (512 + c.tiles_m - 1) / c.tiles_m;
+  c.dx_most = best.dx * n;
+  if (c.dx_most < some) c.dx_most = some < 24 * n ? some : 24 * n;
+  c.dw_most = best.dw * c.tiles_of(vocab);
   return c;
 }
 
 Plan plan_of(const void* w, uint64_t w_stride, uint64_t tokens, uint64_t columns, uint64_t vocab,
-             uint64_t top, uint32_t dw_dtype, bool grad) {
+             uint64_t top, uint32_t dw_dtype, bool grad, bool has_dx, bool has_dw) {
   Plan p = {};
   p.small = tokens <= 64;
   p.bm = p.small ? 128 : 256, p.bn = p.small ? 64 : 256;
@@ -834,12 +906,12 @@ Plan plan_of(const void* w, uint64_t w_stride, uint64_t tokens, uint64_t columns
   p.stats = take(rows * p.spans * 8);
   if (grad) {
     p.e = take(rows * p.e_stride * 2);
-    const uint32_t mt = (uint32_t)((columns + p.bm - 1) / p.bm);
-    p.dx = cut_of(mt, p.bn, columns, p.piece ? p.piece : 1, (uint32_t)((vocab + 31) / 32), p.small);
-    p.dw = cut_of(mt, p.bn, columns, vocab, (uint32_t)(rows / 32), p.small);
-    const uint64_t w4 = up(columns, 4) * 4 * p.bn, none = up(vocab, p.bn) / p.bn;
-    const uint64_t a = p.dx.most * w4, b = p.dw.most > none ? p.dw.most * w4 : 0;
-    p.partial = take(a > b ? a : b);
+    p.cut = cut_of(p.small, (uint32_t)columns, (uint32_t)(p.piece ? p.piece : 1), (uint32_t)vocab,
+                   has_dx, has_dw);
+    const uint64_t tile = up(columns, 4) * 4 * p.bn;
+    p.dx_parts = take(has_dx ? p.cut.dx_most * tile : 0);
+    p.dw_parts = take(has_dw && p.cut.dw_most > p.cut.tiles_of((uint32_t)vocab)
+                          ? p.cut.dw_most * tile : 0);
     p.sums = take(dw_dtype != ARK_HEAD_F32 && p.pieces > 1 ? vocab * columns * 4 : 0);
   }
   p.bytes = at;
@@ -900,18 +972,20 @@ int launch_logits(const LogitsArgs& a, uint32_t blocks, hipStream_t s) {
   return ARK_OPT_OK;
 }
 
-template <typename P, bool DX>
-int launch_product(const ProductArgs& g, const Cut& cut, uint32_t height, hipStream_t s) {
+template <typename X, typename W>
+int launch_grad(const GradArgs& g, const Cut& cut, uint32_t rows, hipStream_t s) {
   static std::atomic<uint64_t> ready{0};
-  if (int rc = with_lds(product_kernel<P, DX>, P::kLds, &ready)) return rc;
-  const uint32_t n = (height + P::BN - 1) / P::BN;  // blocks without a part leave at once
-  const uint32_t blocks = g.tiles_m * (cut.most > n ? cut.most : n);
-  hipLaunchKernelGGL((product_kernel<P, DX>), dim3(blocks), dim3(P::kLanes), P::kLds, s, g);
+  static_assert(X::kLanes == W::kLanes && X::kLds == W::kLds && X::BN == W::BN, "one launch");
+  if (int rc = with_lds(grad_kernel<X, W>, X::kLds, &ready)) return rc;
+  // as many blocks as any number of live rows may ask for; the others leave at once
+  uint32_t nx = 0, nw = 0;
+  if (g.dx.out.p) nx = cut.dx_most > cut.tiles_of(rows) ? cut.dx_most : cut.tiles_of(rows);
+  if (g.dw.out.p) nw = cut.dw_most;
+  const uint32_t blocks = (uint32_t)(up(g.tiles_m * nx, 8) + up(g.tiles_m * nw, 8));
+  hipLaunchKernelGGL((grad_kernel<X, W>), dim3(blocks), dim3(X::kLanes), X::kLds, s, g);
   ARK_HIP(hipGetLastError());
-  if (DX ? cut.most > 1 : cut.most >= 2 * n) {
-    const uint64_t each = ((uint64_t)height * ((g.out.width + 3) / 4) + kLanes - 1) / kLanes;
-    hipLaunchKernelGGL(join_kernel<DX>, dim3((uint32_t)(each < 65536 ? each : 65536)), dim3(kLanes),
-                       0, s, (const float*)g.partial, g.out);
+  if ((g.dx.out.p && cut.dx_most > 1) || (g.dw.out.p && nw > cut.tiles_of(cut.vocab))) {
+    hipLaunchKernelGGL(join_kernel, dim3(2048), dim3(kLanes), 0, s, g);
     ARK_HIP(hipGetLastError());
   }
   return ARK_OPT_OK;
@@ -962,8 +1036,7 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
   ra.grads = c.grads ? c.grads + t0 : nullptr;
   ra.grad = c.grad, ra.scale = c.scale;
   ra.with_grad = c.with_grad;
-  ra.dx = p.dx, ra.dw = p.dw;
-  ra.vocab = (uint32_t)c.vocab;
+  ra.cut = p.cut;
   ga.x = (const uint16_t*)c.x + t0 * c.x_stride;
   ga.x_stride = c.x_stride;
   ga.columns = (uint32_t)c.columns;
@@ -1019,25 +1092,28 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
                        da);
     ARK_HIP(hipGetLastError());
   }
-  ProductArgs pa = {};
-  pa.b = la.e, pa.b_stride = p.e_stride, pa.b_width = (uint32_t)p.e_stride;
-  pa.partial = (float*)(ws + p.partial);
-  pa.meta = meta;
-  Out& o = pa.out;
-  o.meta = meta;
-  o.width = (uint32_t)c.columns;
+  if (!c.dx && !c.dw) return ARK_OPT_OK;
+  GradArgs gr = {};
+  gr.tiles_m = p.cut.tiles_m;
+  gr.meta = meta;
+  for (ProductArgs* g : {&gr.dx, &gr.dw}) {
+    g->b = la.e, g->b_stride = p.e_stride, g->b_width = (uint32_t)p.e_stride;
+    g->a_width = p.padded;
+    g->out.meta = meta;
+    g->out.width = (uint32_t)c.columns;
+  }
   if (c.dx && tokens) {
-    pa.a = w, pa.a_stride = w_stride, pa.a_width = p.padded, pa.a_rows = (uint32_t)c.vocab;
-    pa.tiles_m = p.dx.tiles_m;
+    Out& o = gr.dx.out;
+    gr.dx.a = w, gr.dx.a_stride = w_stride, gr.dx.a_rows = (uint32_t)c.vocab;
+    gr.dx.partial = (float*)(ws + p.dx_parts);
     o.p = ga.dx, o.stride = c.dx_stride, o.dtype = c.dtype, o.rows = rows, o.height = tokens;
     o.vec = c.dx_stride % 4 == 0 && (uintptr_t)c.dx % 8 == 0;
-    if ((rc = launch_product<typename Size::template P<T, true, false>, true>(pa, p.dx, tokens, s)))
-      return rc;
   }
   if (c.dw) {
-    pa.a = x, pa.a_stride = p.padded, pa.a_width = p.padded, pa.a_rows = 0;
-    pa.tiles_m = p.dw.tiles_m;
-    o.rows = nullptr, o.height = (uint32_t)c.vocab;
+    Out& o = gr.dw.out;
+    gr.dw.a = x, gr.dw.a_stride = p.padded;
+    gr.dw.partial = (float*)(ws + p.dw_parts);
+    o.height = (uint32_t)c.vocab;
     // fp32 sums over the pieces, in dw itself or beside it
     const bool last = piece + 1 == p.pieces, wide = c.dw_dtype == ARK_HEAD_F32;
     float* sums = wide ? (float*)c.dw : (float*)(ws + p.sums);
@@ -1049,10 +1125,9 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
     o.stride = final ? c.dw_stride : sums_stride;
     o.dtype = final ? c.dw_dtype : ARK_HEAD_F32;
     o.vec = o.stride % 4 == 0 && (uintptr_t)o.p % 16 == 0;
-    if ((rc = launch_product<typename Size::template P<T, true, true>, false>(pa, p.dw, o.height, s)))
-      return rc;
   }
-  return ARK_OPT_OK;
+  return launch_grad<typename Size::template P<T, true, false>,
+                     typename Size::template P<T, true, true>>(gr, p.cut, tokens, s);
 }
 
 template <typename T>
@@ -1146,7 +1221,7 @@ int run(Call c) {
       (uintptr_t)c.loss % 4 || (uintptr_t)c.grads % 4)
     return fail(ARK_OPT_EINVAL, "an array is not aligned to its elements");
   const Plan p = plan_of(c.w, c.w_stride, c.tokens, c.columns, c.vocab, c.top,
-                         c.dw ? c.dw_dtype : ARK_HEAD_F32, c.with_grad);
+                         c.dw ? c.dw_dtype : ARK_HEAD_F32, c.with_grad, c.dx, c.dw);
   if (c.tokens == 0 && (!c.dw || (c.flags & ARK_HEAD_ACCUMULATE))) return ARK_OPT_OK;
   if (c.ws_bytes < p.bytes)
     return fail(ARK_OPT_EINVAL, "workspace of %llu B, %llu B needed",
@@ -1192,8 +1267,11 @@ int ark_head_workspace(const void* w, uint64_t w_stride, uint64_t tokens, uint64
                        uint64_t* bytes) {
   if (!bytes) return fail(ARK_OPT_EINVAL, "bytes is NULL");
   *bytes = 0;
+  if (grad & ~(ARK_HEAD_GRAD | ARK_HEAD_DX | ARK_HEAD_DW))
+    return fail(ARK_OPT_EINVAL, "grad %#x unknown", grad);
   if (int rc = check_sizes(tokens, columns, vocab, top, dw_dtype)) return rc;
-  *bytes = plan_of(w, w_stride, tokens, columns, vocab, top, dw_dtype, grad != 0).bytes;
+  *bytes = plan_of(w, w_stride, tokens, columns, vocab, top, dw_dtype, grad != 0,
+                   grad & ARK_HEAD_DX, grad & ARK_HEAD_DW).bytes;
   return ARK_OPT_OK;
 }
 

@@ -112,7 +112,9 @@ def _loss_grad(x, w, call, top, args, grad, dx, dw, accumulate):
     xp, xs = (None, 0) if dx is False else _rows(dx, "dx")
     wp, wstride = (None, 0) if dw is False else _rows(dw, "dw")
     code = _abi.HEAD_F32 if dw is False else _code(dw, "dw")
-    need = _workspace(head[2] % 16 == 0, *head[3:4], *head[5:8], top, code, 1)
+    need = _workspace(head[2] % 16 == 0, *head[3:4], *head[5:8], top, code,
+                      _abi.HEAD_GRAD | (0 if dx is False else _abi.HEAD_DX)
+                      | (0 if dw is False else _abi.HEAD_DW))
     loss = x.new_empty(x.shape[0], dtype=torch.float32)
     # torch's allocator hands a stream's memory back to it without waiting
     ws = x.new_empty(need, dtype=torch.uint8)

@@ -378,6 +378,9 @@ pub const ARK_HEAD_BF16: u32 = 1;
 pub const ARK_HEAD_F32: u32 = 2;
 pub const ARK_HEAD_MAX_TOP: u64 = 256;
 pub const ARK_HEAD_ACCUMULATE: u32 = 1;
+pub const ARK_HEAD_DX: u32 = 1;
+pub const ARK_HEAD_DW: u32 = 2;
+pub const ARK_HEAD_GRAD: u32 = 4;
 
 extern "C" {
     pub fn ark_head_workspace(w: *const c_void, w_stride: u64, tokens: u64, columns: u64,

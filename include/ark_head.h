@@ -65,8 +65,14 @@ extern "C" {
 /* Flags. */
 #define ARK_HEAD_ACCUMULATE 1u /* add to dw (fp32) instead of overwriting it */
 
+/* What a call forms besides the loss, for its workspace. */
+#define ARK_HEAD_DX 1u
+#define ARK_HEAD_DW 2u
+#define ARK_HEAD_GRAD 4u
+
 /* Bytes of workspace of a call: top is 1 for cross entropy; grad is 0 for the
- * loss alone, 1 with gradients.  The address and stride of w count, as the
+ * loss alone, otherwise ARK_HEAD_GRAD, with ARK_HEAD_DX and ARK_HEAD_DW for the
+ * gradients that are formed.  The address and stride of w count, as the
  * products read w itself where rows of 16-byte pieces allow it and a copy
  * otherwise. */
 int ark_head_workspace(const void *w, uint64_t w_stride, uint64_t tokens, uint64_t columns,

@@ -14,7 +14,7 @@ def _msg():
     return _lib.lib().ark_opt_last_error().decode()
 
 
-def _need(tokens=64, columns=64, vocab=100, top=1, dw=F32, grad=1, w=GB, stride=64):
+def _need(tokens=64, columns=64, vocab=100, top=1, dw=F32, grad=7, w=GB, stride=64):
     out = C.c_uint64(7)
     rc = _lib.lib().ark_head_workspace(w, stride, tokens, columns, vocab, top, dw, grad,
                                        C.byref(out))
@@ -27,7 +27,8 @@ def test_workspace_of_the_loss():
     few, many = _need(16384, 64, 32000)[1], _need(1 << 20, 64, 32000)[1]
     assert many < 1.1 * few < 1.3 * 2 ** 30
     assert _need(1 << 20, 64, 1 << 21)[1] < 3 * 2 ** 30
-    assert _need(grad=0)[1] < _need()[1]
+    assert _need(grad=0)[1] < _need(grad=4)[1] < _need(grad=5)[1] <= _need()[1]
+    assert _need(grad=8) == (_abi.EINVAL, 0)
     # a copy of w where its rows are not whole 16-byte pieces
     assert _need(stride=66)[1] >= _need()[1] + 100 * 64 * 2
     assert _need(w=GB + 2)[1] == _need(stride=66)[1]
