@@ -756,10 +756,11 @@ __device__ __forceinline__ void product_block(const ProductArgs& g, const Meta& 
   const Operand oa = {g.a + m0, g.a_stride, g.a_width - m0, ks};
   const Operand ob = DX ? Operand{g.b + n0 * g.b_stride, g.b_stride, P::BN, 0}
                         : Operand{g.b + n0, g.b_stride, g.b_width - n0, ks};
-  p.run(oa, ob, s0, s1, (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds);
+  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  p.run(oa, ob, s0, s1, at);
   const uint64_t w4 = (g.out.width + 3) / 4 * 4;
   float* partial = g.partial + (uint64_t)part * height * w4;
-  p.each([&](uint32_t m, uint32_t n, f32x4 v) __attribute__((always_inline)) {
+  p.each(at, [&](uint32_t m, uint32_t n, f32x4 v) __attribute__((always_inline)) {
     m += m0, n += n0;
     if (m >= g.out.width || n >= height) return;
     if (parts > 1)

@@ -259,16 +259,33 @@ struct Product {
     }
   }
 
-  // f(m, n, v): four outputs at m .. m + 3 of row n, both from the tile's start,
-  // for every fragment of the lane.
+  // f(m, n, v): four outputs at m .. m + 3 of row n, both from the tile's start.  They
+  // pass through LDS (the block's own again, after a barrier), sixteen rows of a wave
+  // at a time, so that neighbouring lanes have neighbouring m: a row's come as whole
+  // lines of memory (1.3B gradients 3.50 ms, 3.58 straight from the sums' lanes).
   template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const uint32_t m0 = wave % WM * 16 * MF + lane / 16 * 4, n0 = wave / WM * 16 * NF + lane % 16;
+  __device__ __forceinline__ void each(uint32_t lds, F f) const {
+    constexpr uint32_t kRowBytes = MF * 64, kChunks = kRowBytes / 16, kMask = kChunks < 16 ? kChunks - 1 : 15;
+    static_assert(16 * kRowBytes * WM * WN <= kLds, "a part of LDS for each wave");
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, row = lane % 16;
+    const uint32_t mine = lds + wave * 16 * kRowBytes;
+    const uint32_t m0 = wave % WM * 16 * MF, n0 = wave / WM * 16 * NF;
+    __syncthreads();
 #pragma unroll
-    for (uint32_t j = 0; j < NF; ++j)
+    for (uint32_t j = 0; j < NF; ++j) {
 #pragma unroll
-      for (uint32_t i = 0; i < MF; ++i) f(m0 + 16 * i, n0 + 16 * j, acc[i][j]);
+      for (uint32_t i = 0; i < MF; ++i)
+        ARK_LDS_AT(f32x4, mine + row * kRowBytes + ((i * 4 + lane / 16) ^ (row & kMask)) * 16) =
+            acc[i][j];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (uint32_t i = 0; i < kRowBytes / 64; ++i) {
+        const uint32_t q = i * 64 + lane, r = q / kChunks, c = q % kChunks;
+        f(m0 + c * 4, n0 + j * 16 + r,
+          ARK_LDS_AT(f32x4, mine + r * kRowBytes + (c ^ (r & kMask)) * 16));
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
   }
 };
 
