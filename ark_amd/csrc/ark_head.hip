@@ -5,6 +5,7 @@
 // layer W and sparse targets p, a piece of the tokens takes these steps:
 //
 //   rank_kernel     which tokens are live, and what follows from how many there are
+//                   (for few tokens gather_kernel's)
 //   gather_kernel   X, padded to whole steps of the products, and z at its targets in
 //                   fp32 (X_t . W_target; a teacher's entries: dots_kernel); zeros
 //                   for the tokens without a loss
@@ -38,7 +39,7 @@ constexpr uint32_t kLanes = 256;
 constexpr uint32_t kRowPad = 256;   // rows of a piece are laid out for whole tiles
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr uint32_t kMaxPiece = 16384;  // tokens: what rank_kernel's block ranks
-constexpr uint32_t kFew = 64;          // tokens that a wave ranks by itself
+constexpr uint32_t kFew = 1024;        // tokens that gather_kernel's blocks rank themselves
 
 // What a piece's kernels leave for each other.
 struct Meta {
@@ -142,10 +143,34 @@ struct Targets {
   const uint32_t* there;  // [tokens]
   uint32_t top, vocab;
 
-  __device__ __forceinline__ bool live(uint32_t t) const {
-    if (!targets) return ld_g<uint32_t>(there + t) != 0;
-    const int64_t y = ld_int(targets, bytes, t);
+  __device__ __forceinline__ bool is_target(int64_t y) const {
     return y != ignore && y >= 0 && y < (int64_t)vocab;
+  }
+  // Which of tokens t, t + step, ... (N of them, below n) have a loss; their loads all
+  // together.
+  template <uint32_t N>
+  __device__ __forceinline__ void live(uint32_t t, uint32_t step, uint32_t n, bool (&out)[N]) const {
+    if (!targets) {
+      uint32_t v[N];
+#pragma unroll
+      for (uint32_t k = 0; k < N; ++k) v[k] = t + k * step < n ? ld_g<uint32_t>(there + t + k * step) : 0u;
+#pragma unroll
+      for (uint32_t k = 0; k < N; ++k) out[k] = v[k] != 0;
+    } else if (bytes == 8) {
+      int64_t v[N];
+#pragma unroll
+      for (uint32_t k = 0; k < N; ++k)
+        v[k] = t + k * step < n ? ld_g<int64_t>((const int64_t*)targets + t + k * step) : -1;
+#pragma unroll
+      for (uint32_t k = 0; k < N; ++k) out[k] = is_target(v[k]);
+    } else {
+      int32_t v[N];
+#pragma unroll
+      for (uint32_t k = 0; k < N; ++k)
+        v[k] = t + k * step < n ? ld_g<int32_t>((const int32_t*)targets + t + k * step) : -1;
+#pragma unroll
+      for (uint32_t k = 0; k < N; ++k) out[k] = is_target(v[k]);
+    }
   }
   __device__ __forceinline__ uint32_t at(uint32_t t, uint32_t k) const {
     return targets ? (uint32_t)ld_int(targets, bytes, t) : ld_g<uint32_t>(index + (uint64_t)t * top + k);
@@ -259,12 +284,17 @@ __global__ __launch_bounds__(kRankLanes) void rank_kernel(RankArgs a) {
   const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   uint64_t mask[kRankEach];
   uint32_t most = 0;
+  bool live[kRankEach];
+  a.targets.live<kRankEach>(threadIdx.x, kRankLanes, a.tokens, live);
 #pragma unroll
-  for (uint32_t k = 0; k < kRankEach; ++k) {
-    const uint32_t t = k * kRankLanes + threadIdx.x;
-    const bool live = t < a.tokens && a.targets.live(min(t, a.tokens - 1));
-    mask[k] = __ballot(live);
-    if (live && a.grads) most = max(most, grad_size(a, t));
+  for (uint32_t k = 0; k < kRankEach; ++k) mask[k] = __ballot(live[k]);
+  if (a.grads) {
+#pragma unroll
+    for (uint32_t k = 0; k < kRankEach; ++k) {
+      const uint32_t t = k * kRankLanes + threadIdx.x;
+      const uint32_t g = t < a.tokens ? grad_size(a, t) : 0u;
+      most = max(most, live[k] ? g : 0u);
+    }
   }
   most = wave_max_bits(most);
   if (lane == 0) {
@@ -274,6 +304,7 @@ __global__ __launch_bounds__(kRankLanes) void rank_kernel(RankArgs a) {
   }
   __syncthreads();
   static_assert(kRankEach * kRankWaves == 256, "four counts a lane");
+  uint32_t live_all = 0;
   if (wave == 0) {
     uint32_t c[4], sum = 0;
 #pragma unroll
@@ -287,9 +318,7 @@ __global__ __launch_bounds__(kRankLanes) void rank_kernel(RankArgs a) {
     uint32_t from = incl - sum;
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) s_count[4 * lane + k] = from, from += c[k];
-    const float largest = a.grads ? __uint_as_float(wave_max_bits(s_most[lane % kRankWaves]))
-                                  : fabsf(a.grad);
-    write_meta(a, (uint32_t)__builtin_amdgcn_readlane(incl, 63), largest);
+    live_all = (uint32_t)__builtin_amdgcn_readlane(incl, 63);
   }
   __syncthreads();
 #pragma unroll
@@ -297,10 +326,12 @@ __global__ __launch_bounds__(kRankLanes) void rank_kernel(RankArgs a) {
     const uint32_t t = k * kRankLanes + threadIdx.x;
     if (t >= a.tokens) break;
     const uint32_t row = s_count[k * kRankWaves + wave] + __popcll(mask[k] & ((1ull << lane) - 1));
-    const bool live = mask[k] >> lane & 1;
-    a.rank[t] = live ? row : ~0u;
-    if (live) a.rows[row] = t;
+    a.rank[t] = live[k] ? row : ~0u;
+    if (live[k]) a.rows[row] = t;
   }
+  if (wave == 0)
+    write_meta(a, live_all, a.grads ? __uint_as_float(wave_max_bits(s_most[lane % kRankWaves]))
+                                    : fabsf(a.grad));
 }
 
 struct GatherArgs {
@@ -312,9 +343,11 @@ struct GatherArgs {
   float* loss;
   uint16_t* dx;  // or NULL
   uint64_t dx_stride;
-  const uint16_t* w;
+  const uint16_t* w;  // as given
   uint64_t w_stride;
   float* z;
+  uint16_t* w_out;    // w padded, or NULL
+  uint32_t blocks;    // those after them pad w
 };
 
 // Eight neighbouring 16-bit values at any element's alignment (gfx950 takes
@@ -328,26 +361,74 @@ __device__ __forceinline__ u32x4 load8(const uint16_t* p, uint32_t n) {
   return u32x4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
 }
 
+// W's rows padded to whole steps, where its own cannot be read 16 bytes at a time.
+__device__ __forceinline__ void pad_rows(const GatherArgs& a) {
+  const uint32_t per = a.padded / 8;
+  const uint64_t all = (uint64_t)a.rank.targets.vocab * per;
+  const uint64_t step = (uint64_t)(gridDim.x - a.blocks) * kLanes;
+  for (uint64_t i = (uint64_t)(blockIdx.x - a.blocks) * kLanes + threadIdx.x; i < all; i += step) {
+    const uint64_t row = i / per;
+    const uint32_t c = (uint32_t)(i % per) * 8;
+    *(u32x4*)(a.w_out + row * a.padded + c) =
+        load8(a.w + row * a.w_stride + c, c < a.columns ? a.columns - c : 0u);
+  }
+}
+
 // A wave a token: its row of x, and with one target z there.  The waves past the
-// last token fill X up to a whole step of the products.  FEW: at most 64 tokens,
-// which every wave ranks for itself, without rank_kernel before.
+// last token fill X up to a whole step of the products, the blocks past those pad W.
+// FEW: at most 1024 tokens, which every block ranks for itself, without rank_kernel
+// before (4096 that way: 19 us, with rank_kernel 16).
 template <typename T, bool FEW>
 __global__ __launch_bounds__(kLanes) void gather_kernel(GatherArgs a) {
   typedef T V __attribute__((ext_vector_type(8)));
-  const uint32_t lane = threadIdx.x % 64;
-  const uint32_t t = __builtin_amdgcn_readfirstlane(blockIdx.x * (kLanes / 64) + threadIdx.x / 64);
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  if (blockIdx.x >= a.blocks) {
+    pad_rows(a);
+    return;
+  }
+  const uint32_t t = __builtin_amdgcn_readfirstlane(blockIdx.x * (kLanes / 64) + wave);
   const RankArgs& r = a.rank;
-  uint32_t row, live;
+  uint32_t row = ~0u, live = 0;
   if constexpr (FEW) {
-    const bool mine = lane < r.tokens && r.targets.live(min(lane, r.tokens - 1));
-    const uint64_t mask = __ballot(mine);
-    live = __popcll(mask);
-    row = t < r.tokens && (mask >> t & 1) ? __popcll(mask & ((1ull << t) - 1)) : ~0u;
-    if (t == 0) {
-      const uint32_t g = mine && r.grads ? grad_size(r, lane) : 0u;
-      write_meta(r, live, r.grads ? __uint_as_float(wave_max_bits(g)) : fabsf(r.grad));
-      if (mine) r.rows[__popcll(mask & ((1ull << lane) - 1))] = lane;
+    constexpr uint32_t kEach = kFew / kLanes, kMasks = kFew / 64;
+    __shared__ uint64_t s_mask[kMasks];
+    __shared__ uint32_t s_most[kLanes / 64];
+    bool mine[kEach];
+    r.targets.live<kEach>(threadIdx.x, kLanes, r.tokens, mine);
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+      const uint64_t m = __ballot(mine[k]);
+      if (lane == 0) s_mask[k * (kLanes / 64) + wave] = m;
     }
+    if (blockIdx.x == 0 && r.grads) {
+      uint32_t most = 0;
+#pragma unroll
+      for (uint32_t k = 0; k < kEach; ++k)
+        if (mine[k]) most = max(most, grad_size(r, k * kLanes + threadIdx.x));
+      most = wave_max_bits(most);
+      if (lane == 0) s_most[wave] = most;
+    }
+    __syncthreads();
+    // the live tokens before each 64, a lane each
+    const uint64_t m = s_mask[lane % kMasks];
+    const uint32_t count = lane < kMasks ? __popcll(m) : 0u;
+    uint32_t incl = count;
+#pragma unroll
+    for (int o = 1; o < (int)kMasks; o <<= 1) {
+      const uint32_t y = __shfl_up(incl, o);
+      if (lane >= (uint32_t)o) incl += y;
+    }
+    live = (uint32_t)__builtin_amdgcn_readlane(incl, kMasks - 1);
+    if (t < r.tokens) {
+      const uint64_t own = s_mask[t / 64];
+      const uint32_t before = (uint32_t)__builtin_amdgcn_readlane(incl - count, t / 64);
+      if (own >> (t % 64) & 1) row = before + __popcll(own & ((1ull << (t % 64)) - 1));
+    }
+    if (row != ~0u && lane == 0) r.rows[row] = t;
+    if (t == 0)
+      write_meta(r, live,
+                 r.grads ? __uint_as_float(wave_max_bits(s_most[lane % (kLanes / 64)]))
+                         : fabsf(r.grad));
   } else {
     row = t < r.tokens ? r.rank[t] : ~0u;
     live = r.meta->live;
@@ -374,7 +455,8 @@ __global__ __launch_bounds__(kLanes) void gather_kernel(GatherArgs a) {
     const u32x4 v = load8(src + c, c < a.columns ? a.columns - c : 0u);
     *(u32x4*)(dst + c) = v;
     if (dot) {
-      const V x = __builtin_bit_cast(V, v), y = *(const V*)(w + c);
+      const V x = __builtin_bit_cast(V, v);
+      const V y = __builtin_bit_cast(V, load8(w + c, c < a.columns ? a.columns - c : 0u));
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) sum = __builtin_fmaf((float)x[i], (float)y[i], sum);
     }
@@ -382,22 +464,6 @@ __global__ __launch_bounds__(kLanes) void gather_kernel(GatherArgs a) {
   if (dot) {
     sum = wave_sum(sum) * r.scale;
     if (lane == 0) a.z[row] = sum;
-  }
-}
-
-// W's rows padded to whole steps, where its own cannot be read 16 bytes at a time.
-__global__ __launch_bounds__(kLanes) void pad_kernel(const uint16_t* __restrict__ w,
-                                                     uint64_t stride, uint32_t vocab,
-                                                     uint32_t columns, uint32_t padded,
-                                                     uint16_t* __restrict__ out) {
-  const uint32_t per = padded / 8;
-  const uint64_t all = (uint64_t)vocab * per;
-  for (uint64_t i = (uint64_t)blockIdx.x * kLanes + threadIdx.x; i < all;
-       i += (uint64_t)gridDim.x * kLanes) {
-    const uint64_t row = i / per;
-    const uint32_t c = (uint32_t)(i % per) * 8;
-    *(u32x4*)(out + row * padded + c) =
-        load8(w + row * stride + c, c < columns ? columns - c : 0u);
   }
 }
 
@@ -556,29 +622,43 @@ __global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {
   }
 }
 
-// log of the sum of a row's exponentials, from its spans, by `lanes` lanes of a
-// block (a wave or all of it; red: a value a wave).
+// log of the sum of a row's exponentials, from its spans' (largest, sum), by `LANES`
+// lanes of a block (a wave or all of it; red: two values a wave).  One pass, eight
+// spans a lane on their way at once.
 template <uint32_t LANES>
 __device__ __forceinline__ float join_spans(const float* stats, uint32_t spans, uint32_t lane,
                                             float* red) {
-  float most = -INFINITY;
-  for (uint32_t i = lane; i < spans; i += LANES) most = fmaxf(most, stats[2 * i]);
-  most = wave_max(most);
-  if constexpr (LANES > 64) {
-    if (lane % 64 == 0) red[lane / 64] = most;
-    __syncthreads();
-    for (uint32_t w = 0; w < LANES / 64; ++w) most = fmaxf(most, red[w]);
-    __syncthreads();
+  typedef float V __attribute__((ext_vector_type(2)));
+  constexpr uint32_t kEach = 8;
+  float most = -INFINITY, sum = 0.0f;
+  const auto join = [](float& m, float& s, float m2, float s2) {
+    // a NaN among the sums stays; -inf on both sides has no distance
+    const float top = fmaxf(m, m2);
+    s = s * (m == top ? 1.0f : expf(m - top)) + s2 * (m2 == top ? 1.0f : expf(m2 - top));
+    m = top;
+  };
+  for (uint32_t i0 = lane; i0 < spans; i0 += LANES * kEach) {
+    V v[kEach];
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+      const uint32_t i = i0 + k * LANES;
+      v[k] = i < spans ? ld_g<V>(stats + 2 * i) : V{-INFINITY, 0.0f};
+    }
+    float m = most;
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) m = fmaxf(m, v[k].x);
+    sum *= most == m ? 1.0f : expf(most - m);
+    most = m;
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) sum += v[k].y * (v[k].x == m ? 1.0f : expf(v[k].x - m));
   }
-  float sum = 0.0f;
-  for (uint32_t i = lane; i < spans; i += LANES) sum += stats[2 * i + 1] * expf(stats[2 * i] - most);
-  sum = wave_sum(sum);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) join(most, sum, __shfl_xor(most, o), __shfl_xor(sum, o));
   if constexpr (LANES > 64) {
-    if (lane % 64 == 0) red[lane / 64] = sum;
+    if (lane % 64 == 0) red[lane / 64 * 2] = most, red[lane / 64 * 2 + 1] = sum;
     __syncthreads();
-    sum = 0.0f;
-    for (uint32_t w = 0; w < LANES / 64; ++w) sum += red[w];
-    __syncthreads();
+    most = red[0], sum = red[1];
+    for (uint32_t w = 1; w < LANES / 64; ++w) join(most, sum, red[2 * w], red[2 * w + 1]);
   }
   return most + logf(sum);
 }
@@ -620,31 +700,35 @@ struct DzArgs {
   float grad, scale;
   uint16_t* e;
   uint64_t e_stride;
-  uint32_t span;  // values a span covers
+  uint32_t written;  // columns that hold something
+  uint32_t span;   // values a span covers
+  uint32_t share;  // of a row, that a block takes: whole rounds of its lanes
 };
 
-// A row's exponentials to dz, a block a row; rows past the live ones, up to a
-// whole step of the products, to zeros.
+// A row's exponentials to dz, by a block (or with few rows by several, each of which
+// joins the spans for itself); rows past the live ones, up to a whole step of the
+// products, to zeros.  Bound by HBM: 12288 rows of 32000, 1.57 GB, 278 us, 5.6 TB/s.
 template <typename T>
 __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
   typedef T V __attribute__((ext_vector_type(8)));
   constexpr uint32_t DT = kTypeOf<T>;
-  __shared__ float red[kLanes / 64];
+  __shared__ float red[kLanes / 64 * 2];
   __shared__ uint32_t s_index[ARK_HEAD_MAX_TOP];
   __shared__ float s_p[ARK_HEAD_MAX_TOP];
   const LossArgs& l = a.loss;
   const uint32_t row = blockIdx.x, live = l.meta->live, tid = threadIdx.x;
   if (row >= (live + kProductStep - 1) / kProductStep * kProductStep) return;
   uint16_t* e = a.e + row * a.e_stride;
+  const uint32_t from = blockIdx.y * a.share, to = min(from + a.share, a.written);
   if (row >= live) {
-    for (uint32_t c = tid * 8; c < a.e_stride; c += kLanes * 8) *(u32x4*)(e + c) = u32x4{0, 0, 0, 0};
+    for (uint32_t c = from + tid * 8; c < to; c += kLanes * 8) *(u32x4*)(e + c) = u32x4{0, 0, 0, 0};
     return;
   }
   const uint32_t t = l.rows[row], top = l.targets.top;
   const float* stats = l.stats + (uint64_t)row * l.spans * 2;
   const float* z = l.z + (uint64_t)row * top;
   const float lse = join_spans<kLanes>(stats, l.spans, tid, red);
-  if (tid < 64) {
+  if (tid < 64 && blockIdx.y == 0) {
     const float loss = row_loss(l.targets, t, z, lse, tid);
     if (tid == 0) l.loss[t] = loss;
   }
@@ -653,7 +737,7 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
     s_index[k] = l.targets.at(t, k);
     s_p[k] = l.targets.weight(t, k);
   }
-  for (uint32_t c = tid * 8; c < a.e_stride; c += kLanes * 8) {
+  for (uint32_t c = from + tid * 8; c < to; c += kLanes * 8) {
     const float s = expf(stats[c / a.span * 2] - lse) * f;
     const V v = ld_nt<V>(e + c);
     u32x4 o;
@@ -667,7 +751,7 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
   // value twice)
   for (uint32_t k = tid; k < top; k += kLanes) {
     const uint32_t v = s_index[k];
-    if (v == ~0u) continue;
+    if (v < from || v >= to) continue;  // another block's, or left out
     float p = 0.0f;
     for (uint32_t i = 0; i < top; ++i) p += s_index[i] == v ? s_p[i] : 0.0f;
     // q - p without the difference of two numbers near 1
@@ -816,24 +900,20 @@ constexpr uint64_t kDzBytes = 1ull << 30;  // of a piece's dz, at most
 struct Big {
   template <typename T, bool AMC, bool BMC>
   using P = Product<T, AMC, BMC, 8, 4, 2, 4, 4>;
-  template <typename T>
-  using L = P<T, false, false>;
 };
 struct Small {
   template <typename T, bool AMC, bool BMC>
   using P = Product<T, AMC, BMC, 4, 2, 2, 2, 4>;
-  template <typename T>
-  using L = P<T, false, false>;
 };
 
 // How a call is cut, and where things lie in its workspace (offsets of 256).
 struct Plan {
-  bool small;                   // tiles
+  bool small_logits, small;     // tiles
   uint32_t piece;               // tokens
   uint32_t pieces;
   uint32_t padded;              // columns
   bool copy_w;
-  uint32_t bm, bn, span, spans;
+  uint32_t span, spans, written;  // written: columns of dz that hold something
   uint64_t e_stride;
   Cut cut;
   uint64_t meta, rank, rows, index, p, self, there, z, x, w, stats, e, dx_parts, dw_parts, sums, bytes;
@@ -842,16 +922,17 @@ struct Plan {
 uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
 // The cut of a piece of `rows` tokens, with room for the parts that it asks for with
-// every token live, and for some more of dx's when few are.
-Cut cut_of(bool small, uint32_t columns, uint32_t rows, uint32_t vocab, bool has_dx, bool has_dw) {
+// every token live, and for some more of dx's when few are.  *best: what it costs.
+Cut cut_of(bool small, uint32_t columns, uint32_t rows, uint32_t vocab, bool has_dx, bool has_dw,
+           float* best_cost) {
   Cut c = {};
   // measured on MI355X: a large tile has a unit to itself, of small ones three share it;
   // partial sums go out and come back at 5 TB/s
   c.tiles_m = small ? (columns + 127) / 128 : (columns + 255) / 256;
   c.bn = small ? 64 : 256;
   c.units = small ? 768 : 256;
-  c.step = small ? 0.33f : 0.85f;
-  c.part = small ? 3.0f : 6.0f;
+  c.step = small ? 0.59f : 0.85f;
+  c.part = small ? 4.0f : 8.0f;
   c.row = (float)up(columns, 4) * 8.0f / 5e6f;
   c.vocab = vocab, c.has_dx = has_dx, c.has_dw = has_dw;
   c.dx_most = c.dw_most = ~0u;
@@ -867,17 +948,29 @@ Cut cut_of(bool small, uint32_t columns, uint32_t rows, uint32_t vocab, bool has
   c.dx_most = best.dx * n;
   if (c.dx_most < some) c.dx_most = some < 24 * n ? some : 24 * n;
   c.dw_most = best.dw * c.tiles_of(vocab);
+  *best_cost = cost;
   return c;
+}
+
+// What the logits cost, in microseconds: large tiles one a unit; small ones three a
+// unit, whose steps take 0.32 alone and 0.59 when three share it.  Measured: 300 rows,
+// 5003 x 901: 26 with large tiles, 12 with small ones; 517, 32308 x 768: 29 and 52.
+float logits_cost(bool small, uint64_t rows, uint64_t vocab, uint32_t padded) {
+  const float steps = (float)(padded / kProductStep);
+  if (!small) {
+    const uint64_t tiles = (up(vocab, 256) / 256) * (up(rows, 256) / 256);
+    return (float)((tiles + 255) / 256) * (steps * 0.8f + 6.0f);
+  }
+  const uint64_t tiles = (up(vocab, 128) / 128) * (up(rows, 64) / 64);
+  float t = (float)(tiles / 768) * (steps * 0.59f + 3.0f);
+  if (tiles % 768) t += steps * (0.18f + 0.137f * (float)((tiles % 768 + 255) / 256)) + 3.0f;
+  return t;
 }
 
 Plan plan_of(const void* w, uint64_t w_stride, uint64_t tokens, uint64_t columns, uint64_t vocab,
              uint64_t top, uint32_t dw_dtype, bool grad, bool has_dx, bool has_dw) {
   Plan p = {};
-  p.small = tokens <= 64;
-  p.bm = p.small ? 128 : 256, p.bn = p.small ? 64 : 256;
-  p.span = p.small ? 64 : 128;
-  p.e_stride = up(vocab, p.bm);
-  p.spans = (uint32_t)(up(vocab, p.bm) / p.span);
+  p.e_stride = up(vocab, 256);
   p.padded = (uint32_t)up(columns, kProductStep);
   p.copy_w = columns % kProductStep || w_stride % 8 || (uintptr_t)w % 16;
   // pieces of equal sizes, whole tiles
@@ -887,7 +980,13 @@ Plan plan_of(const void* w, uint64_t w_stride, uint64_t tokens, uint64_t columns
   p.pieces = (uint32_t)((tokens + most - 1) / most);
   if (p.pieces == 0) p.pieces = 1;
   p.piece = (uint32_t)(p.pieces == 1 ? tokens : up((tokens + p.pieces - 1) / p.pieces, kRowPad));
-  const uint64_t rows = up(p.piece ? p.piece : 1, kRowPad);
+  const uint32_t piece = p.piece ? p.piece : 1;
+  const uint64_t rows = up(piece, kRowPad);
+  p.small_logits = logits_cost(true, piece, vocab, p.padded) <
+                   logits_cost(false, piece, vocab, p.padded);
+  p.span = p.small_logits ? 64 : 128;
+  p.written = (uint32_t)up(vocab, 2 * p.span);
+  p.spans = p.written / p.span;
   uint64_t at = 0;
   const auto take = [&](uint64_t bytes) {
     const uint64_t here = at;
@@ -907,9 +1006,14 @@ Plan plan_of(const void* w, uint64_t w_stride, uint64_t tokens, uint64_t columns
   p.stats = take(rows * p.spans * 8);
   if (grad) {
     p.e = take(rows * p.e_stride * 2);
-    p.cut = cut_of(p.small, (uint32_t)columns, (uint32_t)(p.piece ? p.piece : 1), (uint32_t)vocab,
-                   has_dx, has_dw);
-    const uint64_t tile = up(columns, 4) * 4 * p.bn;
+    float large, small = INFINITY;
+    p.cut = cut_of(false, (uint32_t)columns, piece, (uint32_t)vocab, has_dx, has_dw, &large);
+    if (large < 500.0f) {  // beyond it small tiles have no chance
+      const Cut c = cut_of(true, (uint32_t)columns, piece, (uint32_t)vocab, has_dx, has_dw, &small);
+      p.small = small < large;
+      if (p.small) p.cut = c;
+    }
+    const uint64_t tile = up(columns, 4) * 4 * p.cut.bn;
     p.dx_parts = take(has_dx ? p.cut.dx_most * tile : 0);
     p.dw_parts = take(has_dw && p.cut.dw_most > p.cut.tiles_of((uint32_t)vocab)
                           ? p.cut.dw_most * tile : 0);
@@ -992,7 +1096,7 @@ int launch_grad(const GradArgs& g, const Cut& cut, uint32_t rows, hipStream_t s)
   return ARK_OPT_OK;
 }
 
-template <typename T, typename Size>
+template <typename T, typename LSize, typename Size>
 int run_piece(const Call& c, const Plan& p, uint32_t piece) {
   const hipStream_t s = c.stream;
   const uint64_t t0 = (uint64_t)piece * p.piece;
@@ -1046,13 +1150,20 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
   ga.loss = c.loss + t0;
   ga.dx = c.dx ? (uint16_t*)c.dx + t0 * c.dx_stride : nullptr;
   ga.dx_stride = c.dx_stride;
-  ga.w = w, ga.w_stride = w_stride, ga.z = z;
+  ga.w = (const uint16_t*)c.w, ga.w_stride = c.w_stride, ga.z = z;
   if (!tokens || tokens > kFew) {  // without tokens for what dw's zeros need
     hipLaunchKernelGGL(rank_kernel, dim3(1), dim3(kRankLanes), 0, s, ra);
     ARK_HIP(hipGetLastError());
   }
   if (tokens) {
-    const dim3 grid((tokens + kProductStep - 1 + 3) / 4);
+    ga.blocks = (tokens + kProductStep - 1 + 3) / 4;
+    uint64_t pad = 0;
+    if (p.copy_w && piece == 0) {
+      ga.w_out = (uint16_t*)(ws + p.w);
+      pad = (c.vocab * (p.padded / 8) + kLanes - 1) / kLanes;
+      if (pad > 16384) pad = 16384;
+    }
+    const dim3 grid(ga.blocks + (uint32_t)pad);
     if (tokens <= kFew)
       hipLaunchKernelGGL((gather_kernel<T, true>), grid, dim3(kLanes), 0, s, ga);
     else
@@ -1071,7 +1182,7 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
   la.padded = p.padded, la.vocab = (uint32_t)c.vocab, la.spans = p.spans;
   la.e_stride = p.e_stride;
   la.scale = c.scale;
-  typedef typename Size::template L<T> L;
+  typedef typename LSize::template P<T, false, false> L;
   la.tiles_m = (uint32_t)((c.vocab + L::BM - 1) / L::BM);
   la.meta = meta;
   la.stats = (float*)(ws + p.stats);
@@ -1087,10 +1198,16 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
   DzArgs da = {};
   da.loss = lo, da.grads = ra.grads;
   da.grad = c.grad, da.scale = c.scale;
-  da.e = la.e, da.e_stride = p.e_stride, da.span = p.span;
+  da.e = la.e, da.e_stride = p.e_stride, da.written = p.written, da.span = p.span;
   if (tokens) {
-    hipLaunchKernelGGL(dz_kernel<T>, dim3((uint32_t)up(tokens, kProductStep)), dim3(kLanes), 0, s,
-                       da);
+    // eight blocks for every compute unit, and two rounds of a block's lanes at least
+    const uint64_t rows32 = up(tokens, kProductStep), round = kLanes * 8;
+    uint64_t parts = (2048 + rows32 - 1) / rows32, rounds = (p.written + round - 1) / round;
+    if (parts > (rounds + 1) / 2) parts = (rounds + 1) / 2;
+    da.share = (uint32_t)((rounds + parts - 1) / parts * round);
+    hipLaunchKernelGGL(dz_kernel<T>,
+                       dim3((uint32_t)rows32, (uint32_t)((p.written + da.share - 1) / da.share)),
+                       dim3(kLanes), 0, s, da);
     ARK_HIP(hipGetLastError());
   }
   if (!c.dx && !c.dw) return ARK_OPT_OK;
@@ -1133,15 +1250,11 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
 
 template <typename T>
 int run_call(const Call& c, const Plan& p) {
-  if (p.copy_w) {
-    const uint64_t n = c.vocab * (p.padded / 8), blocks = (n + kLanes - 1) / kLanes;
-    hipLaunchKernelGGL(pad_kernel, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(kLanes),
-                       0, c.stream, (const uint16_t*)c.w, c.w_stride, (uint32_t)c.vocab,
-                       (uint32_t)c.columns, p.padded, (uint16_t*)(c.ws + p.w));
-    ARK_HIP(hipGetLastError());
-  }
   for (uint32_t i = 0; i < p.pieces; ++i) {
-    const int rc = p.small ? run_piece<T, Small>(c, p, i) : run_piece<T, Big>(c, p, i);
+    const int rc = p.small_logits ? p.small ? run_piece<T, Small, Small>(c, p, i)
+                                            : run_piece<T, Small, Big>(c, p, i)
+                   : p.small      ? run_piece<T, Big, Small>(c, p, i)
+                                  : run_piece<T, Big, Big>(c, p, i);
     if (rc) return rc;
   }
   return ARK_OPT_OK;
