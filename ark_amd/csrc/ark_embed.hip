@@ -9,6 +9,7 @@ using namespace ark::dev;
 using ark::fail;
 
 constexpr uint32_t kLanes = 256;
+constexpr uint64_t kMostBlocks = 1ull << 23;  // a launch has fewer than 2^32 lanes
 
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -270,19 +271,21 @@ template <uint32_t DT, bool WIDE>
 __global__ __launch_bounds__(kLanes) void window_kernel(SumArgs a) {
   typedef Column<WIDE> C;
   const uint32_t tiles = (a.columns + C::kWave - 1) / C::kWave;
-  const uint64_t id = (uint64_t)blockIdx.x * (kLanes / 64) +
-                      __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const uint64_t w = id / tiles;
-  if ((w + 1) * kWindow > a.start[a.tokens.vocab]) return;
-  const uint32_t lo = (uint32_t)w * kWindow;
-  if (a.tokens.at(a.pos[lo]) != a.tokens.at(a.pos[lo + kWindow - 1])) return;
-  const C col((uint32_t)(id % tiles), a.columns);
-  float e[C::kEach] = {};
-  add_rows<DT, WIDE, kWindow>(a, col, e, lo, lo + kWindow);
-  float* out = a.windows + w * window_width(a.columns) + col.c;
-  // a lane's last four may be another's too: written twice alike
+  const uint64_t all = (uint64_t)a.start[a.tokens.vocab] / kWindow * tiles;
+  for (uint64_t id = (uint64_t)blockIdx.x * (kLanes / 64) +
+                     __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+       id < all; id += (uint64_t)gridDim.x * (kLanes / 64)) {
+    const uint64_t w = id / tiles;
+    const uint32_t lo = (uint32_t)w * kWindow;
+    if (a.tokens.at(a.pos[lo]) != a.tokens.at(a.pos[lo + kWindow - 1])) continue;
+    const C col((uint32_t)(id % tiles), a.columns);
+    float e[C::kEach] = {};
+    add_rows<DT, WIDE, kWindow>(a, col, e, lo, lo + kWindow);
+    float* out = a.windows + w * window_width(a.columns) + col.c;
+    // a lane's last four may be another's too: written twice alike
 #pragma unroll
-  for (uint32_t j = 0; j < C::kEach; ++j) out[j] = e[j];
+    for (uint32_t j = 0; j < C::kEach; ++j) out[j] = e[j];
+  }
 }
 
 constexpr uint32_t kBatch = 8;  // half the registers of sixteen, twice the waves
@@ -387,8 +390,8 @@ Layout layout_of(uint64_t n, uint64_t vocab, uint64_t columns) {
 
 int check_sizes(uint64_t n, uint64_t vocab, uint64_t columns) {
   if (n >= (1ull << 31)) return fail(ARK_OPT_EINVAL, "n = %llu too large", (unsigned long long)n);
-  if (vocab == 0 || vocab >= (1ull << 31))
-    return fail(ARK_OPT_EINVAL, "vocab = %llu: 1 to 2^31 - 1", (unsigned long long)vocab);
+  if (vocab == 0 || vocab > (1ull << 28))
+    return fail(ARK_OPT_EINVAL, "vocab = %llu: 1 to 2^28", (unsigned long long)vocab);
   if (columns == 0 || columns > 65536)
     return fail(ARK_OPT_EINVAL, "columns = %llu: 1 to 65536", (unsigned long long)columns);
   return ARK_OPT_OK;
@@ -398,7 +401,7 @@ int rows_bytes(uint64_t rows, uint64_t row, uint64_t stride, uint32_t es, bool w
                const char* what, uint64_t* bytes) {
   *bytes = 0;
   if (rows == 0) return ARK_OPT_OK;
-  if (rows > 1 && stride >= (1ull << 31))
+  if (rows > 1 && (stride >= (1ull << 31) || (rows - 1) * stride >= (1ull << 48)))
     return fail(ARK_OPT_EINVAL, "%s: stride %llu too large", what, (unsigned long long)stride);
   if (written && rows > 1 && stride < row)
     return fail(ARK_OPT_EINVAL, "%s: rows of %llu elements overlap at stride %llu", what,
@@ -432,19 +435,19 @@ void launch_lookup(const LookupArgs& a, uint32_t out, dim3 grid, hipStream_t s) 
     launch_lookup<IN, ARK_EMBED_F32>(a, grid, s);
 }
 
+dim3 blocks_of(uint64_t n) { return dim3((uint32_t)(n < kMostBlocks ? n : kMostBlocks)); }
+
 template <uint32_t DT, bool WIDE>
 int launch_sums(const SumArgs& a, hipStream_t s) {
   const uint64_t tiles = (a.columns + Column<WIDE>::kWave - 1) / Column<WIDE>::kWave;
   const uint64_t windows = a.n / kWindow * tiles;
   if (windows) {
-    hipLaunchKernelGGL((window_kernel<DT, WIDE>), dim3((uint32_t)((windows + 3) / 4)), dim3(kLanes),
-                       0, s, a);
+    hipLaunchKernelGGL((window_kernel<DT, WIDE>), blocks_of((windows + 3) / 4), dim3(kLanes), 0,
+                       s, a);
     ARK_HIP(hipGetLastError());
   }
-  const uint64_t blocks = (((uint64_t)a.tokens.vocab + kRows - 1) / kRows * tiles + 3) / 4;
-  hipLaunchKernelGGL((sum_kernel<DT, WIDE>),
-                     dim3((uint32_t)(blocks < (1u << 23) ? blocks : 1u << 23)), dim3(kLanes), 0, s,
-                     a);
+  const uint64_t waves = ((uint64_t)a.tokens.vocab + kRows - 1) / kRows * tiles;
+  hipLaunchKernelGGL((sum_kernel<DT, WIDE>), blocks_of((waves + 3) / 4), dim3(kLanes), 0, s, a);
   ARK_HIP(hipGetLastError());
   return ARK_OPT_OK;
 }
@@ -488,8 +491,7 @@ int ark_embed_lookup(const void* table, uint64_t table_stride, uint32_t table_dt
   a.table_stride = table_stride, a.out_stride = out_stride, a.n = n;
   a.columns = (uint32_t)columns;
   a.scale = scale;
-  const uint64_t blocks = (n * ((columns + 7) / 8) + kLanes - 1) / kLanes;
-  const dim3 grid((uint32_t)(blocks < (1u << 20) ? blocks : 1u << 20));
+  const dim3 grid = blocks_of((n * (columns < 8 ? columns : (columns + 7) / 8) + kLanes - 1) / kLanes);
   const hipStream_t s = (hipStream_t)stream;
   if (table_dtype == ARK_EMBED_F16)
     launch_lookup<ARK_EMBED_F16>(a, out_dtype, grid, s);

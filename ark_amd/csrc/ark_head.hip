@@ -248,7 +248,7 @@ __device__ __forceinline__ void write_meta(const RankArgs& a, uint32_t live, flo
     // the largest |grad * scale| times `up` lies in [2^13, 2^14)
     largest *= fabsf(a.scale);
     if (largest > 0.0f && largest < INFINITY) {
-      const int shift = min(max(13 - ilogbf(largest), -100), 100);
+      const int shift = min(max(13 - ilogbf(largest), -126), 126);
       m.up = ldexpf(1.0f, shift), m.down = ldexpf(1.0f, -shift);
     }
     // the cheapest of the 64 candidates, a lane each
@@ -265,9 +265,11 @@ __device__ __forceinline__ void write_meta(const RankArgs& a, uint32_t live, flo
   if (threadIdx.x % 64 == 0) *a.meta = m;
 }
 
-// |grad| as a whole number, so that a NaN is the largest.
+// |grad| as a whole number; of an inf or NaN 0: its own token's gradients are not
+// finite at any scale, and the others keep theirs.
 __device__ __forceinline__ uint32_t grad_size(const RankArgs& a, uint32_t t) {
-  return __float_as_uint(a.grads[t]) & 0x7FFFFFFFu;
+  const uint32_t g = __float_as_uint(a.grads[t]) & 0x7FFFFFFFu;
+  return g < 0x7F800000u ? g : 0u;
 }
 __device__ __forceinline__ uint32_t wave_max_bits(uint32_t g) {
 #pragma unroll
@@ -1260,13 +1262,12 @@ int run_call(const Call& c, const Plan& p) {
   return ARK_OPT_OK;
 }
 
-// Bytes that rows x row elements at a row stride span; 0 for none.  Strides are
-// below 2^22 for what the products read themselves, 2^40 otherwise.
+// Bytes that rows x row elements at a row stride span; 0 for none.
 int rows_bytes(uint64_t rows, uint64_t row, uint64_t stride, uint32_t es, bool written,
                const char* what, uint64_t* bytes) {
   *bytes = 0;
   if (rows == 0 || row == 0) return ARK_OPT_OK;
-  if (rows > 1 && stride >= (1ull << 32))
+  if (rows > 1 && (stride >= (1ull << 32) || (rows - 1) * stride >= (1ull << 48)))
     return fail(ARK_OPT_EINVAL, "%s: stride %llu too large", what, (unsigned long long)stride);
   if (written && rows > 1 && stride < row)
     return fail(ARK_OPT_EINVAL, "%s: rows of %llu elements overlap at stride %llu", what,

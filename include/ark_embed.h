@@ -18,7 +18,8 @@
  * Every function is stream ordered and returns an ARK_OPT_* status code
  * (include/ark_opt.h), with the message in ark_opt_last_error().  Pointers are
  * device pointers of the current device, and stream is one of its streams.
- * Strides are of rows, in elements; tokens are int32 (token_bytes 4) or int64 (8).
+ * Strides are of rows, in elements, below 2^31; tokens are int32 (token_bytes 4) or
+ * int64 (8).  n is below 2^31, vocab 1 to 2^28, columns 1 to 65536.
  */
 #ifndef ARK_EMBED_H
 #define ARK_EMBED_H

@@ -33,7 +33,8 @@
  * largest of its row in a piece of the vocabulary, and again, scaled by a power
  * of two so that the largest gradient has 2^14, when the row's sum is known.
  * Entries at targets are rounded once, from fp32.  A loss or gradient formed
- * from an inf or NaN is not finite, and the optimizer step then skips.  Sums run
+ * from an inf or NaN is not finite, and the optimizer step then skips; other tokens'
+ * losses and dx stay what they are.  Sums run
  * in an order that depends on the sizes and on which tokens have a loss: equal
  * calls give equal bits.
  *
@@ -44,7 +45,9 @@
  * Every function is stream ordered and returns an ARK_OPT_* status code
  * (include/ark_opt.h), with the message in ark_opt_last_error().  Pointers are
  * device pointers of the current device, and stream is one of its streams.
- * Strides are in elements.
+ * Strides are in elements, below 2^32, and w's below 2^22.  columns are 1 to 65536,
+ * vocab 1 to 2097152, tokens below 2^31; scale and 1 / temperature are positive and
+ * below 2^126.
  */
 #ifndef ARK_HEAD_H
 #define ARK_HEAD_H

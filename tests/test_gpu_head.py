@@ -323,6 +323,28 @@ def test_sizes_of_the_gradient(grad):
     want.check(*head.cross_entropy_grad(x, w, y, grad=g))
 
 
+@pytest.mark.parametrize("grad", [1e36, 1e-37])
+def test_sizes_of_the_gradient_of_fp16(grad):
+    """dw in fp32 holds what the 16 bits of dz do not."""
+    torch = _torch()
+    x, w, y = make(70, 32, 90, "f16")
+    got = head.cross_entropy_grad(x, w, y, grad=grad, dx=False, dw=torch.empty_like(w).float())
+    ce(x, w, y, g=grad).check(*got)
+
+
+@pytest.mark.parametrize("t", [70, 1500])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_a_token_of_no_finite_gradient_leaves_the_others(value, t):
+    torch = _torch()
+    x, w, y = make(t, 32, 90, "f16", masked=0.0)
+    g = torch.full((t,), 1e-4, device="cuda")
+    g[t // 2] = value
+    loss, dx, _ = head.cross_entropy_grad(x, w, y, grad=g)
+    assert not torch.isfinite(dx[t // 2]).any()
+    g[t // 2], dx[t // 2] = 0.0, 0.0
+    ce(x, w, y, g=g).check(loss, dx, None)
+
+
 def test_loss_by_differences():
     """The sum of the losses along a line, by central differences of step h: off by
     h^2 / 6 of the third derivative, at most twice the cube of the largest range of

@@ -126,3 +126,21 @@ def test_lookup_gradient_refusals():
     assert L.ark_embed_grad_workspace(5, 100, 8, None) == _abi.EINVAL
     assert L.ark_embed_grad_workspace(5, 0, 8, C.byref(out)) == _abi.EINVAL and out.value == 0
     assert L.ark_embed_grad_workspace(5, 100, 8, C.byref(out)) == _abi.OK and out.value > 0
+
+
+def test_strides_whose_bytes_wrap_are_refused():
+    """(tokens - 1) * stride * 8 is past 64 bits: no array, whatever it wraps to."""
+    L = _lib.lib()
+    assert L.ark_head_distill(GB, 64, 2 * GB, 64, F16, 1 << 30, 64, 100, 3 * GB, 8, (1 << 32) - 1,
+                              4 * GB, F32, 4, 4, 1.0, 6 * GB, 9 * GB, 1 << 36,
+                              None) == _abi.EINVAL and "stride" in _msg()
+    assert _grad(t=1 << 30, xs=(1 << 32) - 1) == _abi.EINVAL and "stride" in _msg()
+    assert L.ark_embed_lookup(GB, 8, F16, 100, 8, 8 * GB, 8, (1 << 31) - 1, 1.0, 3 * GB,
+                              (1 << 31) - 1, F32, None) == _abi.EINVAL and "stride" in _msg()
+
+
+def test_the_largest_table():
+    out = C.c_uint64(7)
+    L = _lib.lib()
+    assert L.ark_embed_grad_workspace(5, 1 << 28, 1, C.byref(out)) == _abi.OK and out.value > 1 << 30
+    assert L.ark_embed_grad_workspace(5, (1 << 28) + 1, 1, C.byref(out)) == _abi.EINVAL
