@@ -98,13 +98,13 @@ def _loss_grad(x, w, call, top, args, grad, dx, dw, accumulate):
                              f"{x.device}")
         grads, grad = grad.data_ptr(), 0.0
     if dx is None:
-        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+        dx = x.new_empty(x.shape)
     elif dx is not False and (dx.shape != x.shape or dx.dtype != x.dtype or dx.device != x.device):
         raise ValueError(f"dx is {tuple(dx.shape)} {dx.dtype}, x {tuple(x.shape)} {x.dtype}")
     if dw is None:
         if accumulate:
             raise ValueError("accumulate needs a dw")
-        dw = torch.empty_like(w, memory_format=torch.contiguous_format)
+        dw = w.new_empty(w.shape)
     elif dw is not False and (dw.shape != w.shape or dw.device != x.device
                               or dw.dtype not in (w.dtype, torch.float32)):
         raise ValueError(f"dw is {tuple(dw.shape)} {dw.dtype}, not {tuple(w.shape)} float32 or "
