@@ -6,12 +6,11 @@
 //
 //   rank_kernel     which tokens are live, and what follows from how many there are
 //                   (for few tokens gather_kernel's)
-//   gather_kernel   X, padded to whole steps of the products, and z at its targets in
-//                   fp32 (X_t . W_target; a teacher's entries: dots_kernel); zeros
+//   gather_kernel   X, padded to whole steps of the products, and its targets; zeros
 //                   for the tokens without a loss
-//   logits_kernel   z = scale X W^T in tiles that stay in registers; of every row
-//                   and span of the vocabulary its largest z and its sum of
-//                   exp(z - largest), and with gradients the exponentials
+//   logits_kernel   z = scale X W^T in tiles that stay in registers; z at targets in
+//                   fp32; of every row and span of the vocabulary its largest z and
+//                   its sum of exp(z - largest), and with gradients the exponentials
 //                   themselves, in 16 bits: 2^-9 or 2^-12 of each
 //   loss_kernel     the spans' sums joined: log(sum exp z), the loss
 //   dz_kernel       the same, and the exponentials turned into dz where they lie
@@ -180,6 +179,12 @@ struct Targets {
   }
 };
 
+// Targets of live rows lie in rows of whole 16 bytes, ~0 where there is none, or one
+// behind the other where a row has one.
+__host__ __device__ inline uint32_t entries_width(uint32_t top) {
+  return top == 1 ? 1 : (top + 3) / 4 * 4;
+}
+
 // A teacher's distribution, a wave a token.
 __global__ __launch_bounds__(kLanes) void teacher_kernel(
     const void* __restrict__ index, uint32_t index_bytes, uint64_t index_stride,
@@ -347,7 +352,7 @@ struct GatherArgs {
   uint64_t dx_stride;
   const uint16_t* w;  // as given
   uint64_t w_stride;
-  float* z;
+  uint32_t* entries;  // targets by rows
   uint16_t* w_out;    // w padded, or NULL
   uint32_t blocks;    // those after them pad w
 };
@@ -376,13 +381,12 @@ __device__ __forceinline__ void pad_rows(const GatherArgs& a) {
   }
 }
 
-// A wave a token: its row of x, and with one target z there.  The waves past the
-// last token fill X up to a whole step of the products, the blocks past those pad W.
+// A wave a token: its row of x, and its targets.  The waves past the last token fill X
+// up to a whole step of the products, the blocks past those pad W.
 // FEW: at most 1024 tokens, which every block ranks for itself, without rank_kernel
 // before (4096 that way: 19 us, with rank_kernel 16).
-template <typename T, bool FEW>
+template <bool FEW>
 __global__ __launch_bounds__(kLanes) void gather_kernel(GatherArgs a) {
-  typedef T V __attribute__((ext_vector_type(8)));
   const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   if (blockIdx.x >= a.blocks) {
     pad_rows(a);
@@ -450,68 +454,11 @@ __global__ __launch_bounds__(kLanes) void gather_kernel(GatherArgs a) {
   }
   const uint16_t* src = a.x + t * a.x_stride;
   uint16_t* dst = a.out + (uint64_t)row * a.padded;
-  const bool dot = r.targets.targets != nullptr;
-  const uint16_t* w = a.w + (dot ? r.targets.at(t, 0) : 0u) * a.w_stride;
-  float sum = 0.0f;
-  for (uint32_t c = lane * 8; c < a.padded; c += 512) {
-    const u32x4 v = load8(src + c, c < a.columns ? a.columns - c : 0u);
-    *(u32x4*)(dst + c) = v;
-    if (dot) {
-      const V x = __builtin_bit_cast(V, v);
-      const V y = __builtin_bit_cast(V, load8(w + c, c < a.columns ? a.columns - c : 0u));
-#pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) sum = __builtin_fmaf((float)x[i], (float)y[i], sum);
-    }
-  }
-  if (dot) {
-    sum = wave_sum(sum) * r.scale;
-    if (lane == 0) a.z[row] = sum;
-  }
-}
-
-// z at a teacher's entries: a wave takes up to four of a row's.
-constexpr uint32_t kDots = 4;
-template <typename T>
-__global__ __launch_bounds__(kLanes) void dots_kernel(Targets targets,
-                                                      const uint16_t* __restrict__ x,
-                                                      uint32_t padded,
-                                                      const uint16_t* __restrict__ w,
-                                                      uint64_t w_stride,
-                                                      const uint32_t* __restrict__ rows,
-                                                      const Meta* __restrict__ meta, float scale,
-                                                      float* __restrict__ z) {
-  typedef T V __attribute__((ext_vector_type(8)));
-  const uint32_t lane = threadIdx.x % 64;
-  const uint32_t per = (targets.top + kDots - 1) / kDots;
-  const uint64_t id = (uint64_t)blockIdx.x * (kLanes / 64) + threadIdx.x / 64;
-  const uint32_t row = (uint32_t)(id / per), k0 = (uint32_t)(id % per) * kDots;
-  if (row >= meta->live) return;
-  const uint32_t t = rows[row], n = min(targets.top - k0, kDots);
-  const uint16_t* xr = x + (uint64_t)row * padded;
-  const uint16_t* wr[kDots];
-  bool there[kDots];
-#pragma unroll
-  for (uint32_t k = 0; k < kDots; ++k) {
-    const uint32_t v = k < n ? targets.at(t, k0 + k) : ~0u;
-    there[k] = v != ~0u;
-    wr[k] = w + (uint64_t)(there[k] ? v : 0u) * w_stride;
-  }
-  float s[kDots] = {};
-  for (uint32_t c = lane * 8; c < padded; c += 512) {
-    const V a = *(const V*)(xr + c);
-#pragma unroll
-    for (uint32_t k = 0; k < kDots; ++k) {
-      if (!there[k]) continue;
-      const V b = *(const V*)(wr[k] + c);
-#pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) s[k] = __builtin_fmaf((float)a[i], (float)b[i], s[k]);
-    }
-  }
-#pragma unroll
-  for (uint32_t k = 0; k < kDots; ++k) {
-    const float v = wave_sum(s[k]) * scale;
-    if (lane == 0 && k < n) z[(uint64_t)row * targets.top + k0 + k] = v;
-  }
+  for (uint32_t c = lane * 8; c < a.padded; c += 512)
+    *(u32x4*)(dst + c) = load8(src + c, c < a.columns ? a.columns - c : 0u);
+  const uint32_t top = r.targets.top, width = entries_width(top);
+  for (uint32_t k = lane; k < width; k += 64)
+    a.entries[(uint64_t)row * width + k] = k < top ? r.targets.at(t, k) : ~0u;
 }
 
 // The tile of a block: blocks of one XCD (every eighth) take neighbouring tiles,
@@ -542,6 +489,9 @@ struct LogitsArgs {
   const Meta* meta;
   float* stats;  // [row][span] of (largest, sum)
   uint16_t* e;   // [row][e_stride], or NULL
+  const uint32_t* entries;  // [row][entries_width(top)]
+  uint32_t top;
+  float* z;                 // [row][top]: the logits there
 };
 
 template <typename P>
@@ -553,12 +503,15 @@ __global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {
   if (blockIdx.x >= tiles.m * tiles.n) return;
   tiles.find(blockIdx.x, tiles.m * tiles.n, &tm, &tn, &split);
   const uint32_t m0 = tm * P::BM, n0 = tn * P::BN;
+  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t w0 = m0 + wave % P::WM * 16 * P::MF;  // the wave's first of the vocabulary
+  const uint32_t r0 = n0 + wave / P::WM * 16 * P::NF;  // and its first row
+  uint32_t target = ~0u;  // lane i: of row r0 + i
+  if (a.top == 1 && lane < 16 * P::NF && r0 + lane < live) target = a.entries[r0 + lane];
   P p;
   const Operand ow = {a.w + m0 * a.w_stride, a.w_stride, a.vocab - m0, 0};
   const Operand ox = {a.x + (uint64_t)n0 * a.padded, a.padded, P::BN, 0};
   p.run(ow, ox, 0, a.padded / kProductStep, (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds);
-  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const uint32_t w0 = m0 + wave % P::WM * 16 * P::MF;  // the wave's first of the vocabulary
   const uint32_t span = tm * P::WM + wave % P::WM;
   if (m0 + P::BM > a.vocab) {
 #pragma unroll
@@ -570,16 +523,75 @@ __global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {
           for (uint32_t j = 0; j < P::NF; ++j) p.acc[i][j][k] = -INFINITY;
         }
   }
-  if (a.e) __syncthreads();  // LDS is the exponentials' now
+  // a lane's sixteen entries from k on, in four pieces, of one row
+  const auto entries = [&](u32x4 (&v)[4], uint32_t row, uint32_t k) __attribute__((always_inline)) {
+    const uint32_t width = entries_width(a.top);
+#pragma unroll
+    for (uint32_t q = 0; q < 4; ++q) {
+      v[q] = u32x4{~0u, ~0u, ~0u, ~0u};
+      if (k + q * 16 < width)
+        v[q] = ld_g<u32x4>(a.entries + (uint64_t)row * width + k + q * 16);
+    }
+  };
+  u32x4 begin[P::NF][4];  // those of every row's first 64, all on their way at once
+  if (a.top > 1) {
+#pragma unroll
+    for (uint32_t j = 0; j < P::NF; ++j)
+      entries(begin[j], min(r0 + j * 16 + lane / 4, live - 1), lane % 4 * 4);
+  }
+  __syncthreads();  // LDS is the epilogue's now
   // A wave's exponentials of 16 rows pass through LDS of its own, so that a row's
   // leave as whole lines: chunks of 16 bytes, permuted by the row against conflicts.
   constexpr uint32_t kRow = P::MF * 32, kChunks = kRow / 16;  // bytes of a row
-  static_assert(16 * kRow * P::WM * P::WN <= P::kLds, "a part of LDS for each wave");
-  uint8_t* mine = lds + wave * 16 * kRow;
+  // Before them so do the logits of rows that may have a target in the wave's span (64
+  // entries a token of 32000, looked for here: 4.5 us a tile, 256 x 256; gathered rows
+  // of W times x: 55 us for 4096 tokens, of 16 tiles down and 8 rounds).
+  constexpr uint32_t kZRow = P::MF * 64, kSpan = P::MF * 16;
+  static_assert(16 * kZRow * P::WM * P::WN <= P::kLds, "a part of LDS for each wave");
+  uint8_t* mine = lds + wave * 16 * kZRow;
   const float to2 = a.scale * kLog2e;
+  const uint64_t hits = __ballot(target - w0 < kSpan);
 #pragma unroll
   for (uint32_t j = 0; j < P::NF; ++j) {
-    const uint32_t t0 = n0 + wave / P::WM * 16 * P::NF + j * 16, t = t0 + lane % 16;
+    const uint32_t t0 = r0 + j * 16, t = t0 + lane % 16;
+    if (a.top > 1 || hits >> (j * 16) & 0xFFFFu) {
+#pragma unroll
+      for (uint32_t i = 0; i < P::MF; ++i)
+        *(f32x4*)(mine + lane % 16 * kZRow + ((i * 4 + lane / 16) ^ (lane % 16)) * 16) =
+            p.acc[i][j] * a.scale;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const auto z_at = [&](uint32_t row, uint32_t d) {
+        return *(const float*)(mine + row * kZRow + ((d / 4) ^ row) * 16 + d % 4 * 4);
+      };
+      if (a.top == 1) {
+        if (lane / 16 == j && target - w0 < kSpan) a.z[r0 + lane] = z_at(lane % 16, target - w0);
+      } else if (t0 + lane / 4 < live) {
+        const uint64_t row = t0 + lane / 4;
+        const uint32_t width = entries_width(a.top);
+        for (uint32_t k = lane % 4 * 4; k < width; k += 64) {
+          u32x4 v[4];
+          if (k < 16) {
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q) v[q] = begin[j][q];
+          } else {
+            entries(v, (uint32_t)row, k);
+          }
+          // bits of those in the span, entry i in 1 << i; few
+          uint32_t there = 0;
+#pragma unroll
+          for (uint32_t i = 0; i < 16; ++i) there |= v[i / 4][i % 4] - w0 < kSpan ? 1u << i : 0u;
+          while (there) {
+            const uint32_t i = (uint32_t)__ffs(there) - 1u;
+            uint32_t d = 0;
+#pragma unroll
+            for (uint32_t h = 0; h < 16; ++h) d = h == i ? v[h / 4][h % 4] - w0 : d;
+            a.z[row * a.top + k + i / 4 * 16 + i % 4] = z_at(lane / 4, d);
+            there &= there - 1;
+          }
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
     float most = -INFINITY;
 #pragma unroll
     for (uint32_t i = 0; i < P::MF; ++i)
@@ -918,7 +930,7 @@ struct Plan {
   uint32_t span, spans, written;  // written: columns of dz that hold something
   uint64_t e_stride;
   Cut cut;
-  uint64_t meta, rank, rows, index, p, self, there, z, x, w, stats, e, dx_parts, dw_parts, sums, bytes;
+  uint64_t meta, rank, rows, index, p, self, there, entries, z, x, w, stats, e, dx_parts, dw_parts, sums, bytes;
 };
 
 uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
@@ -1002,6 +1014,7 @@ Plan plan_of(const void* w, uint64_t w_stride, uint64_t tokens, uint64_t columns
   p.p = take(rows * top * 4);
   p.self = take(rows * 4);
   p.there = take(rows * 4);
+  p.entries = take(rows * entries_width((uint32_t)top) * 4);
   p.z = take(rows * top * 4);
   p.x = take(rows * p.padded * 2);
   p.w = take(p.copy_w ? vocab * p.padded * 2 : 0);
@@ -1152,7 +1165,8 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
   ga.loss = c.loss + t0;
   ga.dx = c.dx ? (uint16_t*)c.dx + t0 * c.dx_stride : nullptr;
   ga.dx_stride = c.dx_stride;
-  ga.w = (const uint16_t*)c.w, ga.w_stride = c.w_stride, ga.z = z;
+  ga.w = (const uint16_t*)c.w, ga.w_stride = c.w_stride;
+  ga.entries = (uint32_t*)(ws + p.entries);
   if (!tokens || tokens > kFew) {  // without tokens for what dw's zeros need
     hipLaunchKernelGGL(rank_kernel, dim3(1), dim3(kRankLanes), 0, s, ra);
     ARK_HIP(hipGetLastError());
@@ -1167,16 +1181,9 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
     }
     const dim3 grid(ga.blocks + (uint32_t)pad);
     if (tokens <= kFew)
-      hipLaunchKernelGGL((gather_kernel<T, true>), grid, dim3(kLanes), 0, s, ga);
+      hipLaunchKernelGGL((gather_kernel<true>), grid, dim3(kLanes), 0, s, ga);
     else
-      hipLaunchKernelGGL((gather_kernel<T, false>), grid, dim3(kLanes), 0, s, ga);
-    ARK_HIP(hipGetLastError());
-  }
-  if (tokens && c.teacher) {
-    const uint64_t waves = (uint64_t)tokens * ((top + kDots - 1) / kDots);
-    hipLaunchKernelGGL(dots_kernel<T>, dim3((uint32_t)((waves + 3) / 4)), dim3(kLanes), 0, s, g,
-                       (const uint16_t*)x, p.padded, w, w_stride, (const uint32_t*)rows,
-                       (const Meta*)meta, c.scale, z);
+      hipLaunchKernelGGL((gather_kernel<false>), grid, dim3(kLanes), 0, s, ga);
     ARK_HIP(hipGetLastError());
   }
   LogitsArgs la = {};
@@ -1189,6 +1196,7 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
   la.meta = meta;
   la.stats = (float*)(ws + p.stats);
   la.e = c.with_grad ? (uint16_t*)(ws + p.e) : nullptr;
+  la.entries = ga.entries, la.top = top, la.z = z;
   int rc;
   if (tokens && (rc = launch_logits<L>(la, la.tiles_m * ((tokens + L::BN - 1) / L::BN), s))) return rc;
   LossArgs lo = {g, rows, meta, la.stats, p.spans, z, ga.loss};
