@@ -368,17 +368,15 @@ __device__ __forceinline__ u32x4 load8(const uint16_t* p, uint32_t n) {
   return u32x4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
 }
 
-// W's rows padded to whole steps, where its own cannot be read 16 bytes at a time.
+// W's rows padded to whole steps, where its own cannot be read 16 bytes at a time, a
+// wave a row.
 __device__ __forceinline__ void pad_rows(const GatherArgs& a) {
-  const uint32_t per = a.padded / 8;
-  const uint64_t all = (uint64_t)a.rank.targets.vocab * per;
-  const uint64_t step = (uint64_t)(gridDim.x - a.blocks) * kLanes;
-  for (uint64_t i = (uint64_t)(blockIdx.x - a.blocks) * kLanes + threadIdx.x; i < all; i += step) {
-    const uint64_t row = i / per;
-    const uint32_t c = (uint32_t)(i % per) * 8;
-    *(u32x4*)(a.w_out + row * a.padded + c) =
-        load8(a.w + row * a.w_stride + c, c < a.columns ? a.columns - c : 0u);
-  }
+  const uint32_t lane = threadIdx.x % 64, step = (gridDim.x - a.blocks) * (kLanes / 64);
+  for (uint32_t row = (blockIdx.x - a.blocks) * (kLanes / 64) + threadIdx.x / 64;
+       row < a.rank.targets.vocab; row += step)
+    for (uint32_t c = lane * 8; c < a.padded; c += 512)
+      *(u32x4*)(a.w_out + (uint64_t)row * a.padded + c) =
+          load8(a.w + row * a.w_stride + c, c < a.columns ? a.columns - c : 0u);
 }
 
 // A wave a token: its row of x, and its targets.  The waves past the last token fill X
@@ -1176,8 +1174,8 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
     uint64_t pad = 0;
     if (p.copy_w && piece == 0) {
       ga.w_out = (uint16_t*)(ws + p.w);
-      pad = (c.vocab * (p.padded / 8) + kLanes - 1) / kLanes;
-      if (pad > 16384) pad = 16384;
+      pad = (c.vocab + kLanes / 64 - 1) / (kLanes / 64);
+      if (pad > 8192) pad = 8192;
     }
     const dim3 grid(ga.blocks + (uint32_t)pad);
     if (tokens <= kFew)
