@@ -120,7 +120,7 @@ constexpr uint32_t kKept = 16;  // tokens a lane asks for at once
 constexpr uint32_t kWindow = 16;
 
 // KEEP: each lane has kKept tokens at most, which stay in registers for the second
-// time (16384 tokens into 250 groups: 16 us without).
+// time.  Bound by a block's latency: 16384 tokens into 250 groups 10.6 us, 16 without.
 template <bool KEEP>
 __global__ __launch_bounds__(kSortLanes) void sort_kernel(Tokens tokens, uint32_t n,
                                                           uint32_t* __restrict__ start,
@@ -267,6 +267,8 @@ __device__ __forceinline__ uint64_t window_width(uint32_t columns) {
   return (columns + 3) / 4 * 4;
 }
 
+// Latency: 16384 of text's tokens, of which a third of the windows are one token's, 768
+// columns of fp16, 5 us.
 template <uint32_t DT, bool WIDE>
 __global__ __launch_bounds__(kLanes) void window_kernel(SumArgs a) {
   typedef Column<WIDE> C;
@@ -340,7 +342,7 @@ __device__ __forceinline__ void sum_row(const SumArgs& a, const Column<WIDE>& co
 
 // Every row of the table, or those of tokens that occur.  Most rows have no token
 // (a vocabulary is larger than a batch's words), so what counts is the zeros'
-// way to memory: 16384 tokens into 32000 x 768, 98 MB.
+// way to memory: 16384 tokens into 32000 x 768, 98 MB written and 25 read in 29 us.
 template <uint32_t DT, bool WIDE>
 __global__ __launch_bounds__(kLanes) void sum_kernel(SumArgs a) {
   typedef Column<WIDE> C;

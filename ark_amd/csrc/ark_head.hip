@@ -185,7 +185,7 @@ __host__ __device__ inline uint32_t entries_width(uint32_t top) {
   return top == 1 ? 1 : (top + 3) / 4 * 4;
 }
 
-// A teacher's distribution, a wave a token.
+// A teacher's distribution, a wave a token.  Latency: 4096 tokens of 64 entries 5 us.
 __global__ __launch_bounds__(kLanes) void teacher_kernel(
     const void* __restrict__ index, uint32_t index_bytes, uint64_t index_stride,
     const void* __restrict__ logits, uint32_t dtype, uint64_t logits_stride, uint32_t tokens,
@@ -283,7 +283,8 @@ __device__ __forceinline__ uint32_t wave_max_bits(uint32_t g) {
 }
 
 // The live tokens' order, by one block: 1024 tokens at a time side by side, their
-// numbers of live ones summed in the tokens' order.
+// numbers of live ones summed in the tokens' order.  Latency of one block: 16384 tokens
+// 10 us.
 constexpr uint32_t kRankLanes = 1024, kRankWaves = kRankLanes / 64;
 constexpr uint32_t kRankEach = kMaxPiece / kRankLanes;
 __global__ __launch_bounds__(kRankLanes) void rank_kernel(RankArgs a) {
@@ -380,7 +381,9 @@ __device__ __forceinline__ void pad_rows(const GatherArgs& a) {
 }
 
 // A wave a token: its row of x, and its targets.  The waves past the last token fill X
-// up to a whole step of the products, the blocks past those pad W.
+// up to a whole step of the products, the blocks past those pad W.  Bound by HBM:
+// 16384 rows of 2048, 134 MB out and back, 26 us; where W is padded by that too (333
+// tokens, 5003 rows of 901, 18 MB: 7 us).
 // FEW: at most 1024 tokens, which every block ranks for itself, without rank_kernel
 // before (4096 that way: 19 us, with rank_kernel 16).
 template <bool FEW>
@@ -492,6 +495,14 @@ struct LogitsArgs {
   float* z;                 // [row][top]: the logits there
 };
 
+// z of a tile of the vocabulary (m) and of rows of X (n), never in memory.  A lane holds
+// MF x 4 logits of one row of X, a wave MF x 16, so a row's largest logit and sum over a
+// wave's span are sums in registers and two exchanges, and the spans' join is left to the
+// next kernel: nothing waits for another block.  Bound by the matrix units at the clock
+// that power leaves them (1.95 GHz), a tile's 24 to 64 steps of 0.8 us and 6 us before and
+// after them, in which the exponentials are the largest part: 12288 x 32000 x 768 fp16
+// 655 us, 0.92 PFLOP/s; 16384 x 32000 x 2048 bf16 2.0 ms, 1.08 PFLOP/s.  8 rows: W's 49 MB
+// go past in 12 us.
 template <typename P>
 __global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {
   extern __shared__ __align__(1024) uint8_t lds[];
@@ -697,6 +708,7 @@ struct LossArgs {
   float* loss;
 };
 
+// The loss alone, a wave a row.  Latency: 4099 rows of 250 spans 6 us.
 __global__ __launch_bounds__(kLanes) void loss_kernel(LossArgs a) {
   const uint32_t row = blockIdx.x * (kLanes / 64) + threadIdx.x / 64, lane = threadIdx.x % 64;
   if (row >= a.meta->live) return;
@@ -866,6 +878,12 @@ __device__ __forceinline__ void product_block(const ProductArgs& g, const Meta& 
   });
 }
 
+// dx and dw in one launch, the longer blocks first (write_meta), so that the shorter ones
+// fill the units that those leave (12288 x 32000 x 768: 7 % of the call less than with a
+// launch each).  Bound as the logits are: 12288 x 32000 x 768 fp16 1.11 ms, 1.09 PFLOP/s;
+// 16384 x 32000 x 2048 bf16 3.55 ms, 1.21 PFLOP/s, where a library product of 8192^3
+// reaches 1.29 and 1.35.  (A rate of 1.94 is what these matrix instructions reach from
+// registers alone; 32 x 32 x 16 ones reach 1.71.)
 template <typename X, typename W>
 __global__ __launch_bounds__(X::kLanes, 2) void grad_kernel(GradArgs g) {
   extern __shared__ __align__(1024) uint8_t lds[];
@@ -884,7 +902,8 @@ __global__ __launch_bounds__(X::kLanes, 2) void grad_kernel(GradArgs g) {
   }
 }
 
-// The parts of both products, added in order.
+// The parts of both products, added in order.  Bound by the caches that the parts are
+// still in: dw's two of 32000 x 768, 18 us.
 __device__ __forceinline__ void join(const float* partial, uint32_t parts, uint32_t height,
                                      const Out& out, uint64_t i, uint64_t step) {
   const uint32_t per = (out.width + 3) / 4;
