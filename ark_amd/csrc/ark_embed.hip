@@ -1,4 +1,6 @@
 // ark_embed.hip -- token lookup and its gradient (include/ark_embed.h).
+#include <type_traits>
+
 #include "ark_act.hpp"
 #include "ark_common.hpp"
 #include "ark_embed.h"
@@ -141,7 +143,7 @@ __global__ __launch_bounds__(kSortLanes) void sort_kernel(Tokens tokens, uint32_
       if (t >= hi) v[k] = ~0u;
     }
   };
-  if (KEEP && n) ask(lo);
+  if (KEEP) ask(lo);
   for (uint32_t t0 = lo; t0 < hi; t0 += 64 * kKept) {
     if (!KEEP) ask(t0);
 #pragma unroll
@@ -228,38 +230,50 @@ struct Column {
   }
 };
 
-// e = e + the rows at sorted positions [lo, hi), in order, kBatch in flight.
-template <uint32_t DT, bool WIDE, uint32_t kBatch>
+__device__ __forceinline__ auto sorted(const SumArgs& a) {
+  return [p = a.pos](uint32_t i) { return ld_g<uint32_t>(p + i); };
+}
+
+// e = e + the rows at sorted positions [lo, hi), in order, kBatch in flight, as they are
+// in memory until they are added.  pos(i): the i-th position.
+template <uint32_t DT, bool WIDE, uint32_t kBatch, typename F>
 __device__ __forceinline__ void add_rows(const SumArgs& a, const Column<WIDE>& col,
                                          float (&e)[Column<WIDE>::kEach], uint32_t lo,
-                                         uint32_t hi) {
+                                         uint32_t hi, F pos) {
   constexpr uint32_t E = Column<WIDE>::kEach;
+  typedef elem_t<DT> T;
+  typedef T V __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  typedef typename std::conditional<WIDE, V, T>::type R;
   for (uint32_t i = lo; i < hi; i += kBatch) {
     // the positions of the rows, a lane one
     const uint32_t k = i + threadIdx.x % kBatch;
-    const uint32_t p = ld_g<uint32_t>(a.pos + min(k, hi - 1));
-    float v[kBatch][E];
-#pragma unroll
-    for (uint32_t k = 0; k < kBatch; ++k) {
+    const uint32_t p = pos(min(k, hi - 1));
+    R v[kBatch];
+    const auto load = [&](uint32_t k) __attribute__((always_inline)) {
       const uint32_t t = __builtin_amdgcn_readlane(p, k);
-      const elem_t<DT>* row = (const elem_t<DT>*)a.dy + t * a.dy_stride;
-      if (i + k < hi) {
-        if constexpr (WIDE) {
-          Some<4> s;
-          s.load<DT>(row, col.c);
+      v[k] = *(const ARK_GLOBAL R*)((const T*)a.dy + t * a.dy_stride + col.c);
+    };
+    const auto add = [&](uint32_t k) __attribute__((always_inline)) {
+      if constexpr (WIDE) {
 #pragma unroll
-          for (uint32_t j = 0; j < E; ++j) v[k][j] = s.v[j];
-        } else {
-          v[k][0] = (float)row[col.c];
-        }
+        for (uint32_t j = 0; j < E; ++j) e[j] += (float)v[k][j];
+      } else {
+        e[0] += (float)v[k];
       }
+    };
+    if (i + kBatch <= hi) {
+#pragma unroll
+      for (uint32_t k = 0; k < kBatch; ++k) load(k);
+#pragma unroll
+      for (uint32_t k = 0; k < kBatch; ++k) add(k);
+    } else {
+#pragma unroll
+      for (uint32_t k = 0; k < kBatch; ++k)
+        if (i + k < hi) load(k);
+#pragma unroll
+      for (uint32_t k = 0; k < kBatch; ++k)
+        if (i + k < hi) add(k);
     }
-#pragma unroll
-    for (uint32_t k = 0; k < kBatch; ++k)
-      if (i + k < hi) {
-#pragma unroll
-        for (uint32_t j = 0; j < E; ++j) e[j] += v[k][j];
-      }
   }
 }
 
@@ -282,7 +296,7 @@ __global__ __launch_bounds__(kLanes) void window_kernel(SumArgs a) {
     if (a.tokens.at(a.pos[lo]) != a.tokens.at(a.pos[lo + kWindow - 1])) continue;
     const C col((uint32_t)(id % tiles), a.columns);
     float e[C::kEach] = {};
-    add_rows<DT, WIDE, kWindow>(a, col, e, lo, lo + kWindow);
+    add_rows<DT, WIDE, kWindow>(a, col, e, lo, lo + kWindow, sorted(a));
     float* out = a.windows + w * window_width(a.columns) + col.c;
     // a lane's last four may be another's too: written twice alike
 #pragma unroll
@@ -294,6 +308,41 @@ constexpr uint32_t kBatch = 8;  // half the registers of sixteen, twice the wave
 
 constexpr uint32_t kRows = 4;     // rows of the table a wave takes, their starts read at once
 
+// e to row v, or added there; zeros.
+template <bool WIDE>
+__device__ __forceinline__ void put_row(const SumArgs& a, const Column<WIDE>& col, uint32_t v,
+                                        float (&e)[Column<WIDE>::kEach]) {
+  typedef Column<WIDE> C;
+  float* row = a.dw + v * a.dw_stride;
+#pragma unroll
+  for (uint32_t j = 0; j < C::kEach; ++j) e[j] *= a.scale;
+  if constexpr (WIDE) {
+    if (col.c == col.own) {
+      Some<4> out;
+      if (a.accumulate) out.load<ARK_EMBED_F32>(row, col.c);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) out.v[j] = a.accumulate ? out.v[j] + e[j] : e[j];
+      out.store<ARK_EMBED_F32>(row, col.c);
+      return;
+    }
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < C::kEach; ++j)
+    if (col.c + j >= col.own) row[col.c + j] = a.accumulate ? row[col.c + j] + e[j] : e[j];
+}
+template <bool WIDE>
+__device__ __forceinline__ void put_zeros(const SumArgs& a, const Column<WIDE>& col, uint32_t v) {
+  float* row = a.dw + v * a.dw_stride;
+  if (WIDE && col.c == col.own) {
+    const Some<4> none = {};
+    none.store<ARK_EMBED_F32>(row, col.c);
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < Column<WIDE>::kEach; ++j)
+      if (col.c + j >= col.own) row[col.c + j] = 0.0f;
+  }
+}
+
 template <uint32_t DT, bool WIDE>
 __device__ __forceinline__ void sum_row(const SumArgs& a, const Column<WIDE>& col, uint32_t v,
                                         uint32_t lo, uint32_t hi) {
@@ -301,7 +350,7 @@ __device__ __forceinline__ void sum_row(const SumArgs& a, const Column<WIDE>& co
   float e[C::kEach] = {};
   const uint32_t w0 = (lo + kWindow - 1) / kWindow, w1 = hi / kWindow;  // whole windows
   const bool windows = w0 < w1;
-  add_rows<DT, WIDE, kBatch>(a, col, e, lo, windows ? w0 * kWindow : hi);
+  add_rows<DT, WIDE, kBatch>(a, col, e, lo, windows ? w0 * kWindow : hi, sorted(a));
   if (windows) {
     const uint64_t width = window_width(a.columns);
     for (uint32_t w = w0; w < w1; w += kBatch) {
@@ -320,24 +369,9 @@ __device__ __forceinline__ void sum_row(const SumArgs& a, const Column<WIDE>& co
           for (uint32_t j = 0; j < C::kEach; ++j) e[j] += s[k][j];
         }
     }
-    add_rows<DT, WIDE, kBatch>(a, col, e, w1 * kWindow, hi);
+    add_rows<DT, WIDE, kBatch>(a, col, e, w1 * kWindow, hi, sorted(a));
   }
-  float* row = a.dw + v * a.dw_stride;
-#pragma unroll
-  for (uint32_t j = 0; j < C::kEach; ++j) e[j] *= a.scale;
-  if constexpr (WIDE) {
-    if (col.c == col.own) {
-      Some<4> out;
-      if (a.accumulate) out.load<ARK_EMBED_F32>(row, col.c);
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) out.v[j] = a.accumulate ? out.v[j] + e[j] : e[j];
-      out.store<ARK_EMBED_F32>(row, col.c);
-      return;
-    }
-  }
-#pragma unroll
-  for (uint32_t j = 0; j < C::kEach; ++j)
-    if (col.c + j >= col.own) row[col.c + j] = a.accumulate ? row[col.c + j] + e[j] : e[j];
+  put_row(a, col, v, e);
 }
 
 // Every row of the table, or those of tokens that occur.  Most rows have no token
@@ -358,21 +392,86 @@ __global__ __launch_bounds__(kLanes) void sum_kernel(SumArgs a) {
     for (uint32_t k = 0; k <= kRows; ++k) at[k] = a.start[min(v0 + k, vocab)];
     if (!a.accumulate) {
 #pragma unroll
-      for (uint32_t k = 0; k < kRows; ++k) {
-        if (at[k] != at[k + 1] || v0 + k >= vocab) continue;
-        float* row = a.dw + (v0 + k) * a.dw_stride;
-        if (WIDE && col.c == col.own) {
-          const Some<4> none = {};
-          none.store<ARK_EMBED_F32>(row, col.c);
-        } else {
-#pragma unroll
-          for (uint32_t j = 0; j < C::kEach; ++j)
-            if (col.c + j >= col.own) row[col.c + j] = 0.0f;
-        }
-      }
+      for (uint32_t k = 0; k < kRows; ++k)
+        if (at[k] == at[k + 1] && v0 + k < vocab) put_zeros(a, col, v0 + k);
     }
     for (uint32_t k = 0; k < kRows; ++k)
       if (at[k] != at[k + 1]) sum_row<DT, WIDE>(a, col, v0 + k, at[k], at[k + 1]);
+  }
+}
+
+// The whole gradient of few tokens in one launch: a block takes kFewRows rows of the
+// table and a tile of columns for each of its waves, finds the rows' positions among all
+// tokens and puts them in order by counting, for each, those before it.  A row's sums are
+// by sixteen positions.  305 tokens into 14862 x 1837 21.5 us (109 MB of zeros), 276 into
+// 604 x 64 9; sorted and summed in three launches 26 and 16.  512 equal tokens, a row by
+// four waves, take longer than by windows, more of them much longer.
+constexpr uint32_t kFew = 512;
+constexpr uint32_t kFewRows = 16;
+
+template <uint32_t DT, bool WIDE>
+__global__ __launch_bounds__(kLanes) void few_kernel(SumArgs a) {
+  typedef Column<WIDE> C;
+  constexpr uint32_t kWaves = kLanes / 64, kEach = kFew / kLanes;
+  __shared__ uint64_t s_mask[kEach * kWaves];
+  constexpr uint32_t kAtOnce = 16;  // of the ones found, compared with
+  __shared__ __align__(16) uint32_t s_found[kFew + kAtOnce];
+  __shared__ uint32_t s_pos[kFew], s_start[kFewRows + 1];
+  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t v0 = blockIdx.x * kFewRows, rows = min(kFewRows, a.tokens.vocab - v0);
+  uint32_t row[kEach];
+#pragma unroll
+  for (uint32_t k = 0; k < kEach; ++k) {
+    const uint32_t t = k * kLanes + threadIdx.x;
+    row[k] = t < a.n ? a.tokens.at(t) - v0 : ~0u;  // ~0, no row, stays past them
+    const uint64_t mask = __ballot(row[k] < rows);
+    if (lane == 0) s_mask[k * kWaves + wave] = mask;
+  }
+  __syncthreads();
+  uint32_t all = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kEach * kWaves; ++i) {
+    const uint64_t mask = s_mask[i];
+    if (i % kWaves == wave && row[i / kWaves] < rows)
+      s_found[all + __popcll(mask & ((1ull << lane) - 1ull))] =
+          row[i / kWaves] << 16 | (i / kWaves * kLanes + threadIdx.x);
+    all += __popcll(mask);
+  }
+  if (threadIdx.x < kAtOnce) s_found[all + threadIdx.x] = ~0u;
+  __syncthreads();
+  // those found that are below a key
+  const auto below = [&](uint32_t key) {
+    uint32_t at = 0;
+    for (uint32_t j = 0; j < all; j += kAtOnce) {
+      u32x4 v[kAtOnce / 4];
+#pragma unroll
+      for (uint32_t q = 0; q < kAtOnce / 4; ++q) v[q] = *(const u32x4*)(s_found + j + q * 4);
+#pragma unroll
+      for (uint32_t q = 0; q < kAtOnce; ++q) at += v[q / 4][q % 4] < key ? 1 : 0;
+    }
+    return at;
+  };
+  for (uint32_t i = threadIdx.x; i < all; i += kLanes) s_pos[below(s_found[i])] = s_found[i] & 0xFFFFu;
+  if (threadIdx.x <= kFewRows) s_start[threadIdx.x] = below(threadIdx.x << 16);
+  __syncthreads();
+  const uint32_t tile0 = blockIdx.y * kWaves;
+  const uint32_t tiles = min((a.columns + C::kWave - 1) / C::kWave - tile0, kWaves);
+  for (uint32_t i = wave; i < rows * tiles; i += kWaves) {
+    const uint32_t r = i / tiles, lo = s_start[r], hi = s_start[r + 1];
+    const C col(tile0 + i % tiles, a.columns);
+    if (lo == hi) {
+      if (!a.accumulate) put_zeros(a, col, v0 + r);
+      continue;
+    }
+    float e[C::kEach] = {};
+    for (uint32_t g = lo; g < hi; g += kWindow) {
+      float s[C::kEach] = {};
+      add_rows<DT, WIDE, kWindow>(a, col, s, g, min(g + kWindow, hi),
+                                  [&](uint32_t k) { return s_pos[k]; });
+#pragma unroll
+      for (uint32_t j = 0; j < C::kEach; ++j) e[j] += s[j];
+    }
+    put_row(a, col, v0 + r, e);
   }
 }
 
@@ -442,6 +541,21 @@ dim3 blocks_of(uint64_t n) { return dim3((uint32_t)(n < kMostBlocks ? n : kMostB
 template <uint32_t DT, bool WIDE>
 int launch_sums(const SumArgs& a, hipStream_t s) {
   const uint64_t tiles = (a.columns + Column<WIDE>::kWave - 1) / Column<WIDE>::kWave;
+  if (a.n <= kFew) {
+    const uint32_t blocks = (a.tokens.vocab + kFewRows - 1) / kFewRows;
+    const uint32_t tiles4 = (uint32_t)((tiles + kLanes / 64 - 1) / (kLanes / 64));
+    hipLaunchKernelGGL((few_kernel<DT, WIDE>), dim3(blocks, tiles4), dim3(kLanes), 0, s, a);
+    ARK_HIP(hipGetLastError());
+    return ARK_OPT_OK;
+  }
+  const dim3 groups((a.tokens.vocab + kGroup - 1) / kGroup);
+  if (a.n <= kSortLanes * kKept)
+    hipLaunchKernelGGL(sort_kernel<true>, groups, dim3(kSortLanes), 0, s, a.tokens, a.n,
+                       (uint32_t*)a.start, (uint32_t*)a.pos);
+  else
+    hipLaunchKernelGGL(sort_kernel<false>, groups, dim3(kSortLanes), 0, s, a.tokens, a.n,
+                       (uint32_t*)a.start, (uint32_t*)a.pos);
+  ARK_HIP(hipGetLastError());
   const uint64_t windows = a.n / kWindow * tiles;
   if (windows) {
     hipLaunchKernelGGL((window_kernel<DT, WIDE>), blocks_of((windows + 3) / 4), dim3(kLanes), 0,
@@ -562,14 +676,6 @@ int ark_embed_grad(const void* dy, uint64_t dy_stride, uint32_t dy_dtype, const 
   a.n = (uint32_t)n, a.columns = (uint32_t)columns;
   a.accumulate = flags & ARK_EMBED_ACCUMULATE ? 1u : 0u;
   a.scale = scale;
-  const dim3 groups((uint32_t)((vocab + kGroup - 1) / kGroup));
-  if (n <= kSortLanes * kKept)
-    hipLaunchKernelGGL(sort_kernel<true>, groups, dim3(kSortLanes), 0, s, a.tokens, a.n,
-                       (uint32_t*)a.start, (uint32_t*)a.pos);
-  else
-    hipLaunchKernelGGL(sort_kernel<false>, groups, dim3(kSortLanes), 0, s, a.tokens, a.n,
-                       (uint32_t*)a.start, (uint32_t*)a.pos);
-  ARK_HIP(hipGetLastError());
   if (dy_dtype == ARK_EMBED_F16) return launch_sums<ARK_EMBED_F16>(a, s);
   if (dy_dtype == ARK_EMBED_BF16) return launch_sums<ARK_EMBED_BF16>(a, s);
   return launch_sums<ARK_EMBED_F32>(a, s);

@@ -114,6 +114,34 @@ def test_gradient(n, v, d, kind, name):
     assert torch.equal(embed.lookup_grad(whole, tokens, v).double(), want)
 
 
+@pytest.mark.parametrize("kind", ["any", "text", "same"])
+@pytest.mark.parametrize("n,v,d", [(511, 1000, 1100), (512, 17, 3), (512, 33, 2053), (513, 17, 3),
+                                   (513, 33, 1029), (16384, 129, 8), (16385, 129, 8)])
+def test_gradient_on_both_sides_of_its_kernels_sizes(n, v, d, kind):
+    test_gradient(n, v, d, kind, "bf16")
+
+
+@pytest.mark.parametrize("n", [30, 600])
+def test_few_and_many_tokens_of_slices(n):
+    torch = _torch()
+    tokens = _tokens(n, 90, "text")
+    base = torch.randn((n, 61), device="cuda").half()
+    for off, d in ((3, 40), (1, 3), (60, 1)):
+        dy = base[:, off:off + d]
+        big = torch.full((90, 61), 7.0, device="cuda")
+        embed.lookup_grad(dy, tokens, 90, dw=big[:, off:off + d])
+        _check(big[:, off:off + d], dy, tokens, 90)
+        embed.lookup_grad(dy, tokens, 90, dw=big[:, off:off + d], accumulate=True)
+        assert (big[:, :off] == 7).all() and (big[:, off + d:] == 7).all()
+    clean = embed.lookup_grad(base, tokens, 90)
+    base[tokens == -1] = float("nan")
+    tokens[:n // 2] = 90
+    base[:n // 2] = float("nan")
+    got = embed.lookup_grad(base, tokens, 90)
+    assert torch.isfinite(got).all() and got.shape == clean.shape
+    _check(got, base, tokens, 90)
+
+
 def test_rows_without_a_token_are_not_read():
     torch = _torch()
     tokens = _tokens(500, 64, "text")
