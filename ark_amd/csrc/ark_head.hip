@@ -751,6 +751,15 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
   const uint32_t t = l.rows[row], top = l.targets.top;
   const float* stats = l.stats + (uint64_t)row * l.spans * 2;
   const float* z = l.z + (uint64_t)row * top;
+  // four rounds of the block's lanes on their way, the first four while the spans join
+  constexpr uint32_t kAhead = 4, kRound = kLanes * 8;
+  V v[kAhead];
+  const auto fetch = [&](uint32_t c) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t q = 0; q < kAhead; ++q)
+      if (c + q * kRound < to) v[q] = ld_nt<V>(e + c + q * kRound);
+  };
+  fetch(from + tid * 8);
   const float lse = join_spans<kLanes>(stats, l.spans, tid, red);
   if (tid < 64 && blockIdx.y == 0) {
     const float loss = row_loss(l.targets, t, z, lse, tid);
@@ -761,14 +770,19 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
     s_index[k] = l.targets.at(t, k);
     s_p[k] = l.targets.weight(t, k);
   }
-  for (uint32_t c = from + tid * 8; c < to; c += kLanes * 8) {
-    const float s = expf(stats[c / a.span * 2] - lse) * f;
-    const V v = ld_nt<V>(e + c);
-    u32x4 o;
+  for (uint32_t c0 = from + tid * 8; c0 < to; c0 += kAhead * kRound) {
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i)
-      o[i] = narrow2<DT>((float)v[2 * i] * s, (float)v[2 * i + 1] * s);
-    *(u32x4*)(e + c) = o;
+    for (uint32_t q = 0; q < kAhead; ++q) {
+      const uint32_t c = c0 + q * kRound;
+      if (c >= to) break;
+      const float s = expf(stats[c / a.span * 2] - lse) * f;
+      u32x4 o;
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i)
+        o[i] = narrow2<DT>((float)v[q][2 * i] * s, (float)v[q][2 * i + 1] * s);
+      *(u32x4*)(e + c) = o;
+    }
+    fetch(c0 + kAhead * kRound);
   }
   __syncthreads();
   // the targets' own entries, from fp32 (an index that comes twice writes the same
@@ -911,7 +925,16 @@ __device__ __forceinline__ void join(const float* partial, uint32_t parts, uint3
   for (; i < all; i += step) {
     const f32x4* p = (const f32x4*)partial + i;
     f32x4 v = p[0];
-    for (uint32_t s = 1; s < parts; ++s) v += p[s * all];
+    constexpr uint32_t kBatch = 4;  // on their way at once
+    for (uint32_t s = 1; s < parts; s += kBatch) {
+      f32x4 more[kBatch];
+#pragma unroll
+      for (uint32_t k = 0; k < kBatch; ++k)
+        if (s + k < parts) more[k] = p[(s + k) * all];
+#pragma unroll
+      for (uint32_t k = 0; k < kBatch; ++k)
+        if (s + k < parts) v += more[k];
+    }
     out.put((uint32_t)(i / per), (uint32_t)(i % per) * 4, v);
   }
 }
@@ -1122,7 +1145,11 @@ int launch_grad(const GradArgs& g, const Cut& cut, uint32_t rows, hipStream_t s)
   hipLaunchKernelGGL((grad_kernel<X, W>), dim3(blocks), dim3(X::kLanes), X::kLds, s, g);
   ARK_HIP(hipGetLastError());
   if ((g.dx.out.p && cut.dx_most > 1) || (g.dw.out.p && nw > cut.tiles_of(cut.vocab))) {
-    hipLaunchKernelGGL(join_kernel, dim3(2048), dim3(kLanes), 0, s, g);
+    const uint64_t rows_dx = g.dx.out.p ? rows : 0, rows_dw = g.dw.out.p ? cut.vocab : 0;
+    const uint64_t most = (rows_dx > rows_dw ? rows_dx : rows_dw) * ((g.dx.out.width + 3) / 4);
+    const uint64_t join_blocks = (most + kLanes - 1) / kLanes;
+    hipLaunchKernelGGL(join_kernel, dim3(join_blocks < 2048 ? (uint32_t)join_blocks : 2048u),
+                       dim3(kLanes), 0, s, g);
     ARK_HIP(hipGetLastError());
   }
   return ARK_OPT_OK;
