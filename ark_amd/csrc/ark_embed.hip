@@ -541,8 +541,8 @@ dim3 blocks_of(uint64_t n) { return dim3((uint32_t)(n < kMostBlocks ? n : kMostB
 template <uint32_t DT, bool WIDE>
 int launch_sums(const SumArgs& a, hipStream_t s) {
   const uint64_t tiles = (a.columns + Column<WIDE>::kWave - 1) / Column<WIDE>::kWave;
-  if (a.n <= kFew) {
-    const uint32_t blocks = (a.tokens.vocab + kFewRows - 1) / kFewRows;
+  const uint32_t blocks = (a.tokens.vocab + kFewRows - 1) / kFewRows;
+  if (a.n <= kFew && blocks <= kMostBlocks) {
     const uint32_t tiles4 = (uint32_t)((tiles + kLanes / 64 - 1) / (kLanes / 64));
     hipLaunchKernelGGL((few_kernel<DT, WIDE>), dim3(blocks, tiles4), dim3(kLanes), 0, s, a);
     ARK_HIP(hipGetLastError());
