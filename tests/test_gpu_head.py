@@ -615,3 +615,29 @@ def test_refusals():
             head.distill(x, w, index, logits)
         head.distill_grad(x, w, index, logits)
         t.requires_grad_(False)
+
+
+def test_threads_with_a_stream_each():
+    """Calls from several host threads at once, sizes of their own: the bits of calls
+    one after another."""
+    import threading
+    torch = _torch()
+    sets = [make(t, d, v, name) for t, d, v, name in ((300, 64, 700, "f16"), (40, 100, 900, "bf16"),
+                                                      (1100, 72, 300, "f16"))]
+    want = [head.cross_entropy_grad(*s, grad=2.0) for s in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = head.cross_entropy_grad(*sets[i], grad=2.0)
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
