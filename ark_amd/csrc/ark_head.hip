@@ -9,17 +9,19 @@
 //   gather_kernel   X, padded to whole steps of the products, and its targets; zeros
 //                   for the tokens without a loss
 //   logits_kernel   z = scale X W^T in tiles that stay in registers; z at targets in
-//                   fp32; of every row and span of the vocabulary its largest z and
-//                   its sum of exp(z - largest), and with gradients the exponentials
-//                   themselves, in 16 bits: 2^-9 or 2^-12 of each
+//                   fp32; of every row and span of the vocabulary a power of two 2^t
+//                   next to its largest exp(z) and its sum of exp(z) / 2^t, and with
+//                   gradients these exponentials themselves, in 16 bits: 2^-9 or
+//                   2^-12 of each
 //   loss_kernel     the spans' sums joined: log(sum exp z), the loss
 //   dz_kernel       the same, and the exponentials turned into dz where they lie
 //   grad_kernel     dx = dz W and dw = dz^T X, in one launch
 //   join_kernel     sums that were formed in parts
 //
 // The sums over spans make one pass over the vocabulary do: a span's exponentials
-// are relative to its own largest logit, as a row's is not known yet, and take the
-// row's scale when dz is formed.
+// are relative to its own largest, as a row's is not known yet, and take the row's
+// scale when dz is formed.  Powers of two, because a largest z times log2 e would be
+// rounded, the same way for all of a span, which a logit of 1000 shows in the loss.
 #include <math.h>
 
 #include <atomic>
@@ -36,7 +38,7 @@ using ark::fail;
 
 constexpr uint32_t kLanes = 256;
 constexpr uint32_t kRowPad = 256;   // rows of a piece are laid out for whole tiles
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr uint32_t kMaxPiece = 16384;  // tokens: what rank_kernel's block ranks
 constexpr uint32_t kFew = 1024;        // tokens that gather_kernel's blocks rank themselves
 
@@ -488,11 +490,11 @@ struct LogitsArgs {
   float scale;
   uint32_t tiles_m;
   const Meta* meta;
-  float* stats;  // [row][span] of (largest, sum)
+  float* stats;  // [row][span] of (t, sum of 2^(z log2 e - t)), t whole, next to the largest
   uint16_t* e;   // [row][e_stride], or NULL
   const uint32_t* entries;  // [row][entries_width(top)]
   uint32_t top;
-  float* z;                 // [row][top]: the logits there
+  float* z;                 // [row][top]: the products there, before scale
 };
 
 // z of a tile of the vocabulary (m) and of rows of X (n), never in memory.  A lane holds
@@ -567,7 +569,7 @@ __global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {
 #pragma unroll
       for (uint32_t i = 0; i < P::MF; ++i)
         *(f32x4*)(mine + lane % 16 * kZRow + ((i * 4 + lane / 16) ^ (lane % 16)) * 16) =
-            p.acc[i][j] * a.scale;
+            p.acc[i][j];
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       const auto z_at = [&](uint32_t row, uint32_t d) {
         return *(const float*)(mine + row * kZRow + ((d / 4) ^ row) * 16 + d % 4 * 4);
@@ -608,7 +610,9 @@ __global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {
       for (uint32_t k = 0; k < 4; ++k) most = fmaxf(most, p.acc[i][j][k]);
     most = fmaxf(most, __shfl_xor(most, 16));
     most = fmaxf(most, __shfl_xor(most, 32));
-    const float from = most == -INFINITY ? 0.0f : -most * to2;
+    // a whole power of two: no rounding of its own, which all of the span would share
+    const float top = most == -INFINITY ? most : rintf(most * to2);
+    const float from = most == -INFINITY ? 0.0f : -top;
     float sum = 0.0f;
 #pragma unroll
     for (uint32_t i = 0; i < P::MF; ++i)
@@ -622,7 +626,7 @@ __global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {
     sum += __shfl_xor(sum, 32);
     if (lane < 16 && t < live) {
       float* s = a.stats + ((uint64_t)t * a.spans + span) * 2;
-      s[0] = most * a.scale, s[1] = sum;
+      s[0] = top, s[1] = sum;
     }
     if (!a.e) continue;
     const uint32_t row = lane % 16;
@@ -645,19 +649,28 @@ __global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {
   }
 }
 
-// log of the sum of a row's exponentials, from its spans' (largest, sum), by `LANES`
-// lanes of a block (a wave or all of it; red: two values a wave).  One pass, eight
-// spans a lane on their way at once.
+// The sum of a row's exponentials.
+struct RowSum {
+  float top, log;  // log2 of it is top + log; top is whole, so that what is near it stays exact
+  // log2 of the probability at a product x . w
+  __device__ __forceinline__ float log2_q(float product, float to2) const {
+    return __builtin_fmaf(product, to2, -top) - log;
+  }
+};
+
+// It from its spans' (t, sum), by `LANES` lanes of a block (a wave or all of it; red: two
+// values a wave).  One pass, eight spans a lane on their way at once.  Spans' t are
+// whole, so that their sums join without rounding but the sum's own.
 template <uint32_t LANES>
-__device__ __forceinline__ float join_spans(const float* stats, uint32_t spans, uint32_t lane,
-                                            float* red) {
+__device__ __forceinline__ RowSum join_spans(const float* stats, uint32_t spans, uint32_t lane,
+                                             float* red) {
   typedef float V __attribute__((ext_vector_type(2)));
   constexpr uint32_t kEach = 8;
   float most = -INFINITY, sum = 0.0f;
   const auto join = [](float& m, float& s, float m2, float s2) {
     // a NaN among the sums stays; -inf on both sides has no distance
     const float top = fmaxf(m, m2);
-    s = s * (m == top ? 1.0f : expf(m - top)) + s2 * (m2 == top ? 1.0f : expf(m2 - top));
+    s = s * (m == top ? 1.0f : exp2f(m - top)) + s2 * (m2 == top ? 1.0f : exp2f(m2 - top));
     m = top;
   };
   for (uint32_t i0 = lane; i0 < spans; i0 += LANES * kEach) {
@@ -670,10 +683,10 @@ __device__ __forceinline__ float join_spans(const float* stats, uint32_t spans, 
     float m = most;
 #pragma unroll
     for (uint32_t k = 0; k < kEach; ++k) m = fmaxf(m, v[k].x);
-    sum *= most == m ? 1.0f : expf(most - m);
+    sum *= most == m ? 1.0f : exp2f(most - m);
     most = m;
 #pragma unroll
-    for (uint32_t k = 0; k < kEach; ++k) sum += v[k].y * (v[k].x == m ? 1.0f : expf(v[k].x - m));
+    for (uint32_t k = 0; k < kEach; ++k) sum += v[k].y * (v[k].x == m ? 1.0f : exp2f(v[k].x - m));
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) join(most, sum, __shfl_xor(most, o), __shfl_xor(sum, o));
@@ -683,18 +696,18 @@ __device__ __forceinline__ float join_spans(const float* stats, uint32_t spans, 
     most = red[0], sum = red[1];
     for (uint32_t w = 1; w < LANES / 64; ++w) join(most, sum, red[2 * w], red[2 * w + 1]);
   }
-  return most + logf(sum);
+  return {most, log2f(sum)};
 }
 
 // A token's loss: sum of p (log p - log q), by a wave.
-__device__ __forceinline__ float row_loss(const Targets& g, uint32_t t, const float* z, float lse,
-                                          uint32_t lane) {
+__device__ __forceinline__ float row_loss(const Targets& g, uint32_t t, const float* z,
+                                          const RowSum& sum, float to2, uint32_t lane) {
   float s = 0.0f;
   for (uint32_t k = lane; k < g.top; k += 64) {
     const float p = g.weight(t, k);
-    if (p != 0.0f) s += p * (lse - z[k]);
+    if (p != 0.0f) s -= p * sum.log2_q(z[k], to2);
   }
-  s = wave_sum(s);
+  s = wave_sum(s) * kLn2;
   return g.targets ? s : s + g.self[t];
 }
 
@@ -706,6 +719,7 @@ struct LossArgs {
   uint32_t spans;
   const float* z;
   float* loss;
+  float scale;
 };
 
 // The loss alone, a wave a row.  Latency: 4099 rows of 250 spans 6 us.
@@ -713,15 +727,16 @@ __global__ __launch_bounds__(kLanes) void loss_kernel(LossArgs a) {
   const uint32_t row = blockIdx.x * (kLanes / 64) + threadIdx.x / 64, lane = threadIdx.x % 64;
   if (row >= a.meta->live) return;
   const uint32_t t = a.rows[row];
-  const float lse = join_spans<64>(a.stats + (uint64_t)row * a.spans * 2, a.spans, lane, nullptr);
-  const float loss = row_loss(a.targets, t, a.z + (uint64_t)row * a.targets.top, lse, lane);
+  const RowSum sum = join_spans<64>(a.stats + (uint64_t)row * a.spans * 2, a.spans, lane, nullptr);
+  const float loss =
+      row_loss(a.targets, t, a.z + (uint64_t)row * a.targets.top, sum, a.scale * kLog2e, lane);
   if (lane == 0) a.loss[t] = loss;
 }
 
 struct DzArgs {
   LossArgs loss;
   const float* grads;  // or NULL
-  float grad, scale;
+  float grad;
   uint16_t* e;
   uint64_t e_stride;
   uint32_t written;  // columns that hold something
@@ -760,12 +775,13 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
       if (c + q * kRound < to) v[q] = ld_nt<V>(e + c + q * kRound);
   };
   fetch(from + tid * 8);
-  const float lse = join_spans<kLanes>(stats, l.spans, tid, red);
+  const RowSum sum = join_spans<kLanes>(stats, l.spans, tid, red);
+  const float to2 = l.scale * kLog2e;
   if (tid < 64 && blockIdx.y == 0) {
-    const float loss = row_loss(l.targets, t, z, lse, tid);
+    const float loss = row_loss(l.targets, t, z, sum, to2, tid);
     if (tid == 0) l.loss[t] = loss;
   }
-  const float f = (a.grads ? a.grads[t] : a.grad) * a.scale * l.meta->up;
+  const float f = (a.grads ? a.grads[t] : a.grad) * l.scale * l.meta->up;
   for (uint32_t k = tid; k < top; k += kLanes) {
     s_index[k] = l.targets.at(t, k);
     s_p[k] = l.targets.weight(t, k);
@@ -775,7 +791,7 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
     for (uint32_t q = 0; q < kAhead; ++q) {
       const uint32_t c = c0 + q * kRound;
       if (c >= to) break;
-      const float s = expf(stats[c / a.span * 2] - lse) * f;
+      const float s = exp2f((stats[c / a.span * 2] - sum.top) - sum.log) * f;
       u32x4 o;
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i)
@@ -793,7 +809,7 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
     float p = 0.0f;
     for (uint32_t i = 0; i < top; ++i) p += s_index[i] == v ? s_p[i] : 0.0f;
     // q - p without the difference of two numbers near 1
-    const float d = (expm1f(z[k] - lse) + (1.0f - p)) * f;
+    const float d = (expm1f(sum.log2_q(z[k], to2) * kLn2) + (1.0f - p)) * f;
     e[v] = (uint16_t)narrow2<DT>(d, 0.0f);
   }
 }
@@ -1243,7 +1259,7 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
   la.entries = ga.entries, la.top = top, la.z = z;
   int rc;
   if (tokens && (rc = launch_logits<L>(la, la.tiles_m * ((tokens + L::BN - 1) / L::BN), s))) return rc;
-  LossArgs lo = {g, rows, meta, la.stats, p.spans, z, ga.loss};
+  LossArgs lo = {g, rows, meta, la.stats, p.spans, z, ga.loss, c.scale};
   if (!c.with_grad) {  // with tokens, or run() ends before
     hipLaunchKernelGGL(loss_kernel, dim3((tokens + 3) / 4), dim3(kLanes), 0, s, lo);
     ARK_HIP(hipGetLastError());
@@ -1251,7 +1267,7 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
   }
   DzArgs da = {};
   da.loss = lo, da.grads = ra.grads;
-  da.grad = c.grad, da.scale = c.scale;
+  da.grad = c.grad;
   da.e = la.e, da.e_stride = p.e_stride, da.written = p.written, da.span = p.span;
   if (tokens) {
     // eight blocks for every compute unit, and two rounds of a block's lanes at least

@@ -29,9 +29,9 @@
  * The gradients of x and w are
  *     dx = dz w          in x's type
  *     dw (+)= dz^T x     in fp32, or in w's type (not added to)
- * dz is rounded to the 16 bits of x's type on the way, twice: relative to the
- * largest of its row in a piece of the vocabulary, and again, scaled by a power
- * of two so that the largest gradient has 2^14, when the row's sum is known.
+ * dz is rounded to the 16 bits of x's type on the way, twice: relative to a power
+ * of two next to the largest of its row in a piece of the vocabulary, and again,
+ * scaled so that the largest gradient has 2^14, when the row's sum is known.
  * Entries at targets are rounded once, from fp32.  A loss or gradient formed
  * from an inf or NaN is not finite, and the optimizer step then skips; other tokens'
  * losses and dx stay what they are.  Sums run

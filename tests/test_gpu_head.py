@@ -284,6 +284,42 @@ def test_far_logits(name):
     assert (dx[0] == 0).all() and (dx[4] == 0).all()
 
 
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("t,v", [(9, 300), (300, 2100)])
+def test_large_logits_close_together(t, v, name):
+    """Whole numbers, whose logits (about 1500) are exact: what is left are an
+    exponential's argument, of its distance r from the row's sum, by 2^-22, its value
+    by 2^-21, the sum of them and the logarithm, in all 2^-18 and 2^-21 of r."""
+    torch = _torch()
+    gen = torch.Generator(device="cuda").manual_seed(v)
+    base = torch.randint(-8, 9, (256,), generator=gen, device="cuda")
+    w = base.repeat(v, 1)
+    w.scatter_add_(1, torch.randint(0, 256, (v, 3), generator=gen, device="cuda"),
+                   torch.randint(-1, 2, (v, 3), generator=gen, device="cuda"))
+    x = base.repeat(t, 1)
+    x.scatter_add_(1, torch.randint(0, 256, (t, 3), generator=gen, device="cuda"),
+                   torch.randint(-1, 2, (t, 3), generator=gen, device="cuda"))
+    y = torch.randint(0, v, (t,), generator=gen, device="cuda")
+    z = (x.double() @ w.double().t()) * 0.25
+    y[::2] = z[::2].argmax(1)
+    x, w = x.to(_dt(name)), w.to(_dt(name))
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    want = (lse - z.gather(1, y[:, None]))[:, 0]
+    far = (torch.exp(z - lse) * (lse - z)).sum(1) + want
+    limit = 2.0 ** -18 + 2.0 ** -21 * far
+    loss, dx, dw = head.cross_entropy_grad(x, w, y, scale=0.25)
+    assert ((loss.double() - want).abs() <= limit).all()
+    assert torch.equal(head.cross_entropy(x, w, y, scale=0.25), loss)
+    ce(x, w, y, scale=0.25).check(loss, dx, dw)
+    index = torch.stack([y, (y + 1) % v, (y + 2) % v], 1)
+    logits = torch.tensor([1.0, 0.5, 0.0], device="cuda").repeat(t, 1)
+    p = torch.softmax(logits.double() / 4, 1)
+    want = (p * (p.log() - (z.gather(1, index) - lse))).sum(1)
+    far = far + (p * (lse - z.gather(1, index))).sum(1)
+    got = head.distill(x, w, index, logits, temperature=4.0)
+    assert ((got.double() - want).abs() <= 2.0 ** -17 + 2.0 ** -21 * far).all()
+
+
 def test_pieces():
     """More tokens than a piece, by tokens and by the vocabulary's size."""
     torch = _torch()
