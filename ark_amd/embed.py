@@ -46,9 +46,11 @@ def lookup(table, tokens, scale=1.0, dtype=None, out=None):
     vocab, columns = table.shape
     if out is None:
         out = table.new_empty((*tokens.shape, columns), dtype=dtype or table.dtype)
+        op, ostride = out.data_ptr(), columns
     elif out.shape[-1] != columns or out.device != table.device or dtype not in (None, out.dtype):
         raise ValueError(f"out is {tuple(out.shape)} {out.dtype} on {out.device}")
-    op, ostride = _flat(out, tokens.shape, "out")
+    else:
+        op, ostride = _flat(out, tokens.shape, "out")
     _queue(table, lib().ark_embed_lookup, tp, tstride, _code(table, "table"), vocab, columns, kp,
            size, n, scale, op, ostride, _code(out, "out"))
     return out
@@ -72,9 +74,11 @@ def lookup_grad(dy, tokens, vocab, scale=1.0, dw=None, accumulate=False):
         if accumulate:
             raise ValueError("accumulate needs a dw")
         dw = dy.new_empty((vocab, columns), dtype=torch.float32)
+        wp, wstride = dw.data_ptr(), columns
     elif tuple(dw.shape) != (vocab, columns) or dw.dtype != torch.float32 or dw.device != dy.device:
         raise ValueError(f"dw is {tuple(dw.shape)} {dw.dtype}, not {(vocab, columns)} float32")
-    wp, wstride = _rows(dw, "dw")
+    else:
+        wp, wstride = _rows(dw, "dw")
     need = _workspace(n, vocab, columns)
     ws = dy.new_empty(need, dtype=torch.uint8)
     _queue(dy, lib().ark_embed_grad, yp, ystride, _code(dy, "dy"), kp, size, n, vocab, columns,
