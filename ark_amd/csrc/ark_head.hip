@@ -818,31 +818,38 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
 struct Out {
   void* p;         // fp32 or 16 bits
   uint64_t stride;
-  uint32_t dtype, vec;      // vec: takes four values at a time
+  uint32_t dtype;
   const float* add;         // fp32 to add, of `add_stride`, or NULL
   uint64_t add_stride;
   const uint32_t* rows;     // row n goes to rows[n], or NULL
   uint32_t width, height;   // m and n that are stored
   const Meta* meta;
 
+  // Four values at any element's alignment.
   __device__ __forceinline__ void put(uint32_t n, uint32_t m, f32x4 v) const {
+    typedef float V4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef uint32_t V2 __attribute__((ext_vector_type(2), aligned(2)));
     v *= meta->down;
     const uint64_t row = rows ? rows[n] : n;
     const uint32_t c = min(width - m, 4u);
     if (add) {
       const float* q = add + row * add_stride + m;
+      if (c == 4) {
+        v += *(const ARK_GLOBAL V4*)q;
+      } else {
 #pragma unroll
-      for (uint32_t k = 0; k < 4; ++k)
-        if (k < c) v[k] += q[k];
+        for (uint32_t k = 0; k < 3; ++k)
+          if (k < c) v[k] += q[k];
+      }
     }
     if (dtype == ARK_HEAD_F32) {
       float* q = (float*)p + row * stride + m;
-      if (vec && c == 4) {
-        *(f32x4*)q = v;
+      if (c == 4) {
+        *(ARK_GLOBAL V4*)q = v;
         return;
       }
 #pragma unroll
-      for (uint32_t k = 0; k < 4; ++k)
+      for (uint32_t k = 0; k < 3; ++k)
         if (k < c) q[k] = v[k];
       return;
     }
@@ -850,12 +857,12 @@ struct Out {
                         ? u32x2{narrow2<ARK_ACT_F16>(v[0], v[1]), narrow2<ARK_ACT_F16>(v[2], v[3])}
                         : u32x2{narrow2<ARK_ACT_BF16>(v[0], v[1]), narrow2<ARK_ACT_BF16>(v[2], v[3])};
     uint16_t* q = (uint16_t*)p + row * stride + m;
-    if (vec && c == 4) {
-      *(u32x2*)q = h;
+    if (c == 4) {
+      *(ARK_GLOBAL V2*)q = h;
       return;
     }
 #pragma unroll
-    for (uint32_t k = 0; k < 4; ++k)
+    for (uint32_t k = 0; k < 3; ++k)
       if (k < c) q[k] = (uint16_t)(h[k / 2] >> (k % 2 * 16));
   }
 };
@@ -1295,7 +1302,6 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
     gr.dx.a = w, gr.dx.a_stride = w_stride, gr.dx.a_rows = (uint32_t)c.vocab;
     gr.dx.partial = (float*)(ws + p.dx_parts);
     o.p = ga.dx, o.stride = c.dx_stride, o.dtype = c.dtype, o.rows = rows, o.height = tokens;
-    o.vec = c.dx_stride % 4 == 0 && (uintptr_t)c.dx % 8 == 0;
   }
   if (c.dw) {
     Out& o = gr.dw.out;
@@ -1312,7 +1318,6 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
     o.p = final ? c.dw : (void*)sums;
     o.stride = final ? c.dw_stride : sums_stride;
     o.dtype = final ? c.dw_dtype : ARK_HEAD_F32;
-    o.vec = o.stride % 4 == 0 && (uintptr_t)o.p % 16 == 0;
   }
   return launch_grad<typename Size::template P<T, true, false>,
                      typename Size::template P<T, true, true>>(gr, p.cut, tokens, s);
