@@ -371,6 +371,17 @@ __device__ __forceinline__ u32x4 load8(const uint16_t* p, uint32_t n) {
   return u32x4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
 }
 
+__device__ __forceinline__ void zero8(uint16_t* p, uint32_t n) {
+  typedef uint32_t V __attribute__((ext_vector_type(4), aligned(2)));
+  if (n >= 8) {
+    *(ARK_GLOBAL V*)p = V{0, 0, 0, 0};
+    return;
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < 8; ++k)
+    if (k < n) p[k] = 0;
+}
+
 // W's rows padded to whole steps, where its own cannot be read 16 bytes at a time, a
 // wave a row.
 __device__ __forceinline__ void pad_rows(const GatherArgs& a) {
@@ -452,7 +463,8 @@ __global__ __launch_bounds__(kLanes) void gather_kernel(GatherArgs a) {
   if (row == ~0u) {
     if (lane == 0) a.loss[t] = 0.0f;
     if (a.dx)
-      for (uint32_t c = lane; c < a.columns; c += 64) a.dx[t * a.dx_stride + c] = 0;
+      for (uint32_t c = lane * 8; c < a.columns; c += 512)
+        zero8(a.dx + t * a.dx_stride + c, a.columns - c);
     return;
   }
   const uint16_t* src = a.x + t * a.x_stride;
@@ -746,28 +758,33 @@ struct DzArgs {
 
 // A row's exponentials to dz, by a block (or with few rows by several, each of which
 // joins the spans for itself); rows past the live ones, up to a whole step of the
-// products, to zeros.  Bound by HBM: 12288 rows of 32000, 1.57 GB, 278 us, 5.6 TB/s.
-template <typename T>
+// products, to zeros.  Bound by HBM: 12288 rows of 32000, 1.57 GB, 276 us, 5.7 TB/s.
+// LANES: a block's, or a wave's where a row is no more than a block's one round (6039
+// rows of 377: 10 us, 18 by blocks; 738 of 1936: 7.9 both ways).
+template <typename T, uint32_t LANES>
 __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
   typedef T V __attribute__((ext_vector_type(8)));
-  constexpr uint32_t DT = kTypeOf<T>;
+  constexpr uint32_t DT = kTypeOf<T>, kTeams = kLanes / LANES;
   __shared__ float red[kLanes / 64 * 2];
-  __shared__ uint32_t s_index[ARK_HEAD_MAX_TOP];
-  __shared__ float s_p[ARK_HEAD_MAX_TOP];
+  __shared__ uint32_t s_index_of[kTeams][ARK_HEAD_MAX_TOP];
+  __shared__ float s_p_of[kTeams][ARK_HEAD_MAX_TOP];
   const LossArgs& l = a.loss;
-  const uint32_t row = blockIdx.x, live = l.meta->live, tid = threadIdx.x;
+  const uint32_t team = threadIdx.x / LANES, tid = threadIdx.x % LANES;
+  const uint32_t row = blockIdx.x * kTeams + team, live = l.meta->live;
+  uint32_t* const s_index = s_index_of[team];
+  float* const s_p = s_p_of[team];
   if (row >= (live + kProductStep - 1) / kProductStep * kProductStep) return;
   uint16_t* e = a.e + row * a.e_stride;
   const uint32_t from = blockIdx.y * a.share, to = min(from + a.share, a.written);
   if (row >= live) {
-    for (uint32_t c = from + tid * 8; c < to; c += kLanes * 8) *(u32x4*)(e + c) = u32x4{0, 0, 0, 0};
+    for (uint32_t c = from + tid * 8; c < to; c += LANES * 8) *(u32x4*)(e + c) = u32x4{0, 0, 0, 0};
     return;
   }
   const uint32_t t = l.rows[row], top = l.targets.top;
   const float* stats = l.stats + (uint64_t)row * l.spans * 2;
   const float* z = l.z + (uint64_t)row * top;
-  // four rounds of the block's lanes on their way, the first four while the spans join
-  constexpr uint32_t kAhead = 4, kRound = kLanes * 8;
+  // four rounds of the lanes on their way, the first four while the spans join
+  constexpr uint32_t kAhead = 4, kRound = LANES * 8;
   V v[kAhead];
   const auto fetch = [&](uint32_t c) __attribute__((always_inline)) {
 #pragma unroll
@@ -775,14 +792,14 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
       if (c + q * kRound < to) v[q] = ld_nt<V>(e + c + q * kRound);
   };
   fetch(from + tid * 8);
-  const RowSum sum = join_spans<kLanes>(stats, l.spans, tid, red);
+  const RowSum sum = join_spans<LANES>(stats, l.spans, tid, red);
   const float to2 = l.scale * kLog2e;
   if (tid < 64 && blockIdx.y == 0) {
     const float loss = row_loss(l.targets, t, z, sum, to2, tid);
     if (tid == 0) l.loss[t] = loss;
   }
   const float f = (a.grads ? a.grads[t] : a.grad) * l.scale * l.meta->up;
-  for (uint32_t k = tid; k < top; k += kLanes) {
+  for (uint32_t k = tid; k < top; k += LANES) {
     s_index[k] = l.targets.at(t, k);
     s_p[k] = l.targets.weight(t, k);
   }
@@ -800,10 +817,13 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
     }
     fetch(c0 + kAhead * kRound);
   }
-  __syncthreads();
+  if constexpr (LANES > 64)
+    __syncthreads();
+  else
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
   // the targets' own entries, from fp32 (an index that comes twice writes the same
   // value twice)
-  for (uint32_t k = tid; k < top; k += kLanes) {
+  for (uint32_t k = tid; k < top; k += LANES) {
     const uint32_t v = s_index[k];
     if (v < from || v >= to) continue;  // another block's, or left out
     float p = 0.0f;
@@ -1282,9 +1302,14 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
     uint64_t parts = (2048 + rows32 - 1) / rows32, rounds = (p.written + round - 1) / round;
     if (parts > (rounds + 1) / 2) parts = (rounds + 1) / 2;
     da.share = (uint32_t)((rounds + parts - 1) / parts * round);
-    hipLaunchKernelGGL(dz_kernel<T>,
-                       dim3((uint32_t)rows32, (uint32_t)((p.written + da.share - 1) / da.share)),
-                       dim3(kLanes), 0, s, da);
+    if (rounds == 1)
+      hipLaunchKernelGGL((dz_kernel<T, 64>), dim3((uint32_t)(rows32 / (kLanes / 64))), dim3(kLanes),
+                         0, s, da);
+    else
+      hipLaunchKernelGGL(
+          (dz_kernel<T, kLanes>),
+          dim3((uint32_t)rows32, (uint32_t)((p.written + da.share - 1) / da.share)), dim3(kLanes),
+          0, s, da);
     ARK_HIP(hipGetLastError());
   }
   if (!c.dx && !c.dw) return ARK_OPT_OK;
