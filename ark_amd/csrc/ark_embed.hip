@@ -121,6 +121,7 @@ constexpr uint32_t kSortWaves = kSortLanes / 64;
 constexpr uint32_t kKept = 16;  // tokens a lane asks for at once
 constexpr uint32_t kWindow = 16;
 
+// n is 1 at least: lanes past it read the last token again.
 // KEEP: each lane has kKept tokens at most, which stay in registers for the second
 // time.  Bound by a block's latency: 16384 tokens into 250 groups 10.6 us, 16 without.
 template <bool KEEP>
@@ -475,6 +476,18 @@ __global__ __launch_bounds__(kLanes) void few_kernel(SumArgs a) {
   }
 }
 
+// The gradient of no tokens: every row zeros, with nothing to count or to read.
+template <bool WIDE>
+__global__ __launch_bounds__(kLanes) void zero_kernel(SumArgs a) {
+  typedef Column<WIDE> C;
+  const uint32_t tiles = (a.columns + C::kWave - 1) / C::kWave;
+  const uint64_t all = (uint64_t)a.tokens.vocab * tiles;
+  for (uint64_t id = (uint64_t)blockIdx.x * (kLanes / 64) +
+                     __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+       id < all; id += (uint64_t)gridDim.x * (kLanes / 64))
+    put_zeros(a, C((uint32_t)(id % tiles), a.columns), (uint32_t)(id / tiles));
+}
+
 // ---- host -------------------------------------------------------------------
 
 struct Layout {
@@ -541,6 +554,12 @@ dim3 blocks_of(uint64_t n) { return dim3((uint32_t)(n < kMostBlocks ? n : kMostB
 template <uint32_t DT, bool WIDE>
 int launch_sums(const SumArgs& a, hipStream_t s) {
   const uint64_t tiles = (a.columns + Column<WIDE>::kWave - 1) / Column<WIDE>::kWave;
+  if (a.n == 0) {
+    hipLaunchKernelGGL(zero_kernel<WIDE>, blocks_of((a.tokens.vocab * tiles + 3) / 4),
+                       dim3(kLanes), 0, s, a);
+    ARK_HIP(hipGetLastError());
+    return ARK_OPT_OK;
+  }
   const uint32_t blocks = (a.tokens.vocab + kFewRows - 1) / kFewRows;
   if (a.n <= kFew && blocks <= kMostBlocks) {
     const uint32_t tiles4 = (uint32_t)((tiles + kLanes / 64 - 1) / (kLanes / 64));

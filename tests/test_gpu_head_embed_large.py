@@ -117,3 +117,17 @@ def test_the_largest_table(n):
     dw = embed.lookup_grad(dy, tokens, v)
     assert dw[v - 1] >= 1 and dw[0] >= 1 and dw.sum(dtype=torch.float64) == n - 1
     assert torch.equal(embed.lookup(dw, tokens)[:2], dw[tokens[:2]])
+
+
+@pytest.mark.parametrize("d", [1, 5])
+@pytest.mark.parametrize("v", [7, (1 << 27) + 1, 1 << 28])
+def test_no_tokens_and_the_largest_table(v, d):
+    """An empty batch's gradient is zeros, in tables whose few tokens are sorted too."""
+    torch = _torch()
+    none = torch.empty(0, dtype=torch.long, device="cuda")
+    dw = torch.full((v, d + 1), 7.0, device="cuda")
+    embed.lookup_grad(torch.empty((0, d), device="cuda"), none, v, dw=dw[:, :d])
+    assert not dw[:, :d].any() and (dw[:, d] == 7).all()
+    dw.fill_(1.0)
+    embed.lookup_grad(torch.empty((0, d), device="cuda"), none, v, dw=dw[:, :d], accumulate=True)
+    assert (dw == 1).all()
