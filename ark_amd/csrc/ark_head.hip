@@ -47,7 +47,8 @@ struct Meta {
   uint32_t live;                  // rows with a loss
   uint32_t dx_parts, dw_parts;    // that the products' sums are cut into
   uint32_t dw_first;              // dw's blocks are the longer ones
-  float up, down;                 // dz is formed times up, a power of two, and taken down after
+  int32_t shift;                  // dz is formed times 2^shift
+  float down;                     // 2^-shift, for the products
 };
 
 // How both products' work is cut, decided where the number of live rows is known:
@@ -248,15 +249,27 @@ struct RankArgs {
   Cut cut;
 };
 
+// grad * scale as part 2^e: the product itself may lie outside fp32's range on either
+// side and still be one that dz, times 2^shift, holds.
+struct GradScale {
+  float part;  // of finite ones 0 or 1/4 to 1 in magnitude
+  int e;
+};
+__device__ __forceinline__ GradScale grad_scale(float grad, float scale) {
+  int eg = 0, es = 0;
+  const float g = frexpf(grad, &eg), s = frexpf(scale, &es);
+  return {g * s, g - g == 0.0f ? eg + es : 0};
+}
+
 // By one wave, with the number of live tokens and the largest |grad| over them.
 __device__ __forceinline__ void write_meta(const RankArgs& a, uint32_t live, float largest) {
-  Meta m = {live, 1, 1, 0, 1.0f, 1.0f};
+  Meta m = {live, 1, 1, 0, 0, 1.0f};
   if (a.with_grad) {
-    // the largest |grad * scale| times `up` lies in [2^13, 2^14)
-    largest *= fabsf(a.scale);
-    if (largest > 0.0f && largest < INFINITY) {
-      const int shift = min(max(13 - ilogbf(largest), -126), 126);
-      m.up = ldexpf(1.0f, shift), m.down = ldexpf(1.0f, -shift);
+    // the largest |grad * scale| times 2^shift lies in [2^13, 2^14)
+    if (largest > 0.0f && largest * a.scale < INFINITY) {
+      const GradScale g = grad_scale(largest, a.scale);
+      m.shift = min(max(14 - g.e + (g.part < 0.5f ? 1 : 0), -126), 126);
+      m.down = ldexpf(1.0f, -m.shift);
     }
     // the cheapest of the 64 candidates, a lane each
     const Cut::Parts mine = Cut::candidate(threadIdx.x % 64);
@@ -272,11 +285,11 @@ __device__ __forceinline__ void write_meta(const RankArgs& a, uint32_t live, flo
   if (threadIdx.x % 64 == 0) *a.meta = m;
 }
 
-// |grad| as a whole number; of an inf or NaN 0: its own token's gradients are not
-// finite at any scale, and the others keep theirs.
+// |grad| as a whole number; 0 where it or its product with scale is not finite: its own
+// token's gradients are not finite at any scale, and the others keep theirs.
 __device__ __forceinline__ uint32_t grad_size(const RankArgs& a, uint32_t t) {
-  const uint32_t g = __float_as_uint(a.grads[t]) & 0x7FFFFFFFu;
-  return g < 0x7F800000u ? g : 0u;
+  const float g = fabsf(a.grads[t]);
+  return g * a.scale < INFINITY ? __float_as_uint(g) : 0u;
 }
 __device__ __forceinline__ uint32_t wave_max_bits(uint32_t g) {
 #pragma unroll
@@ -798,7 +811,8 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
     const float loss = row_loss(l.targets, t, z, sum, to2, tid);
     if (tid == 0) l.loss[t] = loss;
   }
-  const float f = (a.grads ? a.grads[t] : a.grad) * l.scale * l.meta->up;
+  const GradScale gs = grad_scale(a.grads ? a.grads[t] : a.grad, l.scale);
+  const float f = ldexpf(gs.part, gs.e + l.meta->shift);
   for (uint32_t k = tid; k < top; k += LANES) {
     s_index[k] = l.targets.at(t, k);
     s_p[k] = l.targets.weight(t, k);

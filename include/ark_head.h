@@ -34,7 +34,8 @@
  * scaled so that the largest gradient has 2^14, when the row's sum is known.
  * Entries at targets are rounded once, from fp32.  A loss or gradient formed
  * from an inf or NaN is not finite, and the optimizer step then skips; other tokens'
- * losses and dx stay what they are.  Sums run
+ * losses and dx stay what they are.  (A token whose grad * scale is past fp32's range
+ * does not count for the largest gradient either.)  Sums run
  * in an order that depends on the sizes and on which tokens have a loss: equal
  * calls give equal bits.
  *

@@ -677,3 +677,42 @@ def test_threads_with_a_stream_each():
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("t", [70, 1500])
+@pytest.mark.parametrize("grad,scale", [(3e38, 2.0), (2.0 ** 127, 4.0)])
+def test_a_token_whose_gradient_passes_fp32_leaves_the_others(grad, scale, t):
+    """|grad| is finite and |grad * scale| is not: as an infinite one."""
+    torch = _torch()
+    x, w, y = make(t, 32, 90, "f16", masked=0.0)
+    x = x / scale  # the logits as they were
+    for others in (1e-4, 3e-9):
+        g = torch.full((t,), others, device="cuda")
+        g[t // 2] = grad
+        loss, dx, _ = head.cross_entropy_grad(x, w, y, grad=g, scale=scale)
+        assert not torch.isfinite(dx[t // 2]).any()
+        g[t // 2], dx[t // 2] = 0.0, 0.0
+        ce(x, w, y, scale=scale, g=g).check(loss, dx, None)
+        index, logits = y[:, None], torch.zeros((t, 1), device="cuda")
+        g[t // 2] = grad
+        loss, dx, _ = head.distill_grad(x, w, index, logits, grad=g, temperature=1.0 / scale)
+        assert not torch.isfinite(dx[t // 2]).any()
+        g[t // 2], dx[t // 2] = 0.0, 0.0
+        ce(x, w, y, scale=scale, g=g).check(loss, dx, None)
+
+
+@pytest.mark.parametrize("t", [70, 1500])
+def test_a_gradient_whose_product_with_scale_is_below_fp32(t):
+    """grad * scale is 5.2 of the smallest fp32, or none of it, and dw, its product
+    with large rows of x, is an ordinary number."""
+    torch = _torch()
+    x, w, y = make(t, 32, 90, "bf16")
+    scale = 2.0 ** -43
+    x, w = x * 2.0 ** 66, w * 2.0 ** -23
+    for grad in (1.3 * 2.0 ** -104, 1.3 * 2.0 ** -109):
+        g = torch.full((t,), grad, device="cuda")
+        want = ce(x, w, y, scale=scale, g=g)
+        for one in (grad, g):
+            got = head.cross_entropy_grad(x, w, y, grad=one, scale=scale,
+                                          dw=torch.empty((90, 32), device="cuda"))
+            want.check(*got)
