@@ -205,7 +205,7 @@ __global__ __launch_bounds__(kLanes) void teacher_kernel(
     id[i] = ~0u, a[i] = -INFINITY;
     if (k < top) {
       const int64_t v = ld_int(index, index_bytes, t * index_stride + k);
-      const float l = ld_float(logits, dtype, t * logits_stride + k) * scale;
+      const float l = ld_float(logits, dtype, t * logits_stride + k);
       if (v >= 0 && v < (int64_t)vocab && l != -INFINITY) id[i] = (uint32_t)v, a[i] = l;
     }
     most = fmaxf(most, a[i]);
@@ -215,7 +215,8 @@ __global__ __launch_bounds__(kLanes) void teacher_kernel(
   bool any = false;
 #pragma unroll
   for (uint32_t i = 0; i < kEach; ++i)
-    if (id[i] != ~0u) a[i] -= most, sum += expf(a[i]), any = true;
+    // the difference before the scale, with which a logit alone may pass fp32
+    if (id[i] != ~0u) a[i] = (a[i] - most) * scale, sum += expf(a[i]), any = true;
   sum = wave_sum(sum);
   const float log_sum = logf(sum);
   float own = 0.0f;

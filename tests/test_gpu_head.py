@@ -716,3 +716,20 @@ def test_a_gradient_whose_product_with_scale_is_below_fp32(t):
             got = head.cross_entropy_grad(x, w, y, grad=one, scale=scale,
                                           dw=torch.empty((90, 32), device="cuda"))
             want.check(*got)
+
+
+@pytest.mark.parametrize("name", TYPES)
+def test_distill_from_logits_that_pass_fp32_over_the_temperature(name):
+    """p is a softmax of differences: logits whose quotient is not finite still have
+    one, and those below the largest by as much have a p of 0."""
+    torch = _torch()
+    x, w, _ = make(6, 32, 90, name)
+    x[:] = 0  # student's logits of 0
+    index = torch.tensor([[3, 80, 5]], device="cuda").repeat(6, 1)
+    logits = torch.tensor([[100.0, 50.0, -100.0], [-100.0, -50.0, -200.0], [100.0, 100.0, 0.0],
+                           [-100.0, -100.0, -100.0], [3e38, -3e38, 0.0], [-1e3, -1e3, -1e4]],
+                          device="cuda")
+    tau = 1e-37
+    got = head.distill_grad(x, w, index, logits, grad=tau, temperature=tau)
+    kl(x, w, index, logits, tau, tau).check(*got)
+    assert torch.equal(head.distill(x, w, index, logits, temperature=tau), got[0])
