@@ -25,20 +25,27 @@ def _tokens(tokens, device):
     size = _INTEGERS.get(tokens.dtype)
     if size is None or tokens.device != device or not tokens.is_contiguous():
         raise ValueError(f"tokens must be contiguous int32 or int64 on {device}, not "
-                         f"{tokens.dtype} on {tokens.device}")
+                         f"{tokens.dtype} on {tokens.device} of strides {tokens.stride()}")
     return tokens.data_ptr(), size, tokens.numel()
 
 
 def _flat(t, shape, what):
     """t, of ``shape`` and one more dimension, as (address, stride) of its rows."""
-    if t.shape[:-1] != shape:
+    if not t.dim() or t.shape[:-1] != shape:
         raise ValueError(f"{what} is {tuple(t.shape)}, the tokens {tuple(shape)}")
-    return _rows(t.view(-1, t.shape[-1]) if t.dim() != 2 else t, what)
+    if t.dim() != 2:
+        try:
+            t = t.view(shape.numel(), t.shape[-1])
+        except RuntimeError:
+            raise ValueError(f"{what}: rows of {tuple(t.shape)} at strides {t.stride()} are not one "
+                             "stride apart: pass a contiguous copy") from None
+    return _rows(t, what)
 
 
 def lookup(table, tokens, scale=1.0, dtype=None, out=None):
-    """scale * table[tokens], tokens of any shape: (*tokens.shape, columns) of the
-    table's type or ``dtype``, in ``out`` or a new tensor."""
+    """scale * table[tokens], contiguous tokens of any shape: (*tokens.shape, columns)
+    of the table's type or ``dtype``, in ``out`` (its rows one stride apart) or a new
+    tensor."""
     if table.requires_grad:
         _no_graph("lookup")
     tp, tstride = _rows(table, "table")
@@ -47,7 +54,8 @@ def lookup(table, tokens, scale=1.0, dtype=None, out=None):
     if out is None:
         out = table.new_empty((*tokens.shape, columns), dtype=dtype or table.dtype)
         op, ostride = out.data_ptr(), columns
-    elif out.shape[-1] != columns or out.device != table.device or dtype not in (None, out.dtype):
+    elif (out.shape[-1:] != (columns,) or out.device != table.device
+          or dtype not in (None, out.dtype)):
         raise ValueError(f"out is {tuple(out.shape)} {out.dtype} on {out.device}")
     else:
         op, ostride = _flat(out, tokens.shape, "out")
@@ -65,8 +73,9 @@ def _workspace(n, vocab, columns):
 
 def lookup_grad(dy, tokens, vocab, scale=1.0, dw=None, accumulate=False):
     """dw (+)= scale * the sums of dy's rows (*tokens.shape, columns) by token:
-    float32 (vocab, columns), rows of any stride; a new tensor when None.  Rows of
-    tokens that do not occur become zeros, or stay with ``accumulate``."""
+    float32 (vocab, columns), rows of any stride; a new tensor when None.  (dy's rows
+    are one stride apart, whatever the tokens' shape.)  Rows of tokens that do not
+    occur become zeros, or stay with ``accumulate``."""
     kp, size, n = _tokens(tokens, dy.device)
     yp, ystride = _flat(dy, tokens.shape, "dy")
     columns = dy.shape[-1]

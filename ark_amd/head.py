@@ -57,7 +57,9 @@ def _targets(targets, x):
     size = _INTEGERS.get(targets.dtype)
     if (size is None or targets.device != x.device or targets.numel() != x.shape[0]
             or not targets.is_contiguous()):
-        raise ValueError(f"targets must be {x.shape[0]} contiguous int32 or int64 on {x.device}")
+        raise ValueError(f"targets must be {x.shape[0]} contiguous int32 or int64 on {x.device}, not "
+                         f"{tuple(targets.shape)} {targets.dtype} on {targets.device} of strides "
+                         f"{targets.stride()}")
     return targets.data_ptr(), size
 
 

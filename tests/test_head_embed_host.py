@@ -135,3 +135,30 @@ def test_what_would_lose_a_graph_is_refused(gpus):
 def test_an_ignored_target_is_an_int32(gpus, ignore):
     with pytest.raises(ValueError, match="int32"):
         head.cross_entropy(Fake((5, 8)), Fake((7, 8)), Fake((5,), torch.int64), ignore=ignore)
+
+
+def test_rows_and_tokens_of_no_one_stride_are_refused_by_name():
+    """Slices that users take (a sequence without its last token) are no matrix of
+    rows, and no list: a refusal of the module's own says so."""
+    text, rows = torch.zeros((3, 9), dtype=torch.int64), torch.zeros((3, 9, 8))
+    table = torch.zeros((7, 8))
+    with pytest.raises(ValueError, match="tokens.*contiguous.*strides"):
+        embed.lookup(Table(table), text[:, :-1])
+    with pytest.raises(ValueError, match="dy.*contiguous"):
+        embed.lookup_grad(rows[:, :-1], text[:, :-1].contiguous(), 7)
+    with pytest.raises(ValueError, match="out.*contiguous"):
+        embed.lookup(Table(table), text[:, :-1].contiguous(), out=rows[:, :-1])
+    for call in (lambda: embed.lookup_grad(torch.zeros(()), text[0, 0], 7),
+                 lambda: embed.lookup(Table(table), text[0, 0], out=torch.zeros(()))):
+        with pytest.raises(ValueError, match="dy is|out is"):
+            call()
+    with pytest.raises(ValueError, match="targets.*contiguous"):
+        head.cross_entropy(Fake((24, 8)), Fake((7, 8)), text[:, :-1])
+
+
+class Table(Fake):
+    """A table beside host tensors, for what is refused before a call."""
+
+    def __init__(self, like):
+        super().__init__(like.shape, like.dtype)
+        self.device = like.device
