@@ -1007,7 +1007,7 @@ __global__ __launch_bounds__(kLanes) void join_kernel(GradArgs g) {
 
 // ---- host -------------------------------------------------------------------
 
-constexpr uint64_t kDzBytes = 1ull << 30;  // of a piece's dz, at most
+constexpr uint64_t kPieceBytes = 1ull << 30;  // of a piece's dz, or of its spans' sums, at most
 
 struct Big {
   template <typename T, bool AMC, bool BMC>
@@ -1085,8 +1085,10 @@ Plan plan_of(const void* w, uint64_t w_stride, uint64_t tokens, uint64_t columns
   p.e_stride = up(vocab, 256);
   p.padded = (uint32_t)up(columns, kProductStep);
   p.copy_w = columns % kProductStep || w_stride % 8 || (uintptr_t)w % 16;
-  // pieces of equal sizes, whole tiles
-  uint64_t most = grad ? kDzBytes / (p.e_stride * 2) / kRowPad * kRowPad : kMaxPiece;
+  // pieces of equal sizes, whole tiles, bounded by what a token's row takes: dz, or for the
+  // loss alone its spans' sums (of the narrower spans)
+  const uint64_t row = grad ? p.e_stride * 2 : p.e_stride / 64 * 8;
+  uint64_t most = kPieceBytes / row / kRowPad * kRowPad;
   if (most < kRowPad) most = kRowPad;
   if (most > kMaxPiece) most = kMaxPiece;
   p.pieces = (uint32_t)((tokens + most - 1) / most);

@@ -1,7 +1,8 @@
 /*
  * ark_head.h -- the loss over a vocabulary from a model's last hidden rows and
- * its output layer, and the gradients of both, on MI355X (gfx950), without the
- * logits in memory.  The reference forms the logits with a tied 1x1 convolution
+ * its output layer, and the gradients of both, on MI355X (gfx950).  The logits
+ * are never in memory; the gradients' dz, of their size in 16 bits, is, in pieces.
+ * The reference forms the logits with a tied 1x1 convolution
  * (proyecto_ark/ark01/objc/bridge.m:414-503) and its cross entropy on the CPU
  * (:954-976); these are this library's own definitions.
  *
@@ -39,9 +40,10 @@
  * in an order that depends on the sizes and on which tokens have a loss: equal
  * calls give equal bits.
  *
- * A call works through the tokens in pieces, whose 16-bit dz (at most 1 GiB) and
- * copied rows lie in the caller's workspace (ark_head_workspace), in use until the
- * call's work ends.  Tokens without a loss cost no products.
+ * A call works through the tokens in pieces, whose copied rows and 16-bit dz (of the
+ * logits' size, at most 1 GiB; for the loss alone sums of 64 or 128 logits each, at most
+ * 1 GiB) lie in the caller's workspace (ark_head_workspace), in use until the call's
+ * work ends.  Tokens without a loss cost no products.
  *
  * Every function is stream ordered and returns an ARK_OPT_* status code
  * (include/ark_opt.h), with the message in ark_opt_last_error().  Pointers are

@@ -733,3 +733,14 @@ def test_distill_from_logits_that_pass_fp32_over_the_temperature(name):
     got = head.distill_grad(x, w, index, logits, grad=tau, temperature=tau)
     kl(x, w, index, logits, tau, tau).check(*got)
     assert torch.equal(head.distill(x, w, index, logits, temperature=tau), got[0])
+
+
+def test_pieces_of_the_loss_alone_of_a_large_vocabulary():
+    """4200 tokens over 2^21 are two pieces: rows of both against 64 bits."""
+    torch = _torch()
+    x, w, y = make(4200, 8, 1 << 21, "f16")
+    loss = head.cross_entropy(x, w, y)
+    assert torch.isfinite(loss).all()
+    for lo in (0, 2070, 4180):
+        part = slice(lo, lo + 20)
+        ce(x[part], w, y[part]).check(loss[part], None, None)

@@ -144,3 +144,10 @@ def test_the_largest_table():
     L = _lib.lib()
     assert L.ark_embed_grad_workspace(5, 1 << 28, 1, C.byref(out)) == _abi.OK and out.value > 1 << 30
     assert L.ark_embed_grad_workspace(5, (1 << 28) + 1, 1, C.byref(out)) == _abi.EINVAL
+
+
+@pytest.mark.parametrize("tokens", [16384, 1 << 20])
+def test_workspace_of_the_loss_alone_of_a_large_vocabulary(tokens):
+    """The spans' sums of a piece are bounded as dz is, whatever the vocabulary."""
+    for vocab in (1 << 19, 1 << 20, (1 << 21) - 5, 1 << 21):
+        assert _need(tokens, 64, vocab, grad=0)[1] < 1.1 * 2 ** 30
