@@ -1,11 +1,9 @@
 // launches.cpp -- the kernels that a call would launch, without a GPU: a library that
 // is loaded before libark_opt.so and stands in for the parts of the runtime that its
 // entry points use.  Every address is device memory, nothing runs, and a launch is a
-// line of text: the kernel's name and grid.  (tests/launches.py)
-#include <cxxabi.h>
+// line of text: grid, block and the kernel's (mangled) name.  (tests/launches.py)
 #include <hip/hip_runtime_api.h>
 
-#include <cstdlib>
 #include <map>
 #include <string>
 
@@ -19,10 +17,7 @@ const char* launches_lines() { return lines.c_str(); }
 
 void __hipRegisterFunction(void**, const void* host, char*, const char* name, unsigned, void*,
                            void*, void*, void*, int*) {
-  int rc = 0;
-  char* plain = abi::__cxa_demangle(name, nullptr, nullptr, &rc);
-  names[host] = plain ? plain : name;
-  std::free(plain);
+  names[host] = name;
 }
 
 // what <<<grid, block>>> hands to the kernel's stub

@@ -28,6 +28,13 @@ TYPES = ["f16", "bf16"]
 SIZES = [(1, 1, 1), (1, 64, 300), (3, 8, 5), (64, 64, 256), (65, 96, 257), (63, 129, 1000),
          (257, 72, 513), (300, 100, 33), (130, 256, 2049), (513, 65, 640), (16, 1030, 70)]
 
+# whose logits and gradients are of the large tiles (checked without a GPU): rows of
+# several tiles, a last one of few rows and of few columns, and steps that go through
+# their buffers several times
+LARGE = [(517, 768, 32308), (1100, 800, 20011), (1290, 160, 32001)]
+LARGE_LOGITS = [(745, 134, 9082)]  # of the logits alone
+LARGE_GRADS = [(259, 644, 15187)]  # of the gradients alone
+
 
 def _torch():
     import torch
@@ -744,3 +751,60 @@ def test_pieces_of_the_loss_alone_of_a_large_vocabulary():
     for lo in (0, 2070, 4180):
         part = slice(lo, lo + 20)
         ce(x[part], w, y[part]).check(loss[part], None, None)
+
+
+# ---- large tiles --------------------------------------------------------------------
+
+def _scattered(y, seed):
+    """y with a third masked: some here and there, and whole stretches."""
+    torch = _torch()
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    y = torch.where(torch.rand(y.shape, generator=gen, device="cuda") < 0.2, -100, y)
+    y[100:180] = y[255:258] = -100
+    return y
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("t,d,v", LARGE + LARGE_LOGITS + LARGE_GRADS)
+def test_large_tiles(t, d, v, name):
+    torch = _torch()
+    x, w, y = make(t, d, v, name)
+    y = _scattered(y, t)
+    y[::50], y[1::50] = v - 1, 0  # the last, ragged span, and the first
+    live = (y >= 0) & (y < v)
+    x[~live] = float("nan")
+    g = torch.rand(t, device="cuda")
+    want = ce(x, w, y, g=g)
+    want.check(head.cross_entropy(x, w, y), None, None)
+    first = head.cross_entropy_grad(x, w, y, grad=g)
+    want.check(*first)
+    assert (first[1][~live] == 0).all() and (first[0][~live] == 0).all()
+    before = torch.randn((v, d), device="cuda")
+    dw = before.clone()
+    loss, dx, _ = head.cross_entropy_grad(x, w, y, grad=g, dw=dw, accumulate=True)
+    assert torch.equal(loss, first[0]) and torch.equal(dx, first[1])
+    off = (dw.double() - before.double() - want.dw).abs()
+    assert (off <= want.b_dw + 2.0 ** -23 * (before.abs().double() + want.dw.abs())).all()
+    again = head.cross_entropy_grad(x, w, y, grad=g)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("t,d,v", LARGE + LARGE_LOGITS + LARGE_GRADS)
+@pytest.mark.parametrize("k", [1, 8, 65, 130, 256])
+def test_distill_of_large_tiles(k, t, d, v, name):
+    torch = _torch()
+    x, w, _ = make(t, d, v, name)
+    index, logits = teacher(t, v, k)
+    index[100:180] = -1
+    index[200:210, 0] = v - 1
+    logits[200:210, 0] = 3.0
+    index[210:230] = torch.arange(k, device="cuda") + 120  # neighbours, over spans' ends
+    logits[210:230] = torch.randn((20, k), device="cuda")
+    g = torch.rand(t, device="cuda")
+    want = kl(x, w, index, logits, 2.0, g)
+    want.check(head.distill(x, w, index, logits, 2.0), None, None)
+    first = head.distill_grad(x, w, index, logits, grad=g, temperature=2.0)
+    want.check(*first)
+    again = head.distill_grad(x, w, index, logits, grad=g, temperature=2.0)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
