@@ -54,10 +54,29 @@ struct Tokens {
   const void* p;
   uint32_t bytes, vocab;
   // ~0: no row
-  __device__ __forceinline__ uint32_t at(uint64_t t) const {
-    const int64_t v = bytes == 8 ? ld_g<int64_t>((const int64_t*)p + t)
-                                 : ld_g<int32_t>((const int32_t*)p + t);
+  __device__ __forceinline__ uint32_t row(int64_t v) const {
     return v >= 0 && v < (int64_t)vocab ? (uint32_t)v : ~0u;
+  }
+  __device__ __forceinline__ uint32_t at(uint64_t t) const {
+    return row(bytes == 8 ? ld_g<int64_t>((const int64_t*)p + t)
+                          : ld_g<int32_t>((const int32_t*)p + t));
+  }
+  // Those at t, t + 64, ..., past `last` the last one's; their loads all together, which
+  // a branch on the size for each would keep apart.
+  template <uint32_t N>
+  __device__ __forceinline__ void each(uint32_t t, uint32_t last, uint32_t (&out)[N]) const {
+    const auto load = [&](auto kind) __attribute__((always_inline)) {
+      typedef decltype(kind) T;
+      T v[N];
+#pragma unroll
+      for (uint32_t k = 0; k < N; ++k) v[k] = ld_g<T>((const T*)p + min(t + k * 64, last));
+#pragma unroll
+      for (uint32_t k = 0; k < N; ++k) out[k] = row(v[k]);
+    };
+    if (bytes == 8)
+      load(int64_t());
+    else
+      load(int32_t());
   }
 };
 
@@ -137,12 +156,10 @@ __global__ __launch_bounds__(kSortLanes) void sort_kernel(Tokens tokens, uint32_
   for (uint32_t i = lane; i < kGroup; i += 64) s_at[wave][i] = 0;
   uint32_t below = 0, v[kKept];
   const auto ask = [&](uint32_t t0) __attribute__((always_inline)) {
+    tokens.each<kKept>(t0 + lane, n - 1, v);
 #pragma unroll
-    for (uint32_t k = 0; k < kKept; ++k) {
-      const uint32_t t = t0 + k * 64 + lane;
-      v[k] = tokens.at(min(t, n - 1));
-      if (t >= hi) v[k] = ~0u;
-    }
+    for (uint32_t k = 0; k < kKept; ++k)
+      if (t0 + k * 64 + lane >= hi) v[k] = ~0u;
   };
   if (KEEP) ask(lo);
   for (uint32_t t0 = lo; t0 < hi; t0 += 64 * kKept) {

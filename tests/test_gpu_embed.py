@@ -257,3 +257,16 @@ def test_refusals():
         embed.lookup(table, tokens)
     with torch.no_grad():
         embed.lookup(table, tokens)
+
+
+@pytest.mark.parametrize("n,v", [(40, 300), (700, 300), (16384, 1000), (20000, 1000)])
+def test_tokens_of_32_and_64_bits_give_equal_bits(n, v):
+    torch = _torch()
+    tokens = _tokens(n, v, "any")
+    tokens[::9] = -2 ** 31  # a 32-bit token's sign is its own
+    dy = torch.randn((n, 40), device="cuda").half()
+    table = torch.randn((v, 40), device="cuda")
+    assert torch.equal(embed.lookup_grad(dy, tokens.int(), v), embed.lookup_grad(dy, tokens, v))
+    assert torch.equal(embed.lookup(table, tokens.int()), embed.lookup(table, tokens))
+    tokens[::9] = 2 ** 32 + 1  # and a 64-bit one's upper half counts
+    _check(embed.lookup_grad(dy, tokens, v), dy, tokens, v)
