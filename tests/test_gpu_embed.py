@@ -270,3 +270,41 @@ def test_tokens_of_32_and_64_bits_give_equal_bits(n, v):
     assert torch.equal(embed.lookup(table, tokens.int()), embed.lookup(table, tokens))
     tokens[::9] = 2 ** 32 + 1  # and a 64-bit one's upper half counts
     _check(embed.lookup_grad(dy, tokens, v), dy, tokens, v)
+
+
+@pytest.mark.parametrize("n", [7, 700])
+def test_the_most_columns(n):
+    torch = _torch()
+    v, d = 50, 65536
+    tokens = _tokens(n, v, "any")
+    dy = torch.randn((n, d), device="cuda").half()
+    _check(embed.lookup_grad(dy, tokens, v), dy, tokens, v)
+    table = torch.randn((v, d), device="cuda").bfloat16()
+    ok = (tokens >= 0) & (tokens < v)
+    assert torch.equal(embed.lookup(table, tokens),
+                       torch.where(ok[:, None], table[tokens.clamp(0, v - 1)], 0))
+
+
+@pytest.mark.parametrize("n", [8, 300, 700])
+def test_few_and_many_tokens_in_a_graph(n):
+    torch = _torch()
+    v, d = 900, 72
+    tokens = _tokens(n, v, "text")
+    dy = torch.randn((n, d), device="cuda").half()
+    before = torch.randn((v, d), device="cuda")
+    dw = before.clone()
+    run = lambda o: (embed.lookup_grad(dy, tokens, v, dw=o, accumulate=True),
+                     embed.lookup_grad(dy, tokens, v, 3.0))
+    first = run(dw.clone())
+    assert all(torch.isfinite(o).all() for o in first)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run(dw)
+    for k in range(4):
+        dy.normal_()
+        tokens.random_(-3, (v, 5, 900, 1)[k])
+        dw.copy_(before)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, run(before.clone()))), k

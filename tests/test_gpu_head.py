@@ -808,3 +808,87 @@ def test_distill_of_large_tiles(k, t, d, v, name):
     want.check(*first)
     again = head.distill_grad(x, w, index, logits, grad=g, temperature=2.0)
     assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+# ---- pieces, graphs and strides that the tests above leave out --------------------------
+
+@pytest.mark.parametrize("t,d,v,k", [(16384 * 2 + 77, 8, 40, 5), (700, 8, (1 << 20) + 3, 9)])
+def test_pieces_of_distillation(t, d, v, k):
+    torch = _torch()
+    x, w, _ = make(t, d, v, "f16")
+    index, logits = teacher(t, v, k)
+    wide = torch.full((t, k + 3), 1, device="cuda", dtype=torch.int32)
+    wide[:, 2:2 + k] = index
+    want = kl(x, w, index, logits.bfloat16(), 0.5, 0.25)
+    want.check(head.distill(x, w, wide[:, 2:2 + k], logits.bfloat16(), 0.5), None, None)
+    for dt in (torch.float16, torch.float32):
+        dw = torch.full((v, d), 7.0, dtype=dt, device="cuda")
+        want.check(*head.distill_grad(x, w, wide[:, 2:2 + k], logits.bfloat16(), grad=0.25,
+                                      temperature=0.5, dw=dw))
+    one = head.distill_grad(x, w, index, logits.bfloat16(), grad=0.25, temperature=0.5, dx=False)
+    assert one[1] is None
+    want.check(one[0], None, one[2])
+
+
+def test_all_of_many_tokens_masked():
+    torch = _torch()
+    x, w, y = make(20000, 16, 90, "f16")
+    y[:] = -100
+    x[:] = float("nan")
+    dw = torch.ones((90, 16), device="cuda")
+    loss, dx, _ = head.cross_entropy_grad(x, w, y, dw=dw, accumulate=True)
+    assert not loss.any() and not dx.any() and (dw == 1).all()
+    assert not head.cross_entropy_grad(x, w, y)[2].any()
+    assert not head.cross_entropy(x, w, y).any()
+
+
+@pytest.mark.parametrize("t,d,v", [(1500, 40, 700), (1290, 160, 32001)])
+def test_many_tokens_in_a_graph(t, d, v):
+    """Replays over other masks: other numbers of live rows, parts and tiles than the
+    captured call's."""
+    torch = _torch()
+    x, w, y = make(t, d, v, "f16")
+    before = torch.randn((v, d), device="cuda")
+    dw = before.clone()
+    run = lambda o: (head.cross_entropy(x, w, y),
+                     *head.cross_entropy_grad(x, w, y, grad=0.5, dw=o, accumulate=True),
+                     *head.cross_entropy_grad(x, w, y, grad=0.5))
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        run(dw.clone())
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        out = run(dw)
+    for k, share in enumerate((0.0, 0.97, 1.0, 0.5, 0.0)):
+        x.normal_()
+        y.random_(0, v)
+        y[torch.rand(t, device="cuda") < share] = -100
+        dw.copy_(before)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, run(before.clone())):
+            assert torch.equal(a, b), k
+
+
+@pytest.mark.parametrize("t,d,v,stride", [(150, 64, 290, (1 << 22) - 8), (150, 64, 290, (1 << 22) - 1),
+                                          (600, 60, 200, (1 << 21) + 4)])
+def test_rows_of_w_far_apart(t, d, v, stride):
+    torch = _torch()
+    x, near, y = make(t, d, v, "bf16")
+    far = torch.full(((v - 1) * stride + d,), float("nan"), device="cuda", dtype=near.dtype)
+    w = far.as_strided((v, d), (stride, 1))
+    w.copy_(near)
+    for a, b in zip(head.cross_entropy_grad(x, w, y, grad=0.5), head.cross_entropy_grad(x, near, y, grad=0.5)):
+        assert torch.equal(a, b)
+    assert torch.equal(head.cross_entropy(x, w, y), head.cross_entropy(x, near, y))
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("t,v", [(3, 10), (70, 300)])
+def test_the_most_columns(t, v, name):
+    x, w, y = make(t, 65536, v, name)
+    want = ce(x, w, y, g=0.5)
+    want.check(*head.cross_entropy_grad(x, w, y, grad=0.5))
+    want.check(head.cross_entropy(x, w, y), None, None)
