@@ -523,6 +523,11 @@ struct LogitsArgs {
   float* z;                 // [row][top]: the products there, before scale
 };
 
+// Whether a z log2 e lies where fp32 has whole numbers alone: its rounding is then no
+// longer below the distance that an exponential takes, so what it is taken off is rounded
+// the same way, and the largest is at distance 0.
+__device__ __forceinline__ bool is_far(float z2) { return fabsf(z2) >= 0x1p23f && fabsf(z2) < INFINITY; }
+
 // z of a tile of the vocabulary (m) and of rows of X (n), never in memory.  A lane holds
 // MF x 4 logits of one row of X, a wave MF x 16, so a row's largest logit and sum over a
 // wave's span are sums in registers and two exchanges, and the spans' join is left to the
@@ -638,13 +643,20 @@ __global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {
     most = fmaxf(most, __shfl_xor(most, 32));
     // a whole power of two: no rounding of its own, which all of the span would share
     const float top = most == -INFINITY ? most : rintf(most * to2);
-    const float from = most == -INFINITY ? 0.0f : -top;
+    float mul = to2, from = most == -INFINITY ? 0.0f : -top;
+    if (is_far(top)) {
+      mul = 1.0f, from = 0.0f;
+#pragma unroll
+      for (uint32_t i = 0; i < P::MF; ++i)
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) p.acc[i][j][k] = p.acc[i][j][k] * to2 - top;
+    }
     float sum = 0.0f;
 #pragma unroll
     for (uint32_t i = 0; i < P::MF; ++i)
 #pragma unroll
       for (uint32_t k = 0; k < 4; ++k) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(p.acc[i][j][k], to2, from));
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(p.acc[i][j][k], mul, from));
         p.acc[i][j][k] = e;
         sum += e;
       }
@@ -680,7 +692,7 @@ struct RowSum {
   float top, log;  // log2 of it is top + log; top is whole, so that what is near it stays exact
   // log2 of the probability at a product x . w
   __device__ __forceinline__ float log2_q(float product, float to2) const {
-    return __builtin_fmaf(product, to2, -top) - log;
+    return (is_far(top) ? product * to2 - top : __builtin_fmaf(product, to2, -top)) - log;
   }
 };
 

@@ -892,3 +892,48 @@ def test_the_most_columns(t, v, name):
     want = ce(x, w, y, g=0.5)
     want.check(*head.cross_entropy_grad(x, w, y, grad=0.5))
     want.check(head.cross_entropy(x, w, y), None, None)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("scale", [2.0 ** 12, 2.0 ** 17 * 1.1, 2.0 ** 22 * 1.3, 2.0 ** 30 * 1.7, 1e33])
+def test_logits_past_the_whole_numbers(scale, name):
+    """Products are small whole numbers, of which equal ones have equal logits whatever
+    the scale: a row is shared evenly by its largest, and every other token's q is 0
+    (but for the first scale, e^-4096 at most)."""
+    torch = _torch()
+    t, d, v = 90, 32, 700
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.zeros((t, d), device="cuda")
+    x[torch.arange(t), torch.arange(t) % d] = 1.0
+    w = torch.randint(-40, 41, (v, d), generator=gen, device="cuda").float()
+    w[:, 5] -= 200  # every logit far below 0
+    z = x @ w.t()
+    most = z.max(1, keepdim=True).values
+    top = (z == most).double()
+    y = torch.randint(0, v, (t,), generator=gen, device="cuda")
+    y[::2] = z[::2].argmax(1)
+    q = top / top.sum(1, keepdim=True)
+    p = one_hot(y, y >= 0, v)
+    gap = (most - z.gather(1, y[:, None]))[:, 0].double()
+    s = torch.tensor(scale, dtype=torch.float32).double()
+    want = top.sum(1).log() + gap * s
+    # a logit that far is known to 2^-23 of itself, and so is the distance of another one
+    slack = torch.where(gap > 0, 2.0 ** -22 * s * (most.abs()[:, 0].double() + gap), 0.0)
+    xx, ww = x.to(_dt(name)), w.to(_dt(name))
+    g = 1.0 / scale
+    loss, dx, dw = head.cross_entropy_grad(xx, ww, y, grad=g, scale=scale,
+                                           dw=torch.empty((v, d), device="cuda"))
+    assert ((loss.double() - want).abs() <= slack + 2.0 ** -20 * (1 + want)).all()
+    assert torch.equal(head.cross_entropy(xx, ww, y, scale=scale), loss)
+    dz = s * torch.tensor(g, dtype=torch.float32).double() * (q - p)
+    u = _half(xx.dtype)
+    off = 2.2 * u * (q + p) + 2.0 ** -36
+    assert ((dw.double() - dz.t() @ x.double()).abs() <= off.t() @ x.double() * 1.01).all()
+    b = off @ w.double().abs()
+    assert ((dx.double() - dz @ w.double()).abs() <= b + u * ((dz @ w.double()).abs() + b) + 2.0 ** -24).all()
+    index = torch.stack([y, z.argmax(1)], 1)
+    teacher_says = torch.tensor([[0.0, 0.0]], device="cuda").repeat(t, 1)
+    got = head.distill(xx, ww, index, teacher_says, temperature=1.0 / scale)
+    inv = (1.0 / torch.tensor(1.0 / scale, dtype=torch.float32)).double()
+    want = top.sum(1).log() + 0.5 * gap * inv - math.log(2.0)
+    assert ((got.double() - want).abs() <= slack + 2.0 ** -20 * (1 + want.abs())).all()
