@@ -11,8 +11,7 @@
 //   logits_kernel   z = scale X W^T in tiles that stay in registers; z at targets in
 //                   fp32; of every row and span of the vocabulary a power of two 2^t
 //                   next to its largest exp(z) and its sum of exp(z) / 2^t, and with
-//                   gradients these exponentials themselves, in 16 bits: 2^-9 or
-//                   2^-12 of each
+//                   gradients these exponentials themselves, in 16 bits (Kept)
 //   loss_kernel     the spans' sums joined: log(sum exp z), the loss
 //   dz_kernel       the same, and the exponentials turned into dz where they lie
 //   grad_kernel     dx = dz W and dw = dz^T X, in one launch
@@ -112,6 +111,38 @@ template <typename T>
 constexpr uint32_t kTypeOf = sizeof(T) == 4 ? ARK_HEAD_F32 : ARK_HEAD_F16;
 template <>
 constexpr uint32_t kTypeOf<__bf16> = ARK_HEAD_BF16;
+
+// An exponential from 0 to under 2, relative to its span's 2^t, in 16 bits without a sign:
+// an exponent's low bits and what is left of them for the fraction, so that only dz's own
+// rounding counts.  fp16 4 and 12 bits (2^-13 of itself, below 2^-14 2^-27: dz in fp16 has
+// 2^-11 and, of the largest gradient, 2^-38), bf16 7 and 9 (2^-10, for 2^-8; its dz has
+// small numbers too).  The bits are those of an fp32 times kDown, cut off at kCut.
+template <typename T>
+struct Kept {
+  static constexpr uint32_t kCut = 11;
+  static constexpr float kDown = 0x1p-112f, kUp = 0x1p112f;
+};
+template <>
+struct Kept<__bf16> {
+  static constexpr uint32_t kCut = 14;
+  static constexpr float kDown = 1.0f, kUp = 1.0f;
+};
+// Two of them, to nearest; and back, times kDown.
+template <typename T>
+__device__ __forceinline__ uint32_t keep2(float a, float b) {
+  typedef Kept<T> K;
+  constexpr uint32_t kLeft = 16 - K::kCut, kHalf = 1u << 15;
+  const uint32_t x = (__float_as_uint(a * K::kDown) << kLeft) + kHalf;
+  const uint32_t y = (__float_as_uint(b * K::kDown) << kLeft) + kHalf;
+  return __builtin_amdgcn_perm(y, x, 0x07060302u);
+}
+template <typename T>
+__device__ __forceinline__ void kept2(uint32_t v, float& a, float& b) {
+  typedef Kept<T> K;
+  constexpr uint32_t kMask = 0xFFFFu << K::kCut;
+  a = __uint_as_float((v << K::kCut) & kMask);
+  b = __uint_as_float((v >> (16 - K::kCut)) & kMask);
+}
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -673,8 +704,7 @@ __global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {
       const f32x4 v = p.acc[i][j];
       const uint32_t chunk = (i * 2 + lane / 32) ^ (row % kChunks);
       *(u32x2*)(mine + row * kRow + chunk * 16 + lane / 16 % 2 * 8) =
-          u32x2{narrow2<kTypeOf<typename P::T>>(v[0], v[1]),
-                narrow2<kTypeOf<typename P::T>>(v[2], v[3])};
+          u32x2{keep2<typename P::T>(v[0], v[1]), keep2<typename P::T>(v[2], v[3])};
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
@@ -789,7 +819,6 @@ struct DzArgs {
 // rows of 377: 10 us, 18 by blocks; 738 of 1936: 7.9 both ways).
 template <typename T, uint32_t LANES>
 __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
-  typedef T V __attribute__((ext_vector_type(8)));
   constexpr uint32_t DT = kTypeOf<T>, kTeams = kLanes / LANES;
   __shared__ float red[kLanes / 64 * 2];
   __shared__ uint32_t s_index_of[kTeams][ARK_HEAD_MAX_TOP];
@@ -811,11 +840,11 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
   const float* z = l.z + (uint64_t)row * top;
   // four rounds of the lanes on their way, the first four while the spans join
   constexpr uint32_t kAhead = 4, kRound = LANES * 8;
-  V v[kAhead];
+  u32x4 v[kAhead];
   const auto fetch = [&](uint32_t c) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t q = 0; q < kAhead; ++q)
-      if (c + q * kRound < to) v[q] = ld_nt<V>(e + c + q * kRound);
+      if (c + q * kRound < to) v[q] = ld_nt<u32x4>(e + c + q * kRound);
   };
   fetch(from + tid * 8);
   const RowSum sum = join_spans<LANES>(stats, l.spans, tid, red);
@@ -835,11 +864,14 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
     for (uint32_t q = 0; q < kAhead; ++q) {
       const uint32_t c = c0 + q * kRound;
       if (c >= to) break;
-      const float s = exp2f((stats[c / a.span * 2] - sum.top) - sum.log) * f;
+      const float s = exp2f((stats[c / a.span * 2] - sum.top) - sum.log) * f * Kept<T>::kUp;
       u32x4 o;
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i)
-        o[i] = narrow2<DT>((float)v[q][2 * i] * s, (float)v[q][2 * i + 1] * s);
+      for (uint32_t i = 0; i < 4; ++i) {
+        float x, y;
+        kept2<T>(v[q][i], x, y);
+        o[i] = narrow2<DT>(x * s, y * s);
+      }
       *(u32x4*)(e + c) = o;
     }
     fetch(c0 + kAhead * kRound);

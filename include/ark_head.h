@@ -30,9 +30,10 @@
  * The gradients of x and w are
  *     dx = dz w          in x's type
  *     dw (+)= dz^T x     in fp32, or in w's type (not added to)
- * dz is rounded to the 16 bits of x's type on the way, twice: relative to a power
- * of two next to the largest of its row in a piece of the vocabulary, and again,
- * scaled so that the largest gradient has 2^14, when the row's sum is known.
+ * dz is rounded to the 16 bits of x's type, relative to the largest gradient, which is
+ * scaled to 2^14; until a row's sum is known its exponentials are kept in 16 bits of
+ * their own, to 2^-13 (fp16) or 2^-10 (bf16) of each, a quarter of what dz's rounding is
+ * off by.
  * Entries at targets are rounded once, from fp32.  A loss or gradient formed
  * from an inf or NaN is not finite, and the optimizer step then skips; other tokens'
  * losses and dx stay what they are.  (A token whose grad * scale is past fp32's range

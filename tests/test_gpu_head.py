@@ -937,3 +937,36 @@ def test_logits_past_the_whole_numbers(scale, name):
     inv = (1.0 / torch.tensor(1.0 / scale, dtype=torch.float32)).double()
     want = top.sum(1).log() + 0.5 * gap * inv - math.log(2.0)
     assert ((got.double() - want).abs() <= slack + 2.0 ** -20 * (1 + want.abs())).all()
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("t,d,v", [(1, 1, 300), (9, 32, 2500), (70, 80, 1000), (517, 768, 32308)])
+def test_dz_is_rounded_once_to_its_type(t, d, v, name):
+    """Rows of x that are 1 in one column make dw dz itself.  An exponential is kept to
+    2^-13 or 2^-10 of itself (a quarter of the type's half step) until its row's sum is
+    known, and dz then to half a step; of an exponential, its argument and the row's sum 2^-18 more."""
+    torch = _torch()
+    gen = torch.Generator(device="cuda").manual_seed(t)
+    w = (3 * torch.randn((v, d), generator=gen, device="cuda")).to(_dt(name))
+    x = torch.zeros((t, d), device="cuda", dtype=w.dtype)
+    x[torch.arange(t), torch.arange(t)] = 1.0
+    y = torch.randint(0, v, (t,), generator=gen, device="cuda")
+    index = torch.stack([y, (y + 1) % v], 1)
+    u = _half(w.dtype)
+    q = torch.softmax(w[:, :t].t().double(), 1)
+    for p, call in (
+            (one_hot(y, y >= 0, v), lambda o: head.cross_entropy_grad(x, w, y, grad=0.75, dw=o)),
+            (0.5 * one_hot(y, y >= 0, v) + 0.5 * one_hot(index[:, 1], y >= 0, v),
+             lambda o: head.distill_grad(x, w, index, torch.zeros((t, 2), device="cuda"), grad=0.75,
+                                         dw=o))):
+        dw = call(torch.empty((v, d), device="cuda"))[2]
+        off = (dw[:, :t].t().double() / 0.75 - (q - p)).abs()
+        at = p > 0
+        # an entry at a target is q - p in fp32, rounded once
+        limit = torch.where(at, u * (q - p).abs() + 2.0 ** -18 * (q + p), q * (1.27 * u + 2.0 ** -18))
+        if name == "f16":
+            # an exponential below 2^-14 of 2^t, which its span's largest is to sqrt(2), is off
+            # by 2^-27 of that, a dz below 2^-27 of the largest gradient by 2^-38
+            limit = limit + 2.0 ** -26.5 + 2.0 ** -38
+        assert (off <= limit * (1 + u)).all(), (off / limit).max().item()
+        assert not dw[:, t:].any()
