@@ -46,8 +46,8 @@ struct Meta {
   uint32_t live;                  // rows with a loss
   uint32_t dx_parts, dw_parts;    // that the products' sums are cut into
   uint32_t dw_first;              // dw's blocks are the longer ones
-  int32_t shift;                  // dz is formed times 2^shift
-  float down;                     // 2^-shift, for the products
+  float largest, to, down;        // grad * scale = grad / largest * to * down; the products
+                                  // take dz without down
 };
 
 // How both products' work is cut, decided where the number of live rows is known:
@@ -281,27 +281,20 @@ struct RankArgs {
   Cut cut;
 };
 
-// grad * scale as part 2^e: the product itself may lie outside fp32's range on either
-// side and still be one that dz, times 2^shift, holds.
-struct GradScale {
-  float part;  // of finite ones 0 or 1/4 to 1 in magnitude
-  int e;
-};
-__device__ __forceinline__ GradScale grad_scale(float grad, float scale) {
-  int eg = 0, es = 0;
-  const float g = frexpf(grad, &eg), s = frexpf(scale, &es);
-  return {g * s, g - g == 0.0f ? eg + es : 0};
-}
-
 // By one wave, with the number of live tokens and the largest |grad| over them.
 __device__ __forceinline__ void write_meta(const RankArgs& a, uint32_t live, float largest) {
-  Meta m = {live, 1, 1, 0, 0, 1.0f};
+  Meta m = {live, 1, 1, 0, 1.0f, 1.0f, 1.0f};
   if (a.with_grad) {
-    // the largest |grad * scale| times 2^shift lies in [2^13, 2^14)
+    // grad * scale = f down, f = grad / largest * to: the largest f is 2^14, a power of two
+    // so that the one number of all tokens has no rounding (which they would share), unless
+    // down is then below fp32.  (By parts, as the product may lie below fp32 itself.)
     if (largest > 0.0f && largest * a.scale < INFINITY) {
-      const GradScale g = grad_scale(largest, a.scale);
-      m.shift = min(max(14 - g.e + (g.part < 0.5f ? 1 : 0), -126), 126);
-      m.down = ldexpf(1.0f, -m.shift);
+      int eg, es;
+      const float part = frexpf(largest, &eg) * frexpf(a.scale, &es);  // 1/4 to 1
+      const int e = eg + es;
+      m.largest = largest;
+      m.to = e >= 14 - 124 ? 0x1p14f : ldexpf(part, e + 126);
+      m.down = e >= 14 - 124 ? ldexpf(part, e - 14) : 0x1p-126f;
     }
     // the cheapest of the 64 candidates, a lane each
     const Cut::Parts mine = Cut::candidate(threadIdx.x % 64);
@@ -853,8 +846,8 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
     const float loss = row_loss(l.targets, t, z, sum, to2, tid);
     if (tid == 0) l.loss[t] = loss;
   }
-  const GradScale gs = grad_scale(a.grads ? a.grads[t] : a.grad, l.scale);
-  const float f = ldexpf(gs.part, gs.e + l.meta->shift);
+  const float g = a.grads ? a.grads[t] : a.grad;
+  const float f = fabsf(g) * l.scale < INFINITY ? g / l.meta->largest * l.meta->to : g * l.scale;
   for (uint32_t k = tid; k < top; k += LANES) {
     s_index[k] = l.targets.at(t, k);
     s_p[k] = l.targets.weight(t, k);

@@ -31,7 +31,7 @@
  *     dx = dz w          in x's type
  *     dw (+)= dz^T x     in fp32, or in w's type (not added to)
  * dz is rounded to the 16 bits of x's type, relative to the largest gradient, which is
- * scaled to 2^14; until a row's sum is known its exponentials are kept in 16 bits of
+ * taken as 2^14; until a row's sum is known its exponentials are kept in 16 bits of
  * their own, to 2^-13 (fp16) or 2^-10 (bf16) of each, a quarter of what dz's rounding is
  * off by.
  * Entries at targets are rounded once, from fp32.  A loss or gradient formed

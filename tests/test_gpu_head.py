@@ -970,3 +970,25 @@ def test_dz_is_rounded_once_to_its_type(t, d, v, name):
             limit = limit + 2.0 ** -26.5 + 2.0 ** -38
         assert (off <= limit * (1 + u)).all(), (off / limit).max().item()
         assert not dw[:, t:].any()
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("t", [40, 1100])
+@pytest.mark.parametrize("grad", [1 / 3, 46.88, 1e-3 * 1.0078, -0.7])
+def test_one_gradient_of_all_tokens_is_not_rounded(grad, t, name):
+    """Tokens that are not expected (q of 1 / v) have -grad (1 - q) at their targets:
+    with the one number in its place as a power of two, what is left of its rounding is q,
+    the same direction for all tokens and so in every sum of them otherwise."""
+    torch = _torch()
+    d, v = 1100, 5000
+    w = torch.zeros((v, d), device="cuda", dtype=_dt(name))
+    x = torch.zeros((t, d), device="cuda", dtype=_dt(name))
+    x[torch.arange(t), torch.arange(t) % d] = 1.0
+    y = torch.randperm(v, device="cuda")[:t]
+    dw = head.cross_entropy_grad(x, w, y, grad=grad, dw=torch.empty((v, d), device="cuda"))[2]
+    at = dw[y, torch.arange(t, device="cuda") % d].double()
+    exact = torch.tensor(grad, dtype=torch.float32).double()
+    assert ((at / exact + 1 - 1 / v).abs() <= 1 / v + 2.0 ** -18).all()
+    g = torch.full((t,), grad, device="cuda")
+    again = head.cross_entropy_grad(x, w, y, grad=g, dw=torch.empty((v, d), device="cuda"))[2]
+    assert torch.equal(dw, again)
