@@ -39,13 +39,25 @@ constexpr uint32_t kLanes = 256;
 constexpr uint32_t kRowPad = 256;   // rows of a piece are laid out for whole tiles
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr uint32_t kMaxPiece = 16384;  // tokens: what rank_kernel's block ranks
-constexpr uint32_t kFew = 1024;        // tokens that gather_kernel's blocks rank themselves
+constexpr uint32_t kFew = 1024;  // tokens that gather_kernel's blocks rank themselves
+
+// Calls of at most this many tokens form dz in two 16-bit parts, its rounded value and what
+// is left of it, in rows of their own: X's rows come twice for dw, and join_kernel adds dx's
+// two.  Where tokens are few a rounding of dz shows in full in dx and dw (one token's entry
+// at its target is nearly all of a row of W's gradient): up to 2.2 times the error of their
+// own rounding for one token, 1.55 for 56, and 1.4 of more, and 1.03 in two parts.  It takes
+// a call of up to 32 tokens 0 to 8 % longer (768 x 32000: 54 us and 57 for one token, 57 and
+// 61 for 32), as its rows still fit a tile, of 64 6 to 17 % (60 and 70), of 128 28 %.
+constexpr uint32_t kTwice = 64;
+static_assert(kTwice <= kFew && kTwice % kProductStep == 0 && 2 * kTwice <= kRowPad,
+              "ranked by gather_kernel, and room for the rows of both parts");
 
 // What a piece's kernels leave for each other.
 struct Meta {
   uint32_t live;                  // rows with a loss
   uint32_t dx_parts, dw_parts;    // that the products' sums are cut into
   uint32_t dw_first;              // dw's blocks are the longer ones
+  uint32_t again;                 // rows from dz's first part to its second, or 0
   float largest, to, down;        // grad * scale = grad / largest * to * down; the products
                                   // take dz without down
 };
@@ -142,6 +154,14 @@ __device__ __forceinline__ void kept2(uint32_t v, float& a, float& b) {
   constexpr uint32_t kMask = 0xFFFFu << K::kCut;
   a = __uint_as_float((v << K::kCut) & kMask);
   b = __uint_as_float((v >> (16 - K::kCut)) & kMask);
+}
+
+// What two values' rounded ones leave, rounded.
+template <typename T>
+__device__ __forceinline__ uint32_t left2(float a, float b, uint32_t rounded) {
+  typedef T V __attribute__((ext_vector_type(2)));
+  const V r = __builtin_bit_cast(V, rounded);
+  return narrow2<kTypeOf<T>>(a - (float)r[0], b - (float)r[1]);
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -278,13 +298,21 @@ struct RankArgs {
   const float* grads;  // or NULL: grad
   float grad, scale;
   uint32_t with_grad;
+  uint32_t twice;  // dz has two parts
   Cut cut;
+
+  // Rows of X and dz up to a whole step.
+  static __device__ __forceinline__ uint32_t whole(uint32_t rows) {
+    return (rows + kProductStep - 1) / kProductStep * kProductStep;
+  }
 };
 
 // By one wave, with the number of live tokens and the largest |grad| over them.
 __device__ __forceinline__ void write_meta(const RankArgs& a, uint32_t live, float largest) {
-  Meta m = {live, 1, 1, 0, 1.0f, 1.0f, 1.0f};
+  Meta m = {live, 1, 1, 0, 0, 1.0f, 1.0f, 1.0f};
   if (a.with_grad) {
+    if (a.twice) m.again = live;
+    const uint32_t rows = m.again + live;
     // grad * scale = f down, f = grad / largest * to: the largest f is 2^14, a power of two
     // so that the one number of all tokens has no rounding (which they would share), unless
     // down is then below fp32.  (By parts, as the product may lie below fp32 itself.)
@@ -298,14 +326,14 @@ __device__ __forceinline__ void write_meta(const RankArgs& a, uint32_t live, flo
     }
     // the cheapest of the 64 candidates, a lane each
     const Cut::Parts mine = Cut::candidate(threadIdx.x % 64);
-    const float cost = a.cut.may(mine, live) ? a.cut.cost(mine, live) : INFINITY;
+    const float cost = a.cut.may(mine, rows) ? a.cut.cost(mine, rows) : INFINITY;
     float best = cost;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) best = fminf(best, __shfl_xor(best, o));
     const Cut::Parts p =
         Cut::candidate((uint32_t)__ffsll((unsigned long long)__ballot(cost == best)) - 1u);
     m.dx_parts = p.dx, m.dw_parts = p.dw;
-    m.dw_first = a.cut.length(live, p.dw) > a.cut.length(a.cut.vocab, p.dx) ? 1 : 0;
+    m.dw_first = a.cut.length(rows, p.dw) > a.cut.length(a.cut.vocab, p.dx) ? 1 : 0;
   }
   if (threadIdx.x % 64 == 0) *a.meta = m;
 }
@@ -491,9 +519,10 @@ __global__ __launch_bounds__(kLanes) void gather_kernel(GatherArgs a) {
     row = t < r.tokens ? r.rank[t] : ~0u;
     live = r.meta->live;
   }
+  const uint32_t again = r.twice ? live : 0;  // rows to X's second copy, or 0
   if (t >= r.tokens) {
-    row = live + (t - r.tokens);
-    if (row < (live + kProductStep - 1) / kProductStep * kProductStep)
+    row = again + live + (t - r.tokens);
+    if (row < RankArgs::whole(again + live))
       for (uint32_t c = lane * 8; c < a.padded; c += 512)
         *(u32x4*)(a.out + (uint64_t)row * a.padded + c) = u32x4{0, 0, 0, 0};
     return;
@@ -507,8 +536,11 @@ __global__ __launch_bounds__(kLanes) void gather_kernel(GatherArgs a) {
   }
   const uint16_t* src = a.x + t * a.x_stride;
   uint16_t* dst = a.out + (uint64_t)row * a.padded;
-  for (uint32_t c = lane * 8; c < a.padded; c += 512)
-    *(u32x4*)(dst + c) = load8(src + c, c < a.columns ? a.columns - c : 0u);
+  for (uint32_t c = lane * 8; c < a.padded; c += 512) {
+    const u32x4 v = load8(src + c, c < a.columns ? a.columns - c : 0u);
+    *(u32x4*)(dst + c) = v;
+    if (again) *(u32x4*)(dst + (uint64_t)again * a.padded + c) = v;
+  }
   const uint32_t top = r.targets.top, width = entries_width(top);
   for (uint32_t k = lane; k < width; k += 64)
     a.entries[(uint64_t)row * width + k] = k < top ? r.targets.at(t, k) : ~0u;
@@ -821,11 +853,14 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
   const uint32_t row = blockIdx.x * kTeams + team, live = l.meta->live;
   uint32_t* const s_index = s_index_of[team];
   float* const s_p = s_p_of[team];
-  if (row >= (live + kProductStep - 1) / kProductStep * kProductStep) return;
+  const uint32_t second = l.meta->again;  // rows to dz's second part, or 0
+  if (second + row >= RankArgs::whole(second + live)) return;
   uint16_t* e = a.e + row * a.e_stride;
+  const uint64_t again = second * a.e_stride;
   const uint32_t from = blockIdx.y * a.share, to = min(from + a.share, a.written);
   if (row >= live) {
-    for (uint32_t c = from + tid * 8; c < to; c += LANES * 8) *(u32x4*)(e + c) = u32x4{0, 0, 0, 0};
+    for (uint32_t c = from + tid * 8; c < to; c += LANES * 8)
+      *(u32x4*)(e + again + c) = u32x4{0, 0, 0, 0};
     return;
   }
   const uint32_t t = l.rows[row], top = l.targets.top;
@@ -866,6 +901,15 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
         o[i] = narrow2<DT>(x * s, y * s);
       }
       *(u32x4*)(e + c) = o;
+      if (again) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          float x, y;
+          kept2<T>(v[q][i], x, y);
+          o[i] = left2<T>(x * s, y * s, o[i]);
+        }
+        *(u32x4*)(e + again + c) = o;
+      }
     }
     fetch(c0 + kAhead * kRound);
   }
@@ -882,7 +926,9 @@ __global__ __launch_bounds__(kLanes) void dz_kernel(DzArgs a) {
     for (uint32_t i = 0; i < top; ++i) p += s_index[i] == v ? s_p[i] : 0.0f;
     // q - p without the difference of two numbers near 1
     const float d = (expm1f(sum.log2_q(z[k], to2) * kLn2) + (1.0f - p)) * f;
-    e[v] = (uint16_t)narrow2<DT>(d, 0.0f);
+    const uint32_t o = narrow2<DT>(d, 0.0f);
+    e[v] = (uint16_t)o;
+    if (again) e[again + v] = (uint16_t)left2<T>(d, 0.0f, o);
   }
 }
 
@@ -961,11 +1007,11 @@ template <typename P, bool DX>
 __device__ __forceinline__ void product_block(const ProductArgs& g, const Meta& meta,
                                               const Tiles& tiles, uint32_t block, uint8_t* lds) {
   const uint32_t parts = DX ? meta.dx_parts : meta.dw_parts;
-  const uint32_t height = DX ? meta.live : g.out.height;
+  const uint32_t height = DX ? meta.again + meta.live : g.out.height;
   uint32_t tm, tn, part;
   tiles.find(block, tiles.m * tiles.n * parts, &tm, &tn, &part);
   const uint32_t m0 = tm * P::BM, n0 = tn * P::BN;
-  const uint32_t ks = DX ? g.a_rows : (meta.live + kProductStep - 1) / kProductStep * kProductStep;
+  const uint32_t ks = DX ? g.a_rows : RankArgs::whole(meta.again + meta.live);
   const uint32_t steps = (ks + kProductStep - 1) / kProductStep;
   const uint32_t s0 = (uint32_t)((uint64_t)steps * part / parts);
   const uint32_t s1 = (uint32_t)((uint64_t)steps * (part + 1) / parts);
@@ -980,7 +1026,7 @@ __device__ __forceinline__ void product_block(const ProductArgs& g, const Meta& 
   p.each(at, [&](uint32_t m, uint32_t n, f32x4 v) __attribute__((always_inline)) {
     m += m0, n += n0;
     if (m >= g.out.width || n >= height) return;
-    if (parts > 1)
+    if (parts > 1 || (DX && meta.again))
       *(f32x4*)(partial + n * w4 + m) = v;
     else
       g.out.put(n, m, v);
@@ -997,7 +1043,7 @@ template <typename X, typename W>
 __global__ __launch_bounds__(X::kLanes, 2) void grad_kernel(GradArgs g) {
   extern __shared__ __align__(1024) uint8_t lds[];
   const Meta meta = *g.meta;
-  const Tiles x = {g.tiles_m, g.dx.out.p ? (meta.live + X::BN - 1) / X::BN : 0u};
+  const Tiles x = {g.tiles_m, g.dx.out.p ? (meta.again + meta.live + X::BN - 1) / X::BN : 0u};
   const Tiles w = {g.tiles_m, g.dw.out.p ? (g.dw.out.height + W::BN - 1) / W::BN : 0u};
   const uint32_t nx = x.m * x.n * meta.dx_parts, nw = w.m * w.n * meta.dw_parts;
   // the second kind starts at a multiple of the XCDs
@@ -1011,35 +1057,43 @@ __global__ __launch_bounds__(X::kLanes, 2) void grad_kernel(GradArgs g) {
   }
 }
 
-// The parts of both products, added in order.  Bound by the caches that the parts are
-// still in: dw's two of 32000 x 768, 18 us.
+// The parts of both products, added in order, and then those of the rows `again` further on.
+// Bound by the caches that the parts are still in: dw's two of 32000 x 768, 18 us.
+template <uint32_t kBatch>  // on their way at once
 __device__ __forceinline__ void join(const float* partial, uint32_t parts, uint32_t height,
-                                     const Out& out, uint64_t i, uint64_t step) {
+                                     uint32_t again, const Out& out, uint64_t i, uint64_t step) {
   const uint32_t per = (out.width + 3) / 4;
-  const uint64_t all = (uint64_t)height * per;
-  for (; i < all; i += step) {
+  const uint64_t rows = (uint64_t)height * per, second = (uint64_t)again * per;
+  const uint64_t all = second + rows;
+  const uint32_t sums = again ? 2 * parts : parts;
+  for (; i < rows; i += step) {
     const f32x4* p = (const f32x4*)partial + i;
+    const auto at = [&](uint32_t s) { return s < parts ? s * all : (s - parts) * all + second; };
     f32x4 v = p[0];
-    constexpr uint32_t kBatch = 4;  // on their way at once
-    for (uint32_t s = 1; s < parts; s += kBatch) {
+    for (uint32_t s = 1; s < sums; s += kBatch) {
       f32x4 more[kBatch];
 #pragma unroll
       for (uint32_t k = 0; k < kBatch; ++k)
-        if (s + k < parts) more[k] = p[(s + k) * all];
+        if (s + k < sums) more[k] = p[at(s + k)];
 #pragma unroll
       for (uint32_t k = 0; k < kBatch; ++k)
-        if (s + k < parts) v += more[k];
+        if (s + k < sums) v += more[k];
     }
     out.put((uint32_t)(i / per), (uint32_t)(i % per) * 4, v);
   }
 }
+// TWICE: dx's rows may come twice, whose longer chains have more parts on their way (for all
+// calls dw's two take 23 us for 19, for their registers).
+template <bool TWICE>
 __global__ __launch_bounds__(kLanes) void join_kernel(GradArgs g) {
+  constexpr uint32_t kBatch = TWICE ? 8 : 4;
   const Meta meta = *g.meta;
+  const uint32_t again = TWICE ? meta.again : 0;
   const uint64_t i = (uint64_t)blockIdx.x * kLanes + threadIdx.x, step = (uint64_t)gridDim.x * kLanes;
-  if (g.dx.out.p && meta.dx_parts > 1)
-    join(g.dx.partial, meta.dx_parts, meta.live, g.dx.out, i, step);
+  if (g.dx.out.p && (meta.dx_parts > 1 || again))
+    join<kBatch>(g.dx.partial, meta.dx_parts, meta.live, again, g.dx.out, i, step);
   if (g.dw.out.p && meta.dw_parts > 1)
-    join(g.dw.partial, meta.dw_parts, g.dw.out.height, g.dw.out, i, step);
+    join<kBatch>(g.dw.partial, meta.dw_parts, g.dw.out.height, 0, g.dw.out, i, step);
 }
 
 // ---- host -------------------------------------------------------------------
@@ -1058,6 +1112,7 @@ struct Small {
 // How a call is cut, and where things lie in its workspace (offsets of 256).
 struct Plan {
   bool small_logits, small;     // tiles
+  bool twice;                   // dz in two parts
   uint32_t piece;               // tokens
   uint32_t pieces;
   uint32_t padded;              // columns
@@ -1159,9 +1214,11 @@ Plan plan_of(const void* w, uint64_t w_stride, uint64_t tokens, uint64_t columns
   if (grad) {
     p.e = take(rows * p.e_stride * 2);
     float large, small = INFINITY;
-    p.cut = cut_of(false, (uint32_t)columns, piece, (uint32_t)vocab, has_dx, has_dw, &large);
+    p.twice = tokens <= kTwice;
+    const uint32_t dz_rows = p.twice ? piece * 2 : piece;
+    p.cut = cut_of(false, (uint32_t)columns, dz_rows, (uint32_t)vocab, has_dx, has_dw, &large);
     if (large < 500.0f) {  // beyond it small tiles have no chance
-      const Cut c = cut_of(true, (uint32_t)columns, piece, (uint32_t)vocab, has_dx, has_dw, &small);
+      const Cut c = cut_of(true, (uint32_t)columns, dz_rows, (uint32_t)vocab, has_dx, has_dw, &small);
       p.small = small < large;
       if (p.small) p.cut = c;
     }
@@ -1230,23 +1287,24 @@ int launch_logits(const LogitsArgs& a, uint32_t blocks, hipStream_t s) {
 }
 
 template <typename X, typename W>
-int launch_grad(const GradArgs& g, const Cut& cut, uint32_t rows, hipStream_t s) {
+int launch_grad(const GradArgs& g, const Cut& cut, bool twice, uint32_t tokens, hipStream_t s) {
   static std::atomic<uint64_t> ready{0};
   static_assert(X::kLanes == W::kLanes && X::kLds == W::kLds && X::BN == W::BN, "one launch");
   if (int rc = with_lds(grad_kernel<X, W>, X::kLds, &ready)) return rc;
   // as many blocks as any number of live rows may ask for; the others leave at once
+  const uint32_t rows = twice ? tokens * 2 : tokens;
   uint32_t nx = 0, nw = 0;
   if (g.dx.out.p) nx = cut.dx_most > cut.tiles_of(rows) ? cut.dx_most : cut.tiles_of(rows);
   if (g.dw.out.p) nw = cut.dw_most;
   const uint32_t blocks = (uint32_t)(up(g.tiles_m * nx, 8) + up(g.tiles_m * nw, 8));
   hipLaunchKernelGGL((grad_kernel<X, W>), dim3(blocks), dim3(X::kLanes), X::kLds, s, g);
   ARK_HIP(hipGetLastError());
-  if ((g.dx.out.p && cut.dx_most > 1) || (g.dw.out.p && nw > cut.tiles_of(cut.vocab))) {
-    const uint64_t rows_dx = g.dx.out.p ? rows : 0, rows_dw = g.dw.out.p ? cut.vocab : 0;
+  if ((g.dx.out.p && (cut.dx_most > 1 || twice)) || (g.dw.out.p && nw > cut.tiles_of(cut.vocab))) {
+    const uint64_t rows_dx = g.dx.out.p ? tokens : 0, rows_dw = g.dw.out.p ? cut.vocab : 0;
     const uint64_t most = (rows_dx > rows_dw ? rows_dx : rows_dw) * ((g.dx.out.width + 3) / 4);
     const uint64_t join_blocks = (most + kLanes - 1) / kLanes;
-    hipLaunchKernelGGL(join_kernel, dim3(join_blocks < 2048 ? (uint32_t)join_blocks : 2048u),
-                       dim3(kLanes), 0, s, g);
+    hipLaunchKernelGGL(twice ? join_kernel<true> : join_kernel<false>,
+                       dim3(join_blocks < 2048 ? (uint32_t)join_blocks : 2048u), dim3(kLanes), 0, s, g);
     ARK_HIP(hipGetLastError());
   }
   return ARK_OPT_OK;
@@ -1297,6 +1355,7 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
   ra.grads = c.grads ? c.grads + t0 : nullptr;
   ra.grad = c.grad, ra.scale = c.scale;
   ra.with_grad = c.with_grad;
+  ra.twice = p.twice;
   ra.cut = p.cut;
   ga.x = (const uint16_t*)c.x + t0 * c.x_stride;
   ga.x_stride = c.x_stride;
@@ -1352,7 +1411,9 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
   da.e = la.e, da.e_stride = p.e_stride, da.written = p.written, da.span = p.span;
   if (tokens) {
     // eight blocks for every compute unit, and two rounds of a block's lanes at least
-    const uint64_t rows32 = up(tokens, kProductStep), round = kLanes * 8;
+    // rows with those up to a whole step of the products
+    const uint64_t rows32 = p.twice ? up(tokens + kProductStep - 1, kLanes / 64) : up(tokens, kProductStep);
+    const uint64_t round = kLanes * 8;
     uint64_t parts = (2048 + rows32 - 1) / rows32, rounds = (p.written + round - 1) / round;
     if (parts > (rounds + 1) / 2) parts = (rounds + 1) / 2;
     da.share = (uint32_t)((rounds + parts - 1) / parts * round);
@@ -1399,7 +1460,7 @@ int run_piece(const Call& c, const Plan& p, uint32_t piece) {
     o.dtype = final ? c.dw_dtype : ARK_HEAD_F32;
   }
   return launch_grad<typename Size::template P<T, true, false>,
-                     typename Size::template P<T, true, true>>(gr, p.cut, tokens, s);
+                     typename Size::template P<T, true, true>>(gr, p.cut, p.twice, tokens, s);
 }
 
 template <typename T>

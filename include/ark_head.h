@@ -33,8 +33,9 @@
  * dz is rounded to the 16 bits of x's type, relative to the largest gradient, which is
  * taken as 2^14; until a row's sum is known its exponentials are kept in 16 bits of
  * their own, to 2^-13 (fp16) or 2^-10 (bf16) of each, a quarter of what dz's rounding is
- * off by.
- * Entries at targets are rounded once, from fp32.  A loss or gradient formed
+ * off by.  With at most 64 tokens, whose sums show a rounding in full, what is left of dz
+ * is 16 bits of its own in the products too.
+ * Entries at targets are formed in fp32.  A loss or gradient formed
  * from an inf or NaN is not finite, and the optimizer step then skips; other tokens'
  * losses and dx stay what they are.  (A token whose grad * scale is past fp32's range
  * does not count for the largest gradient either.)  Sums run

@@ -992,3 +992,53 @@ def test_one_gradient_of_all_tokens_is_not_rounded(grad, t, name):
     g = torch.full((t,), grad, device="cuda")
     again = head.cross_entropy_grad(x, w, y, grad=g, dw=torch.empty((v, d), device="cuda"))[2]
     assert torch.equal(dw, again)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("t,d,v", [(1, 40, 300), (7, 32, 2500), (32, 300, 700), (33, 90, 5000),
+                                   (64, 256, 3000), (50, 768, 32000)])
+def test_few_tokens_have_dz_in_two_parts(t, d, v, name):
+    """dw is dz itself where rows of x are 1 in one column, and dx where rows of w are: of
+    at most 64 tokens only the exponentials' 16 bits (a quarter of half a step) are left of
+    dz's rounding, at targets none, and dx has its own.  A first part of half a step u leaves
+    at most u of dz, which the second has to u of itself: u^2 of dz (2^-16 in bf16)."""
+    torch = _torch()
+    gen = torch.Generator(device="cuda").manual_seed(t + d)
+    w = (3 * torch.randn((v, d), generator=gen, device="cuda")).to(_dt(name))
+    x = torch.zeros((t, d), device="cuda", dtype=w.dtype)
+    x[torch.arange(t), torch.arange(t) % d] = 1.0
+    w[: d - 1] = 0
+    w[torch.arange(d - 1), torch.arange(1, d)] = 1.0  # column c is one of row c - 1, and of others
+    w[d - 1:, 1:] = 0  # whose only column is 0
+    y = torch.randint(0, v, (t,), generator=gen, device="cuda")
+    y[1::5] = -100
+    live = y >= 0
+    g = torch.rand(t, generator=gen, device="cuda") + 0.1
+    g[2::7] *= -3e-3
+    u = _half(w.dtype)
+    q = torch.softmax(x.double() @ w.double().t(), 1)
+    p = one_hot(y, live, v)
+    scale = (g.double() * live)[:, None]
+    dz = scale * (q - p)
+    loss, dx, dw = head.cross_entropy_grad(x, w, y, grad=g, dw=torch.empty((v, d), device="cuda"))
+    off = scale.abs() * torch.where(p > 0, 2.0 ** -18 * (q + p), q * (0.25 * u + 2.0 ** -18))
+    off = off * (1 + u) + u * u * dz.abs()
+    if name == "f16":  # a small exponential's 2^-27, and dz's 2^-39 of the largest gradient
+        off = off + scale.abs() * 2.0 ** -26.5 + (scale != 0) * scale.abs().max() * 2.0 ** -38
+    limit = off.t() @ x.double()
+    assert ((dw.double() - dz.t() @ x.double()).abs() <= limit * 1.01 + 1e-30).all()
+    want = dz[:, :d - 1]
+    err = off[:, :d - 1] * 1.01
+    tiny = 2.0 ** -25 if name == "f16" else 0.0
+    assert ((dx[:, 1:].double() - want).abs() <= err + u * (want.abs() + err) + tiny).all()
+    assert not dx[~live].any()
+    # accumulated, and of a teacher's one entry
+    before = torch.randn((v, d), device="cuda")
+    both = head.cross_entropy_grad(x, w, y, grad=g, dw=before.clone(), accumulate=True)[2]
+    assert torch.equal(both, before + dw)
+    again = head.distill_grad(x, w, y[:, None], torch.zeros((t, 1), device="cuda"), grad=g,
+                              dw=torch.empty((v, d), device="cuda"))
+    assert torch.equal(again[1], dx) and torch.equal(again[2], dw)
+    for dropped in ({"dx": False}, {"dw": False}):
+        part = head.cross_entropy_grad(x, w, y, grad=g, **dropped)
+        assert torch.equal(part[1], dx) if part[1] is not None else part[2] is not None
