@@ -9,8 +9,8 @@ feeds the step: rotary positions with the norms of queries and keys (rope.py,
 include/ark_rope.h), and activations kept in 8 bits with the weight gradient
 from them (act.py, include/ark_act.h).  Operators of the two ends of a model
 whose embedding is also its output layer: the loss over the vocabulary, or the
-divergence from a teacher's top logits, with their gradients and without the
-logits in memory (head.py, include/ark_head.h), and the lookup of tokens with
+divergence from a teacher's top logits, with their gradients, the logits never
+in memory (head.py, include/ark_head.h), and the lookup of tokens with
 its gradient (embed.py, include/ark_embed.h).  This package holds the HIP sources
 (csrc/), the built library (lib/), the host-side mirror of the reference's
 optimizer interface (optimizer.py, host/ark_host.hpp for C++) and the seeded

@@ -421,7 +421,7 @@ __global__ __launch_bounds__(kLanes) void sum_kernel(SumArgs a) {
 // The whole gradient of few tokens in one launch: a block takes kFewRows rows of the
 // table and a tile of columns for each of its waves, finds the rows' positions among all
 // tokens and puts them in order by counting, for each, those before it.  A row's sums are
-// by sixteen positions.  305 tokens into 14862 x 1837 21.5 us (109 MB of zeros), 276 into
+// by sixteen positions.  305 tokens into 14862 x 1837 19.7 us (109 MB of zeros), 276 into
 // 604 x 64 9; sorted and summed in three launches 26 and 16.  512 equal tokens, a row by
 // four waves, take longer than by windows, more of them much longer.
 constexpr uint32_t kFew = 512;

@@ -590,7 +590,7 @@ __device__ __forceinline__ bool is_far(float z2) { return fabsf(z2) >= 0x1p23f &
 // next kernel: nothing waits for another block.  Bound by the matrix units at the clock
 // that power leaves them (1.95 GHz), a tile's 24 to 64 steps of 0.8 us and 6 us before and
 // after them, in which the exponentials are the largest part: 12288 x 32000 x 768 fp16
-// 655 us, 0.92 PFLOP/s; 16384 x 32000 x 2048 bf16 2.0 ms, 1.08 PFLOP/s.  8 rows: W's 49 MB
+// 673 us, 0.90 PFLOP/s; 16384 x 32000 x 2048 bf16 2.0 ms, 1.08 PFLOP/s.  8 rows: W's 49 MB
 // go past in 12 us.
 template <typename P>
 __global__ __launch_bounds__(P::kLanes, 2) void logits_kernel(LogitsArgs a) {

@@ -1,6 +1,7 @@
 """The loss over a vocabulary from the last hidden rows and the output layer
 (include/ark_head.h) for torch tensors, with its gradients, and distillation
-from a teacher's top logits; the logits themselves are never in memory.
+from a teacher's top logits.  The logits are never in memory; with gradients
+their gradient is, in 16 bits, in pieces of at most 1 GiB.
 
 ``cross_entropy(x, w, targets)`` is the loss of every token; with
 ``cross_entropy_grad`` come the gradients of x and of w (the tied embedding),
