@@ -45,7 +45,7 @@ constexpr uint32_t kFew = 1024;  // tokens that gather_kernel's blocks rank them
 // is left of it, in rows of their own: X's rows come twice for dw, and join_kernel adds dx's
 // two.  Where tokens are few a rounding of dz shows in full in dx and dw (one token's entry
 // at its target is nearly all of a row of W's gradient): up to 2.2 times the error of their
-// own rounding for one token, 1.55 for 56, and 1.4 of more, and 1.03 in two parts.  It takes
+// own rounding for one token, 1.55 for 56, 1.4 to 1.5 for more, and 1.0 in two parts.  It takes
 // a call of up to 32 tokens 0 to 8 % longer (768 x 32000: 54 us and 57 for one token, 57 and
 // 61 for 32), as its rows still fit a tile, of 64 6 to 17 % (60 and 70), of 128 28 %.
 constexpr uint32_t kTwice = 64;
